@@ -39,7 +39,8 @@ typedef enum mk_status {
   MK_ERR_NOT_BOUND = 6,      /* mk_forward before mk_bind_weights */
   MK_ERR_BAD_TOKEN = 7,      /* a token id outside [0, vocab) was seen */
   MK_ERR_WORKSPACE = 8,      /* workspace smaller than mk_workspace_size */
-  MK_ERR_TOO_LARGE = 9       /* request exceeds a fixed capacity of the library (see the entry point) */
+  MK_ERR_TOO_LARGE = 9,      /* request exceeds a fixed capacity of the library (see the entry point) */
+  MK_ERR_CACHE = 10          /* a cache row lacks a page that it needs, or no page was free (see mk_get_error) */
 } mk_status;
 
 /* Model configuration: plugin/minicpm5_mk/model.py:561-567 plus the MiniCPM muP scalars.
@@ -299,6 +300,105 @@ mk_status mk_lm_head_argmax(const float* h, int32_t bs, int32_t H, const void* l
 #define MK_LM_HEAD_NOALLOC_MAX_ROWS 64
 mk_status mk_lm_head_argmax_noalloc(const float* h, int32_t bs, int32_t H, const void* lm_head, int32_t V,
                                     float* logits, int32_t* top1, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit paged key/value cache
+ * No counterpart in the reference, whose path keeps no cache.  With these a prompt is run once and several
+ * continuations of it are scored or generated from its cached keys and values.
+ *
+ *   codes  int8 [layers, num_pages, 2, n_kv, page_size, head_dim]   (plane 0 keys, plane 1 values)
+ *   scales f32  [layers, num_pages, 2, n_kv]
+ * value = code * scale: one scale for each block of page_size tokens and head, for keys and for values.
+ * A head's key plane is [page_size, head_dim]; its value plane is [page_size / 4, head_dim, 4] (groups of
+ * four tokens, token innermost).  page_size 16, 32, 64 or 128; head_dim 96 or 128.  Calls that work on one
+ * layer take that layer's codes and scales.
+ *   block_table int32 [rows, width]: page of tokens [j * page_size, (j + 1) * page_size) of a row, -1 past
+ *               its end; lens int32 [rows]; refs int32 [num_pages]: table entries that list a page, 0 = free.
+ * Lengths, tables and counts stay on the device: nothing here copies them to the host.  A row whose table
+ * lacks a page that a call needs, or holds a page id out of range, sets the device error word (mk_get_error:
+ * MK_ERR_CACHE); those tokens are skipped. */
+
+/* Quantises new tokens into positions lens[r] .. lens[r] + n - 1 of each row (lens is not advanced).
+ *   k, v    bf16 [T, n_kv, head_dim], token strides ld_*, head strides head_ld_* (elements, multiples of 8)
+ *   cu_new  int32 [rows + 1]: row r's tokens are [cu_new[r], cu_new[r + 1]); NULL: one token per row (T == rows)
+ *   max_new bound of a row's new tokens
+ * Per page, plane and head: scale' = max(scale if the page already holds tokens of the row, max|new| / 127);
+ * new codes are rint(x / scale'), codes already there rint(code * scale / scale') (round half to even).
+ * Keys or values that are not finite make the page head's scale NaN.  Pages written to must belong to one
+ * row only (mk_kv_fork gives each row a last page of its own). */
+mk_status mk_kv_append(const void* k, const void* v, int64_t ld_k, int64_t head_ld_k, int64_t ld_v, int64_t head_ld_v,
+                       int32_t T, void* codes, float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                       int32_t head_dim, const int32_t* block_table, int32_t rows, int32_t width, const int32_t* lens,
+                       const int32_t* cu_new, int32_t max_new, void* stream);
+
+/* Reads positions start[r] .. start[r] + count[r] - 1 back: k, v bf16 [rows, max_count, n_kv, head_dim], zeros
+ * from count[r] on. */
+mk_status mk_kv_read(const void* codes, const float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                     int32_t head_dim, const int32_t* block_table, int32_t rows, int32_t width, const int32_t* start,
+                     const int32_t* count, int32_t max_count, void* k, void* v, void* stream);
+
+/* Attention of the last tokens of each row over the row's cached keys and values.
+ *   q       bf16 [T, n_q, head_dim] (strides as in mk_kv_append); query head h reads kv head h / (n_q / n_kv)
+ *   lens    tokens of each row in the cache, the queries' own included
+ *   cu_q    int32 [rows + 1]: row r's queries; query i of n sits at position lens[r] - n + i and sees the keys up
+ *           to it.  NULL: one query per row (T == rows)
+ *   max_q, max_len  bounds of a row's queries and of lens; rows past them are cut to them
+ *   out     bf16 [T, n_q, head_dim];  lse f32 [T, n_q] (optional): ln sum exp of the scaled scores
+ * A query that sees no key (an idle row, lens 0) gives zeros and lse = -inf.
+ * workspace: mk_attention_paged_workspace bytes, 16-byte aligned, free for other use once the call's work is
+ * done; it need not be initialised. */
+mk_status mk_attention_paged_workspace(int32_t T, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t rows, int32_t max_q,
+                                       int32_t max_len, size_t* bytes);
+mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int32_t T, int32_t n_q, const void* codes,
+                             const float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size, int32_t head_dim,
+                             const int32_t* block_table, int32_t rows, int32_t width, const int32_t* lens,
+                             const int32_t* cu_q, int32_t max_q, int32_t max_len, float softmax_scale, void* out,
+                             float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of mk_kv_fork (rows: its new rows) and mk_kv_compact; 16-byte aligned. */
+size_t mk_kv_move_workspace(int32_t rows, int32_t num_pages);
+
+/* New rows that continue old ones: row i of the result continues row parents[i] (-1: an empty row).  A parent
+ * may have several children (they share its whole pages) or none (its pages become free).  The first child
+ * of a parent keeps a partly filled last page, each later one gets a copy of it, in all layers, on a free
+ * page (the lowest ids, in row order).  new_table [new_rows, width] and new_lens are written, refs (all
+ * num_pages) is written anew from new_table.  At most 8192 new rows. */
+mk_status mk_kv_fork(void* codes, float* scales, int32_t layers, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                     int32_t head_dim, const int32_t* block_table, const int32_t* lens, int32_t rows, int32_t width,
+                     const int32_t* parents, int32_t new_rows, int32_t* new_table, int32_t* new_lens, int32_t* refs,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gives each row, in place, the pages of its next n_new[r] tokens that it does not have yet (n_new NULL: one
+ * token each), lowest free ids first, in row order, and counts them in refs.  At most 8192 rows. */
+mk_status mk_kv_reserve(int32_t* block_table, const int32_t* lens, int32_t rows, int32_t width, const int32_t* n_new,
+                        int32_t* refs, int32_t num_pages, int32_t page_size, void* stream);
+
+/* Moves the pages in use to the lowest ids, in all layers: with n in use, those with ids >= n move into the
+ * holes below, in ascending order.  new_table, new_refs and used[0] = n are written. */
+mk_status mk_kv_compact(void* codes, float* scales, int32_t layers, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                        int32_t head_dim, const int32_t* block_table, int32_t rows, int32_t width, const int32_t* refs,
+                        int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* ---------------------------------------------------------------- scores of given tokens
+ * The prompt log-probabilities that the reference's fast path refuses (plugin/minicpm5_mk/__init__.py:10-32). */
+
+/* For each row of logits [T, ld] (f32: logits_bits 32, bf16: 16; the first V entries) and its token targets[t]:
+ *   logprobs f32: logit - logsumexp;   entropy f32: -sum p ln p;   ranks int32: 1 + logits above the token's
+ *   top_ids int32 [T, top_k], top_logprobs f32 [T, top_k]: the largest logits, equal ones by lower id
+ * A target outside [0, V) gives logprob 0 and rank 0.  Logits of -inf have probability 0; a row of nothing else
+ * gives logprobs -inf and entropy 0.  A NaN or +inf in a row makes its logprobs and entropy NaN; a NaN ranks
+ * below every number.  0 <= top_k <= 64. */
+mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, int32_t V, int64_t ld,
+                            const int32_t* targets, int32_t top_k, float* logprobs, float* entropy, int32_t* ranks,
+                            int32_t* top_ids, float* top_logprobs, void* stream);
+
+/* The same logprobs and entropy from hidden rows: logits = logit_scale * h @ lm_head^T (f32 accumulation), which
+ * are never written to memory.  h bf16 [T, H] with row stride ld, lm_head bf16 [V, H]; H and ld multiples of 8.
+ * workspace: mk_score_tokens_workspace bytes, 16-byte aligned. */
+mk_status mk_score_tokens_workspace(int32_t T, int32_t H, int32_t V, size_t* bytes);
+mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const void* lm_head, int32_t V,
+                          const int32_t* targets, float logit_scale, float* logprobs, float* entropy, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

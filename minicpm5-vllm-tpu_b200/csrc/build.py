@@ -20,9 +20,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_ROOT = os.path.dirname(HERE)
 REPO = os.path.dirname(PKG_ROOT)
 OUT = os.path.join(PKG_ROOT, "minicpm5_mk", "libminicpm5_mk.so")
-SOURCES = [os.path.join(HERE, "mk_api.cu")]
+SOURCES = [os.path.join(HERE, f) for f in ("mk_api.cu", "mk_cache.cu", "mk_score.cu")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
-              "-shared", "-Xptxas", "-v"]
+              "-shared", "-Xptxas", "-v", "--threads", "0"]
 
 
 def _nvcc() -> str:

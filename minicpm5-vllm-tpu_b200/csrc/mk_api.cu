@@ -16,11 +16,16 @@
 #include "mk_attn_tc.cuh"
 #include "mk_common.cuh"
 #include "mk_gemm.cuh"
+#include "mk_host.cuh"
 #include "mk_small.cuh"
 
 namespace {
 
+using mk::aligned16;
 using mk::AttnLastArgs;
+using mk::cuda_status;
+using mk::launch_k;
+using mk::PFN_encodeTiled;
 using mk::GemmArgs;
 
 // Library device error word (one per device that loads the library); first error wins.
@@ -38,10 +43,6 @@ int lm_launches(int bs, int H) {
   return (bs + nr - 1) / nr;
 }
 
-typedef CUresult (*PFN_encodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 struct DeviceState {
   bool ready = false;
   int sm_count = 0;
@@ -52,19 +53,6 @@ struct DeviceState {
 std::mutex g_mu;
 DeviceState g_dev[kMaxDevices];
 PFN_encodeTiled g_encode = nullptr;
-
-mk_status cuda_status(cudaError_t e) { return e == cudaSuccess ? MK_OK : MK_ERR_CUDA; }
-
-#define MK_CUDA(x)                                   \
-  do {                                               \
-    cudaError_t e_ = (x);                            \
-    if (e_ != cudaSuccess) return MK_ERR_CUDA;       \
-  } while (0)
-#define MK_TRY(x)                \
-  do {                           \
-    mk_status s_ = (x);          \
-    if (s_ != MK_OK) return s_;  \
-  } while (0)
 
 // Per-device one-time set-up: SM count, error-word address, kernel attributes, driver entry point.
 mk_status device_state(DeviceState** out) {
@@ -137,26 +125,6 @@ mk_status device_state(DeviceState** out) {
   return MK_OK;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// Launch `k` on `st`; with `pdl` the launch carries programmatic stream serialization, so the kernel may
-// begin while the previous kernel of the stream drains (every kernel of the forward calls pdl_wait()
-// before touching memory an earlier kernel uses).
-template <typename... KArgs, typename... Args>
-mk_status launch_k(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
-                   Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
-}
 // The same with clusters of two CTAs along x (grid.x even).
 template <typename... KArgs, typename... Args>
 mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
@@ -469,6 +437,15 @@ size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 }  // namespace
 
+mk_status mk::host_device(HostDevice* out) {
+  DeviceState* d = nullptr;
+  MK_TRY(device_state(&d));
+  out->sm_count = d->sm_count;
+  out->err = d->err;
+  out->encode = g_encode;
+  return MK_OK;
+}
+
 struct mk_handle {
   mk_config cfg;
   int device = 0;
@@ -497,6 +474,7 @@ const char* mk_status_string(mk_status s) {
     case MK_ERR_BAD_TOKEN: return "token id out of range";
     case MK_ERR_WORKSPACE: return "workspace too small";
     case MK_ERR_TOO_LARGE: return "request exceeds a fixed library capacity";
+    case MK_ERR_CACHE: return "cache page missing or none free";
   }
   return "unknown status";
 }
@@ -1120,6 +1098,7 @@ mk_status mk_get_error(mk_handle* h, int32_t* device_err) {
   if (device_err) *device_err = v;
   if (v == 0) return MK_OK;
   if (v == mk::DEV_ERR_BAD_TOKEN_ID) return MK_ERR_BAD_TOKEN;
+  if (v == mk::DEV_ERR_BAD_PAGE || v == mk::DEV_ERR_NO_PAGE) return MK_ERR_CACHE;
   return MK_ERR_DEVICE_TIMEOUT;
 }
 

@@ -1,0 +1,219 @@
+// C ABI of the 8-bit paged key/value cache: append, read-back, attention over it, and page moves.
+// See include/minicpm5_mk.h.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "mk_attn_paged.cuh"
+#include "mk_cache.cuh"
+#include "mk_host.cuh"
+
+namespace {
+
+using mk::aligned16;
+using mk::cuda_status;
+using mk::HostDevice;
+using mk::KvPages;
+using mk::launch_k;
+
+// Checks one layer's (or all layers') pages and fills the kernel's view of them.
+mk_status kv_pages(KvPages* out, void* codes, float* scales, int num_pages, int n_kv, int page, int hd) {
+  if (!codes || !scales) return MK_ERR_BAD_ARG;
+  if (num_pages <= 0 || n_kv <= 0 || (hd != 96 && hd != 128)) return MK_ERR_BAD_SHAPE;
+  if (page != 16 && page != 32 && page != 64 && page != 128) return MK_ERR_BAD_SHAPE;
+  if (!aligned16(codes) || (reinterpret_cast<uintptr_t>(scales) & 3u)) return MK_ERR_BAD_ALIGN;
+  out->codes = static_cast<int8_t*>(codes);
+  out->scales = scales;
+  out->num_pages = num_pages;
+  out->n_kv = n_kv;
+  out->head_dim = hd;
+  out->page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+  return MK_OK;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+size_t page_bytes(int n_kv, int page, int hd) { return static_cast<size_t>(2) * n_kv * page * hd; }
+
+mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int n_kv, int page, int hd, int max_pairs,
+                     const int2* pairs, const int32_t* n_pairs, cudaStream_t st) {
+  return launch_k(mk::kv_copy_pages_kernel, dim3(std::min(max_pairs, 4096), layers), dim3(mk::COPY_THREADS), 0, st, true,
+                  static_cast<int8_t*>(codes), scales, num_pages, page_bytes(n_kv, page, hd), 2 * n_kv, pairs, n_pairs);
+}
+
+}  // namespace
+
+extern "C" {
+
+mk_status mk_kv_append(const void* k, const void* v, int64_t ld_k, int64_t head_ld_k, int64_t ld_v, int64_t head_ld_v,
+                       int32_t T, void* codes, float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                       int32_t head_dim, const int32_t* block_table, int32_t rows, int32_t width, const int32_t* lens,
+                       const int32_t* cu_new, int32_t max_new, void* stream) {
+  KvPages c;
+  MK_TRY(kv_pages(&c, codes, scales, num_pages, n_kv, page_size, head_dim));
+  if (rows < 0 || width <= 0 || T < 0 || max_new < 0 || (!cu_new && T != rows)) return MK_ERR_BAD_SHAPE;
+  if (rows == 0 || T == 0 || max_new == 0) return MK_OK;
+  if (!k || !v || !block_table || !lens) return MK_ERR_BAD_ARG;
+  if (!aligned16(k) || !aligned16(v) || ld_k % 8 || ld_v % 8 || head_ld_k % 8 || head_ld_v % 8) return MK_ERR_BAD_ALIGN;
+  const int touched = (std::max(1, cu_new ? max_new : 1) + page_size - 2) / page_size + 1;
+  if (static_cast<int64_t>(rows) * touched > INT_MAX || n_kv > 65535) return MK_ERR_TOO_LARGE;
+  HostDevice d;
+  MK_TRY(mk::host_device(&d));
+  return launch_k(mk::kv_append_kernel, dim3(rows * touched, 2, n_kv), dim3(mk::KVA_THREADS), 0,
+                  static_cast<cudaStream_t>(stream), true, static_cast<const __nv_bfloat16*>(k),
+                  static_cast<const __nv_bfloat16*>(v), static_cast<long long>(ld_k), static_cast<long long>(head_ld_k),
+                  static_cast<long long>(ld_v), static_cast<long long>(head_ld_v), T, c, block_table, width, lens, cu_new,
+                  touched, d.err);
+}
+
+mk_status mk_kv_read(const void* codes, const float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                     int32_t head_dim, const int32_t* block_table, int32_t rows, int32_t width, const int32_t* start,
+                     const int32_t* count, int32_t max_count, void* k, void* v, void* stream) {
+  KvPages c;
+  MK_TRY(kv_pages(&c, const_cast<void*>(codes), const_cast<float*>(scales), num_pages, n_kv, page_size, head_dim));
+  if (rows < 0 || width <= 0 || max_count < 0) return MK_ERR_BAD_SHAPE;
+  if (rows == 0 || max_count == 0) return MK_OK;
+  if (!k || !v || !block_table || !start || !count) return MK_ERR_BAD_ARG;
+  if (!aligned16(k) || !aligned16(v)) return MK_ERR_BAD_ALIGN;
+  const int64_t items = (static_cast<int64_t>(max_count) / 4 + 2) * n_kv * (head_dim / 8);
+  if (items > INT_MAX || rows > 65535) return MK_ERR_TOO_LARGE;
+  HostDevice d;
+  MK_TRY(mk::host_device(&d));
+  const int blocks = static_cast<int>((items + mk::KVR_THREADS - 1) / mk::KVR_THREADS);
+  return launch_k(mk::kv_read_kernel, dim3(blocks, rows, 2), dim3(mk::KVR_THREADS), 0, static_cast<cudaStream_t>(stream),
+                  true, c, block_table, width, start, count, max_count, static_cast<__nv_bfloat16*>(k),
+                  static_cast<__nv_bfloat16*>(v), d.err);
+}
+
+mk_status mk_attention_paged_workspace(int32_t T, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t rows, int32_t max_q,
+                                       int32_t max_len, size_t* bytes) {
+  if (!bytes) return MK_ERR_BAD_ARG;
+  if (T < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || (head_dim != 96 && head_dim != 128) || rows < 0 || max_q < 0 ||
+      max_len < 0)
+    return MK_ERR_BAD_SHAPE;
+  *bytes = 0;
+  return MK_OK;
+}
+
+mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int32_t T, int32_t n_q, const void* codes,
+                             const float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size, int32_t head_dim,
+                             const int32_t* block_table, int32_t rows, int32_t width, const int32_t* lens,
+                             const int32_t* cu_q, int32_t max_q, int32_t max_len, float softmax_scale, void* out,
+                             float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  KvPages c;
+  MK_TRY(kv_pages(&c, const_cast<void*>(codes), const_cast<float*>(scales), num_pages, n_kv, page_size, head_dim));
+  size_t need = 0;
+  MK_TRY(mk_attention_paged_workspace(T, n_q, n_kv, head_dim, rows, max_q, max_len, &need));
+  if (width <= 0 || (!cu_q && T != rows)) return MK_ERR_BAD_SHAPE;
+  if (T == 0 || rows == 0) return MK_OK;
+  if (!q || !out || !block_table || !lens || (need && !workspace)) return MK_ERR_BAD_ARG;
+  if (workspace_bytes < need) return MK_ERR_WORKSPACE;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || ld_q % 8 || head_ld_q % 8) return MK_ERR_BAD_ALIGN;
+  if (n_q > 65535) return MK_ERR_TOO_LARGE;
+  HostDevice d;
+  MK_TRY(mk::host_device(&d));
+  mk::PagedAttnArgs a;
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.ld_q = ld_q;
+  a.hs_q = head_ld_q;
+  a.n_q = n_q;
+  a.rows = rows;
+  a.width = width;
+  a.table = block_table;
+  a.lens = lens;
+  a.cu = cu_q;
+  a.scale = softmax_scale;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.err = d.err;
+  return launch_k(mk::attn_paged_kernel, dim3(T, n_q), dim3(mk::PA_THREADS), 0, static_cast<cudaStream_t>(stream), true, c,
+                  a);
+}
+
+size_t mk_kv_move_workspace(int32_t rows, int32_t num_pages) {
+  if (rows < 0 || num_pages < 0) return 0;
+  // [count][pairs: max(rows, num_pages)][ids: max(rows, num_pages)]
+  const size_t n = static_cast<size_t>(std::max(rows, num_pages));
+  return 256 + align256(n * sizeof(int2)) + align256(n * sizeof(int32_t));
+}
+
+mk_status mk_kv_fork(void* codes, float* scales, int32_t layers, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                     int32_t head_dim, const int32_t* block_table, const int32_t* lens, int32_t rows, int32_t width,
+                     const int32_t* parents, int32_t new_rows, int32_t* new_table, int32_t* new_lens, int32_t* refs,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  KvPages c;
+  MK_TRY(kv_pages(&c, codes, scales, num_pages, n_kv, page_size, head_dim));
+  if (!refs || !workspace) return MK_ERR_BAD_ARG;
+  if (layers <= 0 || rows < 0 || width <= 0 || new_rows < 0) return MK_ERR_BAD_SHAPE;
+  if (new_rows && (!parents || !new_table || !new_lens || !block_table || !lens)) return MK_ERR_BAD_ARG;
+  if (new_rows && (new_table == block_table || new_lens == lens)) return MK_ERR_BAD_ARG;
+  if (workspace_bytes < mk_kv_move_workspace(new_rows, num_pages)) return MK_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MK_ERR_BAD_ALIGN;
+  if (new_rows > mk::PG_ROWS_MAX || layers > 65535) return MK_ERR_TOO_LARGE;
+  HostDevice d;
+  MK_TRY(mk::host_device(&d));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  int32_t* count = reinterpret_cast<int32_t*>(ws);
+  int2* pairs = reinterpret_cast<int2*>(ws + 256);
+  int32_t* src = reinterpret_cast<int32_t*>(ws + 256 + align256(static_cast<size_t>(std::max(new_rows, num_pages)) * sizeof(int2)));
+  MK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(num_pages) * sizeof(int32_t), st));
+  if (new_rows == 0) return MK_OK;
+  MK_TRY(launch_k(mk::kv_fork_rows_kernel, dim3(new_rows), dim3(mk::FORK_THREADS), 0, st, false, block_table, lens, rows,
+                  width, parents, num_pages, c.page_shift, new_table, new_lens, refs, src, d.err));
+  MK_TRY(launch_k(mk::kv_assign_kernel, dim3(1), dim3(mk::PG_THREADS), static_cast<size_t>(new_rows) * sizeof(int), st, true,
+                  new_table, static_cast<const int32_t*>(new_lens), new_rows, width, static_cast<const int32_t*>(nullptr),
+                  static_cast<const int32_t*>(src), pairs, count, refs, num_pages, c.page_shift, d.err));
+  return copy_pages(codes, scales, layers, num_pages, n_kv, page_size, head_dim, new_rows, pairs, count, st);
+}
+
+mk_status mk_kv_reserve(int32_t* block_table, const int32_t* lens, int32_t rows, int32_t width, const int32_t* n_new,
+                        int32_t* refs, int32_t num_pages, int32_t page_size, void* stream) {
+  if (rows < 0 || width <= 0 || num_pages <= 0) return MK_ERR_BAD_SHAPE;
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return MK_ERR_BAD_SHAPE;
+  if (rows == 0) return MK_OK;
+  if (!refs || !block_table || !lens) return MK_ERR_BAD_ARG;
+  if (rows > mk::PG_ROWS_MAX) return MK_ERR_TOO_LARGE;
+  HostDevice d;
+  MK_TRY(mk::host_device(&d));
+  const int shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+  return launch_k(mk::kv_assign_kernel, dim3(1), dim3(mk::PG_THREADS), static_cast<size_t>(rows) * sizeof(int),
+                  static_cast<cudaStream_t>(stream), true, block_table, lens, rows, width, n_new,
+                  static_cast<const int32_t*>(nullptr), static_cast<int2*>(nullptr), static_cast<int32_t*>(nullptr), refs,
+                  num_pages, shift, d.err);
+}
+
+mk_status mk_kv_compact(void* codes, float* scales, int32_t layers, int32_t num_pages, int32_t n_kv, int32_t page_size,
+                        int32_t head_dim, const int32_t* block_table, int32_t rows, int32_t width, const int32_t* refs,
+                        int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  KvPages c;
+  MK_TRY(kv_pages(&c, codes, scales, num_pages, n_kv, page_size, head_dim));
+  if (!refs || !new_refs || !used || !workspace) return MK_ERR_BAD_ARG;
+  if (layers <= 0 || rows < 0 || width <= 0) return MK_ERR_BAD_SHAPE;
+  if (rows && (!block_table || !new_table)) return MK_ERR_BAD_ARG;
+  if (refs == new_refs) return MK_ERR_BAD_ARG;
+  if (workspace_bytes < mk_kv_move_workspace(rows, num_pages)) return MK_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MK_ERR_BAD_ALIGN;
+  if (layers > 65535) return MK_ERR_TOO_LARGE;
+  HostDevice d;
+  MK_TRY(mk::host_device(&d));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  int32_t* count = reinterpret_cast<int32_t*>(ws);
+  int2* pairs = reinterpret_cast<int2*>(ws + 256);
+  int32_t* to = reinterpret_cast<int32_t*>(ws + 256 + align256(static_cast<size_t>(std::max(rows, num_pages)) * sizeof(int2)));
+  MK_TRY(launch_k(mk::kv_compact_plan_kernel, dim3(1), dim3(mk::PG_THREADS), 0, st, true, refs, num_pages, new_refs, to,
+                  pairs, count, used));
+  const size_t entries = static_cast<size_t>(rows) * width;
+  if (entries) {
+    const size_t blocks = std::min<size_t>((entries + 255) / 256, static_cast<size_t>(d.sm_count) * 8);
+    MK_TRY(launch_k(mk::kv_remap_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, true, block_table, entries,
+                    static_cast<const int32_t*>(to), num_pages, new_table, d.err));
+  }
+  return copy_pages(codes, scales, layers, num_pages, n_kv, page_size, head_dim, (num_pages + 1) / 2, pairs, count, st);
+}
+
+}  // extern "C"

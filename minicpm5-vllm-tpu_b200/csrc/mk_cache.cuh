@@ -1,0 +1,488 @@
+// The 8-bit paged key/value cache: quantising append, read-back, and the moves of whole pages.
+//
+// Layout.  codes int8 [layers, pages, 2, n_kv, page, hd], scales f32 [layers, pages, 2, n_kv]; plane 0 holds
+// keys, plane 1 values, and value = code * scale: one scale for each (page, plane, head).  A head's key plane
+// is [page, hd] row by row.  Its value plane is [page / 4, hd, 4]: the four bytes of one 32-bit word are one
+// channel of four consecutive tokens, which is the operand order of the probability-value product (the
+// tokens are its contraction), so attention reads neither plane through a transpose.  Any 16 consecutive
+// tokens of a plane are 16 * hd contiguous bytes in both.
+#pragma once
+
+#include "mk_common.cuh"
+
+namespace mk {
+
+constexpr float kCodeMax = 127.f;
+
+// One layer's pages (or all layers', for page moves) and the rows of pages that index them.
+struct KvPages {
+  int8_t* codes;
+  float* scales;
+  int num_pages, n_kv, page_shift, head_dim;  // page = 1 << page_shift tokens
+};
+
+// Elements of one (page, plane, head), one plane of a page, and one page of a layer.
+__device__ __forceinline__ size_t kv_head_elems(const KvPages& c) {
+  return static_cast<size_t>(c.head_dim) << c.page_shift;
+}
+__device__ __forceinline__ int8_t* kv_head_ptr(const KvPages& c, int page, int plane, int head) {
+  return c.codes + ((static_cast<size_t>(page) * 2 + plane) * c.n_kv + head) * kv_head_elems(c);
+}
+__device__ __forceinline__ float* kv_scale_ptr(const KvPages& c, int page, int plane, int head) {
+  return c.scales + (static_cast<size_t>(page) * 2 + plane) * c.n_kv + head;
+}
+
+// Page of slot `slot` of row `row`, -1 (and the error word set) where the table has no such page.
+__device__ __forceinline__ int kv_page_of(const int32_t* table, int width, int num_pages, int row, int slot, int* err) {
+  const int page = slot < width ? table[static_cast<size_t>(row) * width + slot] : -1;
+  if (page >= 0 && page < num_pages) return page;
+  if (err) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+  return -1;
+}
+
+// round-half-even(x / s) as a code; s > 0
+__device__ __forceinline__ int quant1(float x, float s) {
+  return max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))));
+}
+
+// ---------------------------------------------------------------------------------- append
+// New tokens of each row, quantised into the pages that hold positions lens[r] .. lens[r] + n - 1.
+//
+//   scale' = max(scale of the tokens already in the page, max |new| / 127)      (a page begun anew: the latter)
+//   code   = rint(x / scale') for new tokens,  rint(code * scale / scale') for those already there
+//
+// so a page's scale only grows, and a token already there is rounded again (by at most half a step of the
+// new scale) only when a larger one joins it.  Where the new tokens or the page's scale hold a NaN or an
+// infinity the scale becomes NaN: the page then reads as NaN instead of as a plausible number.
+//
+// Bounds: 2 bytes read and 1 written per element.  One CTA owns one (page, plane, head), so the scale has one
+// writer and nothing is atomic.  A thread's item is 4 tokens x 8 channels: four 16-byte loads, and 32
+// contiguous bytes of the value plane or four 8-byte pieces of the key plane.  The items stay in registers
+// between the maximum and the rounding, so the input is read once.
+constexpr int KVA_THREADS = 256;
+constexpr int KVA_ITEMS = 2;  // 4 x 8 items per thread: 128 tokens x 128 channels
+
+__global__ void __launch_bounds__(KVA_THREADS)
+    kv_append_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long ld_k,
+                     long long hs_k, long long ld_v, long long hs_v, int T, KvPages c, const int32_t* __restrict__ table,
+                     int width, const int32_t* __restrict__ lens, const int32_t* __restrict__ cu, int touched, int* err) {
+  __shared__ uint32_t red[KVA_THREADS / 32];
+  pdl_wait();
+  pdl_trigger();
+  const int row = blockIdx.x / touched, plane = blockIdx.y, head = blockIdx.z;
+  const int tok0 = cu ? cu[row] : row, n = cu ? cu[row + 1] - tok0 : 1;
+  const int len = lens[row], page_tokens = 1 << c.page_shift;
+  if (n <= 0 || len < 0 || tok0 < 0 || tok0 + n > T) return;
+  const int slot = (len >> c.page_shift) + blockIdx.x % touched;
+  const int pos0 = slot << c.page_shift;
+  if (pos0 >= len + n) return;
+  const int page = kv_page_of(table, width, c.num_pages, row, slot, err);
+  if (page < 0) return;
+  const int hd = c.head_dim, chunks = hd >> 3, items = (page_tokens >> 2) * chunks;
+  const __nv_bfloat16* src = plane ? v : k;
+  const long long ld = plane ? ld_v : ld_k;
+  src += head * (plane ? hs_v : hs_k);
+  int8_t* dst = kv_head_ptr(c, page, plane, head);
+  float* sp = kv_scale_ptr(c, page, plane, head);
+  const bool had = pos0 < len;
+  const float was = had ? *sp : 0.f;
+
+  uint4 x[KVA_ITEMS][4];
+  uint32_t top = 0;  // largest |x| as bf16 bits, two halves
+#pragma unroll
+  for (int i = 0; i < KVA_ITEMS; ++i) {
+    const int it = threadIdx.x + i * KVA_THREADS, g = it / chunks, ch = it - g * chunks;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int pos = pos0 + 4 * g + t;
+      x[i][t] = make_uint4(0, 0, 0, 0);
+      if (it < items && pos >= len && pos < len + n)
+        x[i][t] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(tok0 + pos - len) * ld + ch * 8));
+      const uint32_t a = __vmaxu2(x[i][t].x & 0x7fff7fffu, x[i][t].y & 0x7fff7fffu);
+      const uint32_t b = __vmaxu2(x[i][t].z & 0x7fff7fffu, x[i][t].w & 0x7fff7fffu);
+      top = __vmaxu2(top, __vmaxu2(a, b));
+    }
+  }
+  top = max(top & 0xffffu, top >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+  for (int w = 0; w < KVA_THREADS / 32; ++w) top = max(top, red[w]);
+  // 0x7f80 and above are infinity and NaN
+  const float amax = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __uint_as_float(top << 16);
+  const float fresh = __fdiv_rn(amax, kCodeMax);
+  const float now = fresh != fresh || was != was ? __int_as_float(0x7fffffff) : fmaxf(was, fresh);
+  const bool finite = now - now == 0.f;
+  const float by = finite && now > 0.f ? now : 1.f;
+  const bool again = had && now != was;  // the tokens already there change their codes
+  if (threadIdx.x == 0) *sp = now;
+
+#pragma unroll
+  for (int i = 0; i < KVA_ITEMS; ++i) {
+    const int it = threadIdx.x + i * KVA_THREADS, g = it / chunks, ch = it - g * chunks;
+    if (it >= items) continue;
+    const int pos = pos0 + 4 * g;
+    // tokens of this group: [0, o) were there, [o, m) are new, [m, 4) are past the end
+    const int o = min(4, max(0, len - pos)), m = min(4, max(0, len + n - pos));
+    if (m == o && !(again && o > 0)) continue;
+    uint32_t w[4][2];  // [token][8 codes]
+    if (o > 0 || (plane && m < 4)) {  // bytes that stay or are rescaled
+      if (plane) {
+        const uint4 lo = *reinterpret_cast<const uint4*>(dst + (static_cast<size_t>(g) * hd + ch * 8) * 4);
+        const uint4 hi = *reinterpret_cast<const uint4*>(dst + (static_cast<size_t>(g) * hd + ch * 8) * 4 + 16);
+        const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          w[t][0] = w[t][1] = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[t][e >> 2] |= ((u[e] >> (8 * t)) & 0xffu) << (8 * (e & 3));
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint2 u = *reinterpret_cast<const uint2*>(dst + static_cast<size_t>(4 * g + t) * hd + ch * 8);
+          w[t][0] = u.x;
+          w[t][1] = u.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (t >= o && t < m) {
+        const uint32_t u[4] = {x[i][t].x, x[i][t].y, x[i][t].z, x[i][t].w};
+        uint32_t r[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_bf16x2(u[e]);
+          const uint32_t a = finite ? static_cast<uint32_t>(quant1(f.x, by)) & 0xffu : 0u;
+          const uint32_t b = finite ? static_cast<uint32_t>(quant1(f.y, by)) & 0xffu : 0u;
+          r[e >> 1] |= (a | b << 8) << (16 * (e & 1));
+        }
+        w[t][0] = r[0];
+        w[t][1] = r[1];
+      } else if (t < o && again) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float cd = static_cast<float>(static_cast<int8_t>(w[t][h] >> (8 * e)));
+            r |= (finite ? static_cast<uint32_t>(quant1(__fmul_rn(cd, was), by)) & 0xffu : 0u) << (8 * e);
+          }
+          w[t][h] = r;
+        }
+      }
+    }
+    if (plane) {
+      uint32_t u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        u[e] = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) u[e] |= ((w[t][e >> 2] >> (8 * (e & 3))) & 0xffu) << (8 * t);
+      }
+      uint4* p = reinterpret_cast<uint4*>(dst + (static_cast<size_t>(g) * hd + ch * 8) * 4);
+      p[0] = make_uint4(u[0], u[1], u[2], u[3]);
+      p[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (t < m && (t >= o || again))
+          *reinterpret_cast<uint2*>(dst + static_cast<size_t>(4 * g + t) * hd + ch * 8) = make_uint2(w[t][0], w[t][1]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------- read back
+// out[r, i] = bf16 of the keys (plane 0) and values of position start[r] + i, zero from count[r] on.
+// An item is 4 tokens x 8 channels of one head, at a 4-token boundary of the cache, as in the append.
+constexpr int KVR_THREADS = 256;
+__global__ void __launch_bounds__(KVR_THREADS)
+    kv_read_kernel(KvPages c, const int32_t* __restrict__ table, int width, const int32_t* __restrict__ start,
+                   const int32_t* __restrict__ count, int max_count, __nv_bfloat16* __restrict__ ko,
+                   __nv_bfloat16* __restrict__ vo, int* err) {
+  pdl_wait();
+  pdl_trigger();
+  const int row = blockIdx.y, plane = blockIdx.z;
+  const int hd = c.head_dim, chunks = hd >> 3, per_group = chunks * c.n_kv;
+  const int s0 = start[row], n = s0 < 0 ? 0 : min(count[row], max_count);
+  const int it = blockIdx.x * KVR_THREADS + threadIdx.x;
+  const int g = it / per_group, hc = it - g * per_group, head = hc / chunks, ch = hc - head * chunks;
+  const int lead = max(s0, 0) & 3;           // tokens of the first group before the range
+  const int i0 = 4 * g - lead;               // output row of the group's first token
+  if (i0 >= max_count) return;
+  uint32_t u[4][4] = {};
+  if (i0 < n) {
+    const int pos = s0 + i0;
+    const int page = kv_page_of(table, width, c.num_pages, row, pos >> c.page_shift, err);
+    if (page >= 0) {
+      const int in = pos & ((1 << c.page_shift) - 1);
+      const int8_t* src = kv_head_ptr(c, page, plane, head);
+      const float sc = *kv_scale_ptr(c, page, plane, head);
+      if (plane) {
+        const uint4* p = reinterpret_cast<const uint4*>(src + static_cast<size_t>(in) * hd + ch * 32);
+        const uint4 lo = p[0], hi = p[1];
+        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            u[t][e] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(w[2 * e] >> (8 * t))) * sc,
+                                  static_cast<float>(static_cast<int8_t>(w[2 * e + 1] >> (8 * t))) * sc);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint2 p = *reinterpret_cast<const uint2*>(src + static_cast<size_t>(in + t) * hd + ch * 8);
+          const uint32_t w[2] = {p.x, p.y};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            u[t][e] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(w[e >> 1] >> (16 * (e & 1)))) * sc,
+                                  static_cast<float>(static_cast<int8_t>(w[e >> 1] >> (16 * (e & 1) + 8))) * sc);
+        }
+      }
+    }
+  }
+  __nv_bfloat16* out = plane ? vo : ko;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int i = i0 + t;
+    if (i < 0 || i >= max_count) continue;
+    const bool in = i < n;
+    *reinterpret_cast<uint4*>(out + ((static_cast<size_t>(row) * max_count + i) * c.n_kv + head) * hd + ch * 8) =
+        in ? make_uint4(u[t][0], u[t][1], u[t][2], u[t][3]) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------------- page moves
+// Pages are handed out lowest id first and in row order, so the same calls give the same tables.
+
+// Inclusive scan over the CTA's 1024 threads; `total` is the sum.
+constexpr int PG_THREADS = 1024;
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[w] = v;
+  __syncthreads();
+  int s = warp_sums[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  total = __shfl_sync(0xffffffffu, s, 31);
+  const int before = __shfl_sync(0xffffffffu, s, (w + 31) & 31);
+  return v + (w ? before : 0);
+}
+
+// new_table[i] = the pages of row parents[i] (-1: an empty row), refs[p] = the rows that list p.  The first
+// child of a parent keeps a partly filled last page; later children ask for one of their own: src[i] holds the
+// page to copy, -1 where none.  One CTA per new row; refs starts at zero.
+constexpr int FORK_THREADS = 128;
+__global__ void __launch_bounds__(FORK_THREADS)
+    kv_fork_rows_kernel(const int32_t* __restrict__ table, const int32_t* __restrict__ lens, int rows_in, int width,
+                        const int32_t* __restrict__ parents, int num_pages, int page_shift, int32_t* __restrict__ new_table,
+                        int32_t* __restrict__ new_lens, int32_t* __restrict__ refs, int32_t* __restrict__ src, int* err) {
+  pdl_wait();
+  pdl_trigger();
+  const int i = blockIdx.x;
+  int p = parents[i];
+  if (p >= rows_in) {
+    if (threadIdx.x == 0) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+    p = -1;
+  }
+  int len = p < 0 ? 0 : max(0, lens[p]);
+  const int n = min(width, (len + (1 << page_shift) - 1) >> page_shift);
+  if (threadIdx.x == 0 && len > (width << page_shift)) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+  bool twin = false;  // an earlier row continues the same parent
+  if (p >= 0)
+    for (int j = threadIdx.x; j < i; j += FORK_THREADS) twin |= parents[j] == p;
+  const bool part = (len & ((1 << page_shift) - 1)) != 0;
+  const bool copy = __syncthreads_or(twin) && part && n > 0;
+  for (int j = threadIdx.x; j < width; j += FORK_THREADS) {
+    int page = -1;
+    if (j < n) page = kv_page_of(table, width, num_pages, p, j, err);
+    const bool last = copy && j == n - 1;
+    if (page >= 0 && !last) atomicAdd(refs + page, 1);
+    if (last) src[i] = page;
+    new_table[static_cast<size_t>(i) * width + j] = last ? -1 : page;
+  }
+  if (threadIdx.x == 0) {
+    new_lens[i] = len;
+    if (!copy) src[i] = -1;
+  }
+}
+
+// Hands free pages (refs == 0, lowest first) to the rows that ask for them, in row order.
+//   fork:    row i asks for one page where src[i] >= 0: it becomes its last page, and pairs[k] = (src, page)
+//   reserve: row i asks for the missing pages of positions lens[i] .. lens[i] + n_new[i] - 1
+// The requests are scanned into shared memory, then one pass over refs deals out the pages.  One CTA: the
+// pass reads 4 bytes a page, and stops once every request is served.
+constexpr int PG_ROWS_MAX = 8192;
+__global__ void __launch_bounds__(PG_THREADS)
+    kv_assign_kernel(int32_t* __restrict__ table, const int32_t* __restrict__ lens, int rows, int width,
+                     const int32_t* __restrict__ n_new, const int32_t* __restrict__ src, int2* __restrict__ pairs,
+                     int32_t* __restrict__ n_pairs, int32_t* __restrict__ refs, int num_pages, int page_shift, int* err) {
+  extern __shared__ int upto[];  // requests of rows 0 .. i
+  __shared__ int sums[32];
+  pdl_wait();
+  pdl_trigger();
+  const int page_tokens = 1 << page_shift;
+  int asked = 0;
+  for (int base = 0; base < rows; base += PG_THREADS) {
+    const int i = base + threadIdx.x;
+    int want = 0;
+    if (i < rows) {
+      if (src) {
+        want = src[i] >= 0;
+      } else {
+        const int len = max(0, lens[i]), add = n_new ? max(0, n_new[i]) : 1;
+        const int first = len >> page_shift, end = (len + add + page_tokens - 1) >> page_shift;
+        if (add > 0 && end > width) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
+        for (int j = first; j < min(end, width); ++j) want += table[static_cast<size_t>(i) * width + j] < 0;
+      }
+    }
+    int total;
+    const int inc = block_scan(want, sums, total);
+    if (i < rows) upto[i] = asked + inc;
+    asked += total;
+  }
+  __syncthreads();
+  int given = 0;
+  for (int base = 0; base < num_pages && given < asked; base += PG_THREADS) {
+    const int page = base + threadIdx.x;
+    const int is_free = page < num_pages && refs[page] == 0;
+    int total;
+    const int k = given + block_scan(is_free, sums, total) - 1;
+    if (is_free && k < asked) {
+      int lo = 0, hi = rows - 1;  // first row with upto > k
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (upto[mid] > k) hi = mid; else lo = mid + 1;
+      }
+      const int len = max(0, lens[lo]);
+      int32_t* mine = table + static_cast<size_t>(lo) * width;
+      if (src) {
+        mine[min(width, (len + page_tokens - 1) >> page_shift) - 1] = page;
+        pairs[k] = make_int2(src[lo], page);
+      } else {
+        // the row's r-th missing slot; its other requests are served at other slots by other threads, so a
+        // slot counts as missing whether or not it has been filled meanwhile: `first` on, the row's slots
+        // with pages come before those without
+        const int r = k - (lo ? upto[lo - 1] : 0), add = n_new ? max(0, n_new[lo]) : 1;
+        const int end = min(width, (len + add + page_tokens - 1) >> page_shift), mine_n = upto[lo] - (lo ? upto[lo - 1] : 0);
+        mine[end - mine_n + r] = page;
+      }
+      refs[page] = 1;
+    }
+    given += total;
+  }
+  if (threadIdx.x == 0) {
+    if (given < asked) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
+    if (n_pairs) *n_pairs = min(given, asked);
+  }
+}
+
+// Compaction: with `used` live pages, those at `used` and above move into the holes below, lowest to lowest.
+// to[p] = the page's new id (-1: free), new_refs, pairs, n_used.  Two passes of one CTA over refs.
+__global__ void __launch_bounds__(PG_THREADS)
+    kv_compact_plan_kernel(const int32_t* __restrict__ refs, int num_pages, int32_t* __restrict__ new_refs,
+                           int32_t* __restrict__ to, int2* __restrict__ pairs, int32_t* __restrict__ n_pairs,
+                           int32_t* __restrict__ n_used) {
+  __shared__ int sums[32];
+  pdl_wait();
+  pdl_trigger();
+  int mine = 0;
+  for (int p = threadIdx.x; p < num_pages; p += PG_THREADS) mine += refs[p] > 0;
+  int used;
+  block_scan(mine, sums, used);
+  int holes = 0;
+  for (int base = 0; base < used; base += PG_THREADS) {
+    const int p = base + threadIdx.x, r = p < used ? refs[p] : 1;
+    int total;
+    const int k = holes + block_scan(r <= 0, sums, total) - 1;
+    if (p < used) {
+      to[p] = r > 0 ? p : -1;
+      if (r > 0) new_refs[p] = r; else pairs[k].y = p;
+    }
+    holes += total;
+  }
+  __syncthreads();  // the holes are written
+  int moved = 0;
+  for (int base = used; base < num_pages; base += PG_THREADS) {
+    const int p = base + threadIdx.x, r = p < num_pages ? refs[p] : 0;
+    int total;
+    const int k = moved + block_scan(r > 0, sums, total) - 1;
+    if (p < num_pages) {
+      new_refs[p] = 0;
+      to[p] = -1;
+      if (r > 0) {  // as many live pages above as holes below
+        const int hole = pairs[k].y;
+        pairs[k].x = p;
+        to[p] = hole;
+        new_refs[hole] = r;
+      }
+    }
+    moved += total;
+  }
+  if (threadIdx.x == 0) {
+    *n_pairs = moved;
+    *n_used = used;
+  }
+}
+
+// new_table = table through `to`; -1 where the table holds no page.
+__global__ void kv_remap_kernel(const int32_t* __restrict__ table, size_t n, const int32_t* __restrict__ to, int num_pages,
+                                int32_t* __restrict__ new_table, int* err) {
+  pdl_wait();
+  pdl_trigger();
+  for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n;
+       i += static_cast<size_t>(gridDim.x) * blockDim.x) {
+    const int p = table[i];
+    int q = -1;
+    if (p >= 0 && p < num_pages) q = to[p];
+    else if (p >= num_pages) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+    new_table[i] = q;
+  }
+}
+
+// codes and scales of page pairs[k].x to page pairs[k].y in every layer.  No source is a destination.
+constexpr int COPY_THREADS = 256;
+constexpr int COPY_VEC = 6;  // 16-byte vectors in flight per thread
+__global__ void __launch_bounds__(COPY_THREADS)
+    kv_copy_pages_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, int num_pages, size_t page_bytes,
+                         int page_scales, const int2* __restrict__ pairs, const int32_t* __restrict__ n_pairs) {
+  pdl_wait();
+  pdl_trigger();
+  const int n = *n_pairs, layer = blockIdx.y;
+  const size_t vecs = page_bytes / 16;
+  for (int k = blockIdx.x; k < n; k += gridDim.x) {
+    const int2 pr = pairs[k];
+    if (pr.x < 0 || pr.y < 0 || pr.x >= num_pages || pr.y >= num_pages) continue;
+    const size_t lead = static_cast<size_t>(layer) * num_pages;
+    const uint4* s = reinterpret_cast<const uint4*>(codes + (lead + pr.x) * page_bytes);
+    uint4* d = reinterpret_cast<uint4*>(codes + (lead + pr.y) * page_bytes);
+    for (size_t b = 0; b < vecs; b += COPY_THREADS * COPY_VEC) {
+      uint4 t[COPY_VEC];
+#pragma unroll
+      for (int e = 0; e < COPY_VEC; ++e) {
+        const size_t i = b + e * COPY_THREADS + threadIdx.x;
+        if (i < vecs) t[e] = s[i];
+      }
+#pragma unroll
+      for (int e = 0; e < COPY_VEC; ++e) {
+        const size_t i = b + e * COPY_THREADS + threadIdx.x;
+        if (i < vecs) d[i] = t[e];
+      }
+    }
+    for (int i = threadIdx.x; i < page_scales; i += COPY_THREADS)
+      scales[(lead + pr.y) * page_scales + i] = scales[(lead + pr.x) * page_scales + i];
+  }
+}
+
+}  // namespace mk

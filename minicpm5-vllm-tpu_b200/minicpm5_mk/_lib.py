@@ -18,12 +18,14 @@ EXPORTED = (
     "mk_get_error", "mk_destroy", "mk_gemm_w8a16", "mk_attention_prefill", "mk_rope", "mk_rms_rstd", "mk_embed",
     "mk_lm_head_parts", "mk_lm_head_argmax", "mk_launches_per_forward", "mk_lm_head_argmax_noalloc",
     "mk_topk_logprobs", "mk_forward_timed", "mk_sp_block", "mk_workspace_size_sp", "mk_forward_sp",
-    "mk_gemm_w8a16_fused", "mk_set_sp_key_split",
+    "mk_gemm_w8a16_fused", "mk_set_sp_key_split", "mk_kv_append", "mk_kv_read", "mk_attention_paged_workspace",
+    "mk_attention_paged", "mk_kv_move_workspace", "mk_kv_fork", "mk_kv_reserve", "mk_kv_compact", "mk_token_logprobs",
+    "mk_score_tokens_workspace", "mk_score_tokens",
 )
 
 MK_GEMM_ROWSCALE, MK_GEMM_RESID, MK_GEMM_SWIGLU, MK_GEMM_COLSCALE, MK_GEMM_RESID32 = 0, 1, 2, 3, 4
 
-_i32, _f32, _vp, _sz = ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_i32, _i64, _f32, _vp, _sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
 
 class MkConfigC(ctypes.Structure):
@@ -103,11 +105,27 @@ def lib() -> ctypes.CDLL:
         L.mk_lm_head_argmax.argtypes = [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]
         L.mk_lm_head_argmax_noalloc.argtypes = [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp]
         L.mk_topk_logprobs.argtypes = [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]
+        L.mk_kv_append.argtypes = [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32,
+                                   _i32, _vp, _vp, _i32, _vp]
+        L.mk_kv_read.argtypes = [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp]
+        L.mk_attention_paged_workspace.argtypes = [_i32] * 7 + [ctypes.POINTER(_sz)]
+        L.mk_attention_paged.argtypes = [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _i32,
+                                         _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _sz, _vp]
+        L.mk_kv_move_workspace.argtypes = [_i32, _i32]
+        L.mk_kv_move_workspace.restype = _sz
+        L.mk_kv_fork.argtypes = [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp,
+                                 _vp, _sz, _vp]
+        L.mk_kv_reserve.argtypes = [_vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _vp]
+        L.mk_kv_compact.argtypes = [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _sz,
+                                    _vp]
+        L.mk_token_logprobs.argtypes = [_vp, _i32, _i32, _i32, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp]
+        L.mk_score_tokens_workspace.argtypes = [_i32, _i32, _i32, ctypes.POINTER(_sz)]
+        L.mk_score_tokens.argtypes = [_vp, _i32, _i32, _i64, _vp, _i32, _vp, _f32, _vp, _vp, _vp, _sz, _vp]
         L.mk_launches_per_forward.restype = _i32
         L.mk_launches_per_forward.argtypes = [_vp, _i32, _i32]
         for name in EXPORTED:
             if name not in ("mk_status_string", "mk_version", "mk_destroy", "mk_lm_head_parts",
-                            "mk_launches_per_forward"):
+                            "mk_launches_per_forward", "mk_kv_move_workspace"):
                 getattr(L, name).restype = _i32
         _LIB = L
     return _LIB

@@ -1,0 +1,92 @@
+"""Refusals of the cache and scoring entry points at the C ABI, before any device work (no GPU), and the
+definitions that their GPU tests compare with, checked against one another."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import cache_ref as ref
+from minicpm5_mk import _lib
+
+
+def test_bad_arguments_are_status_codes():
+    L = _lib.lib()
+    n = ctypes.c_size_t()
+    kv = lambda **c: L.mk_kv_append(  # noqa: E731
+        *[{**dict(k=16, v=16, ld_k=96, hk=96, ld_v=96, hv=96, T=1, codes=16, scales=16, pages=4, n_kv=1, page=16, hd=96,
+                  table=16, rows=1, width=1, lens=16, cu=None, max_new=1, stream=None), **c}[a]
+          for a in "k v ld_k hk ld_v hv T codes scales pages n_kv page hd table rows width lens cu max_new stream".split()])
+    assert kv(page=24) == 1 and kv(hd=64) == 1 and kv(pages=0) == 1 and kv(T=2) == 1 and kv(width=0) == 1
+    assert kv(codes=8) == 2 and kv(k=8) == 2 and kv(ld_k=97) == 2 and kv(hv=4) == 2
+    assert kv(codes=None) == 5 and kv(lens=None) == 5 and kv(k=None) == 5
+    assert kv(T=0, rows=0) == 0
+    assert L.mk_attention_paged_workspace(1, 3, 2, 96, 1, 1, 10, ctypes.byref(n)) == 1
+    assert L.mk_attention_paged_workspace(1, 4, 2, 80, 1, 1, 10, ctypes.byref(n)) == 1
+    assert L.mk_attention_paged_workspace(1, 4, 2, 96, 1, 1, 10, None) == 5
+    assert L.mk_kv_reserve(16, 16, 9000, 4, None, 16, 10, 16, None) == 9
+    assert L.mk_kv_reserve(16, 16, 4, 4, None, 16, 10, 20, None) == 1
+    assert L.mk_kv_fork(16, 16, 1, 4, 1, 16, 96, 16, 16, 1, 1, 16, 1, 32, 64, 48, 16, 0, None) == 8
+    assert L.mk_kv_fork(16, 16, 1, 4, 1, 16, 96, 16, 16, 1, 1, 16, 1, 16, 64, 48, 16, 1 << 20, None) == 5  # in place
+    assert L.mk_kv_compact(16, 16, 1, 4, 1, 16, 96, 16, 1, 1, 48, 32, 48, 64, 16, 1 << 20, None) == 5
+    assert L.mk_token_logprobs(16, 8, 1, 10, 10, 16, 0, 16, 16, 16, None, None, None) == 5
+    assert L.mk_token_logprobs(16, 32, 1, 10, 10, 16, 11, 16, 16, 16, 16, 16, None) == 1
+    assert L.mk_token_logprobs(18, 32, 1, 10, 10, 16, 0, 16, 16, 16, None, None, None) == 2
+    assert L.mk_score_tokens_workspace(1, 12, 10, ctypes.byref(n)) == 1
+    assert L.mk_score_tokens(16, 1, 16, 16, 16, 10, 16, 1.0, 16, 16, 16, 0, None) == 8
+    assert L.mk_status_string(10) == b"cache page missing or none free"
+
+
+def test_append_definition_is_near_its_input():
+    """Half a step of the scale for tokens rounded once."""
+    n_kv, page, hd = 2, 16, 96
+    codes, scales = ref.pool(3, n_kv, page, hd, 1)
+    x = torch.randn((20, n_kv, hd), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    table = ref.tables([20], page, 3, 1)
+    ref.append(x, x, codes, scales, table, [0], [0, 20])
+    for y in ref.planes(codes, scales, table[0].long()):
+        step = scales[table[0].long()].amax()
+        assert float((y[:20] - x.double()).abs().max()) <= float(step) * 0.5 * (1 + 1e-6)
+
+
+def test_fork_then_compact_keeps_every_row():
+    page, hd, layers, pages = 16, 96, 2, 60
+    lens = [40, 16, 0, 33]
+    codes, scales = ref.pool(pages, 1, page, hd, 3, layers)
+    table = ref.tables(lens, page, pages, 3)
+    read = lambda t, n, layer: [ref.planes(codes[layer], scales[layer], r[:-(-int(m) // page)].long())[1][:int(m)]  # noqa: E731
+                                for r, m in zip(t, n)]
+    before = [read(table, lens, i) for i in range(layers)]
+    par = [0, 3, 0, -1, 0, 3]
+    t, n, refs = ref.fork(codes, scales, table, lens, par, pages)
+    t, refs, used = ref.compact(codes, scales, t, refs)
+    assert int(t.max()) < used == int((refs > 0).sum())
+    for i in range(layers):
+        for got, p in zip(read(t, n, i), par):
+            assert torch.equal(got, before[i][p]) if p >= 0 else got.numel() == 0
+
+
+def test_scores_definition():
+    x = torch.randn((4, 50), generator=torch.Generator().manual_seed(2), dtype=torch.float64)
+    x[1, 7] = -math.inf
+    t = torch.tensor([3, 7, 49, 0])
+    lp, ent, rank, ids, tlp = ref.scores(x, t, 5)
+    want = torch.log_softmax(x, -1)
+    assert np.allclose(lp, want.gather(1, t[:, None])[:, 0]) and np.allclose(tlp, want.topk(5)[0])
+    assert np.allclose(ent, -(want.exp() * torch.where(want == -math.inf, 0, want)).sum(-1))
+    assert rank.tolist() == [1 + int((x[i] > x[i, t[i]]).sum()) for i in range(4)]
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_attend_definition_matches_dense_softmax(page):
+    lens, cu = [30, 5], [0, 3, 5]
+    codes, scales = ref.pool(6, 2, page, 96, 1)
+    table = ref.tables(lens, page, 6, 1)
+    q = torch.randn((5, 4, 96), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    out, lse, _, _ = ref.attend(q, codes, scales, table, lens, cu, 0.1)
+    k, v = ref.planes(codes, scales, table[0, :-(-30 // page)].long())
+    x = torch.einsum("thd,jhd->thj", q[:3].double(), k[:30].repeat_interleave(2, 1)) * 0.1
+    x = x.masked_fill(torch.arange(30) > torch.tensor([27, 28, 29])[:, None, None], -math.inf)
+    assert torch.allclose(out[:3], torch.einsum("thj,jhd->thd", x.softmax(-1), v[:30].repeat_interleave(2, 1)))
+    assert torch.allclose(lse[:3], x.logsumexp(-1))

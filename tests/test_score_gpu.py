@@ -1,0 +1,197 @@
+"""Scores of given tokens on a B200, from logits and from hidden rows, against 64 bits (tests/cache_ref.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import cache_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda", 0)
+
+
+def _check(got, want, x, k):
+    """ids and ranks are equal; logprobs and entropy differ by f32 roundings: 2^-24 of the logit's and the
+    maximum's size and a few 2^-22 for the exponentials and their sum (entropy: weighted by |u| up to the
+    spread that still has weight, at most ln V + its own size)."""
+    lp, ent, rank, ids, tlp = [g.cpu().numpy() for g in got]
+    fin = torch.where(x.isfinite(), x, 0).double().abs().amax(-1).numpy()
+    tol = 2.0 ** -22 * (4 + 2 * fin + math.log(x.shape[1]))
+    for g, w, t in ((lp, want[0], tol), (ent, want[1], 4 * tol), (tlp, want[4], tol[:, None])):
+        assert np.array_equal(np.isnan(g), np.isnan(w)) and np.array_equal(np.isneginf(g), np.isneginf(w))
+        f = np.isfinite(w)
+        d = np.abs(np.where(f, g, 0).astype(np.float64) - np.where(f, w, 0))
+        assert (d <= t).all(), (d / t).max()
+    assert np.array_equal(rank, want[2])
+    assert np.array_equal(ids, want[3]) and ids.shape == (x.shape[0], k)
+
+
+CASES = [(1, 1, 1), (3, 1, 0), (2, 7, 7), (5, 33, 3), (4, 1000, 64), (2, 1025, 20), (7, 4097, 5), (3, 32001, 20),
+         (2, 73448, 64), (1, 130560, 20), (300, 257, 2)]
+
+
+@pytest.mark.parametrize("T,V,k", CASES)
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_token_logprobs(dev, T, V, k, dtype):
+    from minicpm5_mk import ops
+    g = torch.Generator().manual_seed(T + V)
+    x = (3 * torch.randn((T, V), generator=g)).to(dtype)  # in bf16, ties abound
+    t = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    _check(ops.token_logprobs(x.to(dev), t.to(dev), k), ref.scores(x, t, k), x.double(), k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("V", [40, 3001, 70000])
+def test_token_logprobs_orders(dev, V, dtype):
+    """Rows that rise, fall, stand still, hold one peak, two values, or a few logits among masked ones."""
+    from minicpm5_mk import ops
+    r = torch.linspace(-20, 20, V)
+    x = torch.stack([r, r.flip(0), torch.zeros(V), torch.where(torch.arange(V) == V - 2, 90.0, -5.0),
+                     (torch.arange(V) % 2).float(), torch.where(torch.arange(V) % 9 == 4, r, torch.full((V,), -math.inf)),
+                     -r.abs(), 1e4 * r]).to(dtype)
+    t = torch.tensor([0, V - 1, 5, V - 2, 1, 4, V // 2, V - 1], dtype=torch.int32)
+    k = 30
+    _check(ops.token_logprobs(x.to(dev), t.to(dev), k), ref.scores(x, t, k), x.double(), k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("V", [9, 5000])
+def test_token_logprobs_masked_and_not_finite(dev, V, dtype):
+    """Rows of -inf alone, one finite logit, the type's lowest value, a NaN, a +inf, a masked target, and targets
+    outside the vocabulary."""
+    from minicpm5_mk import ops
+    low = torch.finfo(dtype).min
+    x = torch.randn((11, V), generator=torch.Generator().manual_seed(1))
+    x[0] = -math.inf
+    x[1] = -math.inf
+    x[1, V - 1] = 3.0
+    x[2, 1:] = low
+    x[3] = low
+    x[4, 5] = math.nan
+    x[5, 7] = math.inf
+    x[6, 2] = -math.inf
+    x[9] = math.nan
+    x[10, 3:] = math.nan
+    x = x.to(dtype)
+    t = torch.tensor([0, V - 1, 0, 2, 5, 7, 2, -1, V, 4, 1], dtype=torch.int32)
+    k = 9
+    got = [g.cpu() for g in ops.token_logprobs(x.to(dev), t.to(dev), k)]
+    want = ref.scores(x, t, k)
+    assert got[0][7] == 0 and got[0][8] == 0 and got[2][7] == 0 and got[2][8] == 0  # not scored
+    assert got[0][0] == -math.inf and got[1][0] == 0
+    fine = [0, 1, 2, 3, 6, 7, 8]
+    _check([g[fine] for g in got], [w[fine] for w in want], x[fine].double(), k)
+    odd = [4, 5, 9, 10]
+    assert bool(torch.stack([g[odd] for g in got[:2]]).isnan().all()) and bool(got[4][odd].isnan().all())
+    assert np.array_equal(got[3].numpy()[odd], want[3][odd]) and np.array_equal(got[2].numpy()[odd], want[2][odd])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("first,width", [(0, 2051), (1, 2050), (3, 2049), (5, 3000)])
+def test_token_logprobs_strides(dev, dtype, first, width):
+    """Views that begin off a 16-byte boundary, with row strides of every alignment; one row repeated."""
+    from minicpm5_mk import ops
+    V = 2001
+    base = torch.randn((6, width + 8), generator=torch.Generator().manual_seed(2)).to(dtype)
+    t = torch.arange(6, dtype=torch.int32)
+    x = base.to(dev)[:, first:first + V]
+    _check(ops.token_logprobs(x, t.to(dev), 4), ref.scores(base[:, first:first + V], t, 4), base[:, first:first + V].double(), 4)
+    one = base.to(dev)[2:3, first:first + V].expand(6, V)
+    _check(ops.token_logprobs(one, t.to(dev), 4), ref.scores(one.cpu(), t, 4), one.cpu().double(), 4)
+
+
+def test_token_logprobs_offsets_past_32_bits(dev):
+    from minicpm5_mk import ops
+    V, T = 1 << 20, 2100
+    x = torch.zeros((T, V), dtype=BF, device=dev)
+    x[-1] = torch.randn(V, generator=torch.Generator().manual_seed(2)).to(BF).to(dev)
+    t = torch.full((T,), 77, dtype=torch.int32, device=dev)
+    got = [g[-1:] for g in ops.token_logprobs(x, t, 3)]
+    _check(got, ref.scores(x[-1:].cpu(), t[-1:].cpu(), 3), x[-1:].cpu().double(), 3)
+
+
+# ---------------------------------------------------------------------------------------- from hidden rows
+@pytest.mark.parametrize("T,H,V", [(1, 8, 1), (1, 1536, 1000), (3, 384, 129), (7, 72, 257), (128, 512, 2048), (129, 64, 300),
+                                   (40, 1536, 73448), (700, 520, 4001), (5, 2048, 40000), (260, 40, 5)])
+@pytest.mark.parametrize("scale", [1.0, 256.0 / 1536])
+def test_score_tokens(dev, T, H, V, scale):
+    from minicpm5_mk import ops
+    g = torch.Generator(device=dev).manual_seed(T + H + V)
+    wide = torch.randn((T, H + 16), generator=g, device=dev).to(BF)
+    h = wide[:, 8:8 + H]
+    w = (4 / math.sqrt(H) * torch.randn((V, H), generator=g, device=dev)).to(BF)
+    t = torch.randint(0, V, (T,), generator=g, device=dev, dtype=torch.int32)
+    if T > 2:
+        t[1], t[2] = -1, V
+    lp, ent = ops.score_tokens(h, w, t, logit_scale=scale)
+    x = scale * (h.double() @ w.double().T)
+    want = torch.log_softmax(x, -1)
+    ok = (t >= 0) & (t < V)
+    mine = torch.where(ok, want.gather(1, t.clamp(0, V - 1).long()[:, None])[:, 0], 0)
+    we = -(want.exp() * want).sum(-1)
+    # H products summed in f32: at most H 2^-24 of the sum of magnitudes, for the token's logit and for the
+    # others (lse moves by no more); entropy moves by at most that times twice the spread of logits with weight
+    mag = scale * (h.double().abs() @ w.double().abs().T).amax(-1) * (H + 16) * 2.0 ** -24
+    tol = 2 * mag + 2.0 ** -20 * (4 + x.abs().amax(-1))
+    assert bool(((lp.double() - mine).abs() <= tol).all()), float(((lp.double() - mine).abs() / tol).max())
+    assert bool(((ent.double() - we).abs() <= 4 * tol * (1 + math.log(V))).all())
+    assert bool((lp[~ok] == 0).all())
+
+
+def test_score_tokens_not_finite(dev):
+    """A hidden row with a NaN scores NaN, its neighbours do not; a row of infinities too."""
+    from minicpm5_mk import ops
+    g = torch.Generator(device=dev).manual_seed(1)
+    h = torch.randn((150, 384), generator=g, device=dev).to(BF)
+    w = (0.1 * torch.randn((1000, 384), generator=g, device=dev)).to(BF)
+    t = torch.arange(150, dtype=torch.int32, device=dev)
+    clean = ops.score_tokens(h, w, t)
+    h[3, 5] = math.nan
+    h[140, 7] = math.inf
+    lp, ent = ops.score_tokens(h, w, t)
+    bad = torch.zeros(150, dtype=torch.bool, device=dev)
+    bad[[3, 140]] = True
+    assert lp.isnan().equal(bad) and ent.isnan().equal(bad)
+    assert lp[~bad].equal(clean[0][~bad]) and ent[~bad].equal(clean[1][~bad])
+
+
+def test_score_tokens_agrees_with_token_logprobs(dev):
+    from minicpm5_mk import ops
+    g = torch.Generator(device=dev).manual_seed(1)
+    h = torch.randn((64, 384), generator=g, device=dev).to(BF)
+    w = (0.2 * torch.randn((1000, 384), generator=g, device=dev)).to(BF)
+    t = torch.randint(0, 1000, (64,), generator=g, device=dev, dtype=torch.int32)
+    logits = (h.double() @ w.double().T).float()
+    a, b = ops.score_tokens(h, w, t), ops.token_logprobs(logits, t)
+    for x, y in zip(a, b[:2]):
+        assert bool(((x - y).abs() <= 1e-4).all())
+
+
+def test_refusals(dev):
+    from minicpm5_mk import _lib, ops
+    x, t = torch.zeros((3, 50), device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+    for bad in ((x.half(), t), (x.T, t), (x, t.long()), (x, t[:2]), (x.cpu(), t), (x[0], t), (x, t.cpu())):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(*bad)
+    for k in (-1, 51, 65):
+        with pytest.raises((_lib.MkError, RuntimeError)):
+            ops.token_logprobs(x, t, k)
+    h, w = torch.zeros((3, 64), dtype=BF, device=dev), torch.zeros((50, 64), dtype=BF, device=dev)
+    for bad in ((h.float(), w, t), (h, w.float(), t), (h, w[:, :32], t), (h, w, t[:1]), (h.T, w, t), (h, w.cpu(), t)):
+        with pytest.raises(ValueError):
+            ops.score_tokens(*bad)
+    with pytest.raises(_lib.MkError):  # H not a multiple of 8
+        ops.score_tokens(torch.zeros((3, 60), dtype=BF, device=dev), torch.zeros((50, 60), dtype=BF, device=dev), t)
+    with pytest.raises(_lib.MkError):  # rows off the 16-byte grid
+        ops.score_tokens(torch.zeros((3, 68), dtype=BF, device=dev)[:, :64], w, t)
+    lp, ent, rank, ids, tlp = ops.token_logprobs(x[:0], t[:0], 5)
+    assert lp.shape == (0,) and ids.shape == (0, 5)
+    lp, ent = ops.score_tokens(h[:0], w, t[:0])
+    assert lp.shape == (0,)
