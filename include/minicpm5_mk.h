@@ -341,7 +341,8 @@ mk_status mk_kv_read(const void* codes, const float* scales, int32_t num_pages, 
  *   lens    tokens of each row in the cache, the queries' own included
  *   cu_q    int32 [rows + 1]: row r's queries; query i of n sits at position lens[r] - n + i and sees the keys up
  *           to it.  NULL: one query per row (T == rows)
- *   max_q, max_len  bounds of a row's queries and of lens; rows past them are cut to them
+ *   max_q, max_len  what a row's queries and lens are expected to reach: they choose the launch shape and the
+ *           workspace; longer rows are computed all the same
  *   out     bf16 [T, n_q, head_dim];  lse f32 [T, n_q] (optional): ln sum exp of the scaled scores
  * A query that sees no key (an idle row, lens 0) gives zeros and lse = -inf.
  * workspace: mk_attention_paged_workspace bytes, 16-byte aligned, free for other use once the call's work is

@@ -4,7 +4,18 @@
 //   o   = sum_j exp(s_j - m) * vscale * vcode_j / sum_j exp(s_j - m),   lse = m + ln sum_j exp(s_j - m)
 //
 // A row that sees no key (an idle row of the batch) gives zeros and lse = -inf.
+//
+// What bounds it: one new token reads every key and value byte of its row once and does 2 n_q / n_kv products
+// with each (16 for 8 query heads per key/value head), far below the tensor cores' rate, so the cache's bytes
+// are the floor and the conversion of codes to f16 is the next limit.  The kernel therefore works on the
+// transposed products, S^T = K Q^T and O^T = V^T P^T, with keys (then channels) as the matrix rows and the
+// query heads that share a key/value head as its 8 columns: mma.sync m16n8k16 fits that without padding, and a
+// 128-row tcgen05 tile would be 15/16 empty.  The order of the contraction index is free, so each lane's
+// fragment is made of bytes that are contiguous in memory: keys and values go from global memory to
+// registers in 16-byte loads and become operands without touching shared memory.
 #pragma once
+
+#include <cuda_fp16.h>
 
 #include "mk_cache.cuh"
 
@@ -13,80 +24,539 @@ namespace mk {
 struct PagedAttnArgs {
   const __nv_bfloat16* q;
   long long ld_q, hs_q;
-  int n_q, rows, width;
+  int n_q, group, rows, width;  // group = n_q / n_kv
   const int32_t* table;
   const int32_t* lens;
   const int32_t* cu;
-  float scale;
+  float scale;  // softmax scale * log2 e
   __nv_bfloat16* out;
   float* lse;
+  float* part_o;   // [2 * CTAs][rows of a tile][hd]
+  float2* part_ml; // [2 * CTAs][rows of a tile]
+  int4* desc;      // [CTAs]
   int* err;
 };
 
-// One CTA per (token, query head): 128 keys at a time, one score per thread, then one channel per thread.
-constexpr int PA_THREADS = 128;
-__global__ void __launch_bounds__(PA_THREADS) attn_paged_kernel(KvPages c, PagedAttnArgs a) {
-  __shared__ float qs[128], ps[PA_THREADS], red[PA_THREADS / 32];
+constexpr int PA_WARPS = 4;
+constexpr int PA_THREADS = PA_WARPS * 32;
+constexpr int PA_UNIT = 16 * PA_WARPS;  // keys of one unit of work: 16 per warp
+constexpr int PA_GROUPS = 64;           // 16-key groups whose pages and scales are staged at a time
+// m may lag the true maximum by up to 2^kLag: it moves only then, which spares a warp reduction and a rescaling
+// of O per 16 keys.
+//
+// The probabilities p = exp(s - m) * vscale are rounded for their product with the codes.  With up to 16 query
+// rows per tile the tensor pipe idles behind the loads, and p goes in as two bf16 parts (p rounded, and what
+// that left over): 17 bits, and the range of f32, so that keys far below the maximum still count where the
+// others have a zero.  With 32 rows the products and conversions are the limit, and p is one f16 (11 bits), held
+// times kPOff: the largest operand is 2^15, and a key that weighs less than 2^-31 of the maximum is lost.
+constexpr float kPOff = 128.f;
+constexpr float kLag = 8.f;
+
+// Loads of bytes that are read once (not kept in L1).
+__device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream(const uint2* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Four codes (one word) to two f16 pairs, exact: byte ^ 0x80 under 0x64 is 1024 + 128 + code.
+__device__ __forceinline__ void i8x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+  const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias), y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Work.  A pair is (row, tile of 8 NT query rows, key/value head), a query row being (token, head of the
+// group); a pair's keys are cut into units of PA_UNIT.  All units of all pairs, in order, are dealt out in equal
+// contiguous shares, one per CTA, from the lengths on the device: ragged batches, one long row and many short
+// ones all fill the GPU alike.  A pair that lies inside one share is finished there; a share holds at most one
+// piece of a pair that began earlier (slot 0) and one of a pair that continues later (slot 1, named in desc),
+// which attn_paged_join_kernel puts together in order.
+//
+// A warp takes every PA_WARPS-th 16-key group of its CTA's share.  Fragments of lane (r = lane / 4, c = lane % 4):
+//   K Q^T   A rows r, r + 8 are keys 4 (r / 2) + r % 2 and that + 2; a 4-byte word of a key gives k-slots
+//           2c, 2c + 1, 2c + 8, 2c + 9 of one step.  Lane c holds bytes 16c .. of a key (and 64 + 16c .., hd 128,
+//           or 64 + 8c .., hd 96), and the queries' B fragments the same channels.
+//   V^T P^T after a transpose of P (movmatrix) lane c's k-slots are keys 4c .. 4c + 3, one word of the value
+//           plane; a 16-byte load holds them for channels 32j + 4r .. + 3, two of each 16-row tile.
+template <int HD, int NT>
+__global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
+  constexpr int KS = HD / 16, MT = HD / 16, ROWS = 8 * NT, LDO = HD + 4;
+  constexpr bool SPLIT = NT <= 2;  // p as two bf16 parts
+  __shared__ long long s_scan[PA_WARPS], s_base;
+  __shared__ int s_row;
+  __shared__ int s_page[PA_GROUPS];
+  __shared__ float s_ks[PA_GROUPS], s_vs[PA_GROUPS], s_red[PA_WARPS];
+  __shared__ uint2 s_q[NT > 1 ? NT * KS * 32 : 1];
+  __shared__ float s_m[PA_WARPS][ROWS], s_l[PA_WARPS][ROWS];
+  __shared__ __align__(16) float s_o[PA_WARPS][8][LDO];
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+  const int G = a.group, n_kv = cp.n_kv, page_mask = (1 << cp.page_shift) - 1;
+
+  auto row_tokens = [&](int row, int& first) {
+    first = a.cu ? a.cu[row] : row;
+    return a.cu ? a.cu[row + 1] - first : 1;
+  };
+  auto row_tiles = [&](int n) { return (n * G + ROWS - 1) / ROWS; };
+  auto pair_units = [&](int row) { return (max(a.lens[row], 0) + PA_UNIT - 1) / PA_UNIT; };
+  // an idle row still has its zeros to write: one unit
+  auto row_units = [&](int row) {
+    int first;
+    const int n = row_tokens(row, first);
+    return n <= 0 ? 0ll : static_cast<long long>(max(pair_units(row), 1)) * row_tiles(n) * n_kv;
+  };
+
+  // this CTA's share [u0, u1) of the N units, and the row where it begins
+  const int per = (a.rows + PA_THREADS - 1) / PA_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) mine += row_units(i);
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 31) s_scan[warp] = inc;
+  __syncthreads();
+  long long N = 0;
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) {
+    if (w < warp) inc += s_scan[w];
+    N += s_scan[w];
+  }
+  const long long C = min(static_cast<long long>(gridDim.x), N), cta = blockIdx.x;
+  if (tid == 0) a.desc[cta] = make_int4(-1, 0, 0, 0);
+  if (cta >= C) return;
+  const long long u0 = cta * N / C, u1 = (cta + 1) * N / C;
+  if (inc - mine <= u0 && u0 < inc) {
+    long long base = inc - mine;
+    int i = i0;
+    for (long long n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
+    s_row = i;
+    s_base = base;
+  }
+  __syncthreads();
+  int row = s_row;
+  long long base = s_base;
+
+  for (long long u = u0; u < u1;) {
+    const long long ru = row_units(row);
+    if (u >= base + ru) {
+      base += ru;
+      ++row;
+      continue;
+    }
+    int first;
+    const int n = row_tokens(row, first), len = max(a.lens[row], 0), tiles = row_tiles(n);
+    const int upp = max(pair_units(row), 1), local_pair = static_cast<int>((u - base) / upp);
+    const int ua = static_cast<int>((u - base) % upp), ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
+    const int g = local_pair / tiles, rt = local_pair % tiles;
+    const int r0 = rt * ROWS, R = n * G;
+    // a query row's token sees the keys below its limit
+    auto limit = [&](int qr) { return qr < R ? len - n + qr / G + 1 : 0; };
+    const int lim_min = r0 + ROWS <= R ? limit(r0) : 0, lim_max = limit(min(r0 + ROWS, R) - 1);
+    const int kbeg = ua * PA_UNIT, kend = min(ub * PA_UNIT, lim_max);
+
+    // queries as f16, each row scaled by a power of two to about 1 (its exponent joins the score's factor)
+    uint32_t qf[NT == 1 ? KS : 1][2];
+    float rf[NT][2];   // score factor of this lane's two columns of each 8-row tile
+    int lim[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int qr = r0 + t * 8 + r;
+      uint32_t w[KS][2];
+      float top = 0.f;
+      const __nv_bfloat16* qp = a.q;
+      if (qr < R) qp += static_cast<long long>(first + qr / G) * a.ld_q + static_cast<long long>(g * G + qr % G) * a.hs_q;
+#pragma unroll
+      for (int s = 0; s < KS; s += 2) {  // 8 channels: two words' worth
+        const int ch = s < 4 ? 16 * c + 4 * s : HD == 128 ? 64 + 16 * c + 4 * (s - 4) : 64 + 8 * c;
+        const uint4 v = qr < R ? __ldg(reinterpret_cast<const uint4*>(qp + ch)) : make_uint4(0, 0, 0, 0);
+        w[s][0] = v.x;
+        w[s][1] = v.y;
+        w[s + 1][0] = v.z;
+        w[s + 1][1] = v.w;
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = unpack_bf16x2(w[s][e]);
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        uint32_t h[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = unpack_bf16x2(w[s][e]);
+          h[e] = pack_f16x2(f.x * down, f.y * down);
+        }
+        if constexpr (NT == 1) {
+          qf[s][0] = h[0];
+          qf[s][1] = h[1];
+        } else if (warp == t % PA_WARPS) {
+          s_q[(t * KS + s) * 32 + lane] = make_uint2(h[0], h[1]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rf[t][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4) * a.scale;
+        lim[t][e] = limit(r0 + t * 8 + 2 * c + e);
+      }
+    }
+
+    float m[NT][2], l[NT][2], o[MT][NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
+    }
+    float vref = 0.f;  // the largest value scale so far: O is in units of vref / kPOff
+
+    for (int kb = kbeg; kb < kend; kb += PA_GROUPS * 16) {
+      const int ng = min(PA_GROUPS, (kend - kb + 15) >> 4);
+      __syncthreads();  // the last groups' pages and scales (and s_q, s_o) are no longer read
+      float vs = 0.f;
+      if (tid < ng) {
+        const int page = kv_page_of(a.table, a.width, cp.num_pages, row, (kb + tid * 16) >> cp.page_shift, a.err);
+        s_page[tid] = page;
+        vs = page < 0 ? 0.f : *kv_scale_ptr(cp, page, 1, g);
+        s_ks[tid] = page < 0 ? 0.f : *kv_scale_ptr(cp, page, 0, g);
+      }
+      float top = vs;  // (a NaN scale does not take part, and makes its own group NaN)
+#pragma unroll
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      if (lane == 0) s_red[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_red[w]);
+      const float nref = fmaxf(vref, top);
+      if (tid < ng) s_vs[tid] = nref > 0.f ? vs / nref * kPOff : vs;
+      if (nref != vref && vref > 0.f) {
+        const float f = vref / nref;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][t][e] *= f;
+      }
+      vref = nref;
+      __syncthreads();
+
+      uint32_t kw[2][KS];  // two keys' words
+      uint4 vw[HD / 32];
+      auto load_k = [&](int gi) {
+        const int page = max(s_page[gi], 0), in = (kb + gi * 16) & page_mask;
+        const int8_t* p = kv_head_ptr(cp, page, 0, g) + static_cast<size_t>(in + 4 * (r >> 1) + (r & 1)) * HD;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 x = ldg_stream(reinterpret_cast<const uint4*>(p + i * 2 * HD + c * 16));
+          kw[i][0] = x.x;
+          kw[i][1] = x.y;
+          kw[i][2] = x.z;
+          kw[i][3] = x.w;
+          if constexpr (HD == 128) {
+            const uint4 y = ldg_stream(reinterpret_cast<const uint4*>(p + i * 2 * HD + 64 + c * 16));
+            kw[i][4] = y.x;
+            kw[i][5] = y.y;
+            kw[i][6] = y.z;
+            kw[i][7] = y.w;
+          } else {
+            const uint2 y = ldg_stream(reinterpret_cast<const uint2*>(p + i * 2 * HD + 64 + c * 8));
+            kw[i][4] = y.x;
+            kw[i][5] = y.y;
+          }
+        }
+      };
+      auto load_v = [&](int gi) {
+        const int page = max(s_page[gi], 0), in = (kb + gi * 16) & page_mask;
+        const int8_t* p = kv_head_ptr(cp, page, 1, g) + static_cast<size_t>(in) * HD + (c * HD + 4 * r) * 4;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) vw[j] = ldg_stream(reinterpret_cast<const uint4*>(p + j * 128));
+      };
+      if (warp < ng) {
+        load_k(warp);
+        load_v(warp);
+      }
+#pragma unroll 1
+      for (int gi = warp; gi < ng; gi += PA_WARPS) {
+        const bool more = gi + PA_WARPS < ng;
+        float s[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KS; ++w) {
+          uint32_t a0, a1, a2, a3;
+          i8x4_to_f16x4(kw[0][w], a0, a2);
+          i8x4_to_f16x4(kw[1][w], a1, a3);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (NT == 1) {
+              mma_16816(s[t], a0, a1, a2, a3, qf[w][0], qf[w][1]);
+            } else {
+              const uint2 b = s_q[(t * KS + w) * 32 + lane];
+              mma_16816(s[t], a0, a1, a2, a3, b.x, b.y);
+            }
+          }
+        }
+        if (more) load_k(gi + PA_WARPS);
+        const float ks = s_ks[gi], vr = s_vs[gi];
+        const int key = kb + gi * 16 + 4 * (r >> 1) + (r & 1);  // and key + 2
+        const bool masked = kb + gi * 16 + 16 > lim_min || s_page[gi] < 0;
+        uint32_t pb[NT][2], pl[SPLIT ? NT : 1][2];
+        bool raise = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][e] *= rf[t][e & 1] * ks;
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key + (e & 2) >= lim[t][e & 1] || s_page[gi] < 0) s[t][e] = -INFINITY;
+          }
+          raise |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kLag || fmaxf(s[t][1], s[t][3]) > m[t][1] + kLag;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[t][e], s[t][e + 2]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), m[t][e]);
+              const float f = top == m[t][e] ? 1.f : ex2_approx(m[t][e] - top);
+              m[t][e] = top;
+              l[t][e] *= f;
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                o[i][t][e] *= f;
+                o[i][t][e + 2] *= f;
+              }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
+          float p[4];
+          p[0] = ex2_approx(s[t][0] - m0);
+          p[1] = ex2_approx(s[t][1] - m1);
+          p[2] = ex2_approx(s[t][2] - m0);
+          p[3] = ex2_approx(s[t][3] - m1);
+          l[t][0] += p[0] + p[2];
+          l[t][1] += p[1] + p[3];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = masked && s[t][e] == -INFINITY ? 0.f : p[e] * vr;  // 0 even where vr is NaN
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (SPLIT) {
+              const uint32_t hi = pack_bf16x2(p[2 * e], p[2 * e + 1]);
+              const float2 f = unpack_bf16x2(hi);
+              pb[t][e] = movmatrix_trans(hi);
+              pl[t][e] = movmatrix_trans(pack_bf16x2(p[2 * e] - f.x, p[2 * e + 1] - f.y));
+            } else {
+              pb[t][e] = movmatrix_trans(pack_f16x2(p[2 * e], p[2 * e + 1]));
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          const uint32_t w[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            if constexpr (SPLIT) {
+              i8x4_to_bf16x4(w[2 * h], a0, a2);
+              i8x4_to_bf16x4(w[2 * h + 1], a1, a3);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+                mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+              }
+            } else {
+              i8x4_to_f16x4(w[2 * h], a0, a2);
+              i8x4_to_f16x4(w[2 * h + 1], a1, a3);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_16816(o[2 * j + h][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+            }
+          }
+        }
+        if (more) load_v(gi + PA_WARPS);
+      }
+    }
+
+    // the warps' pieces, joined in order
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], d);
+        if (r == 0) {
+          s_m[warp][t * 8 + 2 * c + e] = m[t][e];
+          s_l[warp][t * 8 + 2 * c + e] = l[t][e];
+        }
+      }
+    const bool whole = ua == 0 && ub == upp;
+    const int slot = static_cast<int>(cta) * 2 + (ua == 0 ? 1 : 0);
+    const float unit = vref / kPOff;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int q8 = 2 * c + e;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][t * 8 + q8]);
+        const float f = m[t][e] == -INFINITY ? (m[t][e] == top ? 1.f : 0.f) : ex2_approx(m[t][e] - top);
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j)
+          *reinterpret_cast<float4*>(&s_o[warp][q8][32 * j + 4 * r]) =
+              make_float4(o[2 * j][t][e] * f, o[2 * j][t][e + 2] * f, o[2 * j + 1][t][e] * f, o[2 * j + 1][t][e + 2] * f);
+      }
+      __syncthreads();
+      const int q8 = tid >> 4, qr = r0 + t * 8 + q8;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][t * 8 + q8]);
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) {
+        const float mw = s_m[w][t * 8 + q8];
+        sum += s_l[w][t * 8 + q8] * (mw == -INFINITY ? (mw == top ? 1.f : 0.f) : ex2_approx(mw - top));
+      }
+      if (qr < R) {
+        const long long at = static_cast<long long>(first + qr / G) * a.n_q + g * G + qr % G;
+#pragma unroll
+        for (int d = (tid & 15) * 4; d < HD; d += 64) {
+          float4 x = *reinterpret_cast<const float4*>(&s_o[0][q8][d]);
+#pragma unroll
+          for (int w = 1; w < PA_WARPS; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(&s_o[w][q8][d]);
+            x.x += y.x;
+            x.y += y.y;
+            x.z += y.z;
+            x.w += y.w;
+          }
+          if (whole) {
+            const float f = sum == 0.f ? 0.f : unit / sum;
+            *reinterpret_cast<uint2*>(a.out + at * HD + d) =
+                make_uint2(pack_bf16x2(x.x * f, x.y * f), pack_bf16x2(x.z * f, x.w * f));
+          } else {
+            *reinterpret_cast<float4*>(a.part_o + (static_cast<size_t>(slot) * ROWS + t * 8 + q8) * HD + d) =
+                make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
+          }
+        }
+        if ((tid & 15) == 0) {
+          if (!whole)
+            a.part_ml[static_cast<size_t>(slot) * ROWS + t * 8 + q8] = make_float2(top, sum);
+          else if (a.lse)
+            a.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.693147180559945f;
+        }
+      }
+    }
+    if (!whole && ua == 0 && tid == 0) {
+      const long long last = base + static_cast<long long>(local_pair + 1) * upp - 1;  // the pair's last unit
+      a.desc[cta] = make_int4(row, rt, g, static_cast<int>(((last + 1) * C - 1) / N));
+    }
+    __syncthreads();  // s_o and s_q are free again
+    u += ub - ua;
+  }
+  pdl_trigger();
+}
+
+// Joins the pieces of one query row of a pair that several CTAs worked on, in their order.  CTA (c, i): row i of
+// the pair that began in CTA c and was not finished there.
+constexpr int PJ_PARTS = 4;  // groups of threads over the pieces
+template <int HD>
+__global__ void __launch_bounds__(PJ_PARTS * HD) attn_paged_join_kernel(PagedAttnArgs a) {
+  __shared__ float s_o[PJ_PARTS][HD], s_red[2][32];
   pdl_wait();
   pdl_trigger();
-  const int tok = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, hd = c.head_dim;
-  int row = tok, n = 1, first = tok;
-  if (a.cu) {
-    int lo = 0, hi = a.rows - 1;  // last row that begins at or before the token
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.cu[mid] <= tok) lo = mid; else hi = mid - 1;
-    }
-    row = lo;
-    first = a.cu[row];
-    n = a.cu[row + 1] - first;
-  }
-  const int keys = a.lens[row] - n + (tok - first) + 1;  // keys this query sees
-  const int kvh = h / (a.n_q / c.n_kv);
-  if (tid < hd) qs[tid] = __bfloat162float(a.q[static_cast<long long>(tok) * a.ld_q + h * a.hs_q + tid]);
+  const int4 d = a.desc[blockIdx.x];
+  if (d.x < 0) return;
+  const int ROWS = gridDim.y, i = blockIdx.y, G = a.group;
+  const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1, qr = d.y * ROWS + i;
+  if (qr >= n * G) return;
+  const int pieces = d.w - static_cast<int>(blockIdx.x) + 1;
+  auto slot = [&](int p) { return (static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + i; };
+  const int tid = threadIdx.x, grp = tid / HD, dim = tid % HD, warp = tid >> 5, lane = tid & 31;
+  float top = -INFINITY;
+  for (int p = tid; p < pieces; p += PJ_PARTS * HD) top = fmaxf(top, a.part_ml[slot(p)].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_red[0][warp] = top;
   __syncthreads();
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int base = 0; base < keys; base += PA_THREADS) {
-    const int j = base + tid;
-    float s = -INFINITY;
-    int page = -1;
-    if (j < keys) page = kv_page_of(a.table, a.width, c.num_pages, row, j >> c.page_shift, a.err);
-    if (page >= 0) {
-      const int8_t* kp = kv_head_ptr(c, page, 0, kvh) + static_cast<size_t>(j & ((1 << c.page_shift) - 1)) * hd;
-      float d = 0.f;
-      for (int e = 0; e < hd; ++e) d += qs[e] * static_cast<float>(kp[e]);
-      s = d * (*kv_scale_ptr(c, page, 0, kvh) * a.scale);
-    }
-    float mx = s;
-    for (int w = 16; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    mx = m;
-    for (int w = 0; w < PA_THREADS / 32; ++w) mx = fmaxf(mx, red[w]);
-    const float p = page >= 0 ? expf(s - mx) : 0.f;
-    float sum = p;
-    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = sum;
-    ps[tid] = page >= 0 ? p * *kv_scale_ptr(c, page, 1, kvh) : 0.f;
-    __syncthreads();
-    const float keep = mx == m ? 1.f : expf(m - mx);
-    l *= keep;
-    for (int w = 0; w < PA_THREADS / 32; ++w) l += red[w];
-    o *= keep;
-    m = mx;
-    if (tid < hd)
-      for (int i = 0; i < min(PA_THREADS, keys - base); ++i) {
-        const int pg = kv_page_of(a.table, a.width, c.num_pages, row, (base + i) >> c.page_shift, a.err);
-        if (pg < 0) continue;
-        const int in = (base + i) & ((1 << c.page_shift) - 1);
-        o += ps[i] * static_cast<float>(kv_head_ptr(c, pg, 1, kvh)[(static_cast<size_t>(in >> 2) * hd + tid) * 4 + (in & 3)]);
-      }
-    __syncthreads();
+#pragma unroll
+  for (int w = 0; w < PJ_PARTS * HD / 32; ++w) top = fmaxf(top, s_red[0][w]);
+  float sum = 0.f;
+  for (int p = tid; p < pieces; p += PJ_PARTS * HD) {
+    const float2 ml = a.part_ml[slot(p)];
+    sum += ml.y * (ml.x == -INFINITY ? (ml.x == top ? 1.f : 0.f) : ex2_approx(ml.x - top));
   }
-  if (tid < hd)
-    a.out[(static_cast<size_t>(tok) * a.n_q + h) * hd + tid] = __float2bfloat16(l == 0.f ? 0.f : o / l);
-  if (tid == 0 && a.lse) a.lse[static_cast<size_t>(tok) * a.n_q + h] = l == 0.f ? -INFINITY : m + logf(l);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_red[1][warp] = sum;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int p = grp; p < pieces; p += PJ_PARTS) {
+    const float mp = a.part_ml[slot(p)].x;
+    acc += a.part_o[slot(p) * HD + dim] * (mp == -INFINITY ? (mp == top ? 1.f : 0.f) : ex2_approx(mp - top));
+  }
+  s_o[grp][dim] = acc;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < PJ_PARTS * HD / 32; ++w) sum += s_red[1][w];
+  const long long at = static_cast<long long>(first + qr / G) * a.n_q + d.z * G + qr % G;
+  if (grp == 0) {
+#pragma unroll
+    for (int p = 1; p < PJ_PARTS; ++p) acc += s_o[p][dim];
+    a.out[at * HD + dim] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
+  }
+  if (tid == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.693147180559945f;
 }
 
 }  // namespace mk

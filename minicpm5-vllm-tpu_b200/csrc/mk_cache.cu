@@ -43,6 +43,30 @@ mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int 
                   static_cast<int8_t*>(codes), scales, num_pages, page_bytes(n_kv, page, hd), 2 * n_kv, pairs, n_pairs);
 }
 
+// Launch shape and workspace of the paged attention.  Query rows (tokens times heads of a group) per tile: 8, 16
+// or 32, the smallest that holds a row's queries; a wider tile reads and converts the cache less often but
+// leaves room for two CTAs per SM instead of four.  One wave of CTAs on 148 SMs, fewer when the bounds say that
+// there are fewer units of work.
+struct PagedPlan {
+  int nt, ctas;
+  size_t o_bytes, ml_bytes, bytes;
+};
+PagedPlan paged_plan(int group, int n_kv, int hd, int rows, int max_q, int max_len) {
+  PagedPlan p;
+  const int64_t q_rows = static_cast<int64_t>(std::max(max_q, 1)) * group;
+  p.nt = q_rows <= 8 ? 1 : q_rows <= 16 ? 2 : 4;
+  const int64_t tiles = (q_rows + 8 * p.nt - 1) / (8 * p.nt);
+  const int64_t per_pair = std::max(1, max_len / mk::PA_UNIT + (max_len % mk::PA_UNIT != 0));
+  const int64_t most = 148 * (p.nt == 1 ? 4 : 2);
+  // (each factor is below 2^31: cut before the product can overflow)
+  const int64_t pairs = std::min<int64_t>(most, static_cast<int64_t>(rows) * n_kv) * std::min<int64_t>(most, tiles);
+  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min(most, pairs) * per_pair)));
+  p.o_bytes = static_cast<size_t>(2) * p.ctas * 8 * p.nt * hd * sizeof(float);
+  p.ml_bytes = static_cast<size_t>(2) * p.ctas * 8 * p.nt * sizeof(float2);
+  p.bytes = p.o_bytes + p.ml_bytes + static_cast<size_t>(p.ctas) * sizeof(int4);
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -93,7 +117,7 @@ mk_status mk_attention_paged_workspace(int32_t T, int32_t n_q, int32_t n_kv, int
   if (T < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || (head_dim != 96 && head_dim != 128) || rows < 0 || max_q < 0 ||
       max_len < 0)
     return MK_ERR_BAD_SHAPE;
-  *bytes = 0;
+  *bytes = paged_plan(n_q / n_kv, n_kv, head_dim, rows, max_q, max_len).bytes;
   return MK_OK;
 }
 
@@ -108,28 +132,41 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
   MK_TRY(mk_attention_paged_workspace(T, n_q, n_kv, head_dim, rows, max_q, max_len, &need));
   if (width <= 0 || (!cu_q && T != rows)) return MK_ERR_BAD_SHAPE;
   if (T == 0 || rows == 0) return MK_OK;
-  if (!q || !out || !block_table || !lens || (need && !workspace)) return MK_ERR_BAD_ARG;
+  if (!q || !out || !block_table || !lens || !workspace) return MK_ERR_BAD_ARG;
   if (workspace_bytes < need) return MK_ERR_WORKSPACE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || ld_q % 8 || head_ld_q % 8) return MK_ERR_BAD_ALIGN;
-  if (n_q > 65535) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
+  const PagedPlan p = paged_plan(n_q / n_kv, n_kv, head_dim, rows, max_q, max_len);
   mk::PagedAttnArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.ld_q = ld_q;
   a.hs_q = head_ld_q;
   a.n_q = n_q;
+  a.group = n_q / n_kv;
   a.rows = rows;
   a.width = width;
   a.table = block_table;
   a.lens = lens;
   a.cu = cu_q;
-  a.scale = softmax_scale;
+  a.scale = softmax_scale * 1.4426950408889634f;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
+  char* ws = static_cast<char*>(workspace);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
+  a.desc = reinterpret_cast<int4*>(ws + p.o_bytes + p.ml_bytes);
   a.err = d.err;
-  return launch_k(mk::attn_paged_kernel, dim3(T, n_q), dim3(mk::PA_THREADS), 0, static_cast<cudaStream_t>(stream), true, c,
-                  a);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  void (*k)(KvPages, mk::PagedAttnArgs) =
+      head_dim == 96 ? (p.nt == 1 ? mk::attn_paged_kernel<96, 1> : p.nt == 2 ? mk::attn_paged_kernel<96, 2>
+                                                                             : mk::attn_paged_kernel<96, 4>)
+                     : (p.nt == 1 ? mk::attn_paged_kernel<128, 1> : p.nt == 2 ? mk::attn_paged_kernel<128, 2>
+                                                                              : mk::attn_paged_kernel<128, 4>);
+  MK_TRY(launch_k(k, dim3(p.ctas), dim3(mk::PA_THREADS), 0, st, true, c, a));
+  if (head_dim == 96)
+    return launch_k(mk::attn_paged_join_kernel<96>, dim3(p.ctas, 8 * p.nt), dim3(mk::PJ_PARTS * 96), 0, st, true, a);
+  return launch_k(mk::attn_paged_join_kernel<128>, dim3(p.ctas, 8 * p.nt), dim3(mk::PJ_PARTS * 128), 0, st, true, a);
 }
 
 size_t mk_kv_move_workspace(int32_t rows, int32_t num_pages) {

@@ -411,7 +411,7 @@ def attention_paged(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     """Attention of each row's last tokens over its cached keys and values (mk_attention_paged): (out bf16
     [T, n_q, head_dim], lse f32 [T, n_q]).  q bf16 [T, n_q, head_dim] (strided views allowed); lens counts the
     queries' own tokens; cu_q int32 [rows + 1] gives each row's queries, None one per row.  `max_q` and `max_len`
-    bound the queries and tokens of a row (max_len None: what the table can hold).  A query that sees no key
+    say what the queries and tokens of a row reach, for the launch shape (max_len None: what the table holds).  A query that sees no key
     gives zeros and lse -inf."""
     dev = _pages(codes, scales, 5)
     P, _, n_kv, page, hd = codes.shape
