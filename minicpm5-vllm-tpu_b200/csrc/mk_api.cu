@@ -25,6 +25,7 @@ using mk::aligned16;
 using mk::AttnLastArgs;
 using mk::cuda_status;
 using mk::launch_k;
+using mk::launch_k_pair;
 using mk::PFN_encodeTiled;
 using mk::GemmArgs;
 
@@ -123,27 +124,6 @@ mk_status device_state(DeviceState** out) {
   }
   *out = &d;
   return MK_OK;
-}
-
-// The same with clusters of two CTAs along x (grid.x even).
-template <typename... KArgs, typename... Args>
-mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
-                        Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
 }
 
 // Tokens per GEMM tile for M tokens and N output channels on `sms` SMs.  The persistent GEMM runs

@@ -22,6 +22,7 @@ enum : int {
   DEV_ERR_TIMEOUT_ATTN = 0x200,
   DEV_ERR_BAD_TOKEN_ID = 0x300,
   DEV_ERR_TIMEOUT_ATTN_TC = 0x400,
+  DEV_ERR_TIMEOUT_SCORE = 0x600,
   DEV_ERR_BAD_PAGE = 0x500,  // a row's table holds no page where it needs one, or a page or row id out of range
   DEV_ERR_NO_PAGE = 0x501,   // no free page (or no room in the table) left
 };
@@ -240,6 +241,16 @@ __device__ __forceinline__ void mma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in shared memory: each CTA holds its own 128 rows of A and half of B's columns.
+__device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // Arrive (once) on the barrier at shared::cluster address `bar_cl` when the pair MMAs issued so far by

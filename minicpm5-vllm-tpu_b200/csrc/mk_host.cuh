@@ -50,6 +50,27 @@ mk_status launch_k(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
 }
 
+// The same with clusters of two CTAs along x (grid.x even).
+template <typename... KArgs, typename... Args>
+mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
+                        Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
+}
+
 // What a kernel launch needs to know of the current device (mk_api.cu): the number of SMs, the device
 // error word (first error wins, read by mk_get_error) and the driver's tensor-map encoder.
 struct HostDevice {

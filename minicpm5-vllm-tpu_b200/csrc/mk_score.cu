@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
+#include <mutex>
 
 #include "mk_host.cuh"
 #include "mk_score.cuh"
@@ -13,10 +15,61 @@ namespace {
 using mk::aligned16;
 using mk::HostDevice;
 using mk::launch_k;
-
-constexpr int kScoreParts = 16;
+using mk::launch_k_pair;
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+int64_t id_tiles(int V) { return (static_cast<int64_t>(V) + mk::SC_V - 1) / mk::SC_V; }
+int64_t ld_part(int T) { return (static_cast<int64_t>(T) + 31) / 32 * 32; }
+size_t part_bytes(int T, int V) { return align256(static_cast<size_t>(id_tiles(V)) * 3 * ld_part(T) * sizeof(float)); }
+
+// bf16 rows [rows, ld], boxes of 64 columns x box_rows, 128-byte swizzle; zeros past the last row and column.
+mk_status map_rows(const HostDevice& d, CUtensorMap* m, const void* p, int64_t rows, int cols, int64_t ld, int box_rows) {
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {mk::SC_K, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t es[2] = {1, 1};
+  const CUresult r = d.encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MK_OK : MK_ERR_CUDA;
+}
+
+// Per-device set-up of the scoring kernels: shared memory limits and how many CTA pairs run at once.
+constexpr int kMaxDevices = 64;
+std::mutex g_mu;
+int g_pairs[kMaxDevices];
+bool g_ready[kMaxDevices];
+
+mk_status score_pairs(int sms, int* pairs) {
+  int dev = 0;
+  MK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return MK_ERR_BAD_ARG;
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_ready[dev]) {
+    MK_CUDA(cudaFuncSetAttribute(mk::score_tokens_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(mk::sc_smem_bytes(true))));
+    MK_CUDA(cudaFuncSetAttribute(mk::score_tokens_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(mk::sc_smem_bytes(false))));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (sms / 2));
+    cfg.blockDim = dim3(mk::SC_THREADS);
+    cfg.dynamicSmemBytes = mk::sc_smem_bytes(true);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    MK_CUDA(cudaOccupancyMaxActiveClusters(&n, mk::score_tokens_kernel<true>, &cfg));
+    g_pairs[dev] = n;
+    g_ready[dev] = true;
+  }
+  *pairs = g_pairs[dev];
+  return MK_OK;
+}
 
 }  // namespace
 
@@ -45,7 +98,7 @@ mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, 
 mk_status mk_score_tokens_workspace(int32_t T, int32_t H, int32_t V, size_t* bytes) {
   if (!bytes) return MK_ERR_BAD_ARG;
   if (T < 0 || H <= 0 || H % 8 || V <= 0) return MK_ERR_BAD_SHAPE;
-  *bytes = align256(static_cast<size_t>(T) * kScoreParts * sizeof(mk::ScorePart)) + static_cast<size_t>(T) * sizeof(float);
+  *bytes = part_bytes(T, V) + static_cast<size_t>(T) * sizeof(float);
   return MK_OK;
 }
 
@@ -61,18 +114,37 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   if (!aligned16(h) || !aligned16(lm_head) || !aligned16(workspace) || ld % 8) return MK_ERR_BAD_ALIGN;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
+  int pairs = 0;
+  MK_TRY(score_pairs(d.sm_count, &pairs));
+  // up to 128 tokens half of a pair's products would be with rows past the end
+  const bool pair = T > mk::SC_M && pairs > 0;
+  const int tok_tile = pair ? 2 * mk::SC_M : mk::SC_M;
+  const int64_t tok_tiles = (static_cast<int64_t>(T) + tok_tile - 1) / tok_tile, ids = id_tiles(V);
+  if (tok_tiles * ids > INT_MAX / 2) return MK_ERR_TOO_LARGE;
+  CUtensorMap mh, mw;
+  MK_TRY(map_rows(d, &mh, h, T, H, ld, mk::SC_M));
+  MK_TRY(map_rows(d, &mw, lm_head, V, H, H, mk::sc_b_rows(pair)));
+  mk::ScoreArgs a;
+  a.T = T;
+  a.H = H;
+  a.V = V;
+  a.id_tiles = static_cast<int>(ids);
+  a.tok_tiles = static_cast<int>(tok_tiles);
+  a.targets = targets;
+  a.scale = logit_scale * 1.4426950408889634f;
+  a.part = static_cast<float*>(workspace);
+  a.ld_part = ld_part(T);
+  a.target_logit = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_bytes(T, V));
+  a.err = d.err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  mk::ScorePart* part = static_cast<mk::ScorePart*>(workspace);
-  float* tl = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                       align256(static_cast<size_t>(T) * kScoreParts * sizeof(mk::ScorePart)));
-  const size_t smem = static_cast<size_t>(mk::SC_TOK) * H * sizeof(float);
-  MK_CUDA(cudaFuncSetAttribute(mk::score_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  MK_TRY(launch_k(mk::score_tokens_kernel, dim3((T + mk::SC_TOK - 1) / mk::SC_TOK, kScoreParts), dim3(mk::SC_THREADS), smem,
-                  st, true, static_cast<const __nv_bfloat16*>(h), T, H, static_cast<long long>(ld),
-                  static_cast<const __nv_bfloat16*>(lm_head), V, targets, logit_scale, part, tl));
-  return launch_k(mk::score_join_kernel, dim3((T + 127) / 128), dim3(128), 0, st, true,
-                  static_cast<const mk::ScorePart*>(part), kScoreParts, T, V, targets, static_cast<const float*>(tl),
-                  logprobs, entropy);
+  const int tiles = a.id_tiles * a.tok_tiles;
+  if (pair)
+    MK_TRY(launch_k_pair(mk::score_tokens_kernel<true>, dim3(2 * std::min(pairs, tiles)), dim3(mk::SC_THREADS),
+                         mk::sc_smem_bytes(true), st, true, mh, mw, a));
+  else
+    MK_TRY(launch_k(mk::score_tokens_kernel<false>, dim3(std::min(d.sm_count, tiles)), dim3(mk::SC_THREADS),
+                    mk::sc_smem_bytes(false), st, true, mh, mw, a));
+  return launch_k(mk::score_join_kernel, dim3((T + 31) / 32), dim3(32 * mk::SJ_SLICES), 0, st, true, a, logprobs, entropy);
 }
 
 }  // extern "C"

@@ -124,79 +124,302 @@ __global__ void __launch_bounds__(TL_THREADS)
 }
 
 // ---------------------------------------------------------------------------------- from hidden rows
-// Partial statistics of row t over one part of the vocabulary.
-struct ScorePart {
-  float m, z, w;
+// Row statistics of logits = scale * h W^T, tile by tile.  D[token, v] is computed by tcgen05.mma with tokens on
+// the TMEM lanes, so that an epilogue thread owns one token and walks its tile's 256 logits with (m, z, w) in
+// registers: nothing crosses lanes, and what leaves the kernel is 12 bytes per (token, 256 logits) instead of
+// 1024 (f32 logits of 8192 tokens over 73448 ids would be 2.4 GB written and read again).
+//
+// What bounds it: 2 H operations per logit against five instructions and one exponential in the epilogue; with
+// H = 1536 the tensor cores take 12288 cycles for a 128 x 256 tile and the exponentials 2048, hidden behind the
+// next tile's products (two accumulators fill the 512 TMEM columns).  With few tokens W's bytes are the bound.
+//
+// Layout.  PAIR (more than 128 tokens): two CTAs work on 256 tokens x 256 ids with 2-SM MMAs, each holding its 128
+// tokens and half of the ids, which halves the operand bytes that each SM takes in per product.  Otherwise one
+// CTA works on 128 tokens x 256 ids.  Tiles go out id-major: the CTAs at work share a few id tiles at a time, so W
+// comes from HBM once and the token tiles stay in L2.
+//   warp 0     TMA producer (64 of H per stage, 128-byte swizzle)
+//   warp 1     TMEM allocator and MMA issuer (the even CTA's, for both of a pair)
+//   warps 2-5  epilogue, one per 32-lane quarter of TMEM
+constexpr int SC_M = 128;      // tokens per CTA
+constexpr int SC_V = 256;      // ids per tile
+constexpr int SC_K = 64;       // of H per stage
+constexpr int SC_THREADS = 192;
+constexpr uint32_t SC_A_BYTES = SC_M * SC_K * 2;
+__host__ __device__ constexpr int sc_stages(bool pair) { return pair ? 6 : 4; }
+__host__ __device__ constexpr int sc_b_rows(bool pair) { return pair ? SC_V / 2 : SC_V; }
+__host__ __device__ constexpr uint32_t sc_stage_bytes(bool pair) { return SC_A_BYTES + sc_b_rows(pair) * SC_K * 2; }
+__host__ __device__ constexpr size_t sc_smem_bytes(bool pair) { return 1024 + sc_stages(pair) * sc_stage_bytes(pair) + 256; }
+constexpr float kLn2 = 0.693147180559945f;
+
+struct ScoreArgs {
+  int T, H, V, id_tiles, tok_tiles;
+  const int32_t* targets;
+  float scale;          // logit scale * log2 e: the statistics are in units of log 2
+  float* part;          // [id tiles][3][ld_part]: m, z, w
+  long long ld_part;    // T rounded up
+  float* target_logit;  // [T]
+  int* err;
 };
 
-// SC_TOK hidden rows in shared memory as f32; a warp walks the part's vocabulary rows, its lanes split H.
-constexpr int SC_TOK = 8;
-constexpr int SC_THREADS = 256;
-__global__ void __launch_bounds__(SC_THREADS)
-    score_tokens_kernel(const __nv_bfloat16* __restrict__ h, int T, int H, long long ld, const __nv_bfloat16* __restrict__ W,
-                        int V, const int32_t* __restrict__ targets, float scale, ScorePart* __restrict__ part,
-                        float* __restrict__ target_logit) {
-  extern __shared__ float hs[];  // [SC_TOK][H]
-  __shared__ RowStats red[SC_THREADS / 32][SC_TOK];
-  pdl_wait();
+template <bool PAIR>
+__global__ void __launch_bounds__(SC_THREADS, 1)
+    score_tokens_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
+                        const ScoreArgs args) {
+  constexpr int STAGES = sc_stages(PAIR), B_ROWS = sc_b_rows(PAIR);
+  constexpr uint32_t STAGE = sc_stage_bytes(PAIR);
+  extern __shared__ uint8_t sc_smem_raw[];
+  const uint32_t raw = smem_u32(sc_smem_raw);
+  uint8_t* base = sc_smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + STAGES * STAGE);  // [STAGES] both operands landed
+  uint64_t* empty = full + STAGES;   // [STAGES] the MMAs that read the stage finished
+  uint64_t* tfull = empty + STAGES;  // [2] accumulator ready
+  uint64_t* tempty = tfull + 2;      // [2] accumulator drained
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = PAIR ? cluster_ctarank() : 0u;
+  auto lead_bar = [&](uint64_t* b) { return PAIR ? mapa_cluster(smem_u32(b), 0) : smem_u32(b); };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 4 * (PAIR ? 2 : 1));
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmH);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();
-  const int tok0 = blockIdx.x * SC_TOK, lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < SC_TOK * H; i += SC_THREADS) {
-    const int t = tok0 + i / H;
-    hs[i] = t < T ? __bfloat162float(h[static_cast<long long>(t) * ld + i % H]) : 0.f;
-  }
-  __syncthreads();
-  const int per = (V + gridDim.y - 1) / gridDim.y, v0 = blockIdx.y * per, v1 = min(V, v0 + per);
-  RowStats s[SC_TOK];
-  int tg[SC_TOK];
-#pragma unroll
-  for (int t = 0; t < SC_TOK; ++t) {
-    s[t] = stats_empty();
-    tg[t] = tok0 + t < T ? targets[tok0 + t] : -1;
-  }
-  for (int v = v0 + wp; v < v1; v += SC_THREADS / 32) {
-    float acc[SC_TOK] = {};
-    for (int c = lane; c < H; c += 32) {
-      const float w = __bfloat162float(W[static_cast<size_t>(v) * H + c]);
-#pragma unroll
-      for (int t = 0; t < SC_TOK; ++t) acc[t] += w * hs[t * H + c];
+
+  const int unit = PAIR ? static_cast<int>(blockIdx.x) >> 1 : static_cast<int>(blockIdx.x);
+  const int units = PAIR ? static_cast<int>(gridDim.x) >> 1 : static_cast<int>(gridDim.x);
+  const int tiles = args.id_tiles * args.tok_tiles, my_tiles = (tiles - unit + units - 1) / units;
+  const int KT = (args.H + SC_K - 1) / SC_K;  // past H both operands read zeros
+  auto id_tile = [&](int it) { return (unit + it * units) / args.tok_tiles; };
+  // first token of this CTA's half of the tile
+  auto tok0 = [&](int it) {
+    return ((unit + it * units) % args.tok_tiles) * (PAIR ? 2 * SC_M : SC_M) + static_cast<int>(crank) * SC_M;
+  };
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    pdl_wait();
+    uint32_t issued = 0, issued_par = 0;
+    int idx = 0;
+    bool ok = true;
+    for (int it = 0; ok && it < my_tiles; ++it) {
+      const int t0 = tok0(it), v0 = id_tile(it) * SC_V + static_cast<int>(crank) * (PAIR ? B_ROWS : 0);
+      for (int kt = 0; kt < KT; ++kt, ++idx) {
+        const int s = idx % STAGES;
+        const uint32_t ph = (idx / STAGES) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag));
+        if (!ok) break;
+        if (leader) {
+          uint8_t* at = base + s * STAGE;
+          if constexpr (PAIR) {
+            if (crank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE);
+            const uint32_t fb = lead_bar(&full[s]);
+            tma_load_2d_pair(at, &tmH, fb, kt * SC_K, t0);
+            tma_load_2d_pair(at + SC_A_BYTES, &tmW, fb, kt * SC_K, v0);
+          } else {
+            mbar_arrive_expect_tx(&full[s], STAGE);
+            tma_load_2d(at, &tmH, &full[s], kt * SC_K, t0);
+            tma_load_2d(at + SC_A_BYTES, &tmW, &full[s], kt * SC_K, v0);
+          }
+        }
+        __syncwarp();
+        issued |= 1u << s;
+        issued_par = (issued_par & ~(1u << s)) | (ph << s);
+      }
     }
+    // every issued copy lands before the CTA may exit (a pair's on the even CTA's barriers)
+    if (!PAIR || crank == 0)
+      for (int s = 0; s < STAGES; ++s)
+        if (issued & (1u << s)) mbar_wait_drain(&full[s], (issued_par >> s) & 1u);
+  } else if (warp == 1) {
+    if (!PAIR || crank == 0) {
+      const bool leader = elect_one();
+      const uint32_t idesc = idesc_bf16_f32(PAIR ? 2 * SC_M : SC_M, SC_V);
+      auto commit_all = [&](uint64_t* b) {
+        if constexpr (PAIR) {
+          mma_commit_pair(smem_u32(b));
+          mma_commit_pair(mapa_cluster(smem_u32(b), 1));
+        } else {
+          mma_commit(b);
+        }
+      };
+      int idx = 0;
+      bool ok = true;
+      for (int it = 0; ok && it < my_tiles; ++it) {
+        const int a = it & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&tempty[a], ((it >> 1) & 1) ^ 1u, abort_flag))) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + a * SC_V;
+        for (int kt = 0; kt < KT; ++kt, ++idx) {
+          const int s = idx % STAGES;
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (idx / STAGES) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = sdesc_kmajor_sw128(smem_u32(base + s * STAGE));
+          const uint64_t db = sdesc_kmajor_sw128(smem_u32(base + s * STAGE + SC_A_BYTES));
+          if (leader) {
 #pragma unroll
-    for (int t = 0; t < SC_TOK; ++t) {
-      for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
-      const float x = acc[t] * scale;
-      stats_add(s[t], x);
-      if (v == tg[t] && lane == 0) target_logit[tok0 + t] = x;
+            for (int k = 0; k < SC_K / 16; ++k) {
+              if constexpr (PAIR)
+                mma_f16_ss_pair(d, da + 2 * k, db + 2 * k, idesc, (kt | k) != 0 ? 1u : 0u);
+              else
+                mma_f16_ss(d, da + 2 * k, db + 2 * k, idesc, (kt | k) != 0 ? 1u : 0u);
+            }
+            commit_all(&empty[s]);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (leader) commit_all(&tfull[a]);
+        __syncwarp();
+      }
+      if (leader) {
+        if constexpr (PAIR)
+          mma_commit_pair(smem_u32(drain));
+        else
+          mma_commit(drain);
+      }
+      __syncwarp();
+      mbar_wait_drain(drain, 0);
+    }
+  } else {
+    const int q = warp & 3;  // the TMEM quarter that this warp may read
+    pdl_wait();
+    for (int it = 0; it < my_tiles; ++it) {
+      const int a = it & 1, vt = id_tile(it), t = tok0(it) + q * 32 + lane, v0 = vt * SC_V;
+      const int tg = t < args.T ? args.targets[t] : -1;
+      const int nv = min(SC_V, args.V - v0);
+      if (!mbar_wait(&tfull[a], (it >> 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      float m = -INFINITY, z = 0.f, w = 0.f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < nv; c0 += 32) {
+        uint32_t acc[32];
+        tmem_ld_32x32b_x32(tmem_base + a * SC_V + c0 + (static_cast<uint32_t>(q * 32) << 16), acc);
+        tmem_ld_wait();
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(acc[j]) * args.scale;
+        if (c0 + 32 > nv) {  // ids past the vocabulary weigh nothing
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j >= nv) y[j] = -INFINITY;
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) top = max3f(top, y[j], y[j + 1]);
+        const float ref = top == -INFINITY ? 0.f : top, d = m - ref, f = ex2_approx(d);
+        w = (w + z * fmaxf(d, kFar)) * f;
+        z *= f;
+        m = top;
+        float z1 = 0.f, w1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float ua = y[j] - ref, ub = y[j + 1] - ref, ea = ex2_approx(ua), eb = ex2_approx(ub);
+          z += ea;
+          z1 += eb;
+          w = fmaf(ea, fmaxf(ua, kFar), w);
+          w1 = fmaf(eb, fmaxf(ub, kFar), w1);
+        }
+        z += z1;
+        w += w1;
+        const int at = tg - v0 - c0;
+        if (at >= 0 && at < 32) {
+          float x = y[0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) x = j == at ? y[j] : x;
+          if (tg < args.V) args.target_logit[t] = x;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR)
+          mbar_arrive_cluster(lead_bar(&tempty[a]));
+        else
+          mbar_arrive(&tempty[a]);
+      }
+      if (t < args.T) {
+        float* p = args.part + static_cast<long long>(vt) * 3 * args.ld_part + t;
+        p[0] = m;
+        p[args.ld_part] = z;
+        p[2 * args.ld_part] = w;
+      }
     }
   }
-  if (lane == 0)
-#pragma unroll
-    for (int t = 0; t < SC_TOK; ++t) red[wp][t] = s[t];
+
+  tc_fence_before();
   __syncthreads();
-  if (threadIdx.x < SC_TOK && tok0 + threadIdx.x < T) {
-    RowStats r = red[0][threadIdx.x];
-    for (int i = 1; i < SC_THREADS / 32; ++i) r = stats_join(r, red[i][threadIdx.x]);
-    part[static_cast<size_t>(tok0 + threadIdx.x) * gridDim.y + blockIdx.y] = {r.m, r.z, r.w};
+  tc_fence_after();
+  if constexpr (PAIR) {
+    cluster_sync();  // neither CTA frees its TMEM or leaves while the pair's MMAs may still read its operands
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+  } else {
+    if (warp == 1) tmem_dealloc(tmem_base, 512);
   }
+  if (threadIdx.x == 0 && *abort_flag && args.err) atomicCAS(args.err, 0, DEV_ERR_TIMEOUT_SCORE);
 }
 
-// Joins a row's parts in order.
-__global__ void score_join_kernel(const ScorePart* __restrict__ part, int nparts, int T, int V,
-                                  const int32_t* __restrict__ targets, const float* __restrict__ target_logit,
-                                  float* __restrict__ lp, float* __restrict__ ent) {
+// Joins a token's id tiles: 32 tokens x SJ_SLICES slices of the tiles per CTA, then the slices in order.
+constexpr int SJ_SLICES = 32;
+__device__ __forceinline__ RowStats stats_join2(const RowStats& a, const RowStats& b) {  // units of log 2
+  RowStats r;
+  r.m = fmaxf(a.m, b.m);
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
+  const float da = a.m - ref, db = b.m - ref, ea = ex2_approx(da), eb = ex2_approx(db);
+  r.z = a.z * ea + b.z * eb;
+  r.w = (a.w + a.z * fmaxf(da, kFar)) * ea + (b.w + b.z * fmaxf(db, kFar)) * eb;
+  return r;
+}
+__global__ void __launch_bounds__(32 * SJ_SLICES)
+    score_join_kernel(const ScoreArgs args, float* __restrict__ lp, float* __restrict__ ent) {
+  __shared__ RowStats s_p[SJ_SLICES][33];
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= T) return;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, t = blockIdx.x * 32 + lane;
   RowStats s = stats_empty();
-  for (int i = 0; i < nparts; ++i) {
-    const ScorePart p = part[static_cast<size_t>(t) * nparts + i];
-    s = stats_join(s, {p.m, p.z, p.w});
+  if (t < args.T) {
+#pragma unroll 4
+    for (int vt = slice; vt < args.id_tiles; vt += SJ_SLICES) {
+      const float* p = args.part + static_cast<long long>(vt) * 3 * args.ld_part + t;
+      s = stats_join2(s, {p[0], p[args.ld_part], p[2 * args.ld_part]});
+    }
   }
-  const int tg = targets[t];
-  const float lz = logf(s.z);
-  lp[t] = tg < 0 || tg >= V ? 0.f : s.z == 0.f ? -INFINITY : target_logit[t] - s.m - lz;
-  ent[t] = s.z == 0.f ? 0.f : lz - s.w / s.z;
+  s_p[slice][lane] = s;
+  __syncthreads();
+  if (slice || t >= args.T) return;
+  for (int i = 1; i < SJ_SLICES; ++i) s = stats_join2(s, s_p[i][lane]);
+  const int tg = args.targets[t];
+  const float lz = log2f(s.z);
+  lp[t] = tg < 0 || tg >= args.V ? 0.f : s.z == 0.f ? -INFINITY : (args.target_logit[t] - s.m - lz) * kLn2;
+  ent[t] = s.z == 0.f ? 0.f : (lz - s.w / s.z) * kLn2;
 }
 
 }  // namespace mk
