@@ -50,10 +50,10 @@ mk_status launch_k(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
 }
 
-// The same with clusters of two CTAs along x (grid.x even).
+// The same with clusters of `size` CTAs along x (grid.x a multiple of it).
 template <typename... KArgs, typename... Args>
-mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
-                        Args&&... args) {
+mk_status launch_k_cluster(int size, void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
+                           Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -61,7 +61,7 @@ mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem,
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.x = size;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -69,6 +69,12 @@ mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem,
   cfg.attrs = at;
   cfg.numAttrs = pdl ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
+}
+// Clusters of two CTAs.
+template <typename... KArgs, typename... Args>
+mk_status launch_k_pair(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
+                        Args&&... args) {
+  return launch_k_cluster(2, k, grid, block, smem, st, pdl, std::forward<Args>(args)...);
 }
 
 // What a kernel launch needs to know of the current device (mk_api.cu): the number of SMs, the device

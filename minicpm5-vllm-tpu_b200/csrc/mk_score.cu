@@ -15,13 +15,19 @@ namespace {
 using mk::aligned16;
 using mk::HostDevice;
 using mk::launch_k;
+using mk::launch_k_cluster;
 using mk::launch_k_pair;
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-int64_t id_tiles(int V) { return (static_cast<int64_t>(V) + mk::SC_V - 1) / mk::SC_V; }
+// More than one CTA's tokens go to CTA pairs: up to 128 half of a pair's products would be with rows past the end.
+bool in_pairs(int T) { return T > mk::SC_M; }
+int64_t id_tiles(int T, int V) {
+  const int ids = mk::sc_ids(in_pairs(T));
+  return (static_cast<int64_t>(V) + ids - 1) / ids;
+}
 int64_t ld_part(int T) { return (static_cast<int64_t>(T) + 31) / 32 * 32; }
-size_t part_bytes(int T, int V) { return align256(static_cast<size_t>(id_tiles(V)) * 3 * ld_part(T) * sizeof(float)); }
+size_t part_bytes(int T, int V) { return align256(static_cast<size_t>(id_tiles(T, V)) * 3 * ld_part(T) * sizeof(float)); }
 
 // bf16 rows [rows, ld], boxes of 64 columns x box_rows, 128-byte swizzle; zeros past the last row and column.
 mk_status map_rows(const HostDevice& d, CUtensorMap* m, const void* p, int64_t rows, int cols, int64_t ld, int box_rows) {
@@ -48,13 +54,13 @@ mk_status score_pairs(int sms, int* pairs) {
   std::lock_guard<std::mutex> lk(g_mu);
   if (!g_ready[dev]) {
     MK_CUDA(cudaFuncSetAttribute(mk::score_tokens_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(mk::sc_smem_bytes(true))));
+                                 static_cast<int>(mk::SC_SMEM_BYTES)));
     MK_CUDA(cudaFuncSetAttribute(mk::score_tokens_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(mk::sc_smem_bytes(false))));
+                                 static_cast<int>(mk::SC_SMEM_BYTES)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (sms / 2));
     cfg.blockDim = dim3(mk::SC_THREADS);
-    cfg.dynamicSmemBytes = mk::sc_smem_bytes(true);
+    cfg.dynamicSmemBytes = mk::SC_SMEM_BYTES;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2;
@@ -64,6 +70,7 @@ mk_status score_pairs(int sms, int* pairs) {
     cfg.numAttrs = 1;
     int n = 0;
     MK_CUDA(cudaOccupancyMaxActiveClusters(&n, mk::score_tokens_kernel<true>, &cfg));
+    if (n <= 0) return MK_ERR_CUDA;
     g_pairs[dev] = n;
     g_ready[dev] = true;
   }
@@ -86,13 +93,26 @@ mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, 
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (logits_bits == 32)
-    return launch_k(mk::token_logprobs_kernel<float>, dim3(T), dim3(mk::TL_THREADS), 0, st, true,
-                    static_cast<const float*>(logits), V, static_cast<long long>(ld), targets, top_k, logprobs, entropy,
-                    ranks, top_ids, top_logprobs);
-  return launch_k(mk::token_logprobs_kernel<__nv_bfloat16>, dim3(T), dim3(mk::TL_THREADS), 0, st, true,
-                  static_cast<const __nv_bfloat16*>(logits), V, static_cast<long long>(ld), targets, top_k, logprobs,
-                  entropy, ranks, top_ids, top_logprobs);
+  mk::LogitsArgs a;
+  a.logits = logits;
+  a.V = V;
+  a.k = top_k;
+  a.ld = ld;
+  a.targets = targets;
+  a.lp = logprobs;
+  a.ent = entropy;
+  a.rank = ranks;
+  a.top_ids = top_ids;
+  a.top_lp = top_logprobs;
+  // CTAs per row: four fit on an SM.  Rows are shared while the GPU has room for twice the CTAs and every one
+  // keeps at least a step's 8192 logits.
+  int cluster = 1;
+  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= static_cast<int64_t>(d.sm_count) * 4 &&
+         V / (cluster * 2) >= mk::TL_THREADS * mk::TL_VALUES)
+    cluster *= 2;
+  void (*k)(mk::LogitsArgs, int) =
+      logits_bits == 32 ? mk::token_logprobs_kernel<float> : mk::token_logprobs_kernel<__nv_bfloat16>;
+  return launch_k_cluster(cluster, k, dim3(static_cast<unsigned>(T) * cluster), dim3(mk::TL_THREADS), 0, st, true, a, cluster);
 }
 
 mk_status mk_score_tokens_workspace(int32_t T, int32_t H, int32_t V, size_t* bytes) {
@@ -116,14 +136,13 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   MK_TRY(mk::host_device(&d));
   int pairs = 0;
   MK_TRY(score_pairs(d.sm_count, &pairs));
-  // up to 128 tokens half of a pair's products would be with rows past the end
-  const bool pair = T > mk::SC_M && pairs > 0;
+  const bool pair = in_pairs(T);
   const int tok_tile = pair ? 2 * mk::SC_M : mk::SC_M;
-  const int64_t tok_tiles = (static_cast<int64_t>(T) + tok_tile - 1) / tok_tile, ids = id_tiles(V);
+  const int64_t tok_tiles = (static_cast<int64_t>(T) + tok_tile - 1) / tok_tile, ids = id_tiles(T, V);
   if (tok_tiles * ids > INT_MAX / 2) return MK_ERR_TOO_LARGE;
   CUtensorMap mh, mw;
   MK_TRY(map_rows(d, &mh, h, T, H, ld, mk::SC_M));
-  MK_TRY(map_rows(d, &mw, lm_head, V, H, H, mk::sc_b_rows(pair)));
+  MK_TRY(map_rows(d, &mw, lm_head, V, H, H, mk::SC_B_ROWS));
   mk::ScoreArgs a;
   a.T = T;
   a.H = H;
@@ -131,7 +150,7 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   a.id_tiles = static_cast<int>(ids);
   a.tok_tiles = static_cast<int>(tok_tiles);
   a.targets = targets;
-  a.scale = logit_scale * 1.4426950408889634f;
+  a.scale = static_cast<float>(logit_scale * 1.4426950408889634 * (1.0 + mk::kTruncPerStep * ((H + 15) / 16)));
   a.part = static_cast<float*>(workspace);
   a.ld_part = ld_part(T);
   a.target_logit = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_bytes(T, V));
@@ -140,11 +159,11 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   const int tiles = a.id_tiles * a.tok_tiles;
   if (pair)
     MK_TRY(launch_k_pair(mk::score_tokens_kernel<true>, dim3(2 * std::min(pairs, tiles)), dim3(mk::SC_THREADS),
-                         mk::sc_smem_bytes(true), st, true, mh, mw, a));
+                         mk::SC_SMEM_BYTES, st, true, mh, mw, a));
   else
     MK_TRY(launch_k(mk::score_tokens_kernel<false>, dim3(std::min(d.sm_count, tiles)), dim3(mk::SC_THREADS),
-                    mk::sc_smem_bytes(false), st, true, mh, mw, a));
-  return launch_k(mk::score_join_kernel, dim3((T + 31) / 32), dim3(32 * mk::SJ_SLICES), 0, st, true, a, logprobs, entropy);
+                    mk::SC_SMEM_BYTES, st, true, mh, mw, a));
+  return launch_k(mk::score_join_kernel, dim3((T + mk::SJ_TOKENS - 1) / mk::SJ_TOKENS), dim3(mk::SJ_THREADS), 0, st, true, a, logprobs, entropy);
 }
 
 }  // extern "C"

@@ -18,6 +18,8 @@ struct RowStats {
   float m, z, w;
 };
 constexpr float kFar = -200.f;
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLn2 = 0.693147180559945f;
 __device__ __forceinline__ RowStats stats_empty() { return {-INFINITY, 0.f, 0.f}; }
 __device__ __forceinline__ RowStats stats_join(const RowStats& a, const RowStats& b) {
   RowStats r;
@@ -43,6 +45,23 @@ __device__ __forceinline__ RowStats stats_warp(RowStats s) {
   return s;
 }
 
+// (d0, d1) += (a0, a1) * (b0, b1) in one packed f32x2 FMA.
+__device__ __forceinline__ void fma2_pair(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+// A 16-byte load of bytes that are read once.
+__device__ __forceinline__ uint4 ldg_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 // Order of the alternatives: value descending, then id ascending; zeros of either sign are equal and a NaN
 // comes after every number.  An entry is one 64-bit number, larger = earlier.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -55,79 +74,341 @@ __device__ __forceinline__ unsigned long long order_entry(uint32_t key, int id) 
 __device__ __forceinline__ int order_id(unsigned long long e) { return static_cast<int>(~static_cast<uint32_t>(e)); }
 
 // ---------------------------------------------------------------------------------- from logits
-// One CTA per row: one pass for the statistics and the rank, then one for each alternative, the largest entry
-// that comes after the last pick.
-constexpr int TL_THREADS = 1024;
+// One pass over the logits: statistics, rank and alternatives together.  A cluster of CTAs shares a row (one CTA
+// where there are rows enough), each with a slice of it.
+//
+// Alternatives.  An entry can only be among the k largest if it reaches tau, any value that k entries of the
+// slice reach.  The threads form 64 groups; the k-th largest of the groups' running maxima is such a value.  It is
+// taken after the first 8192 logits, again whenever as many more have been seen, and at the end; logits that
+// reach the current tau go into a list in shared memory (a few per doubling and alternative), and those that
+// reach the last one are put in order by counting.  Rows that defeat it (more than TL_CAP entries listed: long
+// runs of equal or rising logits; fewer than k logits above -inf) fall back to one search of the slice for
+// each alternative that is missing.
+//
+// What bounds it: the bytes of the logits.  Per bf16 logit the arithmetic is about six instructions and one
+// exponential, two thirds of what an SM can issue at the rate at which HBM delivers them.
+constexpr int TL_THREADS = 256;
+constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
+constexpr int TL_GROUPS = 64;     // of TL_THREADS / TL_GROUPS neighbouring lanes
+constexpr int TL_CAP = 2048;      // list entries
+constexpr int TL_CLUSTER_MAX = 8;
+static_assert(TL_TOPK_MAX <= TL_GROUPS && TL_CLUSTER_MAX * TL_TOPK_MAX <= TL_CAP, "alternatives");
+
+__device__ __forceinline__ float order_value(unsigned long long e) {
+  const uint32_t k = static_cast<uint32_t>(e >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+template <typename E>
+__device__ __forceinline__ float logit_at(const E* p, long long i);
+template <>
+__device__ __forceinline__ float logit_at<float>(const float* p, long long i) { return p[i]; }
+template <>
+__device__ __forceinline__ float logit_at<__nv_bfloat16>(const __nv_bfloat16* p, long long i) {
+  return __bfloat162float(p[i]);
+}
+__device__ __forceinline__ unsigned long long ld_cluster_u64(const void* p, uint32_t rank) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_cluster(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+struct LogitsArgs {
+  const void* logits;
+  int V, k;
+  long long ld;
+  const int32_t* targets;
+  float* lp;
+  float* ent;
+  int32_t* rank;
+  int32_t* top_ids;
+  float* top_lp;
+};
 
 template <typename E>
-__device__ __forceinline__ float logit_at(const E* p, size_t i);
-template <>
-__device__ __forceinline__ float logit_at<float>(const float* p, size_t i) { return p[i]; }
-template <>
-__device__ __forceinline__ float logit_at<__nv_bfloat16>(const __nv_bfloat16* p, size_t i) { return __bfloat162float(p[i]); }
-
-template <typename E>
-__global__ void __launch_bounds__(TL_THREADS)
-    token_logprobs_kernel(const E* __restrict__ logits, int V, long long ld, const int32_t* __restrict__ targets, int k,
-                          float* __restrict__ lp, float* __restrict__ ent, int32_t* __restrict__ rank,
-                          int32_t* __restrict__ top_ids, float* __restrict__ top_lp) {
-  __shared__ RowStats rs[32];
-  __shared__ int rc[32];
-  __shared__ unsigned long long pick[32];
+__global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const LogitsArgs a, const int cluster) {
+  constexpr bool BF = sizeof(E) == 2;
+  constexpr int EPV = 16 / sizeof(E);            // logits per 16-byte vector
+  constexpr int VECS = TL_VALUES / EPV;          // vectors per thread and step
+  constexpr uint32_t kNone = BF ? 0xff80ff80u : 0xff800000u;  // -inf
+  __shared__ unsigned long long s_list[TL_CAP], s_kept[TL_CAP], s_top[TL_TOPK_MAX];
+  __shared__ unsigned long long s_pick[TL_THREADS / 32];
+  __shared__ float s_gm[TL_GROUPS], s_tau;
+  __shared__ int s_n, s_kept_n, s_have;
+  __shared__ RowStats s_st[TL_THREADS / 32];
+  __shared__ int s_above[TL_THREADS / 32];
+  __shared__ __align__(8) float s_res[4];        // this CTA's m, z, w, rank count
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wp = tid >> 5;
-  const E* row = logits + static_cast<long long>(b) * ld;
-  const int t = targets[b];
+  const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5, V = a.V, k = a.k;
+  const int part = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const long long b = blockIdx.x / cluster;
+  const E* row = static_cast<const E*>(a.logits) + b * a.ld;
+  const int t = a.targets[b];
   const bool given = t >= 0 && t < V;
-  const float mine = given ? logit_at(row, t) : 0.f;
-  RowStats s = stats_empty();
+  const float mine = given ? logit_at(row, t) : INFINITY;
+
+  // the row: `head` logits up to a 16-byte boundary, nvec vectors, a tail; this CTA's vectors and loose logits
+  const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(E)));
+  const int nvec = (V - head) / EPV, tail0 = head + nvec * EPV;
+  const int per = (nvec + cluster - 1) / cluster, vec0 = min(nvec, part * per), vec1 = min(nvec, vec0 + per);
+  const int lo = part == 0 ? 0 : head + vec0 * EPV, hi = part == cluster - 1 ? V : head + vec1 * EPV;
+  const uint4* vecs = reinterpret_cast<const uint4*>(row + head);
+
+  RowStats st = stats_empty();
+  float top = -INFINITY, tau = -INFINITY;
   int above = 0;
-  for (int i = tid; i < V; i += TL_THREADS) {
-    const float x = logit_at(row, i);
-    stats_add(s, x);
-    above += x > mine || (mine != mine && x == x);
-  }
-  s = stats_warp(s);
-  above = __reduce_add_sync(0xffffffffu, above);
-  if (lane == 0) { rs[wp] = s; rc[wp] = above; }
+  if (tid == 0) s_n = s_kept_n = 0;
   __syncthreads();
-  s = rs[0];
-  above = rc[0];
-  for (int i = 1; i < 32; ++i) { s = stats_join(s, rs[i]); above += rc[i]; }
-  const float lz = logf(s.z);
+  auto list = [&](float x, int id) {
+    if (x >= tau && x > -INFINITY) {
+      const int at = atomicAdd(&s_n, 1);
+      if (at < TL_CAP) s_list[at] = order_entry(order_key(x), id);
+    }
+  };
+  // tau from the groups' maxima (every thread calls it)
+  auto threshold = [&]() {
+    float g = top;
+#pragma unroll
+    for (int o = 1; o < TL_THREADS / TL_GROUPS; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % (TL_THREADS / TL_GROUPS) == 0) s_gm[tid / (TL_THREADS / TL_GROUPS)] = g;
+    __syncthreads();
+    if (tid < TL_GROUPS) {
+      const float mineg = s_gm[tid];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < TL_GROUPS; ++j) {
+        const float o = s_gm[j];
+        r += o > mineg || (o == mineg && j < tid);
+      }
+      if (r == k - 1) s_tau = mineg;
+    }
+    __syncthreads();
+    tau = s_tau;
+  };
+
+  // a loose logit of the head or tail: at most one per thread
+  int loose = -1;
+  if (part == 0 && tid < head) loose = tid;
+  if (part == cluster - 1 && tid >= 32 && tail0 + tid - 32 < V) loose = tail0 + tid - 32;
+  float loose_x = -INFINITY;
+  if (loose >= 0) {
+    loose_x = logit_at(row, loose);
+    stats_add(st, loose_x);
+    top = loose_x == loose_x ? loose_x : top;
+    above += loose_x > mine;
+  }
+
+  const int steps = max(1, (vec1 - vec0 + TL_THREADS * VECS - 1) / (TL_THREADS * VECS));
+  for (int step = 0; step < steps; ++step) {
+    uint4 x[VECS];
+    const int v0 = vec0 + step * TL_THREADS * VECS + tid;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      x[v] = make_uint4(kNone, kNone, kNone, kNone);
+      if (v0 + v * TL_THREADS < vec1) x[v] = ldg_once(vecs + v0 + v * TL_THREADS);
+    }
+    auto words = [&](int v, int w) { return w == 0 ? x[v].x : w == 1 ? x[v].y : w == 2 ? x[v].z : x[v].w; };
+    float vm[VECS], most = st.m;
+    // maxima of the vectors
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      if constexpr (BF) {
+        auto h2 = [&](int w) {
+          const uint32_t u = words(v, w);
+          return *reinterpret_cast<const __nv_bfloat162*>(&u);
+        };
+        const __nv_bfloat162 h = __hmax2(__hmax2(h2(0), h2(1)), __hmax2(h2(2), h2(3)));
+        vm[v] = fmaxf(__low2float(h), __high2float(h));
+      } else {
+        vm[v] = fmaxf(max3f(__uint_as_float(x[v].x), __uint_as_float(x[v].y), __uint_as_float(x[v].z)),
+                      __uint_as_float(x[v].w));
+      }
+      most = fmaxf(most, vm[v]);
+    }
+    top = fmaxf(top, most);
+    // statistics
+    const float ref = most == -INFINITY ? 0.f : most;
+    {
+      const float d = st.m - ref, f = __expf(d);
+      st.w = (st.w + st.z * fmaxf(d, kFar)) * f;
+      st.z *= f;
+      st.m = most;
+    }
+    float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
+    auto two = [&](float p, float q) {
+      float up = p, uq = q;
+      add2_acc(up, uq, -ref, -ref);
+      const float ep = ex2_approx(up * kLog2E), eq = ex2_approx(uq * kLog2E);
+      add2_acc(z0, z1, ep, eq);
+      up = fmaxf(up, kFar);
+      uq = fmaxf(uq, kFar);
+      fma2_pair(w0, w1, ep, eq, up, uq);
+    };
+    if constexpr (BF) {
+      const __nv_bfloat162 m2 = __float2bfloat162_rn(mine);
+      __nv_bfloat162 cnt = __float2bfloat162_rn(0.f);
+#pragma unroll
+      for (int v = 0; v < VECS; ++v)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t u = words(v, w);
+          const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&u);
+          cnt = __hadd2(cnt, __hgt2(h, m2));  // at most VECS * 4 in each half: exact
+          const float2 f = unpack_bf16x2(u);
+          two(f.x, f.y);
+        }
+      above += static_cast<int>(__low2float(cnt)) + static_cast<int>(__high2float(cnt));
+    } else {
+#pragma unroll
+      for (int v = 0; v < VECS; ++v)
+#pragma unroll
+        for (int w = 0; w < 4; w += 2) {
+          const float p = __uint_as_float(words(v, w)), q = __uint_as_float(words(v, w + 1));
+          above += (p > mine) + (q > mine);
+          two(p, q);
+        }
+    }
+    st.z += z0 + z1;
+    st.w += w0 + w1;
+    if (k > 0) {
+      if ((step & (step - 1)) == 0) {  // after 1, 2, 3, 5, 9, ... steps
+        threshold();
+        if (step == 0 && loose >= 0) list(loose_x, loose);
+      }
+#pragma unroll
+      for (int v = 0; v < VECS; ++v)
+        if (vm[v] >= tau) {
+          const int id = head + (v0 + v * TL_THREADS) * EPV;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (BF) {
+              const float2 f = unpack_bf16x2(words(v, w));
+              list(f.x, id + 2 * w);
+              list(f.y, id + 2 * w + 1);
+            } else {
+              list(__uint_as_float(words(v, w)), id + w);
+            }
+          }
+        }
+    }
+  }
+
+  // this CTA's statistics
+  st = stats_warp(st);
+  above = __reduce_add_sync(0xffffffffu, above);
+  if (lane == 0) {
+    s_st[wp] = st;
+    s_above[wp] = above;
+  }
+  if (k > 0) threshold();  // (a barrier; the list is complete)
+  __syncthreads();
   if (tid == 0) {
-    lp[b] = !given ? 0.f : s.z == 0.f ? -INFINITY : mine - s.m - lz;
-    ent[b] = s.z == 0.f ? 0.f : lz - s.w / s.z;
-    rank[b] = given ? above + 1 : 0;
-  }
-  unsigned long long last = ~0ull;
-  for (int r = 0; r < k; ++r) {
-    unsigned long long best = 0;
-    for (int i = tid; i < V; i += TL_THREADS) {
-      const unsigned long long e = order_entry(order_key(logit_at(row, i)), i);
-      if (e < last && e > best) best = e;
+    for (int i = 1; i < TL_THREADS / 32; ++i) {
+      st = stats_join(st, s_st[i]);
+      above += s_above[i];
     }
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    s_res[0] = st.m;
+    s_res[1] = st.z;
+    s_res[2] = st.w;
+    s_res[3] = __int_as_float(above);
+  }
+
+  // this CTA's alternatives, in order
+  const int want = min(k, hi - lo);
+  if (k > 0) {
+    const int n = s_n;
+    if (n <= TL_CAP) {
+      const unsigned long long least = order_entry(order_key(tau), -1);  // any entry of value tau or more is >=
+      for (int i = tid; i < n; i += TL_THREADS)
+        if (s_list[i] >= least) s_kept[atomicAdd(&s_kept_n, 1)] = s_list[i];
+    }
     __syncthreads();
-    if (lane == 0) pick[wp] = best;
+    const int kept = s_kept_n;
+    for (int i = tid; i < kept; i += TL_THREADS) {
+      const unsigned long long e = s_kept[i];
+      int r = 0;
+      for (int j = 0; j < kept; ++j) r += s_kept[j] > e;
+      if (r < k) s_top[r] = e;
+    }
     __syncthreads();
-    for (int i = 0; i < 32; ++i) best = max(best, pick[i]);
-    last = best;
+    for (int have = min(kept, k); have < want; ++have) {
+      const unsigned long long last = have ? s_top[have - 1] : ~0ull;
+      unsigned long long best = 0;
+      for (int i = lo + tid; i < hi; i += TL_THREADS) {
+        const unsigned long long e = order_entry(order_key(logit_at(row, i)), i);
+        if (e < last && e > best) best = e;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (lane == 0) s_pick[wp] = best;
+      __syncthreads();
+      if (tid == 0) {
+        for (int i = 1; i < TL_THREADS / 32; ++i) best = max(best, s_pick[i]);
+        s_top[have] = best;
+      }
+      __syncthreads();
+    }
+    for (int i = want + tid; i < k; i += TL_THREADS) s_top[i] = 0;  // a slice of fewer than k logits
+  }
+  if (tid == 0) s_have = want;
+
+  // the row's
+  if (cluster > 1) cluster_sync(); else __syncthreads();
+  if (part == 0) {
+    st = {s_res[0], s_res[1], s_res[2]};
+    above = __float_as_int(s_res[3]);
+    for (int c = 1; c < cluster; ++c) {
+      const unsigned long long mz = ld_cluster_u64(&s_res[0], c), wa = ld_cluster_u64(&s_res[2], c);
+      st = stats_join(st, {__uint_as_float(static_cast<uint32_t>(mz)), __uint_as_float(static_cast<uint32_t>(mz >> 32)),
+                           __uint_as_float(static_cast<uint32_t>(wa))});
+      above += static_cast<int>(wa >> 32);
+    }
+    if (given && mine != mine) {  // a NaN ranks below every number
+      int numbers = 0;
+      for (int i = tid; i < V; i += TL_THREADS) {
+        const float x = logit_at(row, i);
+        numbers += x == x;
+      }
+      numbers = __reduce_add_sync(0xffffffffu, numbers);
+      __syncthreads();
+      if (lane == 0) s_above[wp] = numbers;
+      __syncthreads();
+      above = 0;
+      for (int i = 0; i < TL_THREADS / 32; ++i) above += s_above[i];
+    }
+    const float lz = logf(st.z);
     if (tid == 0) {
-      const int id = order_id(best);
-      top_ids[static_cast<size_t>(b) * k + r] = id;
-      top_lp[static_cast<size_t>(b) * k + r] = s.z == 0.f ? -INFINITY : logit_at(row, id) - s.m - lz;
+      a.lp[b] = !given ? 0.f : st.z == 0.f ? -INFINITY : mine - st.m - lz;
+      a.ent[b] = st.z == 0.f ? 0.f : lz - st.w / st.z;
+      a.rank[b] = given ? above + 1 : 0;
+    }
+    const int all = cluster * k;
+    if (cluster > 1) {
+      for (int i = tid; i < all; i += TL_THREADS) s_list[i] = ld_cluster_u64(&s_top[i % k], i / k);
+      __syncthreads();
+    }
+    for (int i = tid; i < all; i += TL_THREADS) {
+      const unsigned long long e = cluster > 1 ? s_list[i] : s_top[i];
+      int r = i;
+      if (cluster > 1) {
+        r = 0;
+        for (int j = 0; j < all; ++j) r += s_list[j] > e;
+      }
+      if (r < k && e) {
+        a.top_ids[b * k + r] = order_id(e);
+        a.top_lp[b * k + r] = st.z == 0.f ? -INFINITY : order_value(e) - st.m - lz;
+      }
     }
   }
+  if (cluster > 1) cluster_sync();  // no CTA leaves while its lists may be read
 }
 
 // ---------------------------------------------------------------------------------- from hidden rows
 // Row statistics of logits = scale * h W^T, tile by tile.  D[token, v] is computed by tcgen05.mma with tokens on
 // the TMEM lanes, so that an epilogue thread owns one token and walks its tile's 256 logits with (m, z, w) in
-// registers: nothing crosses lanes, and what leaves the kernel is 12 bytes per (token, 256 logits) instead of
-// 1024 (f32 logits of 8192 tokens over 73448 ids would be 2.4 GB written and read again).
+// registers: nothing crosses lanes, and what leaves the kernel is 12 bytes per (token, id tile) instead of
+// 4 a logit (f32 logits of 8192 tokens over 73448 ids would be 2.4 GB written and read again).
 //
 // What bounds it: 2 H operations per logit against five instructions and one exponential in the epilogue; with
 // H = 1536 the tensor cores take 12288 cycles for a 128 x 256 tile and the exponentials 2048, hidden behind the
@@ -135,21 +416,27 @@ __global__ void __launch_bounds__(TL_THREADS)
 //
 // Layout.  PAIR (more than 128 tokens): two CTAs work on 256 tokens x 256 ids with 2-SM MMAs, each holding its 128
 // tokens and half of the ids, which halves the operand bytes that each SM takes in per product.  Otherwise one
-// CTA works on 128 tokens x 256 ids.  Tiles go out id-major: the CTAs at work share a few id tiles at a time, so W
+// CTA works on 128 tokens x 128 ids (W is then the bound, and the smaller tiles leave less of the last wave idle:
+// 1020 tiles of 130560 ids on 148 SMs fill 98 % of 7 waves, 510 tiles of 256 ids 86 % of 4).  Tiles go out id-major: the CTAs at work share a few id tiles at a time, so W
 // comes from HBM once and the token tiles stay in L2.
 //   warp 0     TMA producer (64 of H per stage, 128-byte swizzle)
 //   warp 1     TMEM allocator and MMA issuer (the even CTA's, for both of a pair)
 //   warps 2-5  epilogue, one per 32-lane quarter of TMEM
 constexpr int SC_M = 128;      // tokens per CTA
-constexpr int SC_V = 256;      // ids per tile
 constexpr int SC_K = 64;       // of H per stage
 constexpr int SC_THREADS = 192;
 constexpr uint32_t SC_A_BYTES = SC_M * SC_K * 2;
-__host__ __device__ constexpr int sc_stages(bool pair) { return pair ? 6 : 4; }
-__host__ __device__ constexpr int sc_b_rows(bool pair) { return pair ? SC_V / 2 : SC_V; }
-__host__ __device__ constexpr uint32_t sc_stage_bytes(bool pair) { return SC_A_BYTES + sc_b_rows(pair) * SC_K * 2; }
-__host__ __device__ constexpr size_t sc_smem_bytes(bool pair) { return 1024 + sc_stages(pair) * sc_stage_bytes(pair) + 256; }
-constexpr float kLn2 = 0.693147180559945f;
+constexpr int SC_B_ROWS = 128;  // ids that a CTA loads per tile
+constexpr int SC_STAGES = 6;
+constexpr uint32_t SC_STAGE_BYTES = SC_A_BYTES + SC_B_ROWS * SC_K * 2;
+constexpr size_t SC_SMEM_BYTES = 1024 + SC_STAGES * SC_STAGE_BYTES + 256;
+__host__ __device__ constexpr int sc_ids(bool pair) { return pair ? 2 * SC_B_ROWS : SC_B_ROWS; }  // ids per tile
+
+// The tensor cores' f32 accumulator rounds toward zero: of sums of products of either sign a step of 16 loses
+// 0.26 * 2^-24 of the final value on average (measured from the entropy's error against 64 bits: 0.23, 0.25, 0.26
+// and 0.27 at H = 256, 768, 1536 and 4096), 1.5e-6 at H = 1536, all logits alike.  The logits are scaled up by that
+// average (the entropy's error falls from 1.2e-6 to that of f32 sums).
+constexpr double kTruncPerStep = 0.26 / (1 << 24);
 
 struct ScoreArgs {
   int T, H, V, id_tiles, tok_tiles;
@@ -165,8 +452,8 @@ template <bool PAIR>
 __global__ void __launch_bounds__(SC_THREADS, 1)
     score_tokens_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
                         const ScoreArgs args) {
-  constexpr int STAGES = sc_stages(PAIR), B_ROWS = sc_b_rows(PAIR);
-  constexpr uint32_t STAGE = sc_stage_bytes(PAIR);
+  constexpr int STAGES = SC_STAGES, SC_V = sc_ids(PAIR);
+  constexpr uint32_t STAGE = SC_STAGE_BYTES;
   extern __shared__ uint8_t sc_smem_raw[];
   const uint32_t raw = smem_u32(sc_smem_raw);
   uint8_t* base = sc_smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -229,7 +516,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
     int idx = 0;
     bool ok = true;
     for (int it = 0; ok && it < my_tiles; ++it) {
-      const int t0 = tok0(it), v0 = id_tile(it) * SC_V + static_cast<int>(crank) * (PAIR ? B_ROWS : 0);
+      const int t0 = tok0(it), v0 = id_tile(it) * SC_V + static_cast<int>(crank) * SC_B_ROWS;
       for (int kt = 0; kt < KT; ++kt, ++idx) {
         const int s = idx % STAGES;
         const uint32_t ph = (idx / STAGES) & 1;
@@ -387,8 +674,6 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
   if (threadIdx.x == 0 && *abort_flag && args.err) atomicCAS(args.err, 0, DEV_ERR_TIMEOUT_SCORE);
 }
 
-// Joins a token's id tiles: 32 tokens x SJ_SLICES slices of the tiles per CTA, then the slices in order.
-constexpr int SJ_SLICES = 32;
 __device__ __forceinline__ RowStats stats_join2(const RowStats& a, const RowStats& b) {  // units of log 2
   RowStats r;
   r.m = fmaxf(a.m, b.m);
@@ -398,24 +683,40 @@ __device__ __forceinline__ RowStats stats_join2(const RowStats& a, const RowStat
   r.w = (a.w + a.z * fmaxf(da, kFar)) * ea + (b.w + b.z * fmaxf(db, kFar)) * eb;
   return r;
 }
-__global__ void __launch_bounds__(32 * SJ_SLICES)
+// Joins a token's id tiles: 8 tokens x 128 slices of the tiles per CTA; a slice in order, then the slices in a
+// fixed order.
+constexpr int SJ_TOKENS = 8;
+constexpr int SJ_THREADS = 1024;
+__global__ void __launch_bounds__(SJ_THREADS)
     score_join_kernel(const ScoreArgs args, float* __restrict__ lp, float* __restrict__ ent) {
-  __shared__ RowStats s_p[SJ_SLICES][33];
+  __shared__ RowStats s_p[SJ_THREADS / 32][SJ_TOKENS];
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, t = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = threadIdx.x % SJ_TOKENS;
+  const int t = blockIdx.x * SJ_TOKENS + k;
   RowStats s = stats_empty();
   if (t < args.T) {
 #pragma unroll 4
-    for (int vt = slice; vt < args.id_tiles; vt += SJ_SLICES) {
+    for (int vt = threadIdx.x / SJ_TOKENS; vt < args.id_tiles; vt += SJ_THREADS / SJ_TOKENS) {
       const float* p = args.part + static_cast<long long>(vt) * 3 * args.ld_part + t;
       s = stats_join2(s, {p[0], p[args.ld_part], p[2 * args.ld_part]});
     }
   }
-  s_p[slice][lane] = s;
+  auto across = [&](int o) {
+    return RowStats{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o),
+                    __shfl_xor_sync(0xffffffffu, s.w, o)};
+  };
+  s = stats_join2(s, across(8));
+  s = stats_join2(s, across(16));
+  if (lane < SJ_TOKENS) s_p[warp][lane] = s;
   __syncthreads();
-  if (slice || t >= args.T) return;
-  for (int i = 1; i < SJ_SLICES; ++i) s = stats_join2(s, s_p[i][lane]);
+  if (warp) return;
+  s = s_p[lane / SJ_TOKENS][k];
+#pragma unroll
+  for (int i = 4; i < SJ_THREADS / 32; i += 4) s = stats_join2(s, s_p[i + lane / SJ_TOKENS][k]);
+  s = stats_join2(s, across(8));
+  s = stats_join2(s, across(16));
+  if (lane >= SJ_TOKENS || t >= args.T) return;
   const int tg = args.targets[t];
   const float lz = log2f(s.z);
   lp[t] = tg < 0 || tg >= args.V ? 0.f : s.z == 0.f ? -INFINITY : (args.target_logit[t] - s.m - lz) * kLn2;
