@@ -39,8 +39,11 @@ struct PagedAttnArgs {
 
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
-constexpr int PA_UNIT = 16 * PA_WARPS;  // keys of one unit of work: 16 per warp
-constexpr int PA_GROUPS = 64;           // 16-key groups whose pages and scales are staged at a time
+// 16-key groups that a warp works on at a time: with 8 query rows two neighbouring ones, whose instructions fill each
+// other's latencies; wider tiles have work enough, and no registers left.
+__host__ __device__ constexpr int pa_groups(int nt) { return nt == 1 ? 2 : 1; }
+__host__ __device__ constexpr int pa_unit(int nt) { return 16 * pa_groups(nt) * PA_WARPS; }  // keys of one unit of work
+constexpr int PA_GROUPS = 64;           // groups whose pages and scales are staged at a time
 // m may lag the true maximum by up to 2^kLag: it moves only then, which spares a warp reduction and a rescaling
 // of O per 16 keys.
 //
@@ -51,6 +54,10 @@ constexpr int PA_GROUPS = 64;           // 16-key groups whose pages and scales 
 // times kPOff: the largest operand is 2^15, and a key that weighs less than 2^-31 of the maximum is lost.
 constexpr float kPOff = 128.f;
 constexpr float kLag = 8.f;
+// m before the first key: low enough that any score raises it, and finite, so that m - m is 0
+constexpr float kLow = -1e30f;
+
+__host__ __device__ constexpr int pa_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 // Loads of bytes that are read once (not kept in L1).
 __device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
@@ -106,14 +113,15 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 // piece of a pair that began earlier (slot 0) and one of a pair that continues later (slot 1, named in desc),
 // which attn_paged_join_kernel puts together in order.
 //
-// A warp takes every PA_WARPS-th 16-key group of its CTA's share.  Fragments of lane (r = lane / 4, c = lane % 4):
+// A warp takes every PA_WARPS-th block of GP 16-key groups of its CTA's share.  Fragments of lane (r = lane / 4, c = lane % 4):
 //   K Q^T   A rows r, r + 8 are keys 4 (r / 2) + r % 2 and that + 2; a 4-byte word of a key gives k-slots
 //           2c, 2c + 1, 2c + 8, 2c + 9 of one step.  Lane c holds bytes 16c .. of a key (and 64 + 16c .., hd 128,
 //           or 64 + 8c .., hd 96), and the queries' B fragments the same channels.
 //   V^T P^T after a transpose of P (movmatrix) lane c's k-slots are keys 4c .. 4c + 3, one word of the value
 //           plane; a 16-byte load holds them for channels 32j + 4r .. + 3, two of each 16-row tile.
 template <int HD, int NT>
-__global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
+__global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
+  constexpr int GP = pa_groups(NT), PA_UNIT = pa_unit(NT);
   constexpr int KS = HD / 16, MT = HD / 16, ROWS = 8 * NT, LDO = HD + 4;
   constexpr bool SPLIT = NT <= 2;  // p as two bf16 parts
   __shared__ long long s_scan[PA_WARPS], s_base;
@@ -191,31 +199,49 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
     const int lim_min = r0 + ROWS <= R ? limit(r0) : 0, lim_max = limit(min(r0 + ROWS, R) - 1);
     const int kbeg = ua * PA_UNIT, kend = min(ub * PA_UNIT, lim_max);
 
-    // queries as f16, each row scaled by a power of two to about 1 (its exponent joins the score's factor)
-    uint32_t qf[NT == 1 ? KS : 1][2];
-    float rf[NT][2];   // score factor of this lane's two columns of each 8-row tile
-    int lim[NT][2];
+    // Asked for first, all at once: the queries, then the pages of the first keys and the scales of those pages.
+    uint32_t qw[NT][KS][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int qr = r0 + t * 8 + r;
-      uint32_t w[KS][2];
-      float top = 0.f;
       const __nv_bfloat16* qp = a.q;
       if (qr < R) qp += static_cast<long long>(first + qr / G) * a.ld_q + static_cast<long long>(g * G + qr % G) * a.hs_q;
 #pragma unroll
       for (int s = 0; s < KS; s += 2) {  // 8 channels: two words' worth
         const int ch = s < 4 ? 16 * c + 4 * s : HD == 128 ? 64 + 16 * c + 4 * (s - 4) : 64 + 8 * c;
         const uint4 v = qr < R ? __ldg(reinterpret_cast<const uint4*>(qp + ch)) : make_uint4(0, 0, 0, 0);
-        w[s][0] = v.x;
-        w[s][1] = v.y;
-        w[s + 1][0] = v.z;
-        w[s + 1][1] = v.w;
+        qw[t][s][0] = v.x;
+        qw[t][s][1] = v.y;
+        qw[t][s + 1][0] = v.z;
+        qw[t][s + 1][1] = v.w;
       }
+    }
+    int page = -1;
+    float page_vs = 0.f, page_ks = 0.f;
+    auto load_pages = [&](int kb, int ng) {  // thread i: the page of group i
+      page = -1;
+      page_vs = page_ks = 0.f;
+      if (tid < ng) page = kv_page_of(a.table, a.width, cp.num_pages, row, (kb + tid * 16) >> cp.page_shift, a.err);
+      if (page >= 0) {
+        page_vs = *kv_scale_ptr(cp, page, 1, g);
+        page_ks = *kv_scale_ptr(cp, page, 0, g);
+      }
+    };
+    auto groups_at = [&](int kb) { return min(PA_GROUPS, (kend - kb + 15) >> 4); };
+    if (kbeg < kend) load_pages(kbeg, groups_at(kbeg));
+
+    // queries as f16, each row scaled by a power of two to about 1 (its exponent joins the score's factor)
+    uint32_t qf[NT == 1 ? KS : 1][2];
+    float rf[NT][2];   // score factor of this lane's two columns of each 8-row tile
+    int lim[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float top = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack_bf16x2(w[s][e]);
+          const float2 f = unpack_bf16x2(qw[t][s][e]);
           top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -227,7 +253,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
         uint32_t h[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack_bf16x2(w[s][e]);
+          const float2 f = unpack_bf16x2(qw[t][s][e]);
           h[e] = pack_f16x2(f.x * down, f.y * down);
         }
         if constexpr (NT == 1) {
@@ -247,7 +273,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
     float m[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      m[t][0] = m[t][1] = -INFINITY;
+      m[t][0] = m[t][1] = kLow;
       l[t][0] = l[t][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
@@ -255,16 +281,12 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
     float vref = 0.f;  // the largest value scale so far: O is in units of vref / kPOff
 
     for (int kb = kbeg; kb < kend; kb += PA_GROUPS * 16) {
-      const int ng = min(PA_GROUPS, (kend - kb + 15) >> 4);
-      __syncthreads();  // the last groups' pages and scales (and s_q, s_o) are no longer read
-      float vs = 0.f;
-      if (tid < ng) {
-        const int page = kv_page_of(a.table, a.width, cp.num_pages, row, (kb + tid * 16) >> cp.page_shift, a.err);
-        s_page[tid] = page;
-        vs = page < 0 ? 0.f : *kv_scale_ptr(cp, page, 1, g);
-        s_ks[tid] = page < 0 ? 0.f : *kv_scale_ptr(cp, page, 0, g);
+      const int ng = groups_at(kb);
+      if (kb != kbeg) {
+        load_pages(kb, ng);
+        __syncthreads();  // the last groups' pages and scales are no longer read
       }
-      float top = vs;  // (a NaN scale does not take part, and makes its own group NaN)
+      float top = page_vs;  // (a NaN scale does not take part, and makes its own group NaN)
 #pragma unroll
       for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       if (lane == 0) s_red[warp] = top;
@@ -272,7 +294,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_red[w]);
       const float nref = fmaxf(vref, top);
-      if (tid < ng) s_vs[tid] = nref > 0.f ? vs / nref * kPOff : vs;
+      if (tid < PA_GROUPS) {  // (past ng: no page)
+        s_page[tid] = page;
+        s_ks[tid] = page_ks;
+        s_vs[tid] = nref > 0.f ? page_vs / nref * kPOff : page_vs;
+      }
       if (nref != vref && vref > 0.f) {
         const float f = vref / nref;
 #pragma unroll
@@ -285,90 +311,145 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
       vref = nref;
       __syncthreads();
 
-      uint32_t kw[2][KS];  // two keys' words
-      uint4 vw[HD / 32];
-      auto load_k = [&](int gi) {
-        const int page = max(s_page[gi], 0), in = (kb + gi * 16) & page_mask;
-        const int8_t* p = kv_head_ptr(cp, page, 0, g) + static_cast<size_t>(in + 4 * (r >> 1) + (r & 1)) * HD;
+      uint32_t kw[GP][2][KS];  // two keys' words
+      uint4 vw[GP][HD / 32];
+      // Where the block's groups lie: in one page from 32 tokens on, so that all loads share one address.
+      const size_t plane = static_cast<size_t>(n_kv) * HD << cp.page_shift;
+      const int8_t* at[GP];
+      auto find = [&](int gi) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 x = ldg_stream(reinterpret_cast<const uint4*>(p + i * 2 * HD + c * 16));
-          kw[i][0] = x.x;
-          kw[i][1] = x.y;
-          kw[i][2] = x.z;
-          kw[i][3] = x.w;
-          if constexpr (HD == 128) {
-            const uint4 y = ldg_stream(reinterpret_cast<const uint4*>(p + i * 2 * HD + 64 + c * 16));
-            kw[i][4] = y.x;
-            kw[i][5] = y.y;
-            kw[i][6] = y.z;
-            kw[i][7] = y.w;
-          } else {
-            const uint2 y = ldg_stream(reinterpret_cast<const uint2*>(p + i * 2 * HD + 64 + c * 8));
-            kw[i][4] = y.x;
-            kw[i][5] = y.y;
-          }
+        for (int p = 0; p < GP; ++p) {
+          if (p == 0 || cp.page_shift == 4)
+            at[p] = kv_head_ptr(cp, max(s_page[gi + p], 0), 0, g) + ((kb + (gi + p) * 16) & page_mask) * HD;
+          else
+            at[p] = at[0] + p * 16 * HD;
         }
       };
-      auto load_v = [&](int gi) {
-        const int page = max(s_page[gi], 0), in = (kb + gi * 16) & page_mask;
-        const int8_t* p = kv_head_ptr(cp, page, 1, g) + static_cast<size_t>(in) * HD + (c * HD + 4 * r) * 4;
+      const int lane_k = (4 * (r >> 1) + (r & 1)) * HD + c * 16, lane_k8 = (4 * (r >> 1) + (r & 1)) * HD + 64 + c * 8;
+      const int lane_v = (c * HD + 4 * r) * 4;
+      auto load_k = [&]() {
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) vw[j] = ldg_stream(reinterpret_cast<const uint4*>(p + j * 128));
-      };
-      if (warp < ng) {
-        load_k(warp);
-        load_v(warp);
-      }
-#pragma unroll 1
-      for (int gi = warp; gi < ng; gi += PA_WARPS) {
-        const bool more = gi + PA_WARPS < ng;
-        float s[NT][4];
+        for (int p = 0; p < GP; ++p)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
-        for (int w = 0; w < KS; ++w) {
-          uint32_t a0, a1, a2, a3;
-          i8x4_to_f16x4(kw[0][w], a0, a2);
-          i8x4_to_f16x4(kw[1][w], a1, a3);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if constexpr (NT == 1) {
-              mma_16816(s[t], a0, a1, a2, a3, qf[w][0], qf[w][1]);
+          for (int i = 0; i < 2; ++i) {
+            const uint4 x = ldg_stream(reinterpret_cast<const uint4*>(at[p] + lane_k + i * 2 * HD));
+            kw[p][i][0] = x.x;
+            kw[p][i][1] = x.y;
+            kw[p][i][2] = x.z;
+            kw[p][i][3] = x.w;
+            if constexpr (HD == 128) {
+              const uint4 y = ldg_stream(reinterpret_cast<const uint4*>(at[p] + lane_k + 64 + i * 2 * HD));
+              kw[p][i][4] = y.x;
+              kw[p][i][5] = y.y;
+              kw[p][i][6] = y.z;
+              kw[p][i][7] = y.w;
             } else {
-              const uint2 b = s_q[(t * KS + w) * 32 + lane];
-              mma_16816(s[t], a0, a1, a2, a3, b.x, b.y);
+              const uint2 y = ldg_stream(reinterpret_cast<const uint2*>(at[p] + lane_k8 + i * 2 * HD));
+              kw[p][i][4] = y.x;
+              kw[p][i][5] = y.y;
             }
           }
-        }
-        if (more) load_k(gi + PA_WARPS);
-        const float ks = s_ks[gi], vr = s_vs[gi];
-        const int key = kb + gi * 16 + 4 * (r >> 1) + (r & 1);  // and key + 2
-        const bool masked = kb + gi * 16 + 16 > lim_min || s_page[gi] < 0;
-        uint32_t pb[NT][2], pl[SPLIT ? NT : 1][2];
-        bool raise = false;
+      };
+      auto load_v = [&]() {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int p = 0; p < GP; ++p)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] *= rf[t][e & 1] * ks;
-          if (masked) {
+          for (int j = 0; j < HD / 32; ++j)
+            vw[p][j] = ldg_stream(reinterpret_cast<const uint4*>(at[p] + plane + lane_v + j * 128));
+      };
+      if (warp * GP < ng) {
+        find(warp * GP);
+        load_k();
+        load_v();
+      }
+#pragma unroll 1
+      for (int gi = warp * GP; gi < ng; gi += PA_WARPS * GP) {
+        const bool more = gi + PA_WARPS * GP < ng;
+        float s[GP][NT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (key + (e & 2) >= lim[t][e & 1] || s_page[gi] < 0) s[t][e] = -INFINITY;
+        for (int p = 0; p < GP; ++p) {
+          // even and odd steps in sums of their own: two chains of products half as long
+          float s1[NT][4];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[p][t][e] = s1[t][e] = 0.f;
+#pragma unroll
+          for (int w = 0; w < KS; ++w) {
+            uint32_t a0, a1, a2, a3;
+            i8x4_to_f16x4(kw[p][0][w], a0, a2);
+            i8x4_to_f16x4(kw[p][1][w], a1, a3);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (NT == 1) {
+                mma_16816(w & 1 ? s1[t] : s[p][t], a0, a1, a2, a3, qf[w][0], qf[w][1]);
+              } else {
+                const uint2 b = s_q[(t * KS + w) * 32 + lane];
+                mma_16816(s[p][t], a0, a1, a2, a3, b.x, b.y);
+              }
+            }
           }
-          raise |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kLag || fmaxf(s[t][1], s[t][3]) > m[t][1] + kLag;
+          if constexpr (NT == 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[p][0][e] += s1[0][e];
         }
-        if (__any_sync(0xffffffffu, raise)) {
+        // keys past a row's limit or of a missing page weigh nothing
+        bool none[GP];
+        float vr[GP], sf[GP][NT][2];
+        bool masked = kb + (gi + GP) * 16 > lim_min;
+#pragma unroll
+        for (int p = 0; p < GP; ++p) {
+          none[p] = s_page[gi + p] < 0;
+          masked |= none[p];
+          const float ks = s_ks[gi + p];
+          vr[p] = s_vs[gi + p];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            sf[p][t][0] = rf[t][0] * ks;
+            sf[p][t][1] = rf[t][1] * ks;
+          }
+        }
+        if (more) {
+          find(gi + PA_WARPS * GP);
+          load_k();
+        }
+        // x = s - m, in units of log 2
+        float x[GP][NT][4];
+        float top = 0.f;
+        auto centre = [&]() {
+          top = -INFINITY;
+#pragma unroll
+          for (int p = 0; p < GP; ++p)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[p][t][e] = fmaf(s[p][t][e], sf[p][t][e & 1], -m[t][e & 1]);
+              if (masked) {
+                const int key = kb + (gi + p) * 16 + 4 * (r >> 1) + (r & 1);  // and key + 2
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (none[p] || key + (e & 2) >= lim[t][e & 1]) x[p][t][e] = -INFINITY;
+              }
+              top = max3f(max3f(top, x[p][t][0], x[p][t][1]), x[p][t][2], x[p][t][3]);
+            }
+        };
+        centre();
+        if (__any_sync(0xffffffffu, top > kLag)) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(s[t][e], s[t][e + 2]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-              top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), m[t][e]);
-              const float f = top == m[t][e] ? 1.f : ex2_approx(m[t][e] - top);
-              m[t][e] = top;
+              float top_s = m[t][e];
+#pragma unroll
+              for (int p = 0; p < GP; ++p)
+#pragma unroll
+                for (int i = e; i < 4; i += 2)
+                  if (x[p][t][i] > 0.f) top_s = fmaxf(top_s, s[p][t][i] * sf[p][t][e]);
+              top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 4));
+              top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 8));
+              top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 16));
+              const float f = ex2_approx(m[t][e] - top_s);
+              m[t][e] = top_s;
               l[t][e] *= f;
 #pragma unroll
               for (int i = 0; i < MT; ++i) {
@@ -376,54 +457,61 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
                 o[i][t][e + 2] *= f;
               }
             }
+          centre();
         }
+        uint32_t pb[GP][NT][2], pl[SPLIT ? GP : 1][NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
-          float p[4];
-          p[0] = ex2_approx(s[t][0] - m0);
-          p[1] = ex2_approx(s[t][1] - m1);
-          p[2] = ex2_approx(s[t][2] - m0);
-          p[3] = ex2_approx(s[t][3] - m1);
-          l[t][0] += p[0] + p[2];
-          l[t][1] += p[1] + p[3];
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = masked && s[t][e] == -INFINITY ? 0.f : p[e] * vr;  // 0 even where vr is NaN
+          for (int p = 0; p < GP; ++p) {
+            float y[4];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if constexpr (SPLIT) {
-              const uint32_t hi = pack_bf16x2(p[2 * e], p[2 * e + 1]);
-              const float2 f = unpack_bf16x2(hi);
-              pb[t][e] = movmatrix_trans(hi);
-              pl[t][e] = movmatrix_trans(pack_bf16x2(p[2 * e] - f.x, p[2 * e + 1] - f.y));
-            } else {
-              pb[t][e] = movmatrix_trans(pack_f16x2(p[2 * e], p[2 * e + 1]));
+            for (int e = 0; e < 4; ++e) {
+              y[e] = ex2_approx(x[p][t][e]);
+              l[t][e & 1] += y[e];
+              y[e] *= vr[p];
             }
-          }
-        }
+            if (masked)  // 0 even where the scale is NaN
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-          const uint32_t w[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
+              for (int e = 0; e < 4; ++e)
+                if (x[p][t][e] == -INFINITY) y[e] = 0.f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            if constexpr (SPLIT) {
-              i8x4_to_bf16x4(w[2 * h], a0, a2);
-              i8x4_to_bf16x4(w[2 * h + 1], a1, a3);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
-                mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (SPLIT) {
+                const uint32_t hi = pack_bf16x2(y[2 * e], y[2 * e + 1]);
+                const float2 f = unpack_bf16x2(hi);
+                pb[p][t][e] = movmatrix_trans(hi);
+                pl[p][t][e] = movmatrix_trans(pack_bf16x2(y[2 * e] - f.x, y[2 * e + 1] - f.y));
+              } else {
+                pb[p][t][e] = movmatrix_trans(pack_f16x2(y[2 * e], y[2 * e + 1]));
               }
-            } else {
-              i8x4_to_f16x4(w[2 * h], a0, a2);
-              i8x4_to_f16x4(w[2 * h + 1], a1, a3);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) mma_16816(o[2 * j + h][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
             }
           }
-        }
-        if (more) load_v(gi + PA_WARPS);
+#pragma unroll
+        for (int p = 0; p < GP; ++p)
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) {
+            const uint32_t w[4] = {vw[p][j].x, vw[p][j].y, vw[p][j].z, vw[p][j].w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t a0, a1, a2, a3;
+              if constexpr (SPLIT) {
+                i8x4_to_bf16x4(w[2 * h], a0, a2);
+                i8x4_to_bf16x4(w[2 * h + 1], a1, a3);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
+                  mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pl[p][t][0], pl[p][t][1]);
+                }
+              } else {
+                i8x4_to_f16x4(w[2 * h], a0, a2);
+                i8x4_to_f16x4(w[2 * h + 1], a1, a3);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma_16816(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
+              }
+            }
+          }
+        if (more) load_v();
       }
     }
 
@@ -448,10 +536,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int q8 = 2 * c + e;
-        float top = -INFINITY;
+        float top = kLow;
 #pragma unroll
         for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][t * 8 + q8]);
-        const float f = m[t][e] == -INFINITY ? (m[t][e] == top ? 1.f : 0.f) : ex2_approx(m[t][e] - top);
+        const float f = ex2_approx(m[t][e] - top);
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j)
           *reinterpret_cast<float4*>(&s_o[warp][q8][32 * j + 4 * r]) =
@@ -459,14 +547,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
       }
       __syncthreads();
       const int q8 = tid >> 4, qr = r0 + t * 8 + q8;
-      float top = -INFINITY, sum = 0.f;
+      float top = kLow, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][t * 8 + q8]);
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) {
-        const float mw = s_m[w][t * 8 + q8];
-        sum += s_l[w][t * 8 + q8] * (mw == -INFINITY ? (mw == top ? 1.f : 0.f) : ex2_approx(mw - top));
-      }
+      for (int w = 0; w < PA_WARPS; ++w) sum += s_l[w][t * 8 + q8] * ex2_approx(s_m[w][t * 8 + q8] - top);
       if (qr < R) {
         const long long at = static_cast<long long>(first + qr / G) * a.n_q + g * G + qr % G;
 #pragma unroll
@@ -507,56 +592,51 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 2) attn_paged_kernel
   pdl_trigger();
 }
 
-// Joins the pieces of one query row of a pair that several CTAs worked on, in their order.  CTA (c, i): row i of
-// the pair that began in CTA c and was not finished there.
-constexpr int PJ_PARTS = 4;  // groups of threads over the pieces
+// Joins the pieces of a pair that several CTAs worked on.  CTA (c, i): rows 8i .. 8i + 7 of the pair that began in
+// CTA c and was not finished there.  A thread owns four channels of a row; PJ_PARTS groups of threads take every
+// PJ_PARTS-th piece in turn, and their results are joined in order.
+constexpr int PJ_PARTS = 4;
 template <int HD>
-__global__ void __launch_bounds__(PJ_PARTS * HD) attn_paged_join_kernel(PagedAttnArgs a) {
-  __shared__ float s_o[PJ_PARTS][HD], s_red[2][32];
+__global__ void __launch_bounds__(PJ_PARTS * 2 * HD) attn_paged_join_kernel(PagedAttnArgs a) {
+  __shared__ __align__(16) float s_o[PJ_PARTS][8][HD];
+  __shared__ float2 s_ml[PJ_PARTS][8];
   pdl_wait();
   pdl_trigger();
   const int4 d = a.desc[blockIdx.x];
   if (d.x < 0) return;
-  const int ROWS = gridDim.y, i = blockIdx.y, G = a.group;
-  const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1, qr = d.y * ROWS + i;
-  if (qr >= n * G) return;
+  const int ROWS = 8 * gridDim.y, G = a.group;
+  const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1;
   const int pieces = d.w - static_cast<int>(blockIdx.x) + 1;
-  auto slot = [&](int p) { return (static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + i; };
-  const int tid = threadIdx.x, grp = tid / HD, dim = tid % HD, warp = tid >> 5, lane = tid & 31;
-  float top = -INFINITY;
-  for (int p = tid; p < pieces; p += PJ_PARTS * HD) top = fmaxf(top, a.part_ml[slot(p)].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) s_red[0][warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < PJ_PARTS * HD / 32; ++w) top = fmaxf(top, s_red[0][w]);
-  float sum = 0.f;
-  for (int p = tid; p < pieces; p += PJ_PARTS * HD) {
-    const float2 ml = a.part_ml[slot(p)];
-    sum += ml.y * (ml.x == -INFINITY ? (ml.x == top ? 1.f : 0.f) : ex2_approx(ml.x - top));
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_red[1][warp] = sum;
-  float acc = 0.f;
+  const int grp = threadIdx.x / (2 * HD), q8 = threadIdx.x % (2 * HD) / (HD / 4), dim = threadIdx.x % (HD / 4) * 4;
+  const int i = blockIdx.y * 8 + q8, qr = d.y * ROWS + i;
+  float m = kLow, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto weight = [](float from, float to) { return ex2_approx(from - to); };
+  auto add = [&](float2 ml, float4 x) {
+    const float top = fmaxf(m, ml.x), f = weight(m, top), e = weight(ml.x, top);
+    m = top;
+    l = l * f + ml.y * e;
+    o.x = o.x * f + x.x * e;
+    o.y = o.y * f + x.y * e;
+    o.z = o.z * f + x.z * e;
+    o.w = o.w * f + x.w * e;
+  };
 #pragma unroll 8
   for (int p = grp; p < pieces; p += PJ_PARTS) {
-    const float mp = a.part_ml[slot(p)].x;
-    acc += a.part_o[slot(p) * HD + dim] * (mp == -INFINITY ? (mp == top ? 1.f : 0.f) : ex2_approx(mp - top));
+    const size_t at = (static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + i;
+    add(a.part_ml[at], *reinterpret_cast<const float4*>(a.part_o + at * HD + dim));
   }
-  s_o[grp][dim] = acc;
+  *reinterpret_cast<float4*>(&s_o[grp][q8][dim]) = o;
+  if (dim == 0) s_ml[grp][q8] = make_float2(m, l);
   __syncthreads();
-  sum = 0.f;
+  if (grp || qr >= n * G) return;
 #pragma unroll
-  for (int w = 0; w < PJ_PARTS * HD / 32; ++w) sum += s_red[1][w];
+  for (int p = 1; p < PJ_PARTS; ++p) add(s_ml[p][q8], *reinterpret_cast<const float4*>(&s_o[p][q8][dim]));
   const long long at = static_cast<long long>(first + qr / G) * a.n_q + d.z * G + qr % G;
-  if (grp == 0) {
-#pragma unroll
-    for (int p = 1; p < PJ_PARTS; ++p) acc += s_o[p][dim];
-    a.out[at * HD + dim] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
-  }
-  if (tid == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.693147180559945f;
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(a.out + at * HD + dim) =
+      make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
+  if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
 }
 
 }  // namespace mk

@@ -45,7 +45,7 @@ mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int 
 
 // Launch shape and workspace of the paged attention.  Query rows (tokens times heads of a group) per tile: 8, 16
 // or 32, the smallest that holds a row's queries; a wider tile reads and converts the cache less often but
-// leaves room for two CTAs per SM instead of four.  One wave of CTAs on 148 SMs, fewer when the bounds say that
+// leaves room for two CTAs per SM instead of three.  One wave of CTAs on 148 SMs, fewer when the bounds say that
 // there are fewer units of work.
 struct PagedPlan {
   int nt, ctas;
@@ -56,8 +56,9 @@ PagedPlan paged_plan(int group, int n_kv, int hd, int rows, int max_q, int max_l
   const int64_t q_rows = static_cast<int64_t>(std::max(max_q, 1)) * group;
   p.nt = q_rows <= 8 ? 1 : q_rows <= 16 ? 2 : 4;
   const int64_t tiles = (q_rows + 8 * p.nt - 1) / (8 * p.nt);
-  const int64_t per_pair = std::max(1, max_len / mk::PA_UNIT + (max_len % mk::PA_UNIT != 0));
-  const int64_t most = 148 * (p.nt == 1 ? 4 : 2);
+  const int unit = mk::pa_unit(p.nt);
+  const int64_t per_pair = std::max(1, max_len / unit + (max_len % unit != 0));
+  const int64_t most = 148 * mk::pa_ctas_per_sm(p.nt);
   // (each factor is below 2^31: cut before the product can overflow)
   const int64_t pairs = std::min<int64_t>(most, static_cast<int64_t>(rows) * n_kv) * std::min<int64_t>(most, tiles);
   p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min(most, pairs) * per_pair)));
@@ -85,11 +86,16 @@ mk_status mk_kv_append(const void* k, const void* v, int64_t ld_k, int64_t head_
   if (static_cast<int64_t>(rows) * touched > INT_MAX || n_kv > 65535) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
-  return launch_k(mk::kv_append_kernel, dim3(rows * touched, 2, n_kv), dim3(mk::KVA_THREADS), 0,
-                  static_cast<cudaStream_t>(stream), true, static_cast<const __nv_bfloat16*>(k),
-                  static_cast<const __nv_bfloat16*>(v), static_cast<long long>(ld_k), static_cast<long long>(head_ld_k),
-                  static_cast<long long>(ld_v), static_cast<long long>(head_ld_v), T, c, block_table, width, lens, cu_new,
-                  touched, d.err);
+  using Kernel = decltype(&mk::kv_append_kernel<96, 4>);
+  static const Kernel kernels[2][4] = {
+      {mk::kv_append_kernel<96, 4>, mk::kv_append_kernel<96, 5>, mk::kv_append_kernel<96, 6>, mk::kv_append_kernel<96, 7>},
+      {mk::kv_append_kernel<128, 4>, mk::kv_append_kernel<128, 5>, mk::kv_append_kernel<128, 6>,
+       mk::kv_append_kernel<128, 7>}};
+  return launch_k(kernels[head_dim == 128][c.page_shift - 4], dim3(rows * touched, 2, n_kv),
+                  dim3(mk::kva_threads(head_dim, c.page_shift)), 0, static_cast<cudaStream_t>(stream), true,
+                  static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v),
+                  static_cast<long long>(ld_k), static_cast<long long>(head_ld_k), static_cast<long long>(ld_v),
+                  static_cast<long long>(head_ld_v), T, c, block_table, width, lens, cu_new, touched, d.err);
 }
 
 mk_status mk_kv_read(const void* codes, const float* scales, int32_t num_pages, int32_t n_kv, int32_t page_size,
@@ -165,8 +171,8 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
                                                                               : mk::attn_paged_kernel<128, 4>);
   MK_TRY(launch_k(k, dim3(p.ctas), dim3(mk::PA_THREADS), 0, st, true, c, a));
   if (head_dim == 96)
-    return launch_k(mk::attn_paged_join_kernel<96>, dim3(p.ctas, 8 * p.nt), dim3(mk::PJ_PARTS * 96), 0, st, true, a);
-  return launch_k(mk::attn_paged_join_kernel<128>, dim3(p.ctas, 8 * p.nt), dim3(mk::PJ_PARTS * 128), 0, st, true, a);
+    return launch_k(mk::attn_paged_join_kernel<96>, dim3(p.ctas, p.nt), dim3(mk::PJ_PARTS * 2 * 96), 0, st, true, a);
+  return launch_k(mk::attn_paged_join_kernel<128>, dim3(p.ctas, p.nt), dim3(mk::PJ_PARTS * 2 * 128), 0, st, true, a);
 }
 
 size_t mk_kv_move_workspace(int32_t rows, int32_t num_pages) {

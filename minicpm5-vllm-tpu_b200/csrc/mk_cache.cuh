@@ -45,6 +45,35 @@ __device__ __forceinline__ int quant1(float x, float s) {
   return max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))));
 }
 
+// The same for eight values at once without a division: t = x * (1 / s) + 1.5 * 2^23 is the nearest integer (ties
+// to even) to within the product's rounding, in the low bits of t.  The quotient and the product differ by less
+// than 2^-22 of 127, so the integers can differ only where the product lies within 2^-14 of a tie; there (one
+// vector in 500 or so) the quotients are taken.  s >= max|x| / 127 up to a rounding, so no integer passes 127.
+__device__ __forceinline__ void quant8(const uint4& x, float inv, float s, uint32_t (&t)[8]) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  float f[8], off = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 p = unpack_bf16x2(u[e]);
+    f[2 * e] = p.x;
+    f[2 * e + 1] = p.y;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = fmaf(f[e], inv, kMagic);
+    off = fmaxf(off, fabsf(fmaf(f[e], inv, kMagic - y)));
+    t[e] = __float_as_uint(y);
+  }
+  if (!(off < 0.5f - 0x1p-14f))
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = static_cast<uint32_t>(quant1(f[e], s));
+}
+// the low bytes of four words as one word
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 // ---------------------------------------------------------------------------------- append
 // New tokens of each row, quantised into the pages that hold positions lens[r] .. lens[r] + n - 1.
 //
@@ -58,30 +87,37 @@ __device__ __forceinline__ int quant1(float x, float s) {
 // Bounds: 2 bytes read and 1 written per element.  One CTA owns one (page, plane, head), so the scale has one
 // writer and nothing is atomic.  A thread's item is 4 tokens x 8 channels: four 16-byte loads, and 32
 // contiguous bytes of the value plane or four 8-byte pieces of the key plane.  The items stay in registers
-// between the maximum and the rounding, so the input is read once.
-constexpr int KVA_THREADS = 256;
-constexpr int KVA_ITEMS = 2;  // 4 x 8 items per thread: 128 tokens x 128 channels
+// between the maximum and the rounding, so the input is read once.  A CTA has a thread for each item, for 128-token
+// pages one for two.
+__host__ __device__ constexpr int kva_items(int page_shift) { return page_shift == 7 ? 2 : 1; }
+__host__ __device__ constexpr int kva_threads(int hd, int page_shift) {
+  return (((1 << page_shift) / 4 * (hd / 8)) / kva_items(page_shift) + 31) / 32 * 32;
+}
 
-__global__ void __launch_bounds__(KVA_THREADS)
+template <int HD, int SHIFT>
+__global__ void __launch_bounds__(kva_threads(HD, SHIFT))
     kv_append_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long ld_k,
                      long long hs_k, long long ld_v, long long hs_v, int T, KvPages c, const int32_t* __restrict__ table,
                      int width, const int32_t* __restrict__ lens, const int32_t* __restrict__ cu, int touched, int* err) {
-  __shared__ uint32_t red[KVA_THREADS / 32];
+  constexpr int KVA_ITEMS = kva_items(SHIFT), THREADS = kva_threads(HD, SHIFT), hd = HD, chunks = HD / 8;
+  constexpr int items = (1 << SHIFT) / 4 * chunks, per = items / KVA_ITEMS;  // per: threads with an item
+  __shared__ uint32_t red[THREADS / 32];
   pdl_wait();
   pdl_trigger();
   const int row = blockIdx.x / touched, plane = blockIdx.y, head = blockIdx.z;
   const int tok0 = cu ? cu[row] : row, n = cu ? cu[row + 1] - tok0 : 1;
-  const int len = lens[row], page_tokens = 1 << c.page_shift;
+  const int len = lens[row];
   if (n <= 0 || len < 0 || tok0 < 0 || tok0 + n > T) return;
-  const int slot = (len >> c.page_shift) + blockIdx.x % touched;
-  const int pos0 = slot << c.page_shift;
+  const int slot = (len >> SHIFT) + blockIdx.x % touched;
+  const int pos0 = slot << SHIFT;
   if (pos0 >= len + n) return;
   const int page = kv_page_of(table, width, c.num_pages, row, slot, err);
   if (page < 0) return;
-  const int hd = c.head_dim, chunks = hd >> 3, items = (page_tokens >> 2) * chunks;
-  const __nv_bfloat16* src = plane ? v : k;
   const long long ld = plane ? ld_v : ld_k;
-  src += head * (plane ? hs_v : hs_k);
+  // (the row of position 0 would be: positions before the new tokens are never read)
+  const __nv_bfloat16* src = (plane ? v : k) + head * (plane ? hs_v : hs_k) + static_cast<long long>(tok0 - len) * ld;
+  const int g0 = threadIdx.x / chunks, ch = threadIdx.x % chunks;
+  const bool mine = threadIdx.x < per;
   int8_t* dst = kv_head_ptr(c, page, plane, head);
   float* sp = kv_scale_ptr(c, page, plane, head);
   const bool had = pos0 < len;
@@ -91,13 +127,13 @@ __global__ void __launch_bounds__(KVA_THREADS)
   uint32_t top = 0;  // largest |x| as bf16 bits, two halves
 #pragma unroll
   for (int i = 0; i < KVA_ITEMS; ++i) {
-    const int it = threadIdx.x + i * KVA_THREADS, g = it / chunks, ch = it - g * chunks;
+    const int g = g0 + i * (per / chunks);
+    const __nv_bfloat16* at = src + static_cast<long long>(pos0 + 4 * g) * ld + ch * 8;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int pos = pos0 + 4 * g + t;
       x[i][t] = make_uint4(0, 0, 0, 0);
-      if (it < items && pos >= len && pos < len + n)
-        x[i][t] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(tok0 + pos - len) * ld + ch * 8));
+      if (mine && pos >= len && pos < len + n) x[i][t] = __ldg(reinterpret_cast<const uint4*>(at + t * ld));
       const uint32_t a = __vmaxu2(x[i][t].x & 0x7fff7fffu, x[i][t].y & 0x7fff7fffu);
       const uint32_t b = __vmaxu2(x[i][t].z & 0x7fff7fffu, x[i][t].w & 0x7fff7fffu);
       top = __vmaxu2(top, __vmaxu2(a, b));
@@ -108,7 +144,7 @@ __global__ void __launch_bounds__(KVA_THREADS)
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-  for (int w = 0; w < KVA_THREADS / 32; ++w) top = max(top, red[w]);
+  for (int w = 0; w < THREADS / 32; ++w) top = max(top, red[w]);
   // 0x7f80 and above are infinity and NaN
   const float amax = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __uint_as_float(top << 16);
   const float fresh = __fdiv_rn(amax, kCodeMax);
@@ -117,15 +153,37 @@ __global__ void __launch_bounds__(KVA_THREADS)
   const float by = finite && now > 0.f ? now : 1.f;
   const bool again = had && now != was;  // the tokens already there change their codes
   if (threadIdx.x == 0) *sp = now;
+  const float inv = __frcp_rn(by);
+  // (a scale so small that its reciprocal is infinite takes the divisions below)
+  const bool fast = finite && inv <= 3.4e38f;
 
 #pragma unroll
   for (int i = 0; i < KVA_ITEMS; ++i) {
-    const int it = threadIdx.x + i * KVA_THREADS, g = it / chunks, ch = it - g * chunks;
-    if (it >= items) continue;
+    const int g = g0 + i * (per / chunks);
+    if (!mine) continue;
     const int pos = pos0 + 4 * g;
     // tokens of this group: [0, o) were there, [o, m) are new, [m, 4) are past the end
     const int o = min(4, max(0, len - pos)), m = min(4, max(0, len + n - pos));
     if (m == o && !(again && o > 0)) continue;
+    if (fast && o == 0 && m == 4) {  // four new tokens: nothing of the page's bytes is read
+      uint32_t t[4][8];
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) quant8(x[i][k4], inv, by, t[k4]);
+      if (plane) {
+        uint32_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = low_bytes(t[0][e], t[1][e], t[2][e], t[3][e]);
+        uint4* p = reinterpret_cast<uint4*>(dst + (static_cast<size_t>(g) * hd + ch * 8) * 4);
+        p[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        p[1] = make_uint4(u[4], u[5], u[6], u[7]);
+      } else {
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4)
+          *reinterpret_cast<uint2*>(dst + static_cast<size_t>(4 * g + k4) * hd + ch * 8) =
+              make_uint2(low_bytes(t[k4][0], t[k4][1], t[k4][2], t[k4][3]), low_bytes(t[k4][4], t[k4][5], t[k4][6], t[k4][7]));
+      }
+      continue;
+    }
     uint32_t w[4][2];  // [token][8 codes]
     if (o > 0 || (plane && m < 4)) {  // bytes that stay or are rescaled
       if (plane) {

@@ -141,7 +141,8 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   const int64_t tok_tiles = (static_cast<int64_t>(T) + tok_tile - 1) / tok_tile, ids = id_tiles(T, V);
   if (tok_tiles * ids > INT_MAX / 2) return MK_ERR_TOO_LARGE;
   CUtensorMap mh, mw;
-  MK_TRY(map_rows(d, &mh, h, T, H, ld, mk::SC_M));
+  const int rows = pair ? mk::SC_M : (T + 7) / 8 * 8;
+  MK_TRY(map_rows(d, &mh, h, T, H, ld, rows));
   MK_TRY(map_rows(d, &mw, lm_head, V, H, H, mk::SC_B_ROWS));
   mk::ScoreArgs a;
   a.T = T;
@@ -149,6 +150,7 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   a.V = V;
   a.id_tiles = static_cast<int>(ids);
   a.tok_tiles = static_cast<int>(tok_tiles);
+  a.rows = rows;
   a.targets = targets;
   a.scale = static_cast<float>(logit_scale * 1.4426950408889634 * (1.0 + mk::kTruncPerStep * ((H + 15) / 16)));
   a.part = static_cast<float*>(workspace);

@@ -45,14 +45,6 @@ __device__ __forceinline__ RowStats stats_warp(RowStats s) {
   return s;
 }
 
-// (d0, d1) += (a0, a1) * (b0, b1) in one packed f32x2 FMA.
-__device__ __forceinline__ void fma2_pair(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 x, y, z;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
-      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "+f"(d0), "+f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
 // A 16-byte load of bytes that are read once.
 __device__ __forceinline__ uint4 ldg_once(const uint4* p) {
   uint4 v;
@@ -77,23 +69,24 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 // One pass over the logits: statistics, rank and alternatives together.  A cluster of CTAs shares a row (one CTA
 // where there are rows enough), each with a slice of it.
 //
-// Alternatives.  An entry can only be among the k largest if it reaches tau, any value that k entries of the
-// slice reach.  The threads form 64 groups; the k-th largest of the groups' running maxima is such a value.  It is
-// taken after the first 8192 logits, again whenever as many more have been seen, and at the end; logits that
-// reach the current tau go into a list in shared memory (a few per doubling and alternative), and those that
-// reach the last one are put in order by counting.  Rows that defeat it (more than TL_CAP entries listed: long
-// runs of equal or rising logits; fewer than k logits above -inf) fall back to one search of the slice for
-// each alternative that is missing.
+// Alternatives.  An entry can only be among the k largest if it reaches tau, any value that k entries reach.  A
+// warp's lanes keep the maxima of two halves of what they have seen, and the k-th largest of the 64 is such a value;
+// it is taken after the first 1024 logits of the warp, again when four times as many have been seen, and so on,
+// and the largest that any warp of the CTA has published serves them all.  16-byte vectors that hold a logit
+// that reaches it go into a list in shared memory; at the end their logits are cut to what reaches the last tau
+// and put in order by counting.  No warp waits for another before the end.  Rows that defeat it (long runs of
+// equal or rising logits that fill the list; fewer than k logits above -inf) fall back to one search of the slice
+// for each alternative missing.
 //
 // What bounds it: the bytes of the logits.  Per bf16 logit the arithmetic is about six instructions and one
 // exponential, two thirds of what an SM can issue at the rate at which HBM delivers them.
 constexpr int TL_THREADS = 256;
 constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
-constexpr int TL_GROUPS = 64;     // of TL_THREADS / TL_GROUPS neighbouring lanes
-constexpr int TL_CAP = 2048;      // list entries
+constexpr int TL_LIST = 1024;     // vectors listed
+constexpr int TL_CAP = 2048;      // logits put in order
 constexpr int TL_CLUSTER_MAX = 8;
-static_assert(TL_TOPK_MAX <= TL_GROUPS && TL_CLUSTER_MAX * TL_TOPK_MAX <= TL_CAP, "alternatives");
+static_assert(TL_TOPK_MAX <= 64 && TL_CLUSTER_MAX * TL_TOPK_MAX <= TL_CAP, "alternatives");
 
 __device__ __forceinline__ float order_value(unsigned long long e) {
   const uint32_t k = static_cast<uint32_t>(e >> 32);
@@ -131,9 +124,11 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
   constexpr int EPV = 16 / sizeof(E);            // logits per 16-byte vector
   constexpr int VECS = TL_VALUES / EPV;          // vectors per thread and step
   constexpr uint32_t kNone = BF ? 0xff80ff80u : 0xff800000u;  // -inf
-  __shared__ unsigned long long s_list[TL_CAP], s_kept[TL_CAP], s_top[TL_TOPK_MAX];
+  __shared__ uint4 s_vec[TL_LIST];
+  __shared__ int s_id[TL_LIST];
+  __shared__ unsigned long long s_kept[TL_CAP], s_top[TL_TOPK_MAX];
   __shared__ unsigned long long s_pick[TL_THREADS / 32];
-  __shared__ float s_gm[TL_GROUPS], s_tau;
+  __shared__ volatile float s_tau[TL_THREADS / 32];
   __shared__ int s_n, s_kept_n, s_have;
   __shared__ RowStats s_st[TL_THREADS / 32];
   __shared__ int s_above[TL_THREADS / 32];
@@ -156,35 +151,30 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
   const uint4* vecs = reinterpret_cast<const uint4*>(row + head);
 
   RowStats st = stats_empty();
-  float top = -INFINITY, tau = -INFINITY;
+  float top = -INFINITY, top1 = -INFINITY, tau = -INFINITY;  // maxima of the even and odd vectors
   int above = 0;
   if (tid == 0) s_n = s_kept_n = 0;
+  if (lane == 0) s_tau[wp] = -INFINITY;
   __syncthreads();
-  auto list = [&](float x, int id) {
-    if (x >= tau && x > -INFINITY) {
-      const int at = atomicAdd(&s_n, 1);
-      if (at < TL_CAP) s_list[at] = order_entry(order_key(x), id);
+  auto list = [&](const uint4& v, int id) {
+    const int at = atomicAdd(&s_n, 1);
+    if (at < TL_LIST) {
+      s_vec[at] = v;
+      s_id[at] = id;
     }
   };
-  // tau from the groups' maxima (every thread calls it)
+  // the warp's tau: one maximum is struck out per round, the lowest lane's among equals
   auto threshold = [&]() {
-    float g = top;
-#pragma unroll
-    for (int o = 1; o < TL_THREADS / TL_GROUPS; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (tid % (TL_THREADS / TL_GROUPS) == 0) s_gm[tid / (TL_THREADS / TL_GROUPS)] = g;
-    __syncthreads();
-    if (tid < TL_GROUPS) {
-      const float mineg = s_gm[tid];
-      int r = 0;
-#pragma unroll 8
-      for (int j = 0; j < TL_GROUPS; ++j) {
-        const float o = s_gm[j];
-        r += o > mineg || (o == mineg && j < tid);
+    uint32_t hi = order_key(fmaxf(top, top1)), lo = order_key(fminf(top, top1)), last = 0;
+    for (int r = 0; r < k; ++r) {
+      last = __reduce_max_sync(0xffffffffu, hi);
+      const uint32_t with = __ballot_sync(0xffffffffu, hi == last);
+      if (lane == __ffs(with) - 1) {
+        hi = lo;
+        lo = 0;
       }
-      if (r == k - 1) s_tau = mineg;
     }
-    __syncthreads();
-    tau = s_tau;
+    tau = last == 0 ? -INFINITY : __uint_as_float(last & 0x80000000u ? last & 0x7fffffffu : ~last);
   };
 
   // a loose logit of the head or tail: at most one per thread
@@ -200,14 +190,19 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
   }
 
   const int steps = max(1, (vec1 - vec0 + TL_THREADS * VECS - 1) / (TL_THREADS * VECS));
-  for (int step = 0; step < steps; ++step) {
-    uint4 x[VECS];
-    const int v0 = vec0 + step * TL_THREADS * VECS + tid;
+  uint4 x[VECS];
+  auto load = [&](int step) {
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
+      const int at = vec0 + (step * VECS + v) * TL_THREADS + tid;
       x[v] = make_uint4(kNone, kNone, kNone, kNone);
-      if (v0 + v * TL_THREADS < vec1) x[v] = ldg_once(vecs + v0 + v * TL_THREADS);
+      if (at < vec1) x[v] = ldg_once(vecs + at);
     }
+  };
+  load(0);
+  int retake = 0;  // the step after which tau is taken next
+  for (int step = 0; step < steps; ++step) {
+    const int v0 = vec0 + step * TL_THREADS * VECS + tid;
     auto words = [&](int v, int w) { return w == 0 ? x[v].x : w == 1 ? x[v].y : w == 2 ? x[v].z : x[v].w; };
     float vm[VECS], most = st.m;
     // maxima of the vectors
@@ -225,8 +220,11 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
                       __uint_as_float(x[v].w));
       }
       most = fmaxf(most, vm[v]);
+      if (v & 1)
+        top1 = fmaxf(top1, vm[v]);
+      else
+        top = fmaxf(top, vm[v]);
     }
-    top = fmaxf(top, most);
     // statistics
     const float ref = most == -INFINITY ? 0.f : most;
     {
@@ -235,63 +233,65 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
       st.z *= f;
       st.m = most;
     }
+    // y = (x - ref) log2 e as one FMA: 2^y is off by the rounding of ref log2 e, which the sums make good.  Where
+    // that product could overflow (logits beyond 1e38) the difference is taken first.
+    const float rl = ref * kLog2E, rest = fmaf(ref, kLog2E, -rl);
+    const bool far = !(fabsf(ref) < 1e38f);
     float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
-    auto two = [&](float p, float q) {
-      float up = p, uq = q;
-      add2_acc(up, uq, -ref, -ref);
-      const float ep = ex2_approx(up * kLog2E), eq = ex2_approx(uq * kLog2E);
-      add2_acc(z0, z1, ep, eq);
-      up = fmaxf(up, kFar);
-      uq = fmaxf(uq, kFar);
-      fma2_pair(w0, w1, ep, eq, up, uq);
+    auto add = [&](float x, float& z, float& w) {
+      const float y = far ? (x - ref) * kLog2E : fmaf(x, kLog2E, -rl), e = ex2_approx(y);
+      z += e;
+      w = fmaf(e, fmaxf(y, kFar), w);
     };
-    if constexpr (BF) {
-      const __nv_bfloat162 m2 = __float2bfloat162_rn(mine);
-      __nv_bfloat162 cnt = __float2bfloat162_rn(0.f);
+    auto all = [&]() {
+      if constexpr (BF) {
+        const __nv_bfloat162 m2 = __float2bfloat162_rn(mine);
+        __nv_bfloat162 cnt = __float2bfloat162_rn(0.f);
 #pragma unroll
-      for (int v = 0; v < VECS; ++v)
+        for (int v = 0; v < VECS; ++v)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t u = words(v, w);
-          const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&u);
-          cnt = __hadd2(cnt, __hgt2(h, m2));  // at most VECS * 4 in each half: exact
-          const float2 f = unpack_bf16x2(u);
-          two(f.x, f.y);
-        }
-      above += static_cast<int>(__low2float(cnt)) + static_cast<int>(__high2float(cnt));
-    } else {
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t u = words(v, w);
+            const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&u);
+            cnt = __hadd2(cnt, __hgt2(h, m2));  // at most VECS * 4 in each half: exact
+            add(__uint_as_float(u << 16), z0, w0);
+            add(__uint_as_float(u & 0xffff0000u), z1, w1);
+          }
+        above += static_cast<int>(__low2float(cnt)) + static_cast<int>(__high2float(cnt));
+      } else {
 #pragma unroll
-      for (int v = 0; v < VECS; ++v)
+        for (int v = 0; v < VECS; ++v)
 #pragma unroll
-        for (int w = 0; w < 4; w += 2) {
-          const float p = __uint_as_float(words(v, w)), q = __uint_as_float(words(v, w + 1));
-          above += (p > mine) + (q > mine);
-          two(p, q);
-        }
-    }
-    st.z += z0 + z1;
-    st.w += w0 + w1;
+          for (int w = 0; w < 4; w += 2) {
+            const float p = __uint_as_float(words(v, w)), q = __uint_as_float(words(v, w + 1));
+            above += (p > mine) + (q > mine);
+            add(p, z0, w0);
+            add(q, z1, w1);
+          }
+      }
+    };
+    if (far) all(); else all();
+    const float back = far ? 1.f : fmaf(-rest, kLn2, 1.f);
+    st.z = fmaf(z0 + z1, back, st.z);
+    st.w = fmaf((w0 + w1) * kLn2, back, st.w);
     if (k > 0) {
-      if ((step & (step - 1)) == 0) {  // after 1, 2, 3, 5, 9, ... steps
+      if (step == retake) {
         threshold();
-        if (step == 0 && loose >= 0) list(loose_x, loose);
+        if (lane == 0) s_tau[wp] = tau;
+        retake = step * 4 + 3;
+      }
+#pragma unroll
+      for (int i = 0; i < TL_THREADS / 32; ++i) tau = fmaxf(tau, s_tau[i]);
+      if (step == 0 && loose_x >= tau && loose_x > -INFINITY) {  // as the first logit of a vector
+        uint32_t first = __float_as_uint(loose_x);
+        if (BF) first = first >> 16 | 0xff800000u;
+        list(make_uint4(first, kNone, kNone, kNone), loose);
       }
 #pragma unroll
       for (int v = 0; v < VECS; ++v)
-        if (vm[v] >= tau) {
-          const int id = head + (v0 + v * TL_THREADS) * EPV;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if constexpr (BF) {
-              const float2 f = unpack_bf16x2(words(v, w));
-              list(f.x, id + 2 * w);
-              list(f.y, id + 2 * w + 1);
-            } else {
-              list(__uint_as_float(words(v, w)), id + w);
-            }
-          }
-        }
+        if (vm[v] >= tau && vm[v] > -INFINITY) list(x[v], head + (v0 + v * TL_THREADS) * EPV);
     }
+    if (step + 1 < steps) load(step + 1);
   }
 
   // this CTA's statistics
@@ -301,8 +301,7 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
     s_st[wp] = st;
     s_above[wp] = above;
   }
-  if (k > 0) threshold();  // (a barrier; the list is complete)
-  __syncthreads();
+  __syncthreads();  // the list is complete
   if (tid == 0) {
     for (int i = 1; i < TL_THREADS / 32; ++i) {
       st = stats_join(st, s_st[i]);
@@ -318,13 +317,22 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
   const int want = min(k, hi - lo);
   if (k > 0) {
     const int n = s_n;
-    if (n <= TL_CAP) {
-      const unsigned long long least = order_entry(order_key(tau), -1);  // any entry of value tau or more is >=
-      for (int i = tid; i < n; i += TL_THREADS)
-        if (s_list[i] >= least) s_kept[atomicAdd(&s_kept_n, 1)] = s_list[i];
+    if (n <= TL_LIST) {
+      threshold();  // of all that each warp has seen; the largest of the warps' serves the CTA
+      if (lane == 0) s_tau[wp] = tau;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < TL_THREADS / 32; ++i) tau = fmaxf(tau, s_tau[i]);
+      for (int i = tid; i < n * EPV; i += TL_THREADS) {
+        const float f = logit_at(reinterpret_cast<const E*>(s_vec), i);
+        if (f >= tau && f > -INFINITY) {
+          const int at = atomicAdd(&s_kept_n, 1);
+          if (at < TL_CAP) s_kept[at] = order_entry(order_key(f), s_id[i / EPV] + i % EPV);
+        }
+      }
     }
     __syncthreads();
-    const int kept = s_kept_n;
+    const int kept = s_kept_n <= TL_CAP ? s_kept_n : 0;
     for (int i = tid; i < kept; i += TL_THREADS) {
       const unsigned long long e = s_kept[i];
       int r = 0;
@@ -385,15 +393,15 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
     }
     const int all = cluster * k;
     if (cluster > 1) {
-      for (int i = tid; i < all; i += TL_THREADS) s_list[i] = ld_cluster_u64(&s_top[i % k], i / k);
+      for (int i = tid; i < all; i += TL_THREADS) s_kept[i] = ld_cluster_u64(&s_top[i % k], i / k);
       __syncthreads();
     }
     for (int i = tid; i < all; i += TL_THREADS) {
-      const unsigned long long e = cluster > 1 ? s_list[i] : s_top[i];
+      const unsigned long long e = cluster > 1 ? s_kept[i] : s_top[i];
       int r = i;
       if (cluster > 1) {
         r = 0;
-        for (int j = 0; j < all; ++j) r += s_list[j] > e;
+        for (int j = 0; j < all; ++j) r += s_kept[j] > e;
       }
       if (r < k && e) {
         a.top_ids[b * k + r] = order_id(e);
@@ -423,13 +431,24 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
 //   warp 1     TMEM allocator and MMA issuer (the even CTA's, for both of a pair)
 //   warps 2-5  epilogue, one per 32-lane quarter of TMEM
 constexpr int SC_M = 128;      // tokens per CTA
-constexpr int SC_K = 64;       // of H per stage
+constexpr int SC_K = 64;       // of H per stage (one 128-byte swizzle row)
 constexpr int SC_THREADS = 192;
 constexpr uint32_t SC_A_BYTES = SC_M * SC_K * 2;
 constexpr int SC_B_ROWS = 128;  // ids that a CTA loads per tile
-constexpr int SC_STAGES = 6;
-constexpr uint32_t SC_STAGE_BYTES = SC_A_BYTES + SC_B_ROWS * SC_K * 2;
-constexpr size_t SC_SMEM_BYTES = 1024 + SC_STAGES * SC_STAGE_BYTES + 256;
+constexpr uint32_t SC_B_BYTES = SC_B_ROWS * SC_K * 2;
+constexpr int SC_STAGES = 6;        // of full token tiles
+constexpr int SC_STAGES_MAX = 11;   // of the smallest
+constexpr uint32_t SC_RING_BYTES = SC_STAGES * (SC_A_BYTES + SC_B_BYTES);
+constexpr size_t SC_SMEM_BYTES = 1024 + SC_RING_BYTES + 256;
+// With few tokens only their rows (a multiple of 8) are loaded, and the room goes to more stages of W: what is in
+// flight of W is what keeps HBM busy.  The MMA reads 128 token rows all the same; the rows after the last come
+// from whatever lies there, and so do their logits, which nobody reads.
+__host__ __device__ constexpr int sc_stages(int rows) {
+  return static_cast<int>(SC_RING_BYTES / (rows * SC_K * 2 + SC_B_BYTES)) < SC_STAGES_MAX
+             ? static_cast<int>(SC_RING_BYTES / (rows * SC_K * 2 + SC_B_BYTES))
+             : SC_STAGES_MAX;
+}
+static_assert(sc_stages(SC_M) == SC_STAGES && SC_B_BYTES + 8 * SC_K * 2 >= SC_A_BYTES, "a token tile read past its rows stays in its stage");
 __host__ __device__ constexpr int sc_ids(bool pair) { return pair ? 2 * SC_B_ROWS : SC_B_ROWS; }  // ids per tile
 
 // The tensor cores' f32 accumulator rounds toward zero: of sums of products of either sign a step of 16 loses
@@ -440,6 +459,7 @@ constexpr double kTruncPerStep = 0.26 / (1 << 24);
 
 struct ScoreArgs {
   int T, H, V, id_tiles, tok_tiles;
+  int rows;             // token rows that a CTA loads per tile
   const int32_t* targets;
   float scale;          // logit scale * log2 e: the statistics are in units of log 2
   float* part;          // [id tiles][3][ld_part]: m, z, w
@@ -452,14 +472,15 @@ template <bool PAIR>
 __global__ void __launch_bounds__(SC_THREADS, 1)
     score_tokens_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
                         const ScoreArgs args) {
-  constexpr int STAGES = SC_STAGES, SC_V = sc_ids(PAIR);
-  constexpr uint32_t STAGE = SC_STAGE_BYTES;
+  constexpr int SC_V = sc_ids(PAIR);
+  const int STAGES = PAIR ? SC_STAGES : sc_stages(args.rows);
+  const uint32_t A_BYTES = PAIR ? SC_A_BYTES : args.rows * SC_K * 2, STAGE = A_BYTES + SC_B_BYTES;
   extern __shared__ uint8_t sc_smem_raw[];
   const uint32_t raw = smem_u32(sc_smem_raw);
   uint8_t* base = sc_smem_raw + (((raw + 1023u) & ~1023u) - raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(base + STAGES * STAGE);  // [STAGES] both operands landed
-  uint64_t* empty = full + STAGES;   // [STAGES] the MMAs that read the stage finished
-  uint64_t* tfull = empty + STAGES;  // [2] accumulator ready
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + SC_RING_BYTES);  // [STAGES] both operands landed
+  uint64_t* empty = full + SC_STAGES_MAX;  // [STAGES] the MMAs that read the stage finished
+  uint64_t* tfull = empty + SC_STAGES_MAX;  // [2] accumulator ready
   uint64_t* tempty = tfull + 2;      // [2] accumulator drained
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -512,14 +533,12 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
   if (warp == 0) {
     const bool leader = elect_one();
     pdl_wait();
-    uint32_t issued = 0, issued_par = 0;
-    int idx = 0;
+    uint32_t issued = 0, issued_par = 0, ph = 0;
+    int s = 0;
     bool ok = true;
     for (int it = 0; ok && it < my_tiles; ++it) {
       const int t0 = tok0(it), v0 = id_tile(it) * SC_V + static_cast<int>(crank) * SC_B_ROWS;
-      for (int kt = 0; kt < KT; ++kt, ++idx) {
-        const int s = idx % STAGES;
-        const uint32_t ph = (idx / STAGES) & 1;
+      for (int kt = 0; kt < KT; ++kt) {
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ph ^ 1u, abort_flag));
         if (!ok) break;
         if (leader) {
@@ -528,16 +547,20 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
             if (crank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE);
             const uint32_t fb = lead_bar(&full[s]);
             tma_load_2d_pair(at, &tmH, fb, kt * SC_K, t0);
-            tma_load_2d_pair(at + SC_A_BYTES, &tmW, fb, kt * SC_K, v0);
+            tma_load_2d_pair(at + A_BYTES, &tmW, fb, kt * SC_K, v0);
           } else {
             mbar_arrive_expect_tx(&full[s], STAGE);
+            tma_load_2d(at + A_BYTES, &tmW, &full[s], kt * SC_K, v0);
             tma_load_2d(at, &tmH, &full[s], kt * SC_K, t0);
-            tma_load_2d(at + SC_A_BYTES, &tmW, &full[s], kt * SC_K, v0);
           }
         }
         __syncwarp();
         issued |= 1u << s;
         issued_par = (issued_par & ~(1u << s)) | (ph << s);
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
       }
     }
     // every issued copy lands before the CTA may exit (a pair's on the even CTA's barriers)
@@ -556,21 +579,21 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
           mma_commit(b);
         }
       };
-      int idx = 0;
+      int s = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (int it = 0; ok && it < my_tiles; ++it) {
         const int a = it & 1;
         if (!__all_sync(0xffffffffu, mbar_wait(&tempty[a], ((it >> 1) & 1) ^ 1u, abort_flag))) break;
         tc_fence_after();
         const uint32_t d = tmem_base + a * SC_V;
-        for (int kt = 0; kt < KT; ++kt, ++idx) {
-          const int s = idx % STAGES;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (idx / STAGES) & 1, abort_flag));
+        for (int kt = 0; kt < KT; ++kt) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], ph, abort_flag));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = sdesc_kmajor_sw128(smem_u32(base + s * STAGE));
-          const uint64_t db = sdesc_kmajor_sw128(smem_u32(base + s * STAGE + SC_A_BYTES));
           if (leader) {
+            const uint64_t da = sdesc_kmajor_sw128(smem_u32(base + s * STAGE));
+            const uint64_t db = sdesc_kmajor_sw128(smem_u32(base + s * STAGE + A_BYTES));
 #pragma unroll
             for (int k = 0; k < SC_K / 16; ++k) {
               if constexpr (PAIR)
@@ -581,6 +604,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
             commit_all(&empty[s]);
           }
           __syncwarp();
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
         if (!ok) break;
         if (leader) commit_all(&tfull[a]);

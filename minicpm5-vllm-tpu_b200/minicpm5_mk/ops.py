@@ -7,6 +7,7 @@ in libminicpm5_mk.so; nothing falls back to torch.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -20,7 +21,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: building a torch.cuda.Stream around it costs 2 us, as much as a kernel launch
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _cuda(t: torch.Tensor, name: str) -> None:
@@ -323,14 +325,19 @@ def topk_logprobs(logits: torch.Tensor, k: int = 20):
 # codes int8 [num_pages, 2, n_kv, page, head_dim] and scales f32 [num_pages, 2, n_kv] of one layer (the calls
 # that move whole pages take [layers, ...]); the layout is described in include/minicpm5_mk.h.  Tables, lengths
 # and counts are int32 tensors on the device; no call here reads them on the host.
+# The argument checks and the calls are written for the host's time: a decoding step calls these once per layer,
+# and several of the kernels run for less than 10 us.
+_I32, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
+
+
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: torch.device) -> None:
-    if t.dtype != dtype or t.dim() != dim or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.ndim != dim or t.device != device or not t.is_contiguous():
         raise ValueError(f"minicpm5_mk: {name} must be a contiguous {dim}-d {dtype} tensor on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
 
 
 def _heads(t: torch.Tensor, name: str, device: torch.device, heads: int, head_dim: int) -> None:
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != device or t.shape[1] != heads or \
+    if t.dtype is not _BF16 or t.ndim != 3 or t.device != device or t.shape[1] != heads or \
             t.shape[2] != head_dim or t.stride(2) != 1:
         raise ValueError(f"minicpm5_mk: {name} must be bf16 [tokens, {heads}, {head_dim}] on {device} with unit "
                          f"stride inside a head, got {tuple(t.shape)} {t.dtype} on {t.device}")
@@ -341,21 +348,26 @@ def _pages(codes: torch.Tensor, scales: torch.Tensor, dim: int) -> torch.device:
         raise ValueError("minicpm5_mk: codes must be a CUDA tensor")
     dev = codes.device
     _need(codes, "codes", torch.int8, dim, dev)
-    _need(scales, "scales", torch.float32, dim - 2, dev)
-    if scales.shape != codes.shape[:-2] or codes.shape[-4] != 2:
+    _need(scales, "scales", _F32, dim - 2, dev)
+    shape = codes.shape
+    if scales.shape != shape[:-2] or shape[-4] != 2:
         raise ValueError("minicpm5_mk: codes are [..., pages, 2, n_kv, page, head_dim] and scales [..., pages, 2, n_kv], "
                          f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
     return dev
 
 
 def _table(block_table: torch.Tensor, lens: Optional[torch.Tensor], name: str, dev: torch.device) -> Tuple[int, int]:
-    _need(block_table, "block_table", torch.int32, 2, dev)
+    _need(block_table, "block_table", _I32, 2, dev)
     rows, width = block_table.shape
     if lens is not None:
-        _need(lens, name, torch.int32, 1, dev)
-        if lens.shape[0] != rows:
-            raise ValueError(f"minicpm5_mk: {name} has {lens.shape[0]} entries for {rows} rows of block_table")
+        _row_values(lens, name, rows, dev)
     return rows, width
+
+
+def _row_values(t: torch.Tensor, name: str, rows: int, dev: torch.device) -> None:
+    _need(t, name, _I32, 1, dev)
+    if t.shape[0] != rows:
+        raise ValueError(f"minicpm5_mk: {name} has {t.shape[0]} entries for {rows} rows")
 
 
 def _cu(cu: Optional[torch.Tensor], name: str, rows: int, tokens: int, dev: torch.device) -> None:
@@ -363,9 +375,17 @@ def _cu(cu: Optional[torch.Tensor], name: str, rows: int, tokens: int, dev: torc
         if tokens != rows:
             raise ValueError(f"minicpm5_mk: without {name} there is one token per row: {tokens} tokens, {rows} rows")
         return
-    _need(cu, name, torch.int32, 1, dev)
+    _need(cu, name, _I32, 1, dev)
     if cu.shape[0] != rows + 1:
         raise ValueError(f"minicpm5_mk: {name} has {cu.shape[0]} entries for {rows} rows")
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(n_q: int, n_kv: int, head_dim: int, rows: int, max_q: int, max_len: int) -> int:
+    n = ctypes.c_size_t()
+    _lib.check(_lib.lib().mk_attention_paged_workspace(0, n_q, n_kv, head_dim, rows, max_q, max_len, ctypes.byref(n)),
+               "mk_attention_paged_workspace")
+    return n.value
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -395,8 +415,8 @@ def kv_read(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor
     dev = _pages(codes, scales, 5)
     P, _, n_kv, page, hd = codes.shape
     rows, width = _table(block_table, start, "start", dev)
-    _table(block_table, count, "count", dev)
-    k = torch.empty((rows, int(max_count), n_kv, hd), dtype=torch.bfloat16, device=dev)
+    _row_values(count, "count", rows, dev)
+    k = torch.empty(rows, int(max_count), n_kv, hd, dtype=_BF16, device=dev)
     v = torch.empty_like(k)
     st = _lib.lib().mk_kv_read(codes.data_ptr(), scales.data_ptr(), P, n_kv, page, hd, block_table.data_ptr(), rows,
                                width, start.data_ptr(), count.data_ptr(), int(max_count), k.data_ptr(), v.data_ptr(),
@@ -419,18 +439,16 @@ def attention_paged(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, 
     _heads(q, "q", dev, n_q, hd)
     rows, width = _table(block_table, lens, "lens", dev)
     _cu(cu_q, "cu_q", rows, T, dev)
-    max_len = width * page if max_len is None else int(max_len)
-    L = _lib.lib()
-    n = ctypes.c_size_t()
-    _lib.check(L.mk_attention_paged_workspace(T, n_q, n_kv, hd, rows, int(max_q), max_len, ctypes.byref(n)),
-               "mk_attention_paged_workspace")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
-    out = torch.empty((T, n_q, hd), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((T, n_q), dtype=torch.float32, device=dev)
-    st = L.mk_attention_paged(q.data_ptr(), q.stride(0), q.stride(1), T, n_q, codes.data_ptr(), scales.data_ptr(), P,
-                              n_kv, page, hd, block_table.data_ptr(), rows, width, lens.data_ptr(), _ptr(cu_q),
-                              int(max_q), max_len, float(softmax_scale), out.data_ptr(), lse.data_ptr(), _ptr(ws),
-                              n.value, _stream(dev))
+    # a multiple of the 64 keys that the plan counts in, so that a growing row asks for the size again only then
+    max_len = width * page if max_len is None else int(max_len) if max_len <= 0 else -(-int(max_len) // 64) * 64
+    nbytes = _attention_workspace(n_q, n_kv, hd, rows, int(max_q), max_len)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    out = torch.empty(T, n_q, hd, dtype=_BF16, device=dev)
+    lse = torch.empty(T, n_q, dtype=_F32, device=dev)
+    st = _lib.lib().mk_attention_paged(q.data_ptr(), q.stride(0), q.stride(1), T, n_q, codes.data_ptr(),
+                                       scales.data_ptr(), P, n_kv, page, hd, block_table.data_ptr(), rows, width,
+                                       lens.data_ptr(), _ptr(cu_q), int(max_q), max_len, float(softmax_scale),
+                                       out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, _stream(dev))
     _lib.check(st, "mk_attention_paged")
     return out, lse
 
@@ -448,13 +466,13 @@ def kv_fork(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor
     dev = _pages(codes, scales, 6)
     layers, P, _, n_kv, page, hd = codes.shape
     rows, width = _table(block_table, lens, "lens", dev)
-    _need(refs, "refs", torch.int32, 1, dev)
-    _need(parents, "parents", torch.int32, 1, dev)
+    _need(refs, "refs", _I32, 1, dev)
+    _need(parents, "parents", _I32, 1, dev)
     if refs.shape[0] != P:
         raise ValueError(f"minicpm5_mk: refs has {refs.shape[0]} entries for {P} pages")
     R = parents.shape[0]
-    table = torch.empty((R, width), dtype=torch.int32, device=dev)
-    new_lens = torch.empty((R,), dtype=torch.int32, device=dev)
+    table = torch.empty(R, width, dtype=_I32, device=dev)
+    new_lens = torch.empty(R, dtype=_I32, device=dev)
     new_refs = torch.empty_like(refs)
     ws = _move_workspace(R, P, dev)
     st = _lib.lib().mk_kv_fork(codes.data_ptr(), scales.data_ptr(), layers, P, n_kv, page, hd, block_table.data_ptr(),
@@ -472,9 +490,9 @@ def kv_reserve(block_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor
         raise ValueError("minicpm5_mk: block_table must be a CUDA tensor")
     dev = block_table.device
     rows, width = _table(block_table, lens, "lens", dev)
-    _need(refs, "refs", torch.int32, 1, dev)
+    _need(refs, "refs", _I32, 1, dev)
     if n_new is not None:
-        _table(block_table, n_new, "n_new", dev)
+        _row_values(n_new, "n_new", rows, dev)
     st = _lib.lib().mk_kv_reserve(block_table.data_ptr(), lens.data_ptr(), rows, width, _ptr(n_new), refs.data_ptr(),
                                   refs.shape[0], int(page), _stream(dev))
     _lib.check(st, "mk_kv_reserve")
@@ -486,11 +504,11 @@ def kv_compact(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
     dev = _pages(codes, scales, 6)
     layers, P, _, n_kv, page, hd = codes.shape
     rows, width = _table(block_table, None, "", dev)
-    _need(refs, "refs", torch.int32, 1, dev)
+    _need(refs, "refs", _I32, 1, dev)
     if refs.shape[0] != P:
         raise ValueError(f"minicpm5_mk: refs has {refs.shape[0]} entries for {P} pages")
     table, new_refs = torch.empty_like(block_table), torch.empty_like(refs)
-    used = torch.empty((1,), dtype=torch.int32, device=dev)
+    used = torch.empty(1, dtype=_I32, device=dev)
     ws = _move_workspace(rows, P, dev)
     st = _lib.lib().mk_kv_compact(codes.data_ptr(), scales.data_ptr(), layers, P, n_kv, page, hd,
                                   block_table.data_ptr(), rows, width, refs.data_ptr(), table.data_ptr(),
@@ -504,47 +522,53 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0):
     """Scores of the tokens targets int32 [T] under rows of logits (f32 or bf16 [T, V], row stride free):
     (logprobs f32 [T], entropy f32 [T], ranks int32 [T], top_ids int32 [T, k], top_logprobs f32 [T, k])
     (mk_token_logprobs).  A target outside [0, V) is not scored: logprob 0, rank 0."""
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or \
+    if not logits.is_cuda or logits.ndim != 2 or logits.dtype not in (_F32, _BF16) or \
             (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("minicpm5_mk: logits must be a row-major f32 or bf16 [T, V] CUDA tensor")
     dev = logits.device
     T, V = logits.shape
-    _need(targets, "targets", torch.int32, 1, dev)
+    _need(targets, "targets", _I32, 1, dev)
     if targets.shape[0] != T:
         raise ValueError(f"minicpm5_mk: {targets.shape[0]} targets for {T} rows of logits")
     k = int(top_k)
-    lp = torch.empty((T,), dtype=torch.float32, device=dev)
+    lp = torch.empty(T, dtype=_F32, device=dev)
     ent = torch.empty_like(lp)
-    rank = torch.empty((T,), dtype=torch.int32, device=dev)
-    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
-    tlp = torch.empty((T, k), dtype=torch.float32, device=dev)
-    st = _lib.lib().mk_token_logprobs(logits.data_ptr(), 16 if logits.dtype == torch.bfloat16 else 32, T, V,
+    rank = torch.empty_like(targets)
+    ids = torch.empty(T, k, dtype=_I32, device=dev)
+    tlp = torch.empty(T, k, dtype=_F32, device=dev)
+    st = _lib.lib().mk_token_logprobs(logits.data_ptr(), 16 if logits.dtype is _BF16 else 32, T, V,
                                       logits.stride(0), targets.data_ptr(), k, lp.data_ptr(), ent.data_ptr(),
                                       rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), _stream(dev))
     _lib.check(st, "mk_token_logprobs")
     return lp, ent, rank, ids, tlp
 
 
+@functools.lru_cache(maxsize=4096)
+def _score_workspace(T: int, H: int, V: int) -> int:
+    n = ctypes.c_size_t()
+    _lib.check(_lib.lib().mk_score_tokens_workspace(T, H, V, ctypes.byref(n)), "mk_score_tokens_workspace")
+    return n.value
+
+
 def score_tokens(h: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor, logit_scale: float = 1.0):
     """(logprobs f32 [T], entropy f32 [T]) of the tokens targets int32 [T] under logits logit_scale * h @ lm_head^T,
     h bf16 [T, H] (row stride free), lm_head bf16 [V, H]; the logits are not written to memory
     (mk_score_tokens).  A target outside [0, V) is not scored: logprob 0."""
-    if not h.is_cuda or h.dim() != 2 or h.dtype != torch.bfloat16 or (h.shape[1] > 1 and h.stride(1) != 1):
+    if not h.is_cuda or h.ndim != 2 or h.dtype is not _BF16 or (h.shape[1] > 1 and h.stride(1) != 1):
         raise ValueError("minicpm5_mk: h must be a row-major bf16 [T, H] CUDA tensor")
     dev = h.device
     T, H = h.shape
-    _need(lm_head, "lm_head", torch.bfloat16, 2, dev)
-    _need(targets, "targets", torch.int32, 1, dev)
+    _need(lm_head, "lm_head", _BF16, 2, dev)
+    _need(targets, "targets", _I32, 1, dev)
     if lm_head.shape[1] != H or targets.shape[0] != T:
         raise ValueError(f"minicpm5_mk: h {tuple(h.shape)}, lm_head {tuple(lm_head.shape)}, {targets.shape[0]} targets")
     V = lm_head.shape[0]
-    L = _lib.lib()
-    n = ctypes.c_size_t()
-    _lib.check(L.mk_score_tokens_workspace(T, H, V, ctypes.byref(n)), "mk_score_tokens_workspace")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    lp = torch.empty((T,), dtype=torch.float32, device=dev)
+    nbytes = _score_workspace(T, H, V)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    lp = torch.empty(T, dtype=_F32, device=dev)
     ent = torch.empty_like(lp)
-    st = L.mk_score_tokens(h.data_ptr(), T, H, h.stride(0), lm_head.data_ptr(), V, targets.data_ptr(),
-                           float(logit_scale), lp.data_ptr(), ent.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
+    st = _lib.lib().mk_score_tokens(h.data_ptr(), T, H, h.stride(0), lm_head.data_ptr(), V, targets.data_ptr(),
+                                    float(logit_scale), lp.data_ptr(), ent.data_ptr(), ws.data_ptr(), nbytes,
+                                    _stream(dev))
     _lib.check(st, "mk_score_tokens")
     return lp, ent
