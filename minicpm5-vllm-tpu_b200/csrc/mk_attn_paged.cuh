@@ -11,8 +11,9 @@
 // transposed products, S^T = K Q^T and O^T = V^T P^T, with keys (then channels) as the matrix rows and the
 // query heads that share a key/value head as its 8 columns: mma.sync m16n8k16 fits that without padding, and a
 // 128-row tcgen05 tile would be 15/16 empty.  The order of the contraction index is free, so each lane's
-// fragment is made of bytes that are contiguous in memory: keys and values go from global memory to
-// registers in 16-byte loads and become operands without touching shared memory.
+// fragment is made of bytes that are contiguous in memory.  Each warp streams its own keys and values through a ring
+// in shared memory with bulk copies (a block's keys are one run of bytes, its values another), a stage or two
+// ahead of its arithmetic, and waits for nobody but the copies.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -58,19 +59,18 @@ constexpr float kLag = 8.f;
 constexpr float kLow = -1e30f;
 
 __host__ __device__ constexpr int pa_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+// Ring of a warp: a stage holds a block's keys and values, and a CTA's rings fill its part of an SM's shared memory
+// (up to 72 KB of 227).
+__host__ __device__ constexpr int pa_stage_bytes(int hd, int nt) { return 2 * 16 * pa_groups(nt) * hd; }
+__host__ __device__ constexpr int pa_stages(int hd, int nt) { return nt == 1 ? (hd == 96 ? 3 : 2) : 4; }
+__host__ __device__ constexpr int pa_ring_bytes(int hd, int nt) { return PA_WARPS * pa_stages(hd, nt) * pa_stage_bytes(hd, nt); }
 
-// Loads of bytes that are read once (not kept in L1).
-__device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg_stream(const uint2* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+// Bulk copy global -> shared (both 16-byte aligned, bytes a multiple of 16), counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 // Four codes (one word) to two f16 pairs, exact: byte ^ 0x80 under 0x64 is 1024 + 128 + code.
@@ -124,13 +124,22 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   constexpr int GP = pa_groups(NT), PA_UNIT = pa_unit(NT);
   constexpr int KS = HD / 16, MT = HD / 16, ROWS = 8 * NT, LDO = HD + 4;
   constexpr bool SPLIT = NT <= 2;  // p as two bf16 parts
+  constexpr int STAGES = pa_stages(HD, NT), STAGE = pa_stage_bytes(HD, NT), HALF = STAGE / 2;
   __shared__ long long s_scan[PA_WARPS], s_base;
   __shared__ int s_row;
   __shared__ int s_page[PA_GROUPS];
   __shared__ float s_ks[PA_GROUPS], s_vs[PA_GROUPS], s_red[PA_WARPS];
   __shared__ uint2 s_q[NT > 1 ? NT * KS * 32 : 1];
   __shared__ float s_m[PA_WARPS][ROWS], s_l[PA_WARPS][ROWS];
-  __shared__ __align__(16) float s_o[PA_WARPS][8][LDO];
+  __shared__ uint64_t s_full[PA_WARPS][STAGES];
+  __shared__ int s_abort;
+  // the rings; after a pair's last block the same bytes hold the warps' results
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  static_assert(sizeof(float) * PA_WARPS * 8 * LDO <= pa_ring_bytes(HD, NT), "results fit");
+  float (*s_o)[8][LDO] = reinterpret_cast<float (*)[8][LDO]>(s_ring);
+  if (threadIdx.x < PA_WARPS * STAGES) mbar_init(&s_full[0][0] + threadIdx.x, 1);
+  if (threadIdx.x == 0) s_abort = 0;
+  fence_mbar_init();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int G = a.group, n_kv = cp.n_kv, page_mask = (1 << cp.page_shift) - 1;
@@ -180,6 +189,9 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   __syncthreads();
   int row = s_row;
   long long base = s_base;
+  uint8_t* ring = s_ring + warp * STAGES * STAGE;
+  int st = 0;           // stage of the next block to be read
+  uint32_t phase = 0;
 
   for (long long u = u0; u < u1;) {
     const long long ru = row_units(row);
@@ -311,63 +323,71 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       vref = nref;
       __syncthreads();
 
-      uint32_t kw[GP][2][KS];  // two keys' words
-      uint4 vw[GP][HD / 32];
-      // Where the block's groups lie: in one page from 32 tokens on, so that all loads share one address.
-      const size_t plane = static_cast<size_t>(n_kv) * HD << cp.page_shift;
-      const int8_t* at[GP];
-      auto find = [&](int gi) {
+      // Asks for the block at group gi (in one page from 32 tokens on).  A missing page is not read: what the stage
+      // holds instead weighs nothing.
+      auto ask = [&](int gi, int stage) {
+        uint8_t* dst = ring + stage * STAGE;
+        uint64_t* bar = &s_full[warp][stage];
+        const size_t plane = static_cast<size_t>(n_kv) * HD << cp.page_shift;
+        if (GP == 1 || cp.page_shift > 4) {
+          const int pg = s_page[gi];
+          mbar_arrive_expect_tx(bar, pg < 0 ? 0 : STAGE);
+          if (pg >= 0) {
+            const int8_t* at = kv_head_ptr(cp, pg, 0, g) + ((kb + gi * 16) & page_mask) * HD;
+            bulk_load(dst, at, HALF, bar);
+            bulk_load(dst + HALF, at + plane, HALF, bar);
+          }
+        } else {
+          uint32_t bytes = 0;
 #pragma unroll
-        for (int p = 0; p < GP; ++p) {
-          if (p == 0 || cp.page_shift == 4)
-            at[p] = kv_head_ptr(cp, max(s_page[gi + p], 0), 0, g) + ((kb + (gi + p) * 16) & page_mask) * HD;
-          else
-            at[p] = at[0] + p * 16 * HD;
+          for (int p = 0; p < GP; ++p) bytes += s_page[gi + p] < 0 ? 0 : STAGE / GP;
+          mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+          for (int p = 0; p < GP; ++p)
+            if (s_page[gi + p] >= 0) {
+              const int8_t* at = kv_head_ptr(cp, s_page[gi + p], 0, g);
+              bulk_load(dst + p * 16 * HD, at, 16 * HD, bar);
+              bulk_load(dst + HALF + p * 16 * HD, at + plane, 16 * HD, bar);
+            }
         }
       };
+      const int blocks = (ng - warp * GP + PA_WARPS * GP - 1) / (PA_WARPS * GP);  // of this warp (none: <= 0)
+      if (lane == 0)
+        for (int i = 0; i < min(blocks, STAGES); ++i) ask((warp + i * PA_WARPS) * GP, (st + i) % STAGES);
       const int lane_k = (4 * (r >> 1) + (r & 1)) * HD + c * 16, lane_k8 = (4 * (r >> 1) + (r & 1)) * HD + 64 + c * 8;
       const int lane_v = (c * HD + 4 * r) * 4;
-      auto load_k = [&]() {
-#pragma unroll
-        for (int p = 0; p < GP; ++p)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 x = ldg_stream(reinterpret_cast<const uint4*>(at[p] + lane_k + i * 2 * HD));
-            kw[p][i][0] = x.x;
-            kw[p][i][1] = x.y;
-            kw[p][i][2] = x.z;
-            kw[p][i][3] = x.w;
-            if constexpr (HD == 128) {
-              const uint4 y = ldg_stream(reinterpret_cast<const uint4*>(at[p] + lane_k + 64 + i * 2 * HD));
-              kw[p][i][4] = y.x;
-              kw[p][i][5] = y.y;
-              kw[p][i][6] = y.z;
-              kw[p][i][7] = y.w;
-            } else {
-              const uint2 y = ldg_stream(reinterpret_cast<const uint2*>(at[p] + lane_k8 + i * 2 * HD));
-              kw[p][i][4] = y.x;
-              kw[p][i][5] = y.y;
-            }
-          }
-      };
-      auto load_v = [&]() {
-#pragma unroll
-        for (int p = 0; p < GP; ++p)
-#pragma unroll
-          for (int j = 0; j < HD / 32; ++j)
-            vw[p][j] = ldg_stream(reinterpret_cast<const uint4*>(at[p] + plane + lane_v + j * 128));
-      };
-      if (warp * GP < ng) {
-        find(warp * GP);
-        load_k();
-        load_v();
-      }
+      int left = blocks;
 #pragma unroll 1
       for (int gi = warp * GP; gi < ng; gi += PA_WARPS * GP) {
-        const bool more = gi + PA_WARPS * GP < ng;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[warp][st], phase, &s_abort))) {
+          for (int i = 0; i < min(left, STAGES); ++i)  // what was asked for lands before the CTA may leave
+            mbar_wait_drain(&s_full[warp][(st + i) % STAGES], phase ^ (st + i >= STAGES ? 1u : 0u));
+          break;
+        }
+        const uint8_t* block = ring + st * STAGE;
         float s[GP][NT][4];
 #pragma unroll
         for (int p = 0; p < GP; ++p) {
+          uint32_t kw[2][KS];  // two keys' words
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(block + p * 16 * HD + lane_k + i * 2 * HD);
+            kw[i][0] = x.x;
+            kw[i][1] = x.y;
+            kw[i][2] = x.z;
+            kw[i][3] = x.w;
+            if constexpr (HD == 128) {
+              const uint4 y = *reinterpret_cast<const uint4*>(block + p * 16 * HD + lane_k + 64 + i * 2 * HD);
+              kw[i][4] = y.x;
+              kw[i][5] = y.y;
+              kw[i][6] = y.z;
+              kw[i][7] = y.w;
+            } else {
+              const uint2 y = *reinterpret_cast<const uint2*>(block + p * 16 * HD + lane_k8 + i * 2 * HD);
+              kw[i][4] = y.x;
+              kw[i][5] = y.y;
+            }
+          }
           // even and odd steps in sums of their own: two chains of products half as long
           float s1[NT][4];
 #pragma unroll
@@ -377,8 +397,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 #pragma unroll
           for (int w = 0; w < KS; ++w) {
             uint32_t a0, a1, a2, a3;
-            i8x4_to_f16x4(kw[p][0][w], a0, a2);
-            i8x4_to_f16x4(kw[p][1][w], a1, a3);
+            i8x4_to_f16x4(kw[0][w], a0, a2);
+            i8x4_to_f16x4(kw[1][w], a1, a3);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               if constexpr (NT == 1) {
@@ -408,10 +428,6 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
             sf[p][t][0] = rf[t][0] * ks;
             sf[p][t][1] = rf[t][1] * ks;
           }
-        }
-        if (more) {
-          find(gi + PA_WARPS * GP);
-          load_k();
         }
         // x = s - m, in units of log 2
         float x[GP][NT][4];
@@ -491,7 +507,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
         for (int p = 0; p < GP; ++p)
 #pragma unroll
           for (int j = 0; j < HD / 32; ++j) {
-            const uint32_t w[4] = {vw[p][j].x, vw[p][j].y, vw[p][j].z, vw[p][j].w};
+            const uint4 x4 = *reinterpret_cast<const uint4*>(block + HALF + p * 16 * HD + lane_v + j * 128);
+            const uint32_t w[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t a0, a1, a2, a3;
@@ -511,7 +528,14 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
               }
             }
           }
-        if (more) load_v();
+        // every lane has used the stage's bytes: it is asked for again
+        __syncwarp();
+        if (lane == 0 && left > STAGES) ask(gi + STAGES * PA_WARPS * GP, st);
+        --left;
+        if (++st == STAGES) {
+          st = 0;
+          phase ^= 1u;
+        }
       }
     }
 
@@ -527,6 +551,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
           s_l[warp][t * 8 + 2 * c + e] = l[t][e];
         }
       }
+    __syncthreads();  // every warp is done with its ring
     const bool whole = ua == 0 && ub == upp;
     const int slot = static_cast<int>(cta) * 2 + (ua == 0 ? 1 : 0);
     const float unit = vref / kPOff;
@@ -586,10 +611,13 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       const long long last = base + static_cast<long long>(local_pair + 1) * upp - 1;  // the pair's last unit
       a.desc[cta] = make_int4(row, rt, g, static_cast<int>(((last + 1) * C - 1) / N));
     }
-    __syncthreads();  // s_o and s_q are free again
+    fence_proxy_async_smem();  // the results before the next copies into the same bytes
+    __syncthreads();           // s_o and s_q are free again
     u += ub - ua;
+    if (s_abort) break;
   }
   pdl_trigger();
+  if (tid == 0 && s_abort) atomicCAS(a.err, 0, DEV_ERR_TIMEOUT_ATTN_PAGED);
 }
 
 // Joins the pieces of a pair that several CTAs worked on.  CTA (c, i): rows 8i .. 8i + 7 of the pair that began in

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <mutex>
 
 #include "mk_attn_paged.cuh"
 #include "mk_cache.cuh"
@@ -66,6 +67,28 @@ PagedPlan paged_plan(int group, int n_kv, int hd, int rows, int max_q, int max_l
   p.ml_bytes = static_cast<size_t>(2) * p.ctas * 8 * p.nt * sizeof(float2);
   p.bytes = p.o_bytes + p.ml_bytes + static_cast<size_t>(p.ctas) * sizeof(int4);
   return p;
+}
+
+// Once per device: the rings are larger than a kernel's default shared memory.
+mk_status paged_ready() {
+  static std::mutex mu;
+  static bool ready[64];
+  int dev = 0;
+  MK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return MK_ERR_BAD_ARG;
+  std::lock_guard<std::mutex> lk(mu);
+  if (ready[dev]) return MK_OK;
+  const auto allow = [](void (*k)(KvPages, mk::PagedAttnArgs), int hd, int nt) {
+    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, mk::pa_ring_bytes(hd, nt));
+  };
+  MK_CUDA(allow(mk::attn_paged_kernel<96, 1>, 96, 1));
+  MK_CUDA(allow(mk::attn_paged_kernel<96, 2>, 96, 2));
+  MK_CUDA(allow(mk::attn_paged_kernel<96, 4>, 96, 4));
+  MK_CUDA(allow(mk::attn_paged_kernel<128, 1>, 128, 1));
+  MK_CUDA(allow(mk::attn_paged_kernel<128, 2>, 128, 2));
+  MK_CUDA(allow(mk::attn_paged_kernel<128, 4>, 128, 4));
+  ready[dev] = true;
+  return MK_OK;
 }
 
 }  // namespace
@@ -169,7 +192,9 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
                                                                              : mk::attn_paged_kernel<96, 4>)
                      : (p.nt == 1 ? mk::attn_paged_kernel<128, 1> : p.nt == 2 ? mk::attn_paged_kernel<128, 2>
                                                                               : mk::attn_paged_kernel<128, 4>);
-  MK_TRY(launch_k(k, dim3(p.ctas), dim3(mk::PA_THREADS), 0, st, true, c, a));
+  const int ring = mk::pa_ring_bytes(head_dim, p.nt);
+  MK_TRY(paged_ready());
+  MK_TRY(launch_k(k, dim3(p.ctas), dim3(mk::PA_THREADS), ring, st, true, c, a));
   if (head_dim == 96)
     return launch_k(mk::attn_paged_join_kernel<96>, dim3(p.ctas, p.nt), dim3(mk::PJ_PARTS * 2 * 96), 0, st, true, a);
   return launch_k(mk::attn_paged_join_kernel<128>, dim3(p.ctas, p.nt), dim3(mk::PJ_PARTS * 2 * 128), 0, st, true, a);

@@ -23,6 +23,7 @@ enum : int {
   DEV_ERR_BAD_TOKEN_ID = 0x300,
   DEV_ERR_TIMEOUT_ATTN_TC = 0x400,
   DEV_ERR_TIMEOUT_SCORE = 0x600,
+  DEV_ERR_TIMEOUT_ATTN_PAGED = 0x700,
   DEV_ERR_BAD_PAGE = 0x500,  // a row's table holds no page where it needs one, or a page or row id out of range
   DEV_ERR_NO_PAGE = 0x501,   // no free page (or no room in the table) left
 };

@@ -104,11 +104,11 @@ mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, 
   a.rank = ranks;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  // CTAs per row: four fit on an SM.  Rows are shared while the GPU has room for twice the CTAs and every one
-  // keeps at least a step's 8192 logits.
+  // CTAs per row: eight fit on an SM.  Rows are shared while the GPU has room for twice the CTAs and every one
+  // keeps at least two steps' 8192 logits.
   int cluster = 1;
-  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= static_cast<int64_t>(d.sm_count) * 4 &&
-         V / (cluster * 2) >= mk::TL_THREADS * mk::TL_VALUES)
+  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= static_cast<int64_t>(d.sm_count) * 8 &&
+         V / (cluster * 2) >= 2 * mk::TL_THREADS * mk::TL_VALUES)
     cluster *= 2;
   void (*k)(mk::LogitsArgs, int) =
       logits_bits == 32 ? mk::token_logprobs_kernel<float> : mk::token_logprobs_kernel<__nv_bfloat16>;

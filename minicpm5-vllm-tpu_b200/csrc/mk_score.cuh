@@ -45,6 +45,25 @@ __device__ __forceinline__ RowStats stats_warp(RowStats s) {
   return s;
 }
 
+// Packed f32x2 arithmetic on register pairs.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // A 16-byte load of bytes that are read once.
 __device__ __forceinline__ uint4 ldg_once(const uint4* p) {
   uint4 v;
@@ -80,11 +99,11 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 //
 // What bounds it: the bytes of the logits.  Per bf16 logit the arithmetic is about six instructions and one
 // exponential, two thirds of what an SM can issue at the rate at which HBM delivers them.
-constexpr int TL_THREADS = 256;
+constexpr int TL_THREADS = 128;   // (256: the work at a row's end, the same for every warp, was a third of all)
 constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
-constexpr int TL_LIST = 1024;     // vectors listed
-constexpr int TL_CAP = 2048;      // logits put in order
+constexpr int TL_LIST = 512;      // vectors listed
+constexpr int TL_CAP = 1024;      // logits put in order
 constexpr int TL_CLUSTER_MAX = 8;
 static_assert(TL_TOPK_MAX <= 64 && TL_CLUSTER_MAX * TL_TOPK_MAX <= TL_CAP, "alternatives");
 
@@ -119,7 +138,7 @@ struct LogitsArgs {
 };
 
 template <typename E>
-__global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const LogitsArgs a, const int cluster) {
+__global__ void __launch_bounds__(TL_THREADS, 8) token_logprobs_kernel(const LogitsArgs a, const int cluster) {
   constexpr bool BF = sizeof(E) == 2;
   constexpr int EPV = 16 / sizeof(E);            // logits per 16-byte vector
   constexpr int VECS = TL_VALUES / EPV;          // vectors per thread and step
@@ -128,7 +147,7 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
   __shared__ int s_id[TL_LIST];
   __shared__ unsigned long long s_kept[TL_CAP], s_top[TL_TOPK_MAX];
   __shared__ unsigned long long s_pick[TL_THREADS / 32];
-  __shared__ volatile float s_tau[TL_THREADS / 32];
+  __shared__ __align__(16) volatile float s_tau[TL_THREADS / 32];
   __shared__ int s_n, s_kept_n, s_have;
   __shared__ RowStats s_st[TL_THREADS / 32];
   __shared__ int s_above[TL_THREADS / 32];
@@ -233,15 +252,23 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
       st.z *= f;
       st.m = most;
     }
-    // y = (x - ref) log2 e as one FMA: 2^y is off by the rounding of ref log2 e, which the sums make good.  Where
-    // that product could overflow (logits beyond 1e38) the difference is taken first.
+    // y = (x - ref) log2 e as one FMA, two logits at a time: 2^y is off by the rounding of ref log2 e, which the
+    // sums make good.  Where that product could overflow (logits beyond 1e38) the difference is taken first.
     const float rl = ref * kLog2E, rest = fmaf(ref, kLog2E, -rl);
     const bool far = !(fabsf(ref) < 1e38f);
-    float z0 = 0.f, z1 = 0.f, w0 = 0.f, w1 = 0.f;
-    auto add = [&](float x, float& z, float& w) {
-      const float y = far ? (x - ref) * kLog2E : fmaf(x, kLog2E, -rl), e = ex2_approx(y);
-      z += e;
-      w = fmaf(e, fmaxf(y, kFar), w);
+    uint64_t z2 = 0, w2 = 0;
+    const uint64_t l2e = pack2(kLog2E, kLog2E), nrl = pack2(-rl, -rl);
+    auto two = [&](float p, float q) {
+      float yp, yq;
+      if (far) {
+        yp = (p - ref) * kLog2E;
+        yq = (q - ref) * kLog2E;
+      } else {
+        unpack2(fma2(pack2(p, q), l2e, nrl), yp, yq);
+      }
+      const uint64_t e = pack2(ex2_approx(yp), ex2_approx(yq));
+      z2 = add2(z2, e);
+      w2 = fma2(e, pack2(fmaxf(yp, kFar), fmaxf(yq, kFar)), w2);
     };
     auto all = [&]() {
       if constexpr (BF) {
@@ -254,8 +281,7 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
             const uint32_t u = words(v, w);
             const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&u);
             cnt = __hadd2(cnt, __hgt2(h, m2));  // at most VECS * 4 in each half: exact
-            add(__uint_as_float(u << 16), z0, w0);
-            add(__uint_as_float(u & 0xffff0000u), z1, w1);
+            two(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
           }
         above += static_cast<int>(__low2float(cnt)) + static_cast<int>(__high2float(cnt));
       } else {
@@ -265,12 +291,14 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(const Log
           for (int w = 0; w < 4; w += 2) {
             const float p = __uint_as_float(words(v, w)), q = __uint_as_float(words(v, w + 1));
             above += (p > mine) + (q > mine);
-            add(p, z0, w0);
-            add(q, z1, w1);
+            two(p, q);
           }
       }
     };
     if (far) all(); else all();
+    float z0, z1, w0, w1;
+    unpack2(z2, z0, z1);
+    unpack2(w2, w0, w1);
     const float back = far ? 1.f : fmaf(-rest, kLn2, 1.f);
     st.z = fmaf(z0 + z1, back, st.z);
     st.w = fmaf((w0 + w1) * kLn2, back, st.w);
