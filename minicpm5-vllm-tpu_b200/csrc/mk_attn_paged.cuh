@@ -620,51 +620,85 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   if (tid == 0 && s_abort) atomicCAS(a.err, 0, DEV_ERR_TIMEOUT_ATTN_PAGED);
 }
 
-// Joins the pieces of a pair that several CTAs worked on.  CTA (c, i): rows 8i .. 8i + 7 of the pair that began in
-// CTA c and was not finished there.  A thread owns four channels of a row; PJ_PARTS groups of threads take every
-// PJ_PARTS-th piece in turn, and their results are joined in order.
-constexpr int PJ_PARTS = 4;
-template <int HD>
-__global__ void __launch_bounds__(PJ_PARTS * 2 * HD) attn_paged_join_kernel(PagedAttnArgs a) {
-  __shared__ __align__(16) float s_o[PJ_PARTS][8][HD];
-  __shared__ float2 s_ml[PJ_PARTS][8];
+// Joins the pieces of the pairs that several CTAs worked on: eight rows of a pair and DIMS of their channels at a
+// time.  A thread owns four channels of a row; PARTS groups of threads take every PARTS-th piece in turn, and their
+// results are joined in order.
+//   LONG  (few pairs, each in many pieces): the CTAs first number the unfinished pairs, and CTA (x, y, z) takes every
+//         gridDim.x-th from the x-th, rows 8y .. and channels 32z .. (8 groups, 32 channels: all SMs have work)
+//   else  CTA (c, y) takes rows 8y .. of the pair that began in CTA c, if one did and was not finished there
+template <int HD, bool LONG>
+struct PagedJoin {
+  static constexpr int PARTS = LONG ? 8 : 2, DIMS = LONG ? 32 : HD, LANES = 8 * DIMS / 4, THREADS = PARTS * LANES;
+};
+template <int HD, bool LONG>
+__global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_kernel(PagedAttnArgs a, int ctas) {
+  using J = PagedJoin<HD, LONG>;
+  __shared__ __align__(16) float s_o[J::PARTS][8][J::DIMS];
+  __shared__ float2 s_ml[J::PARTS][8];
+  __shared__ int s_sum[J::THREADS / 32], s_mine[J::THREADS];
   pdl_wait();
   pdl_trigger();
-  const int4 d = a.desc[blockIdx.x];
-  if (d.x < 0) return;
-  const int ROWS = 8 * gridDim.y, G = a.group;
-  const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1;
-  const int pieces = d.w - static_cast<int>(blockIdx.x) + 1;
-  const int grp = threadIdx.x / (2 * HD), q8 = threadIdx.x % (2 * HD) / (HD / 4), dim = threadIdx.x % (HD / 4) * 4;
-  const int i = blockIdx.y * 8 + q8, qr = d.y * ROWS + i;
-  float m = kLow, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto weight = [](float from, float to) { return ex2_approx(from - to); };
-  auto add = [&](float2 ml, float4 x) {
-    const float top = fmaxf(m, ml.x), f = weight(m, top), e = weight(ml.x, top);
-    m = top;
-    l = l * f + ml.y * e;
-    o.x = o.x * f + x.x * e;
-    o.y = o.y * f + x.y * e;
-    o.z = o.z * f + x.z * e;
-    o.w = o.w * f + x.w * e;
-  };
-#pragma unroll 8
-  for (int p = grp; p < pieces; p += PJ_PARTS) {
-    const size_t at = (static_cast<size_t>(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + i;
-    add(a.part_ml[at], *reinterpret_cast<const float4*>(a.part_o + at * HD + dim));
-  }
-  *reinterpret_cast<float4*>(&s_o[grp][q8][dim]) = o;
-  if (dim == 0) s_ml[grp][q8] = make_float2(m, l);
-  __syncthreads();
-  if (grp || qr >= n * G) return;
+  const int ROWS = 8 * gridDim.y, G = a.group, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int grp = tid / J::LANES, q8 = tid % J::LANES / (J::DIMS / 4), d4 = tid % (J::DIMS / 4) * 4;
+  const int dim = blockIdx.z * J::DIMS + d4;
+  auto join = [&](int cta, const int4& d) {
+    const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1;
+    const int pieces = d.w - cta + 1, i = blockIdx.y * 8 + q8, qr = d.y * ROWS + i;
+    float m = kLow, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 x) {
+      const float top = fmaxf(m, ml.x), f = ex2_approx(m - top), e = ex2_approx(ml.x - top);
+      m = top;
+      l = l * f + ml.y * e;
+      o.x = o.x * f + x.x * e;
+      o.y = o.y * f + x.y * e;
+      o.z = o.z * f + x.z * e;
+      o.w = o.w * f + x.w * e;
+    };
+#pragma unroll 4
+    for (int p = grp; p < pieces; p += J::PARTS) {
+      const size_t at = (static_cast<size_t>(cta + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + i;
+      add(a.part_ml[at], *reinterpret_cast<const float4*>(a.part_o + at * HD + dim));
+    }
+    *reinterpret_cast<float4*>(&s_o[grp][q8][d4]) = o;
+    if (d4 == 0) s_ml[grp][q8] = make_float2(m, l);
+    __syncthreads();
+    if (grp == 0 && qr < n * G) {
 #pragma unroll
-  for (int p = 1; p < PJ_PARTS; ++p) add(s_ml[p][q8], *reinterpret_cast<const float4*>(&s_o[p][q8][dim]));
-  const long long at = static_cast<long long>(first + qr / G) * a.n_q + d.z * G + qr % G;
-  const float f = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(a.out + at * HD + dim) =
-      make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
-  if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
+      for (int p = 1; p < J::PARTS; ++p) add(s_ml[p][q8], *reinterpret_cast<const float4*>(&s_o[p][q8][d4]));
+      const long long at = static_cast<long long>(first + qr / G) * a.n_q + d.z * G + qr % G;
+      const float f = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(a.out + at * HD + dim) =
+          make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
+      if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
+    }
+    __syncthreads();
+  };
+  if constexpr (!LONG) {
+    const int4 d = a.desc[blockIdx.x];
+    if (d.x >= 0) join(blockIdx.x, d);
+  } else {
+    const int gx = gridDim.x, x = blockIdx.x;
+    int before = 0;  // unfinished pairs of earlier rounds
+    for (int c0 = 0; c0 < ctas; c0 += J::THREADS) {
+      const bool open = c0 + tid < ctas && a.desc[c0 + tid].x >= 0;
+      const uint32_t votes = __ballot_sync(0xffffffffu, open);
+      if (lane == 0) s_sum[warp] = __popc(votes);
+      __syncthreads();
+      int number = before + __popc(votes & ((1u << lane) - 1)), total = 0;
+      for (int w = 0; w < J::THREADS / 32; ++w) {
+        if (w < warp) number += s_sum[w];
+        total += s_sum[w];
+      }
+      const int had = (before + gx - 1 - x) / gx;  // of this CTA's pairs
+      if (open && number % gx == x) s_mine[number / gx - had] = c0 + tid;
+      before += total;
+      const int mine = (before + gx - 1 - x) / gx - had;
+      __syncthreads();
+      for (int j = 0; j < mine; ++j) join(s_mine[j], a.desc[s_mine[j]]);
+      __syncthreads();
+    }
+  }
 }
 
 }  // namespace mk

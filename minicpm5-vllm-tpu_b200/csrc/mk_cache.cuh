@@ -45,29 +45,24 @@ __device__ __forceinline__ int quant1(float x, float s) {
   return max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))));
 }
 
-// The same for eight values at once without a division: t = x * (1 / s) + 1.5 * 2^23 is the nearest integer (ties
-// to even) to within the product's rounding, in the low bits of t.  The quotient and the product differ by less
-// than 2^-22 of 127, so the integers can differ only where the product lies within 2^-14 of a tie; there (one
-// vector in 500 or so) the quotients are taken.  s >= max|x| / 127 up to a rounding, so no integer passes 127.
+// The same for eight values at once, as t with the code in its low byte.  The quotient is formed from inv, the
+// correctly rounded 1 / s, as Markstein's method has it (IBM J. Res. Dev. 34, 1990): with q = RN(x inv), the
+// remainder x - q s is exact and RN(q + remainder * inv) is the correctly rounded quotient, as long as nothing
+// underflows.  Adding 1.5 * 2^23 then rounds it to an integer, ties to even.  (Ties are common: x and the largest value
+// of the page are bf16, and their quotient times 127 hits k + 1/2 exactly once in 400 values.)  s >= max|x| / 127 up to
+// a rounding, so no integer passes 127.
 __device__ __forceinline__ void quant8(const uint4& x, float inv, float s, uint32_t (&t)[8]) {
-  constexpr float kMagic = 12582912.f;
   const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-  float f[8], off = 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 p = unpack_bf16x2(u[e]);
-    f[2 * e] = p.x;
-    f[2 * e + 1] = p.y;
-  }
+    const float f[2] = {p.x, p.y};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float y = fmaf(f[e], inv, kMagic);
-    off = fmaxf(off, fabsf(fmaf(f[e], inv, kMagic - y)));
-    t[e] = __float_as_uint(y);
+    for (int i = 0; i < 2; ++i) {
+      const float q = f[i] * inv;
+      t[2 * e + i] = __float_as_uint(fmaf(fmaf(-q, s, f[i]), inv, q) + 12582912.f);
+    }
   }
-  if (!(off < 0.5f - 0x1p-14f))
-#pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = static_cast<uint32_t>(quant1(f[e], s));
 }
 // the low bytes of four words as one word
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -87,9 +82,9 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
 // Bounds: 2 bytes read and 1 written per element.  One CTA owns one (page, plane, head), so the scale has one
 // writer and nothing is atomic.  A thread's item is 4 tokens x 8 channels: four 16-byte loads, and 32
 // contiguous bytes of the value plane or four 8-byte pieces of the key plane.  The items stay in registers
-// between the maximum and the rounding, so the input is read once.  A CTA has a thread for each item, for 128-token
-// pages one for two.
-__host__ __device__ constexpr int kva_items(int page_shift) { return page_shift == 7 ? 2 : 1; }
+// between the maximum and the rounding, so the input is read once.  A thread has up to four
+// items, so that what a page needs once (its address, the maximum over the CTA, two divisions) is shared by 128 values.
+__host__ __device__ constexpr int kva_items(int page_shift) { return page_shift == 7 ? 4 : page_shift == 6 ? 2 : 1; }
 __host__ __device__ constexpr int kva_threads(int hd, int page_shift) {
   return (((1 << page_shift) / 4 * (hd / 8)) / kva_items(page_shift) + 31) / 32 * 32;
 }
@@ -154,8 +149,8 @@ __global__ void __launch_bounds__(kva_threads(HD, SHIFT))
   const bool again = had && now != was;  // the tokens already there change their codes
   if (threadIdx.x == 0) *sp = now;
   const float inv = __frcp_rn(by);
-  // (a scale so small that its reciprocal is infinite takes the divisions below)
-  const bool fast = finite && inv <= 3.4e38f;
+  // (remainders of scales below 2^-90 could underflow: those take the divisions below)
+  const bool fast = finite && by >= 0x1p-90f;
 
 #pragma unroll
   for (int i = 0; i < KVA_ITEMS; ++i) {
@@ -255,18 +250,19 @@ __global__ void __launch_bounds__(kva_threads(HD, SHIFT))
 // ---------------------------------------------------------------------------------- read back
 // out[r, i] = bf16 of the keys (plane 0) and values of position start[r] + i, zero from count[r] on.
 // An item is 4 tokens x 8 channels of one head, at a 4-token boundary of the cache, as in the append.
+// CTA (x, r, plane * n_kv + head).  Bounds: 1 byte read, 2 written per element.
 constexpr int KVR_THREADS = 256;
+template <int HD>
 __global__ void __launch_bounds__(KVR_THREADS)
     kv_read_kernel(KvPages c, const int32_t* __restrict__ table, int width, const int32_t* __restrict__ start,
                    const int32_t* __restrict__ count, int max_count, __nv_bfloat16* __restrict__ ko,
                    __nv_bfloat16* __restrict__ vo, int* err) {
+  constexpr int hd = HD, chunks = HD / 8;
   pdl_wait();
   pdl_trigger();
-  const int row = blockIdx.y, plane = blockIdx.z;
-  const int hd = c.head_dim, chunks = hd >> 3, per_group = chunks * c.n_kv;
+  const int row = blockIdx.y, plane = blockIdx.z >= c.n_kv, head = blockIdx.z - (plane ? c.n_kv : 0);
   const int s0 = start[row], n = s0 < 0 ? 0 : min(count[row], max_count);
-  const int it = blockIdx.x * KVR_THREADS + threadIdx.x;
-  const int g = it / per_group, hc = it - g * per_group, head = hc / chunks, ch = hc - head * chunks;
+  const int it = blockIdx.x * KVR_THREADS + threadIdx.x, g = it / chunks, ch = it % chunks;
   const int lead = max(s0, 0) & 3;           // tokens of the first group before the range
   const int i0 = 4 * g - lead;               // output row of the group's first token
   if (i0 >= max_count) return;
@@ -279,7 +275,7 @@ __global__ void __launch_bounds__(KVR_THREADS)
       const int8_t* src = kv_head_ptr(c, page, plane, head);
       const float sc = *kv_scale_ptr(c, page, plane, head);
       if (plane) {
-        const uint4* p = reinterpret_cast<const uint4*>(src + static_cast<size_t>(in) * hd + ch * 32);
+        const uint4* p = reinterpret_cast<const uint4*>(src + in * hd + ch * 32);
         const uint4 lo = p[0], hi = p[1];
         const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -291,7 +287,7 @@ __global__ void __launch_bounds__(KVR_THREADS)
       } else {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const uint2 p = *reinterpret_cast<const uint2*>(src + static_cast<size_t>(in + t) * hd + ch * 8);
+          const uint2 p = *reinterpret_cast<const uint2*>(src + (in + t) * hd + ch * 8);
           const uint32_t w[2] = {p.x, p.y};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -301,14 +297,13 @@ __global__ void __launch_bounds__(KVR_THREADS)
       }
     }
   }
-  __nv_bfloat16* out = plane ? vo : ko;
+  const size_t ld = static_cast<size_t>(c.n_kv) * hd;
+  __nv_bfloat16* out = (plane ? vo : ko) + static_cast<size_t>(row) * max_count * ld + head * hd + ch * 8;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const int i = i0 + t;
     if (i < 0 || i >= max_count) continue;
-    const bool in = i < n;
-    *reinterpret_cast<uint4*>(out + ((static_cast<size_t>(row) * max_count + i) * c.n_kv + head) * hd + ch * 8) =
-        in ? make_uint4(u[t][0], u[t][1], u[t][2], u[t][3]) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(out + i * ld) = i < n ? make_uint4(u[t][0], u[t][1], u[t][2], u[t][3]) : make_uint4(0, 0, 0, 0);
   }
 }
 

@@ -104,15 +104,20 @@ mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, 
   a.rank = ranks;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  // CTAs per row: eight fit on an SM.  Rows are shared while the GPU has room for twice the CTAs and every one
-  // keeps at least two steps' 8192 logits.
+  // A row is shared by as many CTAs (up to eight) as still have two steps' 8192 logits each, while the GPU has room:
+  // 512 threads run two to an SM.
   int cluster = 1;
-  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= static_cast<int64_t>(d.sm_count) * 8 &&
-         V / (cluster * 2) >= 2 * mk::TL_THREADS * mk::TL_VALUES)
+  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= static_cast<int64_t>(d.sm_count) * 2 &&
+         V / (cluster * 2) >= 8192)
     cluster *= 2;
-  void (*k)(mk::LogitsArgs, int) =
-      logits_bits == 32 ? mk::token_logprobs_kernel<float> : mk::token_logprobs_kernel<__nv_bfloat16>;
-  return launch_k_cluster(cluster, k, dim3(static_cast<unsigned>(T) * cluster), dim3(mk::TL_THREADS), 0, st, true, a, cluster);
+  if (cluster > 1) {
+    void (*k)(mk::LogitsArgs, int) = logits_bits == 32 ? mk::token_logprobs_kernel<float, mk::TL_MANY>
+                                                       : mk::token_logprobs_kernel<__nv_bfloat16, mk::TL_MANY>;
+    return launch_k_cluster(cluster, k, dim3(static_cast<unsigned>(T) * cluster), dim3(mk::TL_MANY), 0, st, true, a, cluster);
+  }
+  void (*k)(mk::LogitsArgs, int) = logits_bits == 32 ? mk::token_logprobs_kernel<float, mk::TL_FEW>
+                                                     : mk::token_logprobs_kernel<__nv_bfloat16, mk::TL_FEW>;
+  return launch_k(k, dim3(static_cast<unsigned>(T)), dim3(mk::TL_FEW), 0, st, true, a, 1);
 }
 
 mk_status mk_score_tokens_workspace(int32_t T, int32_t H, int32_t V, size_t* bytes) {
@@ -158,12 +163,13 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   a.target_logit = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_bytes(T, V));
   a.err = d.err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int tiles = a.id_tiles * a.tok_tiles;
+  const int tiles = a.id_tiles * a.tok_tiles, units = std::min(pair ? pairs : d.sm_count, tiles);
+  a.parts = a.tok_tiles == 1 ? units : a.id_tiles;
   if (pair)
-    MK_TRY(launch_k_pair(mk::score_tokens_kernel<true>, dim3(2 * std::min(pairs, tiles)), dim3(mk::SC_THREADS),
+    MK_TRY(launch_k_pair(mk::score_tokens_kernel<true>, dim3(2 * units), dim3(mk::SC_THREADS),
                          mk::SC_SMEM_BYTES, st, true, mh, mw, a));
   else
-    MK_TRY(launch_k(mk::score_tokens_kernel<false>, dim3(std::min(d.sm_count, tiles)), dim3(mk::SC_THREADS),
+    MK_TRY(launch_k(mk::score_tokens_kernel<false>, dim3(units), dim3(mk::SC_THREADS),
                     mk::SC_SMEM_BYTES, st, true, mh, mw, a));
   return launch_k(mk::score_join_kernel, dim3((T + mk::SJ_TOKENS - 1) / mk::SJ_TOKENS), dim3(mk::SJ_THREADS), 0, st, true, a, logprobs, entropy);
 }

@@ -93,13 +93,15 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 // it is taken after the first 1024 logits of the warp, again when four times as many have been seen, and so on,
 // and the largest that any warp of the CTA has published serves them all.  16-byte vectors that hold a logit
 // that reaches it go into a list in shared memory; at the end their logits are cut to what reaches the last tau
-// and put in order by counting.  No warp waits for another before the end.  Rows that defeat it (long runs of
+// and put in order by counting.  After the first step no warp waits for another before the end.  Rows that defeat it (long runs of
 // equal or rising logits that fill the list; fewer than k logits above -inf) fall back to one search of the slice
 // for each alternative missing.
 //
 // What bounds it: the bytes of the logits.  Per bf16 logit the arithmetic is about six instructions and one
 // exponential, two thirds of what an SM can issue at the rate at which HBM delivers them.
-constexpr int TL_THREADS = 128;   // (256: the work at a row's end, the same for every warp, was a third of all)
+// Threads per CTA.  128 where there are rows enough (the work at a row's end is the same for every warp, and with
+// 256 threads it was a third of all); 512 where a cluster shares a row, so that a slice of 16384 logits is one step.
+constexpr int TL_FEW = 128, TL_MANY = 512;
 constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
 constexpr int TL_LIST = 512;      // vectors listed
@@ -137,8 +139,8 @@ struct LogitsArgs {
   float* top_lp;
 };
 
-template <typename E>
-__global__ void __launch_bounds__(TL_THREADS, 8) token_logprobs_kernel(const LogitsArgs a, const int cluster) {
+template <typename E, int TL_THREADS>
+__global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_kernel(const LogitsArgs a, const int cluster) {
   constexpr bool BF = sizeof(E) == 2;
   constexpr int EPV = 16 / sizeof(E);            // logits per 16-byte vector
   constexpr int VECS = TL_VALUES / EPV;          // vectors per thread and step
@@ -306,6 +308,7 @@ __global__ void __launch_bounds__(TL_THREADS, 8) token_logprobs_kernel(const Log
       if (step == retake) {
         threshold();
         if (lane == 0) s_tau[wp] = tau;
+        if (step == 0) __syncthreads();  // the list begins with the best tau of all warps
         retake = step * 4 + 3;
       }
 #pragma unroll
@@ -490,7 +493,8 @@ struct ScoreArgs {
   int rows;             // token rows that a CTA loads per tile
   const int32_t* targets;
   float scale;          // logit scale * log2 e: the statistics are in units of log 2
-  float* part;          // [id tiles][3][ld_part]: m, z, w
+  int parts;            // per token: one for each id tile, or for each CTA (pair) where it has one token tile only
+  float* part;          // [parts][3][ld_part]: m, z, w
   long long ld_part;    // T rounded up
   float* target_logit;  // [T]
   int* err;
@@ -652,6 +656,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
     }
   } else {
     const int q = warp & 3;  // the TMEM quarter that this warp may read
+    // with one token tile a thread's token stays the same and its statistics go on from tile to tile
+    const bool go_on = args.tok_tiles == 1;
+    float m = -INFINITY, z = 0.f, w = 0.f;
     pdl_wait();
     for (int it = 0; it < my_tiles; ++it) {
       const int a = it & 1, vt = id_tile(it), t = tok0(it) + q * 32 + lane, v0 = vt * SC_V;
@@ -659,7 +666,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
       const int nv = min(SC_V, args.V - v0);
       if (!mbar_wait(&tfull[a], (it >> 1) & 1, abort_flag)) break;
       tc_fence_after();
-      float m = -INFINITY, z = 0.f, w = 0.f;
+      if (!go_on) {
+        m = -INFINITY;
+        z = w = 0.f;
+      }
 #pragma unroll 1
       for (int c0 = 0; c0 < nv; c0 += 32) {
         uint32_t acc[32];
@@ -707,8 +717,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1)
         else
           mbar_arrive(&tempty[a]);
       }
-      if (t < args.T) {
-        float* p = args.part + static_cast<long long>(vt) * 3 * args.ld_part + t;
+      if (t < args.T && (!go_on || it + 1 == my_tiles)) {
+        float* p = args.part + static_cast<long long>(go_on ? unit : vt) * 3 * args.ld_part + t;
         p[0] = m;
         p[args.ld_part] = z;
         p[2 * args.ld_part] = w;
@@ -738,7 +748,7 @@ __device__ __forceinline__ RowStats stats_join2(const RowStats& a, const RowStat
   r.w = (a.w + a.z * fmaxf(da, kFar)) * ea + (b.w + b.z * fmaxf(db, kFar)) * eb;
   return r;
 }
-// Joins a token's id tiles: 8 tokens x 128 slices of the tiles per CTA; a slice in order, then the slices in a
+// Joins a token's parts: 8 tokens x 128 slices of the parts per CTA; a slice in order, then the slices in a
 // fixed order.
 constexpr int SJ_TOKENS = 8;
 constexpr int SJ_THREADS = 1024;
@@ -752,7 +762,7 @@ __global__ void __launch_bounds__(SJ_THREADS)
   RowStats s = stats_empty();
   if (t < args.T) {
 #pragma unroll 4
-    for (int vt = threadIdx.x / SJ_TOKENS; vt < args.id_tiles; vt += SJ_THREADS / SJ_TOKENS) {
+    for (int vt = threadIdx.x / SJ_TOKENS; vt < args.parts; vt += SJ_THREADS / SJ_TOKENS) {
       const float* p = args.part + static_cast<long long>(vt) * 3 * args.ld_part + t;
       s = stats_join2(s, {p[0], p[args.ld_part], p[2 * args.ld_part]});
     }
