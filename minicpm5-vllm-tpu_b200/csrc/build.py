@@ -1,10 +1,11 @@
-"""Build libminicpm5_mk.so (sm_100a) in-tree next to the Python package.
+"""Build libminicpm5_mk.so (sm_100a) and _mk_torch.so in-tree next to the Python package.
 
     python minicpm5-vllm-tpu_b200/csrc/build.py [--force] [--verbose]
 
 nvcc cross-compiles for sm_100a without a GPU.  The library links the CUDA runtime statically and
 takes the driver entry point it needs (cuTensorMapEncodeTiled) through cudaGetDriverEntryPoint, so
-it does not depend on torch or on libcuda at link time.
+it does not depend on torch or on libcuda at link time.  _mk_torch.so is the torch side of the cache and scoring
+operators (host code only, compiled with g++ against torch's headers).
 """
 
 from __future__ import annotations
@@ -23,6 +24,10 @@ OUT = os.path.join(PKG_ROOT, "minicpm5_mk", "libminicpm5_mk.so")
 SOURCES = [os.path.join(HERE, f) for f in ("mk_api.cu", "mk_cache.cu", "mk_score.cu")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
               "-shared", "-Xptxas", "-v", "--threads", "0"]
+
+
+TORCH_OUT = os.path.join(PKG_ROOT, "minicpm5_mk", "_mk_torch.so")
+TORCH_SOURCE = os.path.join(HERE, "mk_torch.cpp")
 
 
 def _nvcc() -> str:
@@ -44,7 +49,33 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in _inputs())
 
 
+def build_torch(force: bool = False) -> str:
+    """The torch-side module, when it is older than its source or the header."""
+    inputs = [TORCH_SOURCE, os.path.join(REPO, "include", "minicpm5_mk.h"), os.path.abspath(__file__)]
+    if not force and os.path.exists(TORCH_OUT) and all(os.path.getmtime(p) <= os.path.getmtime(TORCH_OUT) for p in inputs):
+        return TORCH_OUT
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wno-deprecated",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[a for p in include for a in ("-isystem", p)], TORCH_SOURCE, "-o", TORCH_OUT + ".tmp",
+           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath," + os.path.join(root, "lib")]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"g++ failed ({r.returncode})")
+    os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
+    return TORCH_OUT
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_torch(force)
     if not force and up_to_date():
         return OUT
     cmd = [_nvcc(), *NVCC_FLAGS, "-o", OUT + ".tmp", *SOURCES]

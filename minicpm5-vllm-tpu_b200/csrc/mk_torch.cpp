@@ -1,0 +1,403 @@
+// torch side of the cache and scoring operators (minicpm5_mk/ops.py): argument checks, output tensors and the call
+// into the C ABI, in one step of C++.  In Python the same costs 8 to 15 us a call, more than several of the
+// kernels run for.  The C entry points arrive as addresses from the library that ctypes has loaded
+// (minicpm5_mk/_lib.py), so this module links to torch alone and the library still to nothing.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <sstream>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/minicpm5_mk.h"
+
+namespace {
+
+using at::Tensor;
+
+// Every entry point that this module calls, in the order in which bind() takes their addresses.
+#define MK_TORCH_ENTRIES(X)                                                                                              \
+  X(mk_kv_append) X(mk_kv_read) X(mk_attention_paged_workspace) X(mk_attention_paged) X(mk_kv_move_workspace)            \
+  X(mk_kv_fork) X(mk_kv_reserve) X(mk_kv_compact) X(mk_token_logprobs) X(mk_score_tokens_workspace) X(mk_score_tokens)
+struct Entries {
+#define X(name) decltype(&::name) name = nullptr;
+  MK_TORCH_ENTRIES(X)
+#undef X
+} g;
+PyObject* g_error = nullptr;   // minicpm5_mk._lib.MkError
+PyObject* g_memory = nullptr;  // torch.OutOfMemoryError
+
+struct BadArgument : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+struct BadStatus {
+  const char* what;
+  int status;
+};
+
+void check(mk_status s, const char* what) {
+  if (s != MK_OK) throw BadStatus{what, static_cast<int>(s)};
+}
+
+[[noreturn]] void refuse(const std::string& why) { throw BadArgument("minicpm5_mk: " + why); }
+
+std::string describe(const Tensor& t) {
+  std::ostringstream s;
+  s << t.sizes() << " " << t.scalar_type() << " on " << t.device() << (t.is_contiguous() ? "" : " (strided)");
+  return s.str();
+}
+
+// ------------------------------------------------------------------------------------- arguments
+const Tensor& tensor(PyObject* o, const char* name) {
+  if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
+  return THPVariable_Unpack(o);
+}
+Tensor tensor_or_none(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor(o, name); }
+int32_t integer(PyObject* o, const char* name) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(std::string(name) + " must be an integer");
+  }
+  if (v < INT32_MIN || v > INT32_MAX) refuse(std::string(name) + " is out of range");
+  return static_cast<int32_t>(v);
+}
+float number(PyObject* o, const char* name) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(std::string(name) + " must be a number");
+  }
+  return static_cast<float>(v);
+}
+int32_t size32(const Tensor& t, int d, const char* name) {
+  if (t.size(d) > INT32_MAX) refuse(std::string(name) + " is too large");
+  return static_cast<int32_t>(t.size(d));
+}
+
+void need(const Tensor& t, const char* name, at::ScalarType type, int dim, const at::Device& dev) {
+  if (t.scalar_type() != type || t.dim() != dim || t.device() != dev || !t.is_contiguous()) {
+    std::ostringstream s;
+    s << name << " must be a contiguous " << dim << "-d " << type << " tensor on " << dev << ", got " << describe(t);
+    refuse(s.str());
+  }
+}
+void rows_of(const Tensor& t, const char* name, int64_t rows, const at::Device& dev) {
+  need(t, name, at::kInt, 1, dev);
+  if (t.size(0) != rows) {
+    std::ostringstream s;
+    s << name << " has " << t.size(0) << " entries for " << rows << " rows";
+    refuse(s.str());
+  }
+}
+void heads(const Tensor& t, const char* name, const at::Device& dev, int64_t n, int64_t hd) {
+  if (t.scalar_type() != at::kBFloat16 || t.dim() != 3 || t.device() != dev || (n >= 0 && t.size(1) != n) ||
+      t.size(2) != hd || t.stride(2) != 1) {
+    std::ostringstream s;
+    s << name << " must be bf16 [tokens, heads, " << hd << "] on " << dev << " with unit stride inside a head"
+      << (n >= 0 ? " and " + std::to_string(n) + " heads" : std::string()) << ", got " << describe(t);
+    refuse(s.str());
+  }
+}
+void starts_of(const Tensor& cu, const char* name, int64_t rows, int64_t tokens, const at::Device& dev) {
+  if (!cu.defined()) {
+    if (tokens != rows) {
+      std::ostringstream s;
+      s << "without " << name << " there is one token per row: " << tokens << " tokens, " << rows << " rows";
+      refuse(s.str());
+    }
+    return;
+  }
+  need(cu, name, at::kInt, 1, dev);
+  if (cu.size(0) != rows + 1) {
+    std::ostringstream s;
+    s << name << " has " << cu.size(0) << " entries for " << rows << " rows";
+    refuse(s.str());
+  }
+}
+
+// codes [(layers,) pages, 2, n_kv, page, head_dim] and their scales
+struct Pages {
+  at::Device dev = at::kCPU;
+  void* codes;
+  float* scales;
+  int32_t layers, pages, n_kv, page, hd;
+  Pages(const Tensor& c, const Tensor& s, bool all_layers) {
+    const int dim = all_layers ? 6 : 5;
+    if (!c.is_cuda()) refuse("codes must be a CUDA tensor");
+    dev = c.device();
+    need(c, "codes", at::kChar, dim, dev);
+    need(s, "scales", at::kFloat, dim - 2, dev);
+    if (c.size(dim - 4) != 2 || s.sizes() != c.sizes().slice(0, dim - 2)) {
+      std::ostringstream m;
+      m << "codes are [" << (all_layers ? "layers, " : "") << "pages, 2, n_kv, page, head_dim] and scales ["
+        << (all_layers ? "layers, " : "") << "pages, 2, n_kv], got " << c.sizes() << " and " << s.sizes();
+      refuse(m.str());
+    }
+    codes = c.data_ptr();
+    scales = static_cast<float*>(s.data_ptr());
+    layers = all_layers ? size32(c, 0, "codes") : 1;
+    pages = size32(c, dim - 5, "codes");
+    n_kv = size32(c, dim - 3, "codes");
+    page = size32(c, dim - 2, "codes");
+    hd = size32(c, dim - 1, "codes");
+  }
+};
+
+const int32_t* ids(const Tensor& t) { return t.defined() ? static_cast<const int32_t*>(t.data_ptr()) : nullptr; }
+int32_t* ids_out(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+float* floats(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+void* stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::empty(sizes, at::TensorOptions().dtype(type).device(dev));
+}
+Tensor bytes(size_t n, const at::Device& dev) { return empty({static_cast<int64_t>(n)}, at::kByte, dev); }
+
+PyObject* tuple(std::initializer_list<Tensor> ts) {
+  PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  if (!out) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor& t : ts) {
+    PyObject* o = THPVariable_Wrap(t);
+    if (!o) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i++, o);
+  }
+  return out;
+}
+
+// ------------------------------------------------------------------------------------- operators
+using Args = PyObject* const*;
+
+PyObject* kv_append(Args a) {
+  const Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &table = tensor(a[4], "block_table"),
+               &lens = tensor(a[5], "lens");
+  const Pages c(tensor(a[2], "codes"), tensor(a[3], "scales"), false);
+  const Tensor cu = tensor_or_none(a[6], "cu_new");
+  heads(k, "k", c.dev, c.n_kv, c.hd);
+  heads(v, "v", c.dev, c.n_kv, c.hd);
+  if (k.size(0) != v.size(0)) refuse("k and v have different numbers of tokens");
+  need(table, "block_table", at::kInt, 2, c.dev);
+  rows_of(lens, "lens", table.size(0), c.dev);
+  starts_of(cu, "cu_new", table.size(0), k.size(0), c.dev);
+  const c10::cuda::OptionalCUDAGuard guard(c.dev);
+  check(g.mk_kv_append(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), size32(k, 0, "k"),
+                       c.codes, c.scales, c.pages, c.n_kv, c.page, c.hd, ids(table), size32(table, 0, "block_table"),
+                       size32(table, 1, "block_table"), ids(lens), ids(cu), integer(a[7], "max_new"), stream_of(c.dev)),
+        "mk_kv_append");
+  Py_RETURN_NONE;
+}
+
+PyObject* kv_read(Args a) {
+  const Pages c(tensor(a[0], "codes"), tensor(a[1], "scales"), false);
+  const Tensor &table = tensor(a[2], "block_table"), &start = tensor(a[3], "start"), &count = tensor(a[4], "count");
+  const int32_t most = integer(a[5], "max_count");
+  need(table, "block_table", at::kInt, 2, c.dev);
+  rows_of(start, "start", table.size(0), c.dev);
+  rows_of(count, "count", table.size(0), c.dev);
+  if (most < 0) throw BadStatus{"mk_kv_read", MK_ERR_BAD_SHAPE};
+  const c10::cuda::OptionalCUDAGuard guard(c.dev);
+  const Tensor k = empty({table.size(0), most, c.n_kv, c.hd}, at::kBFloat16, c.dev), v = at::empty_like(k);
+  check(g.mk_kv_read(c.codes, c.scales, c.pages, c.n_kv, c.page, c.hd, ids(table), size32(table, 0, "block_table"),
+                     size32(table, 1, "block_table"), ids(start), ids(count), most, k.data_ptr(), v.data_ptr(),
+                     stream_of(c.dev)),
+        "mk_kv_read");
+  return tuple({k, v});
+}
+
+PyObject* attention_paged(Args a) {
+  const Tensor &q = tensor(a[0], "q"), &table = tensor(a[3], "block_table"), &lens = tensor(a[4], "lens");
+  const Pages c(tensor(a[1], "codes"), tensor(a[2], "scales"), false);
+  const Tensor cu = tensor_or_none(a[5], "cu_q");
+  heads(q, "q", c.dev, -1, c.hd);
+  need(table, "block_table", at::kInt, 2, c.dev);
+  rows_of(lens, "lens", table.size(0), c.dev);
+  starts_of(cu, "cu_q", table.size(0), q.size(0), c.dev);
+  const int32_t T = size32(q, 0, "q"), n_q = size32(q, 1, "q"), rows = size32(table, 0, "block_table");
+  const int32_t width = size32(table, 1, "block_table"), max_q = integer(a[6], "max_q");
+  const int32_t max_len = a[7] == Py_None
+                              ? static_cast<int32_t>(std::min<int64_t>(INT32_MAX, static_cast<int64_t>(width) * c.page))
+                              : integer(a[7], "max_len");
+  size_t n = 0;
+  check(g.mk_attention_paged_workspace(T, n_q, c.n_kv, c.hd, rows, max_q, max_len, &n), "mk_attention_paged_workspace");
+  const c10::cuda::OptionalCUDAGuard guard(c.dev);
+  const Tensor ws = bytes(n, c.dev), out = empty({T, n_q, c.hd}, at::kBFloat16, c.dev), lse = empty({T, n_q}, at::kFloat, c.dev);
+  check(g.mk_attention_paged(q.data_ptr(), q.stride(0), q.stride(1), T, n_q, c.codes, c.scales, c.pages, c.n_kv, c.page, c.hd,
+                             ids(table), rows, width, ids(lens), ids(cu), max_q, max_len, number(a[8], "softmax_scale"),
+                             out.data_ptr(), floats(lse), ws.data_ptr(), n, stream_of(c.dev)),
+        "mk_attention_paged");
+  return tuple({out, lse});
+}
+
+PyObject* kv_fork(Args a) {
+  const Pages c(tensor(a[0], "codes"), tensor(a[1], "scales"), true);
+  const Tensor &table = tensor(a[2], "block_table"), &lens = tensor(a[3], "lens"), &refs = tensor(a[4], "refs"),
+               &parents = tensor(a[5], "parents");
+  need(table, "block_table", at::kInt, 2, c.dev);
+  rows_of(lens, "lens", table.size(0), c.dev);
+  rows_of(refs, "refs", c.pages, c.dev);
+  need(parents, "parents", at::kInt, 1, c.dev);
+  const int32_t R = size32(parents, 0, "parents"), width = size32(table, 1, "block_table");
+  const c10::cuda::OptionalCUDAGuard guard(c.dev);
+  const Tensor out = empty({R, width}, at::kInt, c.dev), new_lens = empty({R}, at::kInt, c.dev), new_refs = at::empty_like(refs);
+  const size_t n = g.mk_kv_move_workspace(R, c.pages);
+  const Tensor ws = bytes(n, c.dev);
+  check(g.mk_kv_fork(c.codes, c.scales, c.layers, c.pages, c.n_kv, c.page, c.hd, ids(table), ids(lens),
+                     size32(table, 0, "block_table"), width, ids(parents), R, ids_out(out), ids_out(new_lens),
+                     ids_out(new_refs), ws.data_ptr(), n, stream_of(c.dev)),
+        "mk_kv_fork");
+  return tuple({out, new_lens, new_refs});
+}
+
+PyObject* kv_reserve(Args a) {
+  const Tensor &table = tensor(a[0], "block_table"), &lens = tensor(a[1], "lens"), &refs = tensor(a[2], "refs");
+  const Tensor n_new = tensor_or_none(a[3], "n_new");
+  if (!table.is_cuda()) refuse("block_table must be a CUDA tensor");
+  const at::Device dev = table.device();
+  need(table, "block_table", at::kInt, 2, dev);
+  rows_of(lens, "lens", table.size(0), dev);
+  need(refs, "refs", at::kInt, 1, dev);
+  if (n_new.defined()) rows_of(n_new, "n_new", table.size(0), dev);
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  check(g.mk_kv_reserve(ids_out(table), ids(lens), size32(table, 0, "block_table"), size32(table, 1, "block_table"), ids(n_new),
+                        ids_out(refs), size32(refs, 0, "refs"), integer(a[4], "page"), stream_of(dev)),
+        "mk_kv_reserve");
+  Py_RETURN_NONE;
+}
+
+PyObject* kv_compact(Args a) {
+  const Pages c(tensor(a[0], "codes"), tensor(a[1], "scales"), true);
+  const Tensor &table = tensor(a[2], "block_table"), &refs = tensor(a[3], "refs");
+  need(table, "block_table", at::kInt, 2, c.dev);
+  rows_of(refs, "refs", c.pages, c.dev);
+  const int32_t rows = size32(table, 0, "block_table");
+  const c10::cuda::OptionalCUDAGuard guard(c.dev);
+  const Tensor out = at::empty_like(table), new_refs = at::empty_like(refs), used = empty({1}, at::kInt, c.dev);
+  const size_t n = g.mk_kv_move_workspace(rows, c.pages);
+  const Tensor ws = bytes(n, c.dev);
+  check(g.mk_kv_compact(c.codes, c.scales, c.layers, c.pages, c.n_kv, c.page, c.hd, ids(table), rows,
+                        size32(table, 1, "block_table"), ids(refs), ids_out(out), ids_out(new_refs), ids_out(used),
+                        ws.data_ptr(), n, stream_of(c.dev)),
+        "mk_kv_compact");
+  return tuple({out, new_refs, used});
+}
+
+PyObject* token_logprobs(Args a) {
+  const Tensor &x = tensor(a[0], "logits"), &targets = tensor(a[1], "targets");
+  const int32_t k = integer(a[2], "top_k");
+  if (!x.is_cuda() || x.dim() != 2 || (x.scalar_type() != at::kFloat && x.scalar_type() != at::kBFloat16) ||
+      (x.size(1) > 1 && x.stride(1) != 1))
+    refuse("logits must be a row-major f32 or bf16 [T, V] CUDA tensor, got " + describe(x));
+  const at::Device dev = x.device();
+  rows_of(targets, "targets", x.size(0), dev);
+  const int32_t T = size32(x, 0, "logits"), V = size32(x, 1, "logits");
+  if (k < 0) throw BadStatus{"mk_token_logprobs", MK_ERR_BAD_SHAPE};
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const Tensor lp = empty({T}, at::kFloat, dev), ent = empty({T}, at::kFloat, dev), rank = empty({T}, at::kInt, dev),
+               top = empty({T, k}, at::kInt, dev), top_lp = empty({T, k}, at::kFloat, dev);
+  check(g.mk_token_logprobs(x.data_ptr(), x.scalar_type() == at::kFloat ? 32 : 16, T, V, x.stride(0), ids(targets), k,
+                            floats(lp), floats(ent), ids_out(rank), ids_out(top), floats(top_lp), stream_of(dev)),
+        "mk_token_logprobs");
+  return tuple({lp, ent, rank, top, top_lp});
+}
+
+PyObject* score_tokens(Args a) {
+  const Tensor &h = tensor(a[0], "h"), &w = tensor(a[1], "lm_head"), &targets = tensor(a[2], "targets");
+  if (!h.is_cuda() || h.dim() != 2 || h.scalar_type() != at::kBFloat16 || (h.size(1) > 1 && h.stride(1) != 1))
+    refuse("h must be a row-major bf16 [T, H] CUDA tensor, got " + describe(h));
+  const at::Device dev = h.device();
+  need(w, "lm_head", at::kBFloat16, 2, dev);
+  if (w.size(1) != h.size(1)) refuse("h is " + describe(h) + ", lm_head " + describe(w));
+  rows_of(targets, "targets", h.size(0), dev);
+  const int32_t T = size32(h, 0, "h"), H = size32(h, 1, "h"), V = size32(w, 0, "lm_head");
+  size_t n = 0;
+  check(g.mk_score_tokens_workspace(T, H, V, &n), "mk_score_tokens_workspace");
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const Tensor ws = bytes(n, dev), lp = empty({T}, at::kFloat, dev), ent = empty({T}, at::kFloat, dev);
+  // (the stride of a single row says nothing)
+  check(g.mk_score_tokens(h.data_ptr(), T, H, T > 1 ? h.stride(0) : H, w.data_ptr(), V, ids(targets), number(a[3], "logit_scale"),
+                          floats(lp), floats(ent), ws.data_ptr(), n, stream_of(dev)),
+        "mk_score_tokens");
+  return tuple({lp, ent});
+}
+
+// bind(MkError, torch.OutOfMemoryError, address, ...): the error classes and the library's entry points.
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  void** to[] = {
+#define X(name) reinterpret_cast<void**>(&g.name),
+      MK_TORCH_ENTRIES(X)
+#undef X
+  };
+  const Py_ssize_t entries = sizeof(to) / sizeof(to[0]);
+  if (n != entries + 2) {
+    PyErr_Format(PyExc_TypeError, "bind takes %zd arguments", entries + 2);
+    return nullptr;
+  }
+  for (Py_ssize_t i = 0; i < entries; ++i) {
+    void* p = PyLong_AsVoidPtr(a[i + 2]);
+    if (!p) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point");
+      return nullptr;
+    }
+    *to[i] = p;
+  }
+  Py_INCREF(a[0]);
+  Py_INCREF(a[1]);
+  Py_XDECREF(g_error);
+  Py_XDECREF(g_memory);
+  g_error = a[0];
+  g_memory = a[1];
+  Py_RETURN_NONE;
+}
+
+// No C++ exception leaves a call: refusals become ValueError, statuses MkError, whatever torch throws RuntimeError.
+template <PyObject* (*F)(Args), int N>
+PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != N) {
+    PyErr_Format(PyExc_TypeError, "%d arguments expected, %zd given", N, n);
+    return nullptr;
+  }
+  if (!g_error) {
+    PyErr_SetString(PyExc_RuntimeError, "minicpm5_mk: the library is not bound");
+    return nullptr;
+  }
+  try {
+    return F(a);
+  } catch (const BadArgument& e) {
+    PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const BadStatus& e) {
+    PyObject* o = PyObject_CallFunction(g_error, "si", e.what, e.status);
+    if (o) {
+      PyErr_SetObject(g_error, o);
+      Py_DECREF(o);
+    }
+  } catch (const c10::OutOfMemoryError& e) {
+    PyErr_SetString(g_memory, e.what());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+#define METHOD(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&call<name, n>)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {
+    {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
+    METHOD(kv_append, 8),
+    METHOD(kv_read, 6),
+    METHOD(attention_paged, 9),
+    METHOD(kv_fork, 6),
+    METHOD(kv_reserve, 5),
+    METHOD(kv_compact, 4),
+    METHOD(token_logprobs, 3),
+    METHOD(score_tokens, 4),
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__mk_torch() { return PyModule_Create(&module); }

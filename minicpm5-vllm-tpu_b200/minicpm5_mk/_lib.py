@@ -131,6 +131,30 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+# The entry points that the torch side (_mk_torch, csrc/mk_torch.cpp) calls, in the order in which it takes them.
+TORCH_ENTRIES = ("mk_kv_append", "mk_kv_read", "mk_attention_paged_workspace", "mk_attention_paged",
+                 "mk_kv_move_workspace", "mk_kv_fork", "mk_kv_reserve", "mk_kv_compact", "mk_token_logprobs",
+                 "mk_score_tokens_workspace", "mk_score_tokens")
+_TORCH = None
+
+
+def torch_side():
+    """The module that checks the tensors of the cache and scoring operators and calls the library for them."""
+    global _TORCH
+    if _TORCH is None:
+        import torch  # first: its libraries are what the module links to
+        try:
+            from . import _mk_torch
+        except ImportError as e:
+            raise RuntimeError("minicpm5_mk: _mk_torch.so is not built, or not for this torch "
+                               "(run `python -c 'import __graft_entry__ as g; g.build()'`)") from e
+        L = lib()
+        _mk_torch.bind(MkError, torch.OutOfMemoryError,
+                       *[ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in TORCH_ENTRIES])
+        _TORCH = _mk_torch
+    return _TORCH
+
+
 def status_string(status: int) -> str:
     try:
         return lib().mk_status_string(int(status)).decode()

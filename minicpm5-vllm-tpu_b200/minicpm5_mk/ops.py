@@ -7,7 +7,6 @@ in libminicpm5_mk.so; nothing falls back to torch.
 from __future__ import annotations
 
 import ctypes
-import functools
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -21,8 +20,7 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(device: torch.device) -> int:
-    # the handle alone: building a torch.cuda.Stream around it costs 2 us, as much as a kernel launch
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _cuda(t: torch.Tensor, name: str) -> None:
@@ -324,251 +322,69 @@ def topk_logprobs(logits: torch.Tensor, k: int = 20):
 # ------------------------------------------------------------------------- 8-bit paged key/value cache
 # codes int8 [num_pages, 2, n_kv, page, head_dim] and scales f32 [num_pages, 2, n_kv] of one layer (the calls
 # that move whole pages take [layers, ...]); the layout is described in include/minicpm5_mk.h.  Tables, lengths
-# and counts are int32 tensors on the device; no call here reads them on the host.
-# The argument checks and the calls are written for the host's time: a decoding step calls these once per layer,
-# and several of the kernels run for less than 10 us.
-_I32, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
-
-
-def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dim: int, device: torch.device) -> None:
-    if t.dtype is not dtype or t.ndim != dim or t.device != device or not t.is_contiguous():
-        raise ValueError(f"minicpm5_mk: {name} must be a contiguous {dim}-d {dtype} tensor on {device}, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}{'' if t.is_contiguous() else ' (strided)'}")
-
-
-def _heads(t: torch.Tensor, name: str, device: torch.device, heads: int, head_dim: int) -> None:
-    if t.dtype is not _BF16 or t.ndim != 3 or t.device != device or t.shape[1] != heads or \
-            t.shape[2] != head_dim or t.stride(2) != 1:
-        raise ValueError(f"minicpm5_mk: {name} must be bf16 [tokens, {heads}, {head_dim}] on {device} with unit "
-                         f"stride inside a head, got {tuple(t.shape)} {t.dtype} on {t.device}")
-
-
-def _pages(codes: torch.Tensor, scales: torch.Tensor, dim: int) -> torch.device:
-    if not codes.is_cuda:
-        raise ValueError("minicpm5_mk: codes must be a CUDA tensor")
-    dev = codes.device
-    _need(codes, "codes", torch.int8, dim, dev)
-    _need(scales, "scales", _F32, dim - 2, dev)
-    shape = codes.shape
-    if scales.shape != shape[:-2] or shape[-4] != 2:
-        raise ValueError("minicpm5_mk: codes are [..., pages, 2, n_kv, page, head_dim] and scales [..., pages, 2, n_kv], "
-                         f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
-    return dev
-
-
-def _table(block_table: torch.Tensor, lens: Optional[torch.Tensor], name: str, dev: torch.device) -> Tuple[int, int]:
-    _need(block_table, "block_table", _I32, 2, dev)
-    rows, width = block_table.shape
-    if lens is not None:
-        _row_values(lens, name, rows, dev)
-    return rows, width
-
-
-def _row_values(t: torch.Tensor, name: str, rows: int, dev: torch.device) -> None:
-    _need(t, name, _I32, 1, dev)
-    if t.shape[0] != rows:
-        raise ValueError(f"minicpm5_mk: {name} has {t.shape[0]} entries for {rows} rows")
-
-
-def _cu(cu: Optional[torch.Tensor], name: str, rows: int, tokens: int, dev: torch.device) -> None:
-    if cu is None:
-        if tokens != rows:
-            raise ValueError(f"minicpm5_mk: without {name} there is one token per row: {tokens} tokens, {rows} rows")
-        return
-    _need(cu, name, _I32, 1, dev)
-    if cu.shape[0] != rows + 1:
-        raise ValueError(f"minicpm5_mk: {name} has {cu.shape[0]} entries for {rows} rows")
-
-
-@functools.lru_cache(maxsize=4096)
-def _attention_workspace(n_q: int, n_kv: int, head_dim: int, rows: int, max_q: int, max_len: int) -> int:
-    n = ctypes.c_size_t()
-    _lib.check(_lib.lib().mk_attention_paged_workspace(0, n_q, n_kv, head_dim, rows, max_q, max_len, ctypes.byref(n)),
-               "mk_attention_paged_workspace")
-    return n.value
-
-
+# and counts are int32 tensors on the device; no call here reads them on the host.  Tensors are checked and outputs
+# allocated in csrc/mk_torch.cpp: a tensor of the wrong type, shape, device or stride raises ValueError, what the
+# library itself refuses MkError.
 def kv_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
               lens: torch.Tensor, cu_new: Optional[torch.Tensor] = None, max_new: int = 1) -> None:
     """Quantise new keys and values (bf16 [T, n_kv, head_dim], strided views allowed) into positions
     lens[r] .. of each row, in place (mk_kv_append).  `cu_new` int32 [rows + 1] gives each row's tokens, None one
     token per row; `max_new` bounds a row's new tokens.  `lens` is not advanced."""
-    dev = _pages(codes, scales, 5)
-    P, _, n_kv, page, hd = codes.shape
-    _heads(k, "k", dev, n_kv, hd)
-    _heads(v, "v", dev, n_kv, hd)
-    if k.shape[0] != v.shape[0]:
-        raise ValueError("minicpm5_mk: k and v have different numbers of tokens")
-    rows, width = _table(block_table, lens, "lens", dev)
-    _cu(cu_new, "cu_new", rows, k.shape[0], dev)
-    st = _lib.lib().mk_kv_append(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                 k.shape[0], codes.data_ptr(), scales.data_ptr(), P, n_kv, page, hd,
-                                 block_table.data_ptr(), rows, width, lens.data_ptr(), _ptr(cu_new), int(max_new),
-                                 _stream(dev))
-    _lib.check(st, "mk_kv_append")
+    _lib.torch_side().kv_append(k, v, codes, scales, block_table, lens, cu_new, max_new)
 
 
 def kv_read(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
-            count: torch.Tensor, max_count: int):
+            count: torch.Tensor, max_count: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """Positions start[r] .. start[r] + count[r] - 1 of each row as (k, v) bf16 [rows, max_count, n_kv, head_dim],
     zeros from count[r] on (mk_kv_read)."""
-    dev = _pages(codes, scales, 5)
-    P, _, n_kv, page, hd = codes.shape
-    rows, width = _table(block_table, start, "start", dev)
-    _row_values(count, "count", rows, dev)
-    k = torch.empty(rows, int(max_count), n_kv, hd, dtype=_BF16, device=dev)
-    v = torch.empty_like(k)
-    st = _lib.lib().mk_kv_read(codes.data_ptr(), scales.data_ptr(), P, n_kv, page, hd, block_table.data_ptr(), rows,
-                               width, start.data_ptr(), count.data_ptr(), int(max_count), k.data_ptr(), v.data_ptr(),
-                               _stream(dev))
-    _lib.check(st, "mk_kv_read")
-    return k, v
+    return _lib.torch_side().kv_read(codes, scales, block_table, start, count, max_count)
 
 
 def attention_paged(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
                     lens: torch.Tensor, cu_q: Optional[torch.Tensor] = None, max_q: int = 1,
-                    max_len: Optional[int] = None, softmax_scale: float = 1.0):
+                    max_len: Optional[int] = None, softmax_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """Attention of each row's last tokens over its cached keys and values (mk_attention_paged): (out bf16
     [T, n_q, head_dim], lse f32 [T, n_q]).  q bf16 [T, n_q, head_dim] (strided views allowed); lens counts the
     queries' own tokens; cu_q int32 [rows + 1] gives each row's queries, None one per row.  `max_q` and `max_len`
-    say what the queries and tokens of a row reach, for the launch shape (max_len None: what the table holds).  A query that sees no key
-    gives zeros and lse -inf."""
-    dev = _pages(codes, scales, 5)
-    P, _, n_kv, page, hd = codes.shape
-    T, n_q = q.shape[0], q.shape[1]
-    _heads(q, "q", dev, n_q, hd)
-    rows, width = _table(block_table, lens, "lens", dev)
-    _cu(cu_q, "cu_q", rows, T, dev)
-    # a multiple of the 64 keys that the plan counts in, so that a growing row asks for the size again only then
-    max_len = width * page if max_len is None else int(max_len) if max_len <= 0 else -(-int(max_len) // 64) * 64
-    nbytes = _attention_workspace(n_q, n_kv, hd, rows, int(max_q), max_len)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    out = torch.empty(T, n_q, hd, dtype=_BF16, device=dev)
-    lse = torch.empty(T, n_q, dtype=_F32, device=dev)
-    st = _lib.lib().mk_attention_paged(q.data_ptr(), q.stride(0), q.stride(1), T, n_q, codes.data_ptr(),
-                                       scales.data_ptr(), P, n_kv, page, hd, block_table.data_ptr(), rows, width,
-                                       lens.data_ptr(), _ptr(cu_q), int(max_q), max_len, float(softmax_scale),
-                                       out.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, _stream(dev))
-    _lib.check(st, "mk_attention_paged")
-    return out, lse
-
-
-def _move_workspace(rows: int, pages: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty(_lib.lib().mk_kv_move_workspace(rows, pages), dtype=torch.uint8, device=dev)
+    say what the queries and tokens of a row reach, for the launch shape (max_len None: what the table holds).  A
+    query that sees no key gives zeros and lse -inf."""
+    return _lib.torch_side().attention_paged(q, codes, scales, block_table, lens, cu_q, max_q, max_len, softmax_scale)
 
 
 def kv_fork(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
-            refs: torch.Tensor, parents: torch.Tensor):
+            refs: torch.Tensor, parents: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Rows that continue old ones (mk_kv_fork): row i of the result continues row parents[i], -1 is an empty
     row.  codes [layers, pages, 2, n_kv, page, head_dim].  Whole pages are shared; of a partly filled last page
     every child but the first gets a copy.  Pages that no new row lists become free.  Returns (table, lens,
     refs), new tensors; the pool changes in place."""
-    dev = _pages(codes, scales, 6)
-    layers, P, _, n_kv, page, hd = codes.shape
-    rows, width = _table(block_table, lens, "lens", dev)
-    _need(refs, "refs", _I32, 1, dev)
-    _need(parents, "parents", _I32, 1, dev)
-    if refs.shape[0] != P:
-        raise ValueError(f"minicpm5_mk: refs has {refs.shape[0]} entries for {P} pages")
-    R = parents.shape[0]
-    table = torch.empty(R, width, dtype=_I32, device=dev)
-    new_lens = torch.empty(R, dtype=_I32, device=dev)
-    new_refs = torch.empty_like(refs)
-    ws = _move_workspace(R, P, dev)
-    st = _lib.lib().mk_kv_fork(codes.data_ptr(), scales.data_ptr(), layers, P, n_kv, page, hd, block_table.data_ptr(),
-                               lens.data_ptr(), rows, width, parents.data_ptr(), R, table.data_ptr(),
-                               new_lens.data_ptr(), new_refs.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
-    _lib.check(st, "mk_kv_fork")
-    return table, new_lens, new_refs
+    return _lib.torch_side().kv_fork(codes, scales, block_table, lens, refs, parents)
 
 
 def kv_reserve(block_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, n_new: Optional[torch.Tensor],
                page: int) -> None:
     """Give each row, in place, the pages of its next n_new[r] tokens (None: one each) that it does not have yet,
     lowest free ids first (mk_kv_reserve)."""
-    if not block_table.is_cuda:
-        raise ValueError("minicpm5_mk: block_table must be a CUDA tensor")
-    dev = block_table.device
-    rows, width = _table(block_table, lens, "lens", dev)
-    _need(refs, "refs", _I32, 1, dev)
-    if n_new is not None:
-        _row_values(n_new, "n_new", rows, dev)
-    st = _lib.lib().mk_kv_reserve(block_table.data_ptr(), lens.data_ptr(), rows, width, _ptr(n_new), refs.data_ptr(),
-                                  refs.shape[0], int(page), _stream(dev))
-    _lib.check(st, "mk_kv_reserve")
+    _lib.torch_side().kv_reserve(block_table, lens, refs, n_new, page)
 
 
-def kv_compact(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, refs: torch.Tensor):
+def kv_compact(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+               refs: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Move the pages in use to the lowest ids, in all layers (mk_kv_compact).  Returns (table, refs, used int32
     [1]), new tensors; the pool changes in place."""
-    dev = _pages(codes, scales, 6)
-    layers, P, _, n_kv, page, hd = codes.shape
-    rows, width = _table(block_table, None, "", dev)
-    _need(refs, "refs", _I32, 1, dev)
-    if refs.shape[0] != P:
-        raise ValueError(f"minicpm5_mk: refs has {refs.shape[0]} entries for {P} pages")
-    table, new_refs = torch.empty_like(block_table), torch.empty_like(refs)
-    used = torch.empty(1, dtype=_I32, device=dev)
-    ws = _move_workspace(rows, P, dev)
-    st = _lib.lib().mk_kv_compact(codes.data_ptr(), scales.data_ptr(), layers, P, n_kv, page, hd,
-                                  block_table.data_ptr(), rows, width, refs.data_ptr(), table.data_ptr(),
-                                  new_refs.data_ptr(), used.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
-    _lib.check(st, "mk_kv_compact")
-    return table, new_refs, used
+    return _lib.torch_side().kv_compact(codes, scales, block_table, refs)
 
 
 # ------------------------------------------------------------------------------- scores of given tokens
-def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0):
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) -> Tuple[torch.Tensor, ...]:
     """Scores of the tokens targets int32 [T] under rows of logits (f32 or bf16 [T, V], row stride free):
     (logprobs f32 [T], entropy f32 [T], ranks int32 [T], top_ids int32 [T, k], top_logprobs f32 [T, k])
     (mk_token_logprobs).  A target outside [0, V) is not scored: logprob 0, rank 0."""
-    if not logits.is_cuda or logits.ndim != 2 or logits.dtype not in (_F32, _BF16) or \
-            (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("minicpm5_mk: logits must be a row-major f32 or bf16 [T, V] CUDA tensor")
-    dev = logits.device
-    T, V = logits.shape
-    _need(targets, "targets", _I32, 1, dev)
-    if targets.shape[0] != T:
-        raise ValueError(f"minicpm5_mk: {targets.shape[0]} targets for {T} rows of logits")
-    k = int(top_k)
-    lp = torch.empty(T, dtype=_F32, device=dev)
-    ent = torch.empty_like(lp)
-    rank = torch.empty_like(targets)
-    ids = torch.empty(T, k, dtype=_I32, device=dev)
-    tlp = torch.empty(T, k, dtype=_F32, device=dev)
-    st = _lib.lib().mk_token_logprobs(logits.data_ptr(), 16 if logits.dtype is _BF16 else 32, T, V,
-                                      logits.stride(0), targets.data_ptr(), k, lp.data_ptr(), ent.data_ptr(),
-                                      rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), _stream(dev))
-    _lib.check(st, "mk_token_logprobs")
-    return lp, ent, rank, ids, tlp
+    return _lib.torch_side().token_logprobs(logits, targets, top_k)
 
 
-@functools.lru_cache(maxsize=4096)
-def _score_workspace(T: int, H: int, V: int) -> int:
-    n = ctypes.c_size_t()
-    _lib.check(_lib.lib().mk_score_tokens_workspace(T, H, V, ctypes.byref(n)), "mk_score_tokens_workspace")
-    return n.value
-
-
-def score_tokens(h: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor, logit_scale: float = 1.0):
+def score_tokens(h: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor,
+                 logit_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """(logprobs f32 [T], entropy f32 [T]) of the tokens targets int32 [T] under logits logit_scale * h @ lm_head^T,
     h bf16 [T, H] (row stride free), lm_head bf16 [V, H]; the logits are not written to memory
     (mk_score_tokens).  A target outside [0, V) is not scored: logprob 0."""
-    if not h.is_cuda or h.ndim != 2 or h.dtype is not _BF16 or (h.shape[1] > 1 and h.stride(1) != 1):
-        raise ValueError("minicpm5_mk: h must be a row-major bf16 [T, H] CUDA tensor")
-    dev = h.device
-    T, H = h.shape
-    _need(lm_head, "lm_head", _BF16, 2, dev)
-    _need(targets, "targets", _I32, 1, dev)
-    if lm_head.shape[1] != H or targets.shape[0] != T:
-        raise ValueError(f"minicpm5_mk: h {tuple(h.shape)}, lm_head {tuple(lm_head.shape)}, {targets.shape[0]} targets")
-    V = lm_head.shape[0]
-    nbytes = _score_workspace(T, H, V)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    lp = torch.empty(T, dtype=_F32, device=dev)
-    ent = torch.empty_like(lp)
-    st = _lib.lib().mk_score_tokens(h.data_ptr(), T, H, h.stride(0), lm_head.data_ptr(), V, targets.data_ptr(),
-                                    float(logit_scale), lp.data_ptr(), ent.data_ptr(), ws.data_ptr(), nbytes,
-                                    _stream(dev))
-    _lib.check(st, "mk_score_tokens")
-    return lp, ent
+    return _lib.torch_side().score_tokens(h, lm_head, targets, logit_scale)
