@@ -40,9 +40,11 @@ size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 size_t page_bytes(int n_kv, int page, int hd) { return static_cast<size_t>(2) * n_kv * page * hd; }
 
 mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int n_kv, int page, int hd, int max_pairs,
-                     const int2* pairs, const int32_t* n_pairs, cudaStream_t st) {
-  return launch_k(mk::kv_copy_pages_kernel, dim3(std::min(max_pairs, 4096), layers), dim3(mk::COPY_THREADS), 0, st, true,
-                  static_cast<int8_t*>(codes), scales, num_pages, page_bytes(n_kv, page, hd), 2 * n_kv, pairs, n_pairs);
+                     const int2* pairs, const int32_t* n_pairs, const int32_t* table, size_t entries, const int32_t* to,
+                     int32_t* new_table, int* err, cudaStream_t st) {
+  return launch_k(mk::kv_copy_pages_kernel, dim3(std::min(std::max(max_pairs, 1), 4096), layers + (entries ? 1 : 0)),
+                  dim3(mk::COPY_THREADS), 0, st, true, static_cast<int8_t*>(codes), scales, num_pages,
+                  page_bytes(n_kv, page, hd), 2 * n_kv, pairs, n_pairs, layers, table, entries, to, new_table, err);
 }
 
 // Launch shape and workspace of the paged attention.  Query rows (tokens times heads of a group) per tile: 8, 16
@@ -228,7 +230,7 @@ mk_status mk_kv_fork(void* codes, float* scales, int32_t layers, int32_t num_pag
   if (new_rows && (new_table == block_table || new_lens == lens)) return MK_ERR_BAD_ARG;
   if (workspace_bytes < mk_kv_move_workspace(new_rows, num_pages)) return MK_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MK_ERR_BAD_ALIGN;
-  if (new_rows > mk::PG_ROWS_MAX || layers > 65535) return MK_ERR_TOO_LARGE;
+  if (new_rows > mk::PG_ROWS_MAX || layers > 65534) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -236,14 +238,24 @@ mk_status mk_kv_fork(void* codes, float* scales, int32_t layers, int32_t num_pag
   int32_t* count = reinterpret_cast<int32_t*>(ws);
   int2* pairs = reinterpret_cast<int2*>(ws + 256);
   int32_t* src = reinterpret_cast<int32_t*>(ws + 256 + align256(static_cast<size_t>(std::max(new_rows, num_pages)) * sizeof(int2)));
-  MK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(num_pages) * sizeof(int32_t), st));
-  if (new_rows == 0) return MK_OK;
-  MK_TRY(launch_k(mk::kv_fork_rows_kernel, dim3(new_rows), dim3(mk::FORK_THREADS), 0, st, false, block_table, lens, rows,
-                  width, parents, num_pages, c.page_shift, new_table, new_lens, refs, src, d.err));
-  MK_TRY(launch_k(mk::kv_assign_kernel, dim3(1), dim3(mk::PG_THREADS), static_cast<size_t>(new_rows) * sizeof(int), st, true,
-                  new_table, static_cast<const int32_t*>(new_lens), new_rows, width, static_cast<const int32_t*>(nullptr),
-                  static_cast<const int32_t*>(src), pairs, count, refs, num_pages, c.page_shift, d.err));
-  return copy_pages(codes, scales, layers, num_pages, n_kv, page_size, head_dim, new_rows, pairs, count, st);
+  if (new_rows == 0) {
+    MK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(num_pages) * sizeof(int32_t), st));
+    return MK_OK;
+  }
+  if (static_cast<int64_t>(new_rows) * width <= mk::FORK_SMALL && num_pages <= mk::FORK_SMALL && new_rows + rows <= 12000) {
+    MK_TRY(launch_k(mk::kv_fork_small_kernel, dim3(1), dim3(mk::PG_THREADS),
+                    (static_cast<size_t>(new_rows) + rows) * sizeof(int), st, true, block_table, lens, rows, width, parents,
+                    new_rows, num_pages, c.page_shift, new_table, new_lens, refs, src, pairs, count, d.err));
+  } else {
+    MK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(num_pages) * sizeof(int32_t), st));
+    MK_TRY(launch_k(mk::kv_fork_rows_kernel, dim3(new_rows), dim3(mk::FORK_THREADS), 0, st, false, block_table, lens, rows,
+                    width, parents, num_pages, c.page_shift, new_table, new_lens, refs, src, d.err));
+    MK_TRY(launch_k(mk::kv_assign_kernel, dim3(1), dim3(mk::PG_THREADS), static_cast<size_t>(new_rows) * sizeof(int), st, true,
+                    new_table, static_cast<const int32_t*>(new_lens), new_rows, width, static_cast<const int32_t*>(nullptr),
+                    static_cast<const int32_t*>(src), pairs, count, refs, num_pages, c.page_shift, d.err));
+  }
+  return copy_pages(codes, scales, layers, num_pages, n_kv, page_size, head_dim, new_rows, pairs, count, nullptr, 0, nullptr,
+                    nullptr, d.err, st);
 }
 
 mk_status mk_kv_reserve(int32_t* block_table, const int32_t* lens, int32_t rows, int32_t width, const int32_t* n_new,
@@ -274,7 +286,7 @@ mk_status mk_kv_compact(void* codes, float* scales, int32_t layers, int32_t num_
   if (refs == new_refs) return MK_ERR_BAD_ARG;
   if (workspace_bytes < mk_kv_move_workspace(rows, num_pages)) return MK_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MK_ERR_BAD_ALIGN;
-  if (layers > 65535) return MK_ERR_TOO_LARGE;
+  if (layers > 65534) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -284,13 +296,8 @@ mk_status mk_kv_compact(void* codes, float* scales, int32_t layers, int32_t num_
   int32_t* to = reinterpret_cast<int32_t*>(ws + 256 + align256(static_cast<size_t>(std::max(rows, num_pages)) * sizeof(int2)));
   MK_TRY(launch_k(mk::kv_compact_plan_kernel, dim3(1), dim3(mk::PG_THREADS), 0, st, true, refs, num_pages, new_refs, to,
                   pairs, count, used));
-  const size_t entries = static_cast<size_t>(rows) * width;
-  if (entries) {
-    const size_t blocks = std::min<size_t>((entries + 255) / 256, static_cast<size_t>(d.sm_count) * 8);
-    MK_TRY(launch_k(mk::kv_remap_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, true, block_table, entries,
-                    static_cast<const int32_t*>(to), num_pages, new_table, d.err));
-  }
-  return copy_pages(codes, scales, layers, num_pages, n_kv, page_size, head_dim, (num_pages + 1) / 2, pairs, count, st);
+  return copy_pages(codes, scales, layers, num_pages, n_kv, page_size, head_dim, (num_pages + 1) / 2, pairs, count,
+                    block_table, static_cast<size_t>(rows) * width, to, new_table, d.err, st);
 }
 
 }  // extern "C"

@@ -371,45 +371,21 @@ __global__ void __launch_bounds__(FORK_THREADS)
   }
 }
 
-// Hands free pages (refs == 0, lowest first) to the rows that ask for them, in row order.
-//   fork:    row i asks for one page where src[i] >= 0: it becomes its last page, and pairs[k] = (src, page)
-//   reserve: row i asks for the missing pages of positions lens[i] .. lens[i] + n_new[i] - 1
-// The requests are scanned into shared memory, then one pass over refs deals out the pages.  One CTA: the
-// pass reads 4 bytes a page, and stops once every request is served.
+// Hands free pages (refs == 0, lowest first) to the rows that ask for them, in row order; upto[i] is the number of
+// requests of rows 0 .. i, in shared memory.  One pass of the CTA over refs, 4 bytes a page, which stops once every
+// request is served.
+//   fork    (src)   row i asks for one page where src[i] >= 0: it becomes its last page, and pairs[k] = (src, page)
+//   reserve (!src)  row i asks for the missing pages of positions lens[i] .. lens[i] + n_new[i] - 1
 constexpr int PG_ROWS_MAX = 8192;
-__global__ void __launch_bounds__(PG_THREADS)
-    kv_assign_kernel(int32_t* __restrict__ table, const int32_t* __restrict__ lens, int rows, int width,
-                     const int32_t* __restrict__ n_new, const int32_t* __restrict__ src, int2* __restrict__ pairs,
-                     int32_t* __restrict__ n_pairs, int32_t* __restrict__ refs, int num_pages, int page_shift, int* err) {
-  extern __shared__ int upto[];  // requests of rows 0 .. i
-  __shared__ int sums[32];
-  pdl_wait();
-  pdl_trigger();
+__device__ __forceinline__ void deal_pages(const int* upto, int asked, int32_t* table, const int32_t* lens, int rows,
+                                           int width, const int32_t* n_new, const int32_t* src, int2* pairs,
+                                           int32_t* n_pairs, int32_t* refs, int num_pages, int page_shift, int* sums,
+                                           int* err) {
   const int page_tokens = 1 << page_shift;
-  int asked = 0;
-  for (int base = 0; base < rows; base += PG_THREADS) {
-    const int i = base + threadIdx.x;
-    int want = 0;
-    if (i < rows) {
-      if (src) {
-        want = src[i] >= 0;
-      } else {
-        const int len = max(0, lens[i]), add = n_new ? max(0, n_new[i]) : 1;
-        const int first = len >> page_shift, end = (len + add + page_tokens - 1) >> page_shift;
-        if (add > 0 && end > width) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
-        for (int j = first; j < min(end, width); ++j) want += table[static_cast<size_t>(i) * width + j] < 0;
-      }
-    }
-    int total;
-    const int inc = block_scan(want, sums, total);
-    if (i < rows) upto[i] = asked + inc;
-    asked += total;
-  }
-  __syncthreads();
   int given = 0;
   for (int base = 0; base < num_pages && given < asked; base += PG_THREADS) {
     const int page = base + threadIdx.x;
-    const int is_free = page < num_pages && refs[page] == 0;
+    const int is_free = page < num_pages && __ldcg(refs + page) == 0;
     int total;
     const int k = given + block_scan(is_free, sums, total) - 1;
     if (is_free && k < asked) {
@@ -424,9 +400,7 @@ __global__ void __launch_bounds__(PG_THREADS)
         mine[min(width, (len + page_tokens - 1) >> page_shift) - 1] = page;
         pairs[k] = make_int2(src[lo], page);
       } else {
-        // the row's r-th missing slot; its other requests are served at other slots by other threads, so a
-        // slot counts as missing whether or not it has been filled meanwhile: `first` on, the row's slots
-        // with pages come before those without
+        // the row's r-th missing slot: a row's slots with pages come before those without
         const int r = k - (lo ? upto[lo - 1] : 0), add = n_new ? max(0, n_new[lo]) : 1;
         const int end = min(width, (len + add + page_tokens - 1) >> page_shift), mine_n = upto[lo] - (lo ? upto[lo - 1] : 0);
         mine[end - mine_n + r] = page;
@@ -439,6 +413,102 @@ __global__ void __launch_bounds__(PG_THREADS)
     if (given < asked) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
     if (n_pairs) *n_pairs = min(given, asked);
   }
+}
+
+// The pages that the rows ask for, counted into upto, and dealt.
+__global__ void __launch_bounds__(PG_THREADS)
+    kv_assign_kernel(int32_t* __restrict__ table, const int32_t* __restrict__ lens, int rows, int width,
+                     const int32_t* __restrict__ n_new, const int32_t* __restrict__ src, int2* __restrict__ pairs,
+                     int32_t* __restrict__ n_pairs, int32_t* __restrict__ refs, int num_pages, int page_shift, int* err) {
+  extern __shared__ int upto[];
+  __shared__ int sums[32];
+  pdl_wait();
+  pdl_trigger();
+  int asked = 0;
+  for (int base = 0; base < rows; base += PG_THREADS) {
+    const int i = base + threadIdx.x;
+    int want = 0;
+    if (i < rows) {
+      if (src) {
+        want = src[i] >= 0;
+      } else {
+        const int len = max(0, lens[i]), add = n_new ? max(0, n_new[i]) : 1;
+        const int first = len >> page_shift, end = (len + add + (1 << page_shift) - 1) >> page_shift;
+        if (add > 0 && end > width) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
+        for (int j = first; j < min(end, width); ++j) want += table[static_cast<size_t>(i) * width + j] < 0;
+      }
+    }
+    int total;
+    const int inc = block_scan(want, sums, total);
+    if (i < rows) upto[i] = asked + inc;
+    asked += total;
+  }
+  __syncthreads();
+  deal_pages(upto, asked, table, lens, rows, width, n_new, src, pairs, n_pairs, refs, num_pages, page_shift, sums, err);
+}
+
+// kv_fork_rows_kernel and kv_assign_kernel in one CTA, for tables and pools that one SM walks through faster than
+// two more launches take: 256 rows of 9 slots over 1500 pages fork in 5 us instead of 12.
+constexpr int FORK_SMALL = 32768;  // table entries, and pages
+__global__ void __launch_bounds__(PG_THREADS)
+    kv_fork_small_kernel(const int32_t* __restrict__ table, const int32_t* __restrict__ lens, int rows_in, int width,
+                         const int32_t* __restrict__ parents, int rows, int num_pages, int page_shift,
+                         int32_t* __restrict__ new_table, int32_t* __restrict__ new_lens, int32_t* refs,
+                         int32_t* __restrict__ src, int2* __restrict__ pairs, int32_t* __restrict__ n_pairs, int* err) {
+  extern __shared__ int smem[];  // [rows] upto, [rows_in] the first child of each parent
+  __shared__ int sums[32];
+  int *upto = smem, *eldest = smem + rows;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x;
+  for (int p = tid; p < num_pages; p += PG_THREADS) refs[p] = 0;
+  for (int p = tid; p < rows_in; p += PG_THREADS) eldest[p] = rows;
+  __syncthreads();
+  for (int i = tid; i < rows; i += PG_THREADS) {
+    const int p = parents[i];
+    if (p >= 0 && p < rows_in) atomicMin(eldest + p, i);
+  }
+  __syncthreads();
+  int asked = 0;
+  for (int base = 0; base < rows; base += PG_THREADS) {
+    const int i = base + tid;
+    int want = 0;
+    if (i < rows) {
+      int p = parents[i];
+      if (p >= rows_in) {
+        atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+        p = -1;
+      }
+      const int len = p < 0 ? 0 : max(0, lens[p]), n = min(width, (len + (1 << page_shift) - 1) >> page_shift);
+      if (len > (width << page_shift)) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+      new_lens[i] = len;
+      src[i] = -1;
+      if (p >= 0 && n > 0 && eldest[p] < i && (len & ((1 << page_shift) - 1))) {
+        const int page = kv_page_of(table, width, num_pages, p, n - 1, err);
+        src[i] = page;
+        want = page >= 0;
+      }
+    }
+    int total;
+    const int inc = block_scan(want, sums, total);
+    if (i < rows) upto[i] = asked + inc;
+    asked += total;
+  }
+  __syncthreads();
+  for (int e = tid; e < rows * width; e += PG_THREADS) {
+    const int i = e / width, j = e - i * width, p = parents[i];
+    const int n = (new_lens[i] + (1 << page_shift) - 1) >> page_shift;
+    const bool ok = p >= 0 && p < rows_in && j < n;
+    const bool copy = ok && j == min(n, width) - 1 && eldest[p] < i && (new_lens[i] & ((1 << page_shift) - 1));
+    int page = -1;
+    if (ok && !copy) page = kv_page_of(table, width, num_pages, p, j, err);
+    if (page >= 0) atomicAdd(refs + page, 1);
+    new_table[e] = page;
+  }
+  __threadfence();
+  __syncthreads();
+  deal_pages(upto, asked, new_table, new_lens, rows, width, nullptr, src, pairs, n_pairs, refs, num_pages, page_shift, sums,
+             err);
 }
 
 // Compaction: with `used` live pages, those at `used` and above move into the holes below, lowest to lowest.
@@ -489,30 +559,27 @@ __global__ void __launch_bounds__(PG_THREADS)
   }
 }
 
-// new_table = table through `to`; -1 where the table holds no page.
-__global__ void kv_remap_kernel(const int32_t* __restrict__ table, size_t n, const int32_t* __restrict__ to, int num_pages,
-                                int32_t* __restrict__ new_table, int* err) {
-  pdl_wait();
-  pdl_trigger();
-  for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n;
-       i += static_cast<size_t>(gridDim.x) * blockDim.x) {
-    const int p = table[i];
-    int q = -1;
-    if (p >= 0 && p < num_pages) q = to[p];
-    else if (p >= num_pages) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
-    new_table[i] = q;
-  }
-}
-
-// codes and scales of page pairs[k].x to page pairs[k].y in every layer.  No source is a destination.
+// codes and scales of page pairs[k].x to page pairs[k].y in every layer.  No source is a destination.  CTAs
+// (x, layers) write new_table = table through `to` (-1 where the table holds no page), where there is one.
 constexpr int COPY_THREADS = 256;
 constexpr int COPY_VEC = 6;  // 16-byte vectors in flight per thread
 __global__ void __launch_bounds__(COPY_THREADS)
     kv_copy_pages_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, int num_pages, size_t page_bytes,
-                         int page_scales, const int2* __restrict__ pairs, const int32_t* __restrict__ n_pairs) {
+                         int page_scales, const int2* __restrict__ pairs, const int32_t* __restrict__ n_pairs, int layers,
+                         const int32_t* __restrict__ table, size_t entries, const int32_t* __restrict__ to,
+                         int32_t* __restrict__ new_table, int* err) {
   pdl_wait();
   pdl_trigger();
   const int n = *n_pairs, layer = blockIdx.y;
+  if (layer == layers) {
+    for (size_t i = blockIdx.x * static_cast<size_t>(COPY_THREADS) + threadIdx.x; i < entries;
+         i += static_cast<size_t>(gridDim.x) * COPY_THREADS) {
+      const int p = table[i];
+      if (p >= num_pages) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+      new_table[i] = p >= 0 && p < num_pages ? to[p] : -1;
+    }
+    return;
+  }
   const size_t vecs = page_bytes / 16;
   for (int k = blockIdx.x; k < n; k += gridDim.x) {
     const int2 pr = pairs[k];
