@@ -1,0 +1,194 @@
+"""Scoring several continuations of one prompt: the prompt runs once, its keys and values stay in an 8-bit paged
+cache, and every candidate answer forks from it.
+
+The whole-model path (`MkEngine.forward`) returns one token per prompt and keeps nothing; scoring N answers with it
+runs the prompt N times.  Here the model is put together from the library's stage operators, with the cache
+(`kv_append`, `attention_paged`, `kv_fork`, `kv_reserve`, `kv_compact`) between them and the scores (`score_tokens`,
+`token_logprobs`) at the end.  Weights are the prepared ones (`mk_weights.prepare_mk_weights`).
+
+    scorer = ContinuationScorer(cfg, weights)
+    prompt_lp = scorer.prefill(prompt_ids)              # log-probabilities of the prompt's own tokens
+    answers = scorer.score([[5, 17], [5, 9, 2], [88]])  # per candidate, of each of its tokens
+    ids, lps = scorer.alternatives(5)                   # best first tokens
+
+`python -m minicpm5_mk.continuations` times it on random weights.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, List, Sequence, Tuple
+
+import torch
+
+from . import _lib, ops
+from .mk_config import MkConfig
+
+
+class ContinuationScorer:
+    """One prompt at a time on one device.  `pages` pages of `page_size` tokens are held for all layers; a prompt
+    and its candidates need ceil(len / page_size) pages for the prompt and for each candidate a copy of the
+    prompt's part-filled last page and the pages of its own tokens.  Running out raises MkError."""
+
+    def __init__(self, cfg: MkConfig, weights: Dict[str, torch.Tensor], device: torch.device | int | str = "cuda", *,
+                 pages: int = 512, page_size: int = 64):
+        cfg.check()
+        self.cfg, self.page = cfg, int(page_size)
+        self.device = torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.w = {k: weights[k].to(self.device) for k in ops.WEIGHT_FIELDS}
+        shape = (cfg.num_layers, int(pages), 2, cfg.n_kv)
+        self.codes = torch.empty((*shape, self.page, cfg.head_dim), dtype=torch.int8, device=self.device)
+        self.scales = torch.empty(shape, dtype=torch.float32, device=self.device)
+        self.width = -(-cfg.max_seq // self.page)
+        self._clear()
+
+    def _clear(self) -> None:
+        # one row, the prompt's; its length is also kept here, where it is set
+        self.table = torch.full((1, self.width), -1, dtype=torch.int32, device=self.device)
+        self.lens = self._int([0])
+        self.refs = torch.zeros(self.codes.shape[1], dtype=torch.int32, device=self.device)
+        self.length = 0
+        self.last = None  # final-normed hidden row of the prompt's last token, bf16 [1, H]
+
+    def _int(self, values: Sequence[int]) -> torch.Tensor:
+        return torch.tensor(list(values), dtype=torch.int32, device=self.device)
+
+    def _check(self) -> None:
+        e = ctypes.c_int32()
+        _lib.check(_lib.lib().mk_get_error(None, ctypes.byref(e)), f"device error word 0x{e.value:x}")
+
+    # ------------------------------------------------------------------ model
+    def _run(self, ids: torch.Tensor, seq: int, pos: int, attend) -> torch.Tensor:
+        """Final-normed hidden rows bf16 [T, H] of tokens at positions pos + t % seq; attend(layer, qkv) gives the
+        attention output of a layer."""
+        c, w = self.cfg, self.w
+        x32, xb = ops.embed(ids, w["embed"], c.scale_emb)
+        h = torch.empty((ids.numel(), c.inter), dtype=torch.bfloat16, device=self.device)
+        for i in range(c.num_layers):
+            qkv = ops.gemm_w8a16(xb, w["w_qkv"][i], w["s_qkv"][i], _lib.MK_GEMM_ROWSCALE, row_scale=ops.rms_rstd(x32, c.eps),
+                                 rope=(w["rope_cos"], w["rope_sin"]), rope_cols=c.q_dim + c.kv_dim, head_dim=c.head_dim,
+                                 rope_seq=seq, rope_pos_base=pos)
+            ops.gemm_w8a16(attend(i, qkv), w["w_o"][i], w["s_o"][i], _lib.MK_GEMM_RESID32, resid_scale=c.residual_scale,
+                           out=xb, resid32=x32)
+            ops.gemm_w8a16(xb, w["w_gu"][i], w["s_gu"][i], _lib.MK_GEMM_SWIGLU, row_scale=ops.rms_rstd(x32, c.eps), out=h)
+            ops.gemm_w8a16(h, w["w_down"][i], w["s_down"][i], _lib.MK_GEMM_RESID32, resid_scale=c.residual_scale, out=xb,
+                           resid32=x32)
+        return (x32 * ops.rms_rstd(x32, c.eps)[:, None] * w["final_norm"]).to(torch.bfloat16)
+
+    def _heads(self, qkv: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        c = self.cfg
+        q, k, v = qkv.split([c.q_dim, c.kv_dim, c.kv_dim], 1)
+        return tuple(t.unflatten(1, (-1, c.head_dim)) for t in (q, k, v))
+
+    # ------------------------------------------------------------------ prompt
+    def prefill(self, ids: Sequence[int]) -> torch.Tensor:
+        """Run the prompt and cache it (whatever was cached before is dropped).  Returns the log-probabilities of
+        its tokens from the second on, f32 [len - 1]."""
+        # the prefill attention takes multiples of 128 tokens; what follows the prompt is seen by none of its tokens
+        c, n = self.cfg, len(ids)
+        padded = -(-n // 128) * 128
+        if not 0 < padded <= c.max_seq:
+            raise ValueError(f"minicpm5_mk: a prompt of {n} tokens (1 to {c.max_seq // 128 * 128})")
+        self._clear()
+        t = self._int(list(ids) + [0] * (padded - n))
+        ops.kv_reserve(self.table, self.lens, self.refs, self._int([n]), self.page)
+        cu = self._int([0, n])
+
+        def attend(layer, qkv):
+            _, k, v = self._heads(qkv)
+            ops.kv_append(k, v, self.codes[layer], self.scales[layer], self.table, self.lens, cu_new=cu, max_new=n)
+            return ops.attention_prefill(qkv, 1, padded, c.n_q, c.n_kv, c.head_dim)
+
+        hidden = self._run(t, padded, 0, attend)[:n]
+        self._check()
+        self.lens, self.length = self._int([n]), n
+        self.last = hidden[n - 1:]
+        if n == 1:
+            return torch.empty(0, device=self.device)
+        return ops.score_tokens(hidden[:n - 1], self.w["lm_head"], t[1:n], logit_scale=c.logit_scale)[0]
+
+    # ------------------------------------------------------------------ candidates
+    def score(self, candidates: Sequence[Sequence[int]]) -> List[torch.Tensor]:
+        """Log-probabilities of each candidate's tokens after the prompt (f32, one tensor per candidate).  The cache
+        is left as it was."""
+        if self.last is None:
+            raise ValueError("minicpm5_mk: score() before prefill()")
+        c, L, C = self.cfg, self.length, len(candidates)
+        M = max((len(a) for a in candidates), default=0)
+        if M == 0:
+            return [torch.empty(0, device=self.device) for _ in candidates]
+        if L + M > c.max_seq:
+            raise ValueError(f"minicpm5_mk: prompt and candidate take {L + M} tokens of {c.max_seq}")
+        # row 0 stays the prompt, rows 1 .. C continue it; candidates are filled up to the longest, and what
+        # follows a candidate's end is seen by none of its tokens
+        ids = self._int([i for a in candidates for i in list(a) + [0] * (M - len(a))])
+        table, lens, refs = ops.kv_fork(self.codes, self.scales, self.table, self.lens, self.refs, self._int([0] * (C + 1)))
+        new = self._int([0] + [M] * C)
+        ops.kv_reserve(table, lens, refs, new, self.page)
+        cu, after = self._int([0] + [M * i for i in range(C + 1)]), lens + new
+
+        def attend(layer, qkv):
+            q, k, v = self._heads(qkv)
+            cache = (self.codes[layer], self.scales[layer], table)
+            ops.kv_append(k, v, *cache, lens, cu_new=cu, max_new=M)
+            out, _ = ops.attention_paged(q, *cache, after, cu_q=cu, max_q=M, max_len=L + M)  # Q carries 1/sqrt(hd)
+            return out.flatten(1)
+
+        hidden = self._run(ids, M, L, attend).view(C, M, c.hidden)
+        # a candidate's first token is predicted by the prompt's last row, the others by the row before
+        rows = torch.cat([self.last.expand(C, 1, -1), hidden[:, :-1]], 1).reshape(C * M, c.hidden)
+        lp, _ = ops.score_tokens(rows, self.w["lm_head"], ids, logit_scale=c.logit_scale)
+        # the candidates' pages go back
+        self.table, self.lens, self.refs = ops.kv_fork(self.codes, self.scales, table, lens, refs, self._int([0]))
+        self._check()
+        return [lp[i * M:i * M + len(a)] for i, a in enumerate(candidates)]
+
+    def alternatives(self, k: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The k most likely first tokens after the prompt: (ids int32 [k], log-probabilities f32 [k])."""
+        if self.last is None:
+            raise ValueError("minicpm5_mk: alternatives() before prefill()")
+        logits, top1 = ops.lm_head_argmax((self.last.float() * self.cfg.logit_scale).contiguous(), self.w["lm_head"])
+        _, _, _, ids, lps = ops.token_logprobs(logits, top1, k)
+        return ids[0], lps[0]
+
+    def compact(self) -> int:
+        """Move the cached pages to the start of the pool; returns how many are in use."""
+        self.table, self.refs, used = ops.kv_compact(self.codes, self.scales, self.table, self.refs)
+        self._check()
+        return int(used)
+
+
+def main() -> None:
+    import argparse
+    import time
+
+    from . import mk_weights
+    from .mk_config import get_config
+    from .mk_init import random_state_dict, synthetic_ids
+
+    ap = argparse.ArgumentParser(description="Score continuations of one prompt on random weights")
+    ap.add_argument("--config", default="minicpm5-1b")
+    ap.add_argument("--prompt", type=int, default=4096, help="prompt tokens")
+    ap.add_argument("--candidates", type=int, default=16)
+    ap.add_argument("--tokens", type=int, default=24, help="tokens per candidate")
+    a = ap.parse_args()
+    cfg = get_config(a.config)
+    pages = -(-a.prompt // 64) + a.candidates * (2 + -(-a.tokens // 64)) + 1
+    s = ContinuationScorer(cfg, mk_weights.prepare_mk_weights(random_state_dict(cfg, seed=1234), cfg), pages=pages)
+    ids = synthetic_ids(1, a.prompt + a.candidates * a.tokens, seed=11, vocab=cfg.vocab)[0].tolist()
+    answers = [ids[a.prompt + i * a.tokens:a.prompt + (i + 1) * a.tokens] for i in range(a.candidates)]
+    for name, call in (("prefill", lambda: s.prefill(ids[:a.prompt])), ("score", lambda: s.score(answers)),
+                       ("alternatives", lambda: s.alternatives(5))):
+        call()
+        torch.cuda.synchronize()
+        t = time.perf_counter()
+        for _ in range(5):
+            call()
+        torch.cuda.synchronize()
+        print(f"{name}: {(time.perf_counter() - t) / 5 * 1e3:.2f} ms")
+
+
+if __name__ == "__main__":
+    main()
