@@ -1,0 +1,522 @@
+// Attention over the 8-bit paged cache for rows with many queries (continuations, chunks of a prompt): the products of
+// mk_attn_paged.cuh with tcgen05.
+//
+// With more than a few dozen query rows per key/value head the cache's bytes are read for little and the products,
+// the conversion of the codes and the exponentials become the work.  Here 256 query rows (tokens times heads of a
+// group) share every 64-key tile, so that a code is converted once for all of them, by warps that do nothing
+// else; S and O lie in TMEM, and the exponentials (16 a clock and SM: 1024 cycles for 256 x 64) are what bounds the
+// loop once it runs.
+//
+//   warp 0      asks for the tile's codes (bulk copies, 3 stages) and looks up its pages and scales
+//   warps 1, 2  MMA issuers of row tiles 0 and 1 (128 rows each), as in mk_attn_tc.cuh:
+//                 S_t(j+1) = Q_t K(j+1)^T (f16, M 128, N 64), then O_t += P_t(j) V(j) (P from TMEM, N hd)
+//   warps 4-11  softmax of tiles 0 and 1, one thread per row, and the rows' queries and results
+//   warps 12-15 int8 -> f16: K rows (64 channels per 128-byte swizzled row) and V as [channel][64 keys], both
+//               K-major operands; a 32-bit word of the value plane is four neighbouring keys of one channel already
+//
+// Queries are scaled by a power of two to f16 without loss (its inverse joins the score's factor), codes are exact, and
+// p = exp(s - m) * vscale goes in as f16 (11 bits), as for the wide tiles of mk_attn_paged.cuh.
+#pragma once
+
+#include "mk_attn_paged.cuh"
+
+namespace mk {
+
+constexpr int PT_ROWS = 256;     // query rows of a CTA's pair
+constexpr int PT_KEYS = 64;      // keys of a tile, and of a unit of work
+constexpr int PT_RAW = 3;        // stages of codes
+constexpr int PT_KV = 3;         // stages of converted tiles
+constexpr int PT_THREADS = 512;
+constexpr int PT_CTAS = 148;
+constexpr uint32_t PT_QCHUNK = 128 * 128;      // 128 rows x 64 channels f16
+constexpr uint32_t PT_KCHUNK = PT_KEYS * 128;  // 64 keys x 64 channels
+__host__ __device__ constexpr uint32_t pt_kv_bytes(int hd) { return 2 * PT_KCHUNK + hd * 128; }
+__host__ __device__ constexpr uint32_t pt_raw_bytes(int hd) { return 2 * PT_KEYS * hd; }
+__host__ __device__ constexpr size_t pt_smem_bytes(int hd) {
+  return 1024 + 4 * PT_QCHUNK + PT_KV * pt_kv_bytes(hd) + PT_RAW * pt_raw_bytes(hd) + 1024;
+}
+// Instruction descriptor for kind::f16 with f16 operands, both K-major.
+__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp, PagedAttnArgs a) {
+  constexpr uint32_t KV = pt_kv_bytes(HD), RAW = pt_raw_bytes(HD);
+  extern __shared__ uint8_t pt_smem_raw[];
+  __shared__ long long s_scan[PT_THREADS / 32], s_base;
+  __shared__ int s_row;
+  const uint32_t raw_addr = smem_u32(pt_smem_raw);
+  uint8_t* sQ = pt_smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);  // [tile][chunk]
+  uint8_t* sKV = sQ + 4 * PT_QCHUNK;                                       // [stage]{K chunk 0, K chunk 1, V}
+  uint8_t* sRaw = sKV + PT_KV * KV;                                        // [stage]{K, V}
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(sRaw + PT_RAW * RAW);
+  uint64_t* raw_empty = raw_full + PT_RAW;
+  uint64_t* kv_full = raw_empty + PT_RAW;
+  uint64_t* kv_empty = kv_full + PT_KV;
+  uint64_t* s_full = kv_empty + PT_KV;  // [tile][buffer]
+  uint64_t* p_ready = s_full + 4;       // [tile][buffer]
+  uint64_t* pv_done = p_ready + 4;      // [tile]
+  uint64_t* q_ready = pv_done + 2;      // [tile]
+  uint64_t* drain = q_ready + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float2* s_sc = reinterpret_cast<float2*>(tmem_slot + 4);  // [8 tiles][4 groups]: key scale, relative value scale
+  int* s_none = reinterpret_cast<int*>(s_sc + 32);          // [8 tiles]: groups without a page
+  float* s_ref = reinterpret_cast<float*>(s_none + 8);      // [16 pieces]: what value scales are relative to
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.group, n_kv = cp.n_kv;
+  if (tid == 0) {
+    for (int i = 0; i < PT_RAW; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < PT_KV; ++i) {
+      mbar_init(&kv_full[i], 4);
+      mbar_init(&kv_empty[i], 2);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&pv_done[t], 1);
+      mbar_init(&q_ready[t], 4);
+    }
+    mbar_init(drain, 2);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  // Work in equal shares of units, as in attn_paged_kernel, here with 256 rows a pair.
+  auto row_tokens = [&](int row, int& first) {
+    first = a.cu ? a.cu[row] : row;
+    return a.cu ? a.cu[row + 1] - first : 1;
+  };
+  auto row_tiles = [&](int n) { return (n * G + PT_ROWS - 1) / PT_ROWS; };
+  auto pair_units = [&](int row) { return max((max(a.lens[row], 0) + PT_KEYS - 1) / PT_KEYS, 1); };
+  auto row_units = [&](int row) {
+    int first;
+    const int n = row_tokens(row, first);
+    return n <= 0 ? 0ll : static_cast<long long>(pair_units(row)) * row_tiles(n) * n_kv;
+  };
+  const int per = (a.rows + PT_THREADS - 1) / PT_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) mine += row_units(i);
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 31) s_scan[warp] = inc;
+  __syncthreads();
+  long long N = 0;
+  for (int w = 0; w < PT_THREADS / 32; ++w) {
+    if (w < warp) inc += s_scan[w];
+    N += s_scan[w];
+  }
+  const long long C = min(static_cast<long long>(gridDim.x), N), cta = blockIdx.x;
+  const bool idle = cta >= C;
+  const long long u0 = idle ? 0 : cta * N / C, u1 = idle ? 0 : (cta + 1) * N / C;
+  if (tid == 0) a.desc[cta] = make_int4(-1, 0, 0, 0);
+  if (!idle && inc - mine <= u0 && u0 < inc) {
+    long long base = inc - mine;
+    int i = i0;
+    for (long long n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
+    s_row = i;
+    s_base = base;
+  }
+  __syncthreads();
+
+  // The share's pieces, walked by every warp for itself.
+  struct Piece {
+    int row, first, n, len, R, r0, g, rt, kbeg, kend, tiles64;  // tiles64: 64-key tiles with a key that a row sees
+    bool whole, begins;
+    long long last;  // the pair's last unit
+  };
+  long long u = u0, base = idle ? 0 : s_base;
+  int row = idle ? 0 : s_row;
+  auto next = [&](Piece& p) {
+    long long ru = 0;
+    while (u < u1 && u >= base + (ru = row_units(row))) {
+      base += ru;
+      ++row;
+    }
+    if (u >= u1) return false;
+    p.row = row;
+    p.n = row_tokens(row, p.first);
+    p.len = max(a.lens[row], 0);
+    p.R = p.n * G;
+    const int upp = pair_units(row), tiles = row_tiles(p.n), pair = static_cast<int>((u - base) / upp);
+    const int ua = static_cast<int>((u - base) % upp), ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
+    p.g = pair / tiles;
+    p.rt = pair % tiles;
+    p.r0 = p.rt * PT_ROWS;
+    p.kbeg = ua * PT_KEYS;
+    p.kend = min(ub * PT_KEYS, p.len - p.n + (min(p.r0 + PT_ROWS, p.R) - 1) / G + 1);
+    p.tiles64 = p.kend > p.kbeg ? (p.kend - p.kbeg + PT_KEYS - 1) / PT_KEYS : 0;
+    p.whole = ua == 0 && ub == upp;
+    p.begins = ua == 0;
+    p.last = base + static_cast<long long>(pair + 1) * upp - 1;
+    u += ub - ua;
+    return true;
+  };
+
+  Piece p;
+  bool ok = true;
+  if (warp == 0) {
+    // ---------------------------------------------------------------- codes, pages and scales
+    int j = 0, piece = 0;
+    while (ok && next(p)) {
+      if (p.tiles64 == 0) continue;
+      float ref = 0.f;
+      for (int s = (p.kbeg >> cp.page_shift) + lane; s <= (p.kend - 1) >> cp.page_shift; s += 32) {
+        const int page = s < a.width ? a.table[static_cast<size_t>(p.row) * a.width + s] : -1;
+        if (page >= 0 && page < cp.num_pages) ref = fmaxf(ref, *kv_scale_ptr(cp, page, 1, p.g));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+      if (lane == 0) s_ref[piece & 15] = ref;
+      ++piece;
+      const int run = min(1 << cp.page_shift, PT_KEYS);  // keys that lie together
+      for (int i = 0; ok && i < p.tiles64; ++i, ++j) {
+        const int st = j % PT_RAW;
+        const int key = p.kbeg + i * PT_KEYS + 16 * lane;
+        int page = -1;
+        float ks = 0.f, vs = 0.f;
+        const bool wanted = lane < 4 && key < p.kend;
+        if (wanted) page = kv_page_of(a.table, a.width, cp.num_pages, p.row, key >> cp.page_shift, a.err);
+        if (page >= 0) {
+          ks = *kv_scale_ptr(cp, page, 0, p.g);
+          vs = *kv_scale_ptr(cp, page, 1, p.g);
+        }
+        const uint32_t none = __ballot_sync(0xffffffffu, wanted && page < 0);
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[st], ((j / PT_RAW) & 1) ^ 1u, abort_flag));
+        if (!ok) break;
+        if (lane < 4) s_sc[(j & 7) * 4 + lane] = make_float2(ks, ref > 0.f ? vs / ref * kPOff : vs);
+        if (lane == 0) s_none[j & 7] = static_cast<int>(none);
+        const bool asks = page >= 0 && (16 * lane) % run == 0;
+        const uint32_t bytes = __reduce_add_sync(0xffffffffu, asks ? 2u * run * HD : 0u);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], bytes);
+        __syncwarp();
+        if (asks) {
+          const int8_t* at = kv_head_ptr(cp, page, 0, p.g) + (key & ((1 << cp.page_shift) - 1)) * HD;
+          uint8_t* dst = sRaw + st * RAW + lane * 16 * HD;
+          bulk_load(dst, at, run * HD, &raw_full[st]);
+          bulk_load(dst + PT_KEYS * HD, at + (static_cast<size_t>(n_kv) * HD << cp.page_shift), run * HD, &raw_full[st]);
+        }
+        __syncwarp();
+      }
+    }
+    // every copy that was asked for lands before the CTA may leave
+    for (int i = max(0, j - PT_RAW); i < j; ++i) mbar_wait_drain(&raw_full[i % PT_RAW], (i / PT_RAW) & 1);
+  } else if (warp == 1 || warp == 2) {
+    // ---------------------------------------------------------------- MMA issuers
+    const int t = warp - 1;
+    const bool leader = elect_one();
+    constexpr uint32_t idesc_s = idesc_f16_f32(128, PT_KEYS), idesc_pv = idesc_f16_f32(128, HD);
+    int j = 0;        // tiles of the CTA
+    int jt = 0, jq = 0;  // tiles and pieces of this row tile
+    auto issue_s = [&](int at, int buffer) {
+      const uint8_t* kb = sKV + (at % PT_KV) * KV;
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint64_t da = sdesc_kmajor_sw128(smem_u32(sQ + (t * 2 + (ks >> 2)) * PT_QCHUNK)) + 2 * (ks & 3);
+          const uint64_t db = sdesc_kmajor_sw128(smem_u32(kb + (ks >> 2) * PT_KCHUNK)) + 2 * (ks & 3);
+          mma_f16_ss(tmem + t * 128 + buffer * 64, da, db, idesc_s, ks > 0 ? 1u : 0u);
+        }
+        mma_commit(&s_full[t * 2 + buffer]);
+      }
+      __syncwarp();
+    };
+    auto wait = [&](uint64_t* b, int parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity & 1, abort_flag)); };
+    while (ok && next(p)) {
+      if (p.tiles64 == 0) continue;
+      if (p.r0 + t * 128 >= p.R) {  // no rows: only lets the tiles go
+        for (int i = 0; ok && i < p.tiles64; ++i, ++j) {
+          ok = wait(&kv_full[j % PT_KV], j / PT_KV);
+          if (ok && lane == 0) mbar_arrive(&kv_empty[j % PT_KV]);
+        }
+        continue;
+      }
+      ok = wait(&q_ready[t], jq) && wait(&kv_full[j % PT_KV], j / PT_KV);
+      ++jq;
+      if (!ok) break;
+      tc_fence_after();
+      issue_s(j, jt & 1);
+      for (int i = 0; ok && i < p.tiles64; ++i, ++j, ++jt) {
+        const int st = j % PT_KV;
+        if (i + 1 < p.tiles64) {
+          ok = wait(&kv_full[(j + 1) % PT_KV], (j + 1) / PT_KV);
+          if (!ok) break;
+          tc_fence_after();
+          // (overwrites P_t(j-1) after O_t += P_t(j-1) V(j-1), which this thread issued before, has read it)
+          issue_s(j + 1, (jt + 1) & 1);
+        }
+        ok = wait(&p_ready[t * 2 + (jt & 1)], jt >> 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int ks = 0; ks < PT_KEYS / 16; ++ks) {
+            const uint64_t db = sdesc_kmajor_sw128(smem_u32(sKV + st * KV + 2 * PT_KCHUNK)) + 2 * ks;
+            mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + (jt & 1) * 64 + ks * 8, db, idesc_pv,
+                       (i > 0 || ks > 0) ? 1u : 0u);
+          }
+          mma_commit(&pv_done[t]);
+          mma_commit(&kv_empty[st]);
+        }
+        __syncwarp();
+      }
+    }
+    if (leader) mma_commit(drain);
+    __syncwarp();
+    mbar_wait_drain(drain, 0);
+  } else if (warp >= 12) {
+    // ---------------------------------------------------------------- int8 -> f16
+    const int ct = tid - 12 * 32;
+    int j = 0;
+    while (ok && next(p)) {
+      for (int i = 0; ok && i < p.tiles64; ++i, ++j) {
+        const int rs = j % PT_RAW, st = j % PT_KV;
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[rs], (j / PT_RAW) & 1, abort_flag) &&
+                                         mbar_wait(&kv_empty[st], ((j / PT_KV) & 1) ^ 1u, abort_flag));
+        if (!ok) break;
+        const uint8_t* rk = sRaw + rs * RAW;
+        const uint8_t* rv = rk + PT_KEYS * HD;
+        uint8_t* dk = sKV + st * KV;
+        uint8_t* dv = dk + 2 * PT_KCHUNK;
+#pragma unroll
+        for (int it = 0; it < PT_KEYS * HD / 16 / 128; ++it) {  // 16 channels of a key
+          const int item = it * 128 + ct, key = item / (HD / 16), c = item % (HD / 16);
+          const uint4 x = *reinterpret_cast<const uint4*>(rk + item * 16);
+          uint4 lo, hi;
+          i8x4_to_f16x4(x.x, lo.x, lo.y);
+          i8x4_to_f16x4(x.y, lo.z, lo.w);
+          i8x4_to_f16x4(x.z, hi.x, hi.y);
+          i8x4_to_f16x4(x.w, hi.z, hi.w);
+          uint8_t* d = dk + (c >> 2) * PT_KCHUNK + key * 128;
+          const int unit = (2 * c) & 7;
+          *reinterpret_cast<uint4*>(d + ((unit ^ (key & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(d + (((unit + 1) ^ (key & 7)) << 4)) = hi;
+        }
+#pragma unroll
+        for (int it = 0; it < 8 * HD / 128; ++it) {  // 8 keys of a channel
+          const int item = it * 128 + ct, pair = item / HD, dim = item % HD;
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(rv + ((2 * pair) * HD + dim) * 4);
+          const uint32_t y = *reinterpret_cast<const uint32_t*>(rv + ((2 * pair + 1) * HD + dim) * 4);
+          uint4 o;
+          i8x4_to_f16x4(x, o.x, o.y);
+          i8x4_to_f16x4(y, o.z, o.w);
+          *reinterpret_cast<uint4*>(dv + dim * 128 + ((pair ^ (dim & 7)) << 4)) = o;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&kv_full[st]);
+          mbar_arrive(&raw_empty[rs]);
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- softmax, queries, results
+    const int t = (warp - 4) >> 2, quarter = warp & 3, trow = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_off + t * 128, tO = tmem + lane_off + 256 + t * 128;
+    int j = 0, jt = 0, piece = 0;
+    while (ok && next(p)) {
+      const int qr = p.r0 + t * 128 + trow;
+      const bool has = qr < p.R;
+      const bool tile_on = p.r0 + t * 128 < p.R;
+      const int limit = has ? p.len - p.n + qr / G + 1 : 0;
+      const long long at = has ? static_cast<long long>(p.first + qr / G) * a.n_q + p.g * G + qr % G : 0;
+      float m = kLow, l = 0.f, ref = 0.f;
+      if (p.tiles64 > 0 && tile_on) {
+        // the row's query, as f16 with its largest channel near 1, into the swizzled operand
+        const __nv_bfloat16* qp = a.q;
+        if (has) qp += static_cast<long long>(p.first + qr / G) * a.ld_q + static_cast<long long>(p.g * G + qr % G) * a.hs_q;
+        float top = 0.f;
+        uint4 qv[HD / 8];
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          qv[c] = has ? __ldg(reinterpret_cast<const uint4*>(qp + c * 8)) : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {qv[c].x, qv[c].y, qv[c].z, qv[c].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_bf16x2(w[e]);
+            top = max3f(top, fabsf(f.x), fabsf(f.y));
+          }
+        }
+        const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+        const float down = __uint_as_float((254u - ex) << 23), sf = __uint_as_float(ex << 23) * a.scale;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint32_t w[4] = {qv[c].x, qv[c].y, qv[c].z, qv[c].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_bf16x2(w[e]);
+            h[e] = pack_f16x2(f.x * down, f.y * down);
+          }
+          *reinterpret_cast<uint4*>(sQ + (t * 2 + (c >> 3)) * PT_QCHUNK + trow * 128 + (((c & 7) ^ (trow & 7)) << 4)) =
+              make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_ready[t]);
+
+        for (int i = 0; ok && i < p.tiles64; ++i, ++j, ++jt) {
+          const int b = jt & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * 2 + b], (jt >> 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t v[64];
+          tmem_ld_32x32b_x32(tS + b * 64, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+          tmem_ld_32x32b_x32(tS + b * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+          tmem_ld_wait();
+          float ks[4], vr[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 sc = s_sc[(j & 7) * 4 + q];
+            ks[q] = sc.x * sf;
+            vr[q] = sc.y;
+          }
+          const int none = s_none[j & 7];
+          // scores in units of log 2, relative to m; keys past the limit or without a page are out
+          const int valid = limit - (p.kbeg + i * PT_KEYS);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * ks[e >> 4]);
+          if (__any_sync(0xffffffffu, valid < PT_KEYS) || none) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (e >= valid || (none >> (e >> 4) & 1)) v[e] = __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int e = 0; e < 64; e += 2)
+            mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool need = m_tile > m + kLag;
+          bool pv_waited = i == 0;
+          if (__any_sync(0xffffffffu, need)) {
+            const float alpha = need ? ex2_approx(m - m_tile) : 1.f;
+            if (i > 0) {
+              // O_t += P_t(j-1) V(j-1) must have landed before O_t is rescaled
+              ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (jt - 1) & 1, abort_flag));
+              if (!ok) break;
+              tc_fence_after();
+              pv_waited = true;
+#pragma unroll
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(tO + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st_32x32b_x32(tO + c * 32, o);
+              }
+              tmem_st_wait();
+            }
+            l *= alpha;
+            if (need) m = m_tile;
+          }
+          uint32_t pk[32];
+          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x0 = __uint_as_float(v[2 * e]) - m, x1 = __uint_as_float(v[2 * e + 1]) - m;
+            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            add2_acc(ls[2 * (e & 1)], ls[2 * (e & 1) + 1], p0, p1);
+            p0 *= vr[e >> 3];
+            p1 *= vr[e >> 3];
+            pk[e] = pack_f16x2(x0 == -INFINITY ? 0.f : p0, x1 == -INFINITY ? 0.f : p1);  // 0 even where vr is NaN
+          }
+          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          if (!pv_waited) {  // a parity barrier is waited for once per phase
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (jt - 1) & 1, abort_flag));
+            if (!ok) break;
+          }
+          tmem_st_32x32b_x32(tS + b * 64, pk);  // P_t(j) over the scores just read
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[t * 2 + b]);
+        }
+        if (ok) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (jt - 1) & 1, abort_flag));
+          tc_fence_after();
+        }
+        if (!ok) break;
+        ref = s_ref[piece & 15];
+      } else {
+        j += p.tiles64;
+      }
+      if (p.tiles64 > 0) ++piece;
+      // the row's result, or its piece of one (all of a piece's rows are written: the join reads them)
+      const size_t slot = (static_cast<size_t>(cta) * 2 + (p.begins ? 1 : 0)) * PT_ROWS + t * 128 + trow;
+      const float f = p.whole ? (l == 0.f ? 0.f : ref / kPOff / l) : ref / kPOff;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();  // (the load wants the whole warp)
+        if (p.tiles64 > 0 && tile_on) {
+          tmem_ld_32x32b_x32(tO + c * 32, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        if (!has) {
+        } else if (p.whole) {
+          uint4* d4 = reinterpret_cast<uint4*>(a.out + at * HD + c * 32);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_bf16x2(__uint_as_float(o[8 * q + 2 * e]) * f, __uint_as_float(o[8 * q + 2 * e + 1]) * f);
+            d4[q] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          float4* d4 = reinterpret_cast<float4*>(a.part_o + slot * HD + c * 32);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            d4[q] = make_float4(__uint_as_float(o[4 * q]) * f, __uint_as_float(o[4 * q + 1]) * f,
+                                __uint_as_float(o[4 * q + 2]) * f, __uint_as_float(o[4 * q + 3]) * f);
+        }
+      }
+      if (has) {
+        if (!p.whole)
+          a.part_ml[slot] = make_float2(m, l);
+        else if (a.lse)
+          a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
+      }
+      if (!p.whole && p.begins && t == 0 && trow == 0)
+        a.desc[cta] = make_int4(p.row, p.rt, p.g, static_cast<int>(((p.last + 1) * C - 1) / N));
+      __syncwarp();
+      tc_fence_before();  // O_t is read before the next piece's first product (ordered by its q_ready and p_ready)
+    }
+  }
+
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (tid == 0 && *abort_flag) atomicCAS(a.err, 0, DEV_ERR_TIMEOUT_ATTN_PAGED);
+}
+
+}  // namespace mk

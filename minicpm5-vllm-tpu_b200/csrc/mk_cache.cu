@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "mk_attn_paged.cuh"
+#include "mk_attn_paged_tc.cuh"
 #include "mk_cache.cuh"
 #include "mk_host.cuh"
 
@@ -48,9 +49,11 @@ mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int 
 }
 
 // Launch shape and workspace of the paged attention.  Query rows (tokens times heads of a group) per tile: 8, 16
-// or 32, the smallest that holds a row's queries; a wider tile reads and converts the cache less often but
-// leaves room for two CTAs per SM instead of three.  One wave of CTAs on 148 SMs, fewer when the bounds say that
+// or 32, the smallest that holds a row's queries (a wider tile reads and converts the cache less often but
+// leaves room for two CTAs per SM instead of three), or 256 with tcgen05 above kPagedWide.  One wave of CTAs on 148 SMs, fewer when the bounds say that
 // there are fewer units of work.
+constexpr int kPagedTc = mk::PT_ROWS / 8;  // the tcgen05 kernel's rows, in eights
+constexpr int kPagedWide = 64;
 struct PagedPlan {
   int nt, ctas, long_join;  // long_join: CTAs that join few pairs of many pieces, 0: one per CTA of the products
   size_t o_bytes, ml_bytes, bytes;
@@ -58,11 +61,11 @@ struct PagedPlan {
 PagedPlan paged_plan(int group, int n_kv, int hd, int rows, int max_q, int max_len) {
   PagedPlan p;
   const int64_t q_rows = static_cast<int64_t>(std::max(max_q, 1)) * group;
-  p.nt = q_rows <= 8 ? 1 : q_rows <= 16 ? 2 : 4;
+  p.nt = q_rows <= 8 ? 1 : q_rows <= 16 ? 2 : q_rows <= kPagedWide ? 4 : kPagedTc;
   const int64_t tiles = (q_rows + 8 * p.nt - 1) / (8 * p.nt);
-  const int unit = mk::pa_unit(p.nt);
+  const int unit = p.nt == kPagedTc ? mk::PT_KEYS : mk::pa_unit(p.nt);
   const int64_t per_pair = std::max(1, max_len / unit + (max_len % unit != 0));
-  const int64_t most = 148 * mk::pa_ctas_per_sm(p.nt);
+  const int64_t most = p.nt == kPagedTc ? mk::PT_CTAS : 148 * mk::pa_ctas_per_sm(p.nt);
   // (each factor is below 2^31: cut before the product can overflow)
   const int64_t pairs = std::min<int64_t>(most, static_cast<int64_t>(rows) * n_kv) * std::min<int64_t>(most, tiles);
   p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min(most, pairs) * per_pair)));
@@ -92,6 +95,10 @@ mk_status paged_ready() {
   MK_CUDA(allow(mk::attn_paged_kernel<128, 1>, 128, 1));
   MK_CUDA(allow(mk::attn_paged_kernel<128, 2>, 128, 2));
   MK_CUDA(allow(mk::attn_paged_kernel<128, 4>, 128, 4));
+  MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<96>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(mk::pt_smem_bytes(96))));
+  MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(mk::pt_smem_bytes(128))));
   ready[dev] = true;
   return MK_OK;
 }
@@ -192,14 +199,16 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
   a.desc = reinterpret_cast<int4*>(ws + p.o_bytes + p.ml_bytes);
   a.err = d.err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool tc = p.nt == kPagedTc;
   void (*k)(KvPages, mk::PagedAttnArgs) =
-      head_dim == 96 ? (p.nt == 1 ? mk::attn_paged_kernel<96, 1> : p.nt == 2 ? mk::attn_paged_kernel<96, 2>
+      tc               ? (head_dim == 96 ? mk::attn_paged_tc_kernel<96> : mk::attn_paged_tc_kernel<128>)
+      : head_dim == 96 ? (p.nt == 1 ? mk::attn_paged_kernel<96, 1> : p.nt == 2 ? mk::attn_paged_kernel<96, 2>
                                                                              : mk::attn_paged_kernel<96, 4>)
                      : (p.nt == 1 ? mk::attn_paged_kernel<128, 1> : p.nt == 2 ? mk::attn_paged_kernel<128, 2>
                                                                               : mk::attn_paged_kernel<128, 4>);
-  const int ring = mk::pa_ring_bytes(head_dim, p.nt);
   MK_TRY(paged_ready());
-  MK_TRY(launch_k(k, dim3(p.ctas), dim3(mk::PA_THREADS), ring, st, true, c, a));
+  MK_TRY(launch_k(k, dim3(p.ctas), dim3(tc ? mk::PT_THREADS : mk::PA_THREADS),
+                  tc ? mk::pt_smem_bytes(head_dim) : mk::pa_ring_bytes(head_dim, p.nt), st, true, c, a));
   const auto join = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     if (p.long_join > 0)

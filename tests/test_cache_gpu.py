@@ -84,6 +84,46 @@ def test_attention_ragged_chunks(dev, hd, page, n_q, n_kv):
     _attend(dev, lens, new, n_q, n_kv, hd, page, 31 + hd + n_q)
 
 
+@pytest.mark.parametrize("hd,page,n_q,n_kv", [(96, 16, 16, 2), (128, 64, 16, 2), (96, 128, 12, 4)])
+@pytest.mark.parametrize("top", [2, 4, 8, 9, 16, 33])
+def test_attention_chunk_sizes(dev, hd, page, n_q, n_kv, top):
+    """Chunks up to `top` tokens: every width of query tile, whole tiles and parts of them."""
+    lens, new = [top, 200, 64, 0, 333, 1000], [top, 1, max(1, top // 2), 0, top, top - 1]
+    _attend(dev, lens, new, n_q, n_kv, hd, page, 57 + hd + top)
+
+
+@pytest.mark.parametrize("hd,page", [(96, 16), (128, 32), (128, 128)])
+def test_attention_chunk_with_a_nan_scale_and_a_missing_page(dev, hd, page):
+    """Wide tiles: a NaN scale shows in the queries that see its page, a missing page is reported, and what lies
+    past a row's end (garbage codes, NaN scales) does not show."""
+    from minicpm5_mk import ops
+    lens, new, n_q, n_kv = [3 * page, 200, 150], [20, 30, 40], 16, 2
+    need = sum(-(-n // page) for n in lens)
+    codes, scales = ref.pool(need + 2, n_kv, page, hd, 4)
+    table = ref.tables(lens, page, need + 2, 4)
+    idle = sorted(set(range(need + 2)) - set(table[table >= 0].tolist()))
+    scales[idle] = math.nan
+    cu = _i32([0, 20, 50, 90])
+    q = torch.randn((90, n_q, hd), generator=torch.Generator().manual_seed(1)).to(BF)
+    want = ref.attend(q, codes, scales, table, lens, cu, 0.1)
+    bad = scales.clone()
+    bad[table[0, 2], 1, 1] = math.nan  # the last page of row 0, values of head 1: seen by the queries from 2 * page on
+    o, lse = ops.attention_paged(*_gpu(dev, q, codes, bad, table, _i32(lens)), cu_q=cu.to(dev), max_q=40, max_len=3 * page,
+                                 softmax_scale=0.1)
+    hit = torch.zeros((90, n_q), dtype=torch.bool)
+    hit[[t for t in range(20) if 3 * page - 20 + t >= 2 * page], 8:] = True
+    assert o.isnan().all(-1).cpu().equal(hit) and o.isnan().any(-1).cpu().equal(hit)
+    ok = ~hit
+    _close(o.cpu()[ok], lse.cpu()[ok], *[w[ok] for w in want])
+    t = table.clone()
+    t[1, 0] = -1
+    o, lse = ops.attention_paged(*_gpu(dev, q, codes, scales, t, _i32(lens)), cu_q=cu.to(dev), max_q=40, softmax_scale=0.1)
+    assert _err() == (10, 0x500)
+    keep = [i for i in range(90) if not 20 <= i < 50]
+    _close(o[keep], lse[keep], *[w[keep] for w in want])
+    assert bool(o[20:50].isfinite().all())
+
+
 def test_attention_queries_before_the_first_key(dev):
     """More queries than tokens (a padded chunk): the first see nothing."""
     _attend(dev, [3, 0, 20], [5, 2, 4], 4, 2, 96, 16, 5)
