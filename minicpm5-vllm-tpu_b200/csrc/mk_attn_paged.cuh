@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   auto row_units = [&](int row) {
     int first;
     const int n = row_tokens(row, first);
-    return n <= 0 ? 0ll : static_cast<long long>(max(pair_units(row), 1)) * row_tiles(n) * n_kv;
+    return n <= 0 ? 0u : static_cast<uint32_t>(max(pair_units(row), 1)) * row_tiles(n) * n_kv;
   };
 
   // this CTA's share [u0, u1) of the N units, and the row where it begins
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   if (inc - mine <= u0 && u0 < inc) {
     long long base = inc - mine;
     int i = i0;
-    for (long long n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
+    for (uint32_t n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
     s_row = i;
     s_base = base;
   }
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   uint32_t phase = 0;
 
   for (long long u = u0; u < u1;) {
-    const long long ru = row_units(row);
+    const uint32_t ru = row_units(row);
     if (u >= base + ru) {
       base += ru;
       ++row;
@@ -202,9 +202,11 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
     }
     int first;
     const int n = row_tokens(row, first), len = max(a.lens[row], 0), tiles = row_tiles(n);
-    const int upp = max(pair_units(row), 1), local_pair = static_cast<int>((u - base) / upp);
-    const int ua = static_cast<int>((u - base) % upp), ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
-    const int g = local_pair / tiles, rt = local_pair % tiles;
+    // (32-bit divisions: a row's units are counted in 32 bits)
+    const uint32_t in = static_cast<uint32_t>(u - base), upp_u = max((len + PA_UNIT - 1) / PA_UNIT, 1), local_pair = in / upp_u;
+    const int upp = upp_u, ua = in - local_pair * upp_u;
+    const int ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
+    const int g = tiles == 1 ? local_pair : local_pair / tiles, rt = local_pair - g * tiles;
     const int r0 = rt * ROWS, R = n * G;
     // a query row's token sees the keys below its limit
     auto limit = [&](int qr) { return qr < R ? len - n + qr / G + 1 : 0; };
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       }
     }
     if (!whole && ua == 0 && tid == 0) {
-      const long long last = base + static_cast<long long>(local_pair + 1) * upp - 1;  // the pair's last unit
+      const long long last = base + (local_pair + 1) * upp_u - 1;  // the pair's last unit
       a.desc[cta] = make_int4(row, rt, g, static_cast<int>(((last + 1) * C - 1) / N));
     }
     fence_proxy_async_smem();  // the results before the next copies into the same bytes
@@ -626,11 +628,12 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 //   LONG  (few pairs, each in many pieces): the CTAs first number the unfinished pairs, and CTA (x, y, z) takes every
 //         gridDim.x-th from the x-th, rows 8y .. and channels 32z .. (8 groups, 32 channels: all SMs have work)
 //   else  CTA (c, y) takes rows 8y .. of the pair that began in CTA c, if one did and was not finished there
+// A piece's O is [row][channel], or (TC: from mk_attn_paged_tc.cuh) [four channels][row][4].
 template <int HD, bool LONG>
 struct PagedJoin {
   static constexpr int PARTS = LONG ? 8 : 2, DIMS = LONG ? 32 : HD, LANES = 8 * DIMS / 4, THREADS = PARTS * LANES;
 };
-template <int HD, bool LONG>
+template <int HD, bool LONG, bool TC>
 __global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_kernel(PagedAttnArgs a, int ctas) {
   using J = PagedJoin<HD, LONG>;
   __shared__ __align__(16) float s_o[J::PARTS][8][J::DIMS];
@@ -639,7 +642,8 @@ __global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_
   pdl_wait();
   pdl_trigger();
   const int ROWS = 8 * gridDim.y, G = a.group, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int grp = tid / J::LANES, q8 = tid % J::LANES / (J::DIMS / 4), d4 = tid % (J::DIMS / 4) * 4;
+  const int grp = tid / J::LANES, in = tid % J::LANES;
+  const int q8 = TC ? in % 8 : in / (J::DIMS / 4), d4 = (TC ? in / 8 : in % (J::DIMS / 4)) * 4;
   const int dim = blockIdx.z * J::DIMS + d4;
   auto join = [&](int cta, const int4& d) {
     const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1;
@@ -657,8 +661,9 @@ __global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_
     };
 #pragma unroll 4
     for (int p = grp; p < pieces; p += J::PARTS) {
-      const size_t at = (static_cast<size_t>(cta + p) * 2 + (p == 0 ? 1 : 0)) * ROWS + i;
-      add(a.part_ml[at], *reinterpret_cast<const float4*>(a.part_o + at * HD + dim));
+      const size_t slot = static_cast<size_t>(cta + p) * 2 + (p == 0 ? 1 : 0), at = slot * ROWS + i;
+      const float* o4 = TC ? a.part_o + ((slot * (HD / 4) + dim / 4) * ROWS + i) * 4 : a.part_o + at * HD + dim;
+      add(a.part_ml[at], *reinterpret_cast<const float4*>(o4));
     }
     *reinterpret_cast<float4*>(&s_o[grp][q8][d4]) = o;
     if (d4 == 0) s_ml[grp][q8] = make_float2(m, l);

@@ -35,6 +35,8 @@ __host__ __device__ constexpr uint32_t pt_raw_bytes(int hd) { return 2 * PT_KEYS
 __host__ __device__ constexpr size_t pt_smem_bytes(int hd) {
   return 1024 + 4 * PT_QCHUNK + PT_KV * pt_kv_bytes(hd) + PT_RAW * pt_raw_bytes(hd) + 1024;
 }
+// In place of a key scale of 0 (a page of zeros): the scores are 0 all the same, and those masked as -inf stay that.
+constexpr float kTinyScale = 1e-30f;
 // Instruction descriptor for kind::f16 with f16 operands, both K-major.
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   auto row_units = [&](int row) {
     int first;
     const int n = row_tokens(row, first);
-    return n <= 0 ? 0ll : static_cast<long long>(pair_units(row)) * row_tiles(n) * n_kv;
+    return n <= 0 ? 0u : static_cast<uint32_t>(pair_units(row)) * row_tiles(n) * n_kv;
   };
   const int per = (a.rows + PT_THREADS - 1) / PT_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
   long long mine = 0;
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   if (!idle && inc - mine <= u0 && u0 < inc) {
     long long base = inc - mine;
     int i = i0;
-    for (long long n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
+    for (uint32_t n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
     s_row = i;
     s_base = base;
   }
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   long long u = u0, base = idle ? 0 : s_base;
   int row = idle ? 0 : s_row;
   auto next = [&](Piece& p) {
-    long long ru = 0;
+    uint32_t ru = 0;
     while (u < u1 && u >= base + (ru = row_units(row))) {
       base += ru;
       ++row;
@@ -158,23 +160,28 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     p.n = row_tokens(row, p.first);
     p.len = max(a.lens[row], 0);
     p.R = p.n * G;
-    const int upp = pair_units(row), tiles = row_tiles(p.n), pair = static_cast<int>((u - base) / upp);
-    const int ua = static_cast<int>((u - base) % upp), ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
+    // (32-bit divisions: a row's units are counted in 32 bits)
+    const uint32_t in = static_cast<uint32_t>(u - base), upp = max((p.len + PT_KEYS - 1) / PT_KEYS, 1);
+    const uint32_t tiles = row_tiles(p.n), pair = in / upp;
+    const int ua = in - pair * upp, ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
     p.g = pair / tiles;
-    p.rt = pair % tiles;
+    p.rt = pair - p.g * tiles;
     p.r0 = p.rt * PT_ROWS;
     p.kbeg = ua * PT_KEYS;
     p.kend = min(ub * PT_KEYS, p.len - p.n + (min(p.r0 + PT_ROWS, p.R) - 1) / G + 1);
     p.tiles64 = p.kend > p.kbeg ? (p.kend - p.kbeg + PT_KEYS - 1) / PT_KEYS : 0;
-    p.whole = ua == 0 && ub == upp;
+    p.whole = ua == 0 && ub == static_cast<int>(upp);
     p.begins = ua == 0;
-    p.last = base + static_cast<long long>(pair + 1) * upp - 1;
+    p.last = base + (pair + 1) * upp - 1;
     u += ub - ua;
     return true;
   };
 
   Piece p;
   bool ok = true;
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
   if (warp == 0) {
     // ---------------------------------------------------------------- codes, pages and scales
     int j = 0, piece = 0;
@@ -190,30 +197,39 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
       if (lane == 0) s_ref[piece & 15] = ref;
       ++piece;
       const int run = min(1 << cp.page_shift, PT_KEYS);  // keys that lie together
+      int page = -1, none8 = 0;
+      float ks = 0.f, vs = 0.f;
       for (int i = 0; ok && i < p.tiles64; ++i, ++j) {
-        const int st = j % PT_RAW;
-        const int key = p.kbeg + i * PT_KEYS + 16 * lane;
-        int page = -1;
-        float ks = 0.f, vs = 0.f;
-        const bool wanted = lane < 4 && key < p.kend;
-        if (wanted) page = kv_page_of(a.table, a.width, cp.num_pages, p.row, key >> cp.page_shift, a.err);
-        if (page >= 0) {
-          ks = *kv_scale_ptr(cp, page, 0, p.g);
-          vs = *kv_scale_ptr(cp, page, 1, p.g);
+        const int st = j % PT_RAW, i8 = i & 7;
+        if (i8 == 0) {  // lane l looks up group l of the next eight tiles
+          const int key = p.kbeg + i * PT_KEYS + 16 * lane;
+          page = -1;
+          ks = vs = 0.f;
+          const bool wanted = key < p.kend;
+          if (wanted) page = kv_page_of(a.table, a.width, cp.num_pages, p.row, key >> cp.page_shift, a.err);
+          if (page >= 0) {
+            ks = *kv_scale_ptr(cp, page, 0, p.g);
+            vs = *kv_scale_ptr(cp, page, 1, p.g);
+          }
+          if (ks == 0.f) ks = kTinyScale;
+          vs = ref > 0.f ? vs / ref * kPOff : vs;
+          none8 = static_cast<int>(__ballot_sync(0xffffffffu, wanted && page < 0));
         }
-        const uint32_t none = __ballot_sync(0xffffffffu, wanted && page < 0);
         ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[st], ((j / PT_RAW) & 1) ^ 1u, abort_flag));
         if (!ok) break;
-        if (lane < 4) s_sc[(j & 7) * 4 + lane] = make_float2(ks, ref > 0.f ? vs / ref * kPOff : vs);
-        if (lane == 0) s_none[j & 7] = static_cast<int>(none);
-        const bool asks = page >= 0 && (16 * lane) % run == 0;
+        const bool here = lane >> 2 == i8;
+        const int in = lane & 3;  // group of the tile
+        if (here) s_sc[(j & 7) * 4 + in] = make_float2(ks, vs);
+        if (lane == 0) s_none[j & 7] = none8 >> (4 * i8) & 15;
+        const bool asks = here && page >= 0 && (16 * in) % run == 0;
         const uint32_t bytes = __reduce_add_sync(0xffffffffu, asks ? 2u * run * HD : 0u);
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], bytes);
         __syncwarp();
         if (asks) {
+          const int key = p.kbeg + i * PT_KEYS + 16 * in;
           const int8_t* at = kv_head_ptr(cp, page, 0, p.g) + (key & ((1 << cp.page_shift) - 1)) * HD;
-          uint8_t* dst = sRaw + st * RAW + lane * 16 * HD;
+          uint8_t* dst = sRaw + st * RAW + in * 16 * HD;
           bulk_load(dst, at, run * HD, &raw_full[st]);
           bulk_load(dst + PT_KEYS * HD, at + (static_cast<size_t>(n_kv) * HD << cp.page_shift), run * HD, &raw_full[st]);
         }
@@ -287,6 +303,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     mbar_wait_drain(drain, 0);
   } else if (warp >= 12) {
     // ---------------------------------------------------------------- int8 -> f16
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int ct = tid - 12 * 32;
     int j = 0;
     while (ok && next(p)) {
@@ -333,6 +350,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax, queries, results
+    // 512 threads x 128 registers at launch: these 256 take 168 each, the others 88
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = (warp - 4) >> 2, quarter = warp & 3, trow = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + lane_off + t * 128, tO = tmem + lane_off + 256 + t * 128;
@@ -361,7 +380,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
           }
         }
         const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-        const float down = __uint_as_float((254u - ex) << 23), sf = __uint_as_float(ex << 23) * a.scale;
+        // (a negative scale turns the queries, so that the scores' factor is not negative)
+        const float down = copysignf(__uint_as_float((254u - ex) << 23), a.scale);
+        const float sf = __uint_as_float(ex << 23) * fabsf(a.scale);
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c) {
           const uint32_t w[4] = {qv[c].x, qv[c].y, qv[c].z, qv[c].w};
@@ -387,28 +408,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
           tmem_ld_32x32b_x32(tS + b * 64, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
           tmem_ld_32x32b_x32(tS + b * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
           tmem_ld_wait();
-          float ks[4], vr[4];
+          float ks[4], vr[4], mx[4][2];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const float2 sc = s_sc[(j & 7) * 4 + q];
             ks[q] = sc.x * sf;
             vr[q] = sc.y;
+            mx[q][0] = mx[q][1] = -INFINITY;
           }
-          const int none = s_none[j & 7];
-          // scores in units of log 2, relative to m; keys past the limit or without a page are out
-          const int valid = limit - (p.kbeg + i * PT_KEYS);
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int e = 0; e < 64; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * ks[e >> 4]);
-          if (__any_sync(0xffffffffu, valid < PT_KEYS) || none) {
+          // keys past the row's limit or without a page are out
+          const int none = s_none[j & 7], valid = limit - (p.kbeg + i * PT_KEYS);
+          const bool masked = __any_sync(0xffffffffu, valid < PT_KEYS) || none;
+          if (masked) {
 #pragma unroll
             for (int e = 0; e < 64; ++e)
               if (e >= valid || (none >> (e >> 4) & 1)) v[e] = __float_as_uint(-INFINITY);
           }
+          // (the factors are not negative: a group's largest product is that of its largest score)
 #pragma unroll
           for (int e = 0; e < 64; e += 2)
-            mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            mx[e >> 4][(e >> 1) & 1] = max3f(mx[e >> 4][(e >> 1) & 1], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          float m_tile = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) m_tile = fmaxf(m_tile, fmaxf(mx[q][0], mx[q][1]) * ks[q]);
           const bool need = m_tile > m + kLag;
           bool pv_waited = i == 0;
           if (__any_sync(0xffffffffu, need)) {
@@ -437,12 +459,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
           float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float x0 = __uint_as_float(v[2 * e]) - m, x1 = __uint_as_float(v[2 * e + 1]) - m;
+            float x0, x1;
+            fma2_sc(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]), ks[e >> 3], -m, x0, x1);
             float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             add2_acc(ls[2 * (e & 1)], ls[2 * (e & 1) + 1], p0, p1);
-            p0 *= vr[e >> 3];
-            p1 *= vr[e >> 3];
-            pk[e] = pack_f16x2(x0 == -INFINITY ? 0.f : p0, x1 == -INFINITY ? 0.f : p1);  // 0 even where vr is NaN
+            fma2_sc(p0, p1, vr[e >> 3], 0.f, p0, p1);
+            pk[e] = pack_f16x2(p0, p1);
+          }
+          if (masked) {  // 0 even where the value scale is NaN
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (__uint_as_float(v[2 * e]) == -INFINITY) pk[e] &= 0xffff0000u;
+              if (__uint_as_float(v[2 * e + 1]) == -INFINITY) pk[e] &= 0x0000ffffu;
+            }
           }
           l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
           if (!pv_waited) {  // a parity barrier is waited for once per phase
@@ -491,11 +520,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
             d4[q] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          float4* d4 = reinterpret_cast<float4*>(a.part_o + slot * HD + c * 32);
+          // [four channels][row]: a warp's rows side by side
+          float4* d4 = reinterpret_cast<float4*>(a.part_o) + (slot / PT_ROWS * (HD / 4) + c * 8) * PT_ROWS + slot % PT_ROWS;
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            d4[q] = make_float4(__uint_as_float(o[4 * q]) * f, __uint_as_float(o[4 * q + 1]) * f,
-                                __uint_as_float(o[4 * q + 2]) * f, __uint_as_float(o[4 * q + 3]) * f);
+            d4[q * PT_ROWS] = make_float4(__uint_as_float(o[4 * q]) * f, __uint_as_float(o[4 * q + 1]) * f,
+                                          __uint_as_float(o[4 * q + 2]) * f, __uint_as_float(o[4 * q + 3]) * f);
         }
       }
       if (has) {

@@ -53,7 +53,7 @@ mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int 
 // leaves room for two CTAs per SM instead of three), or 256 with tcgen05 above kPagedWide.  One wave of CTAs on 148 SMs, fewer when the bounds say that
 // there are fewer units of work.
 constexpr int kPagedTc = mk::PT_ROWS / 8;  // the tcgen05 kernel's rows, in eights
-constexpr int kPagedWide = 64;
+constexpr int kPagedWide = 128;
 struct PagedPlan {
   int nt, ctas, long_join;  // long_join: CTAs that join few pairs of many pieces, 0: one per CTA of the products
   size_t o_bytes, ml_bytes, bytes;
@@ -209,15 +209,17 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
   MK_TRY(paged_ready());
   MK_TRY(launch_k(k, dim3(p.ctas), dim3(tc ? mk::PT_THREADS : mk::PA_THREADS),
                   tc ? mk::pt_smem_bytes(head_dim) : mk::pa_ring_bytes(head_dim, p.nt), st, true, c, a));
-  const auto join = [&](auto hd) {
+  const auto join = [&](auto hd, auto of_tc) {
     constexpr int HD = decltype(hd)::value;
+    constexpr bool TC = decltype(of_tc)::value;
     if (p.long_join > 0)
-      return launch_k(mk::attn_paged_join_kernel<HD, true>, dim3(p.long_join, p.nt, HD / 32),
+      return launch_k(mk::attn_paged_join_kernel<HD, true, TC>, dim3(p.long_join, p.nt, HD / 32),
                       dim3(mk::PagedJoin<HD, true>::THREADS), 0, st, true, a, p.ctas);
-    return launch_k(mk::attn_paged_join_kernel<HD, false>, dim3(p.ctas, p.nt), dim3(mk::PagedJoin<HD, false>::THREADS), 0,
-                    st, true, a, p.ctas);
+    return launch_k(mk::attn_paged_join_kernel<HD, false, TC>, dim3(p.ctas, p.nt), dim3(mk::PagedJoin<HD, false>::THREADS),
+                    0, st, true, a, p.ctas);
   };
-  return head_dim == 96 ? join(std::integral_constant<int, 96>()) : join(std::integral_constant<int, 128>());
+  const auto by_size = [&](auto hd) { return tc ? join(hd, std::true_type()) : join(hd, std::false_type()); };
+  return head_dim == 96 ? by_size(std::integral_constant<int, 96>()) : by_size(std::integral_constant<int, 128>());
 }
 
 size_t mk_kv_move_workspace(int32_t rows, int32_t num_pages) {
