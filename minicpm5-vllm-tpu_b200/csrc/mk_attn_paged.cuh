@@ -25,7 +25,7 @@ namespace mk {
 struct PagedAttnArgs {
   const __nv_bfloat16* q;
   long long ld_q, hs_q;
-  int n_q, group, rows, width;  // group = n_q / n_kv
+  int T, n_q, group, rows, width;  // group = n_q / n_kv
   const int32_t* table;
   const int32_t* lens;
   const int32_t* cu;
@@ -46,15 +46,17 @@ __host__ __device__ constexpr int pa_groups(int nt) { return nt == 1 ? 2 : 1; }
 __host__ __device__ constexpr int pa_unit(int nt) { return 16 * pa_groups(nt) * PA_WARPS; }  // keys of one unit of work
 constexpr int PA_GROUPS = 64;           // groups whose pages and scales are staged at a time
 // m may lag the true maximum by up to 2^kLag: it moves only then, which spares a warp reduction and a rescaling
-// of O per 16 keys.
+// of O per block.
 //
-// The probabilities p = exp(s - m) * vscale are rounded for their product with the codes.  With up to 16 query
-// rows per tile the tensor pipe idles behind the loads, and p goes in as two bf16 parts (p rounded, and what
-// that left over): 17 bits, and the range of f32, so that keys far below the maximum still count where the
-// others have a zero.  With 32 rows the products and conversions are the limit, and p is one f16 (11 bits), held
-// times kPOff: the largest operand is 2^15, and a key that weighs less than 2^-31 of the maximum is lost.
-constexpr float kPOff = 128.f;
-constexpr float kLag = 8.f;
+// The probabilities p = exp(s - m) * vscale are rounded for their product with the codes: to one f16 (11 bits), held
+// times kPOff, so that the largest operand is 2^15.  With up to 16 query rows a block whose smallest p is below f16's
+// normal range (2^-24 of the maximum; or masked) is multiplied in another way, with p as two bf16 parts (p rounded, and
+// what that left over): 17 bits and the range of f32, so that keys far below the maximum still count where the others
+// have a zero.  That conversion and its second product cost a block a quarter more instructions.  With 32 rows the
+// products are the limit, and a key that weighs less than 2^-34 of the maximum is lost.
+constexpr float kPOff = 1024.f;
+constexpr float kLag = 5.f;
+constexpr float kF16Normal = 0x1p-14f;
 // m before the first key: low enough that any score raises it, and finite, so that m - m is 0
 constexpr float kLow = -1e30f;
 
@@ -106,6 +108,17 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A row's queries: [first, first + n); rows that name tokens outside [0, T) have none, and set the error word.
+__device__ __forceinline__ int paged_row_tokens(const PagedAttnArgs& a, int row, int& first) {
+  first = row;
+  if (!a.cu) return 1;
+  first = a.cu[row];
+  const int n = max(a.cu[row + 1] - first, 0);
+  if (n == 0 || (first >= 0 && n <= a.T - first)) return n;
+  atomicCAS(a.err, 0, DEV_ERR_BAD_PAGE);
+  return 0;
+}
+
 // Work.  A pair is (row, tile of 8 NT query rows, key/value head), a query row being (token, head of the
 // group); a pair's keys are cut into units of PA_UNIT.  All units of all pairs, in order, are dealt out in equal
 // contiguous shares, one per CTA, from the lengths on the device: ragged batches, one long row and many short
@@ -123,7 +136,7 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
   constexpr int GP = pa_groups(NT), PA_UNIT = pa_unit(NT);
   constexpr int KS = HD / 16, MT = HD / 16, ROWS = 8 * NT, LDO = HD + 4;
-  constexpr bool SPLIT = NT <= 2;  // p as two bf16 parts
+  constexpr bool SPLIT = NT <= 2;  // p as two bf16 parts where f16 would lose some
   constexpr int STAGES = pa_stages(HD, NT), STAGE = pa_stage_bytes(HD, NT), HALF = STAGE / 2;
   __shared__ long long s_scan[PA_WARPS], s_base;
   __shared__ int s_row;
@@ -144,12 +157,10 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int G = a.group, n_kv = cp.n_kv, page_mask = (1 << cp.page_shift) - 1;
 
-  auto row_tokens = [&](int row, int& first) {
-    first = a.cu ? a.cu[row] : row;
-    return a.cu ? a.cu[row + 1] - first : 1;
-  };
+  auto row_tokens = [&](int row, int& first) { return paged_row_tokens(a, row, first); };
+  auto row_len = [&](int row) { return kv_row_len(a.lens, row, a.width, cp.page_shift, a.err); };
   auto row_tiles = [&](int n) { return (n * G + ROWS - 1) / ROWS; };
-  auto pair_units = [&](int row) { return (max(a.lens[row], 0) + PA_UNIT - 1) / PA_UNIT; };
+  auto pair_units = [&](int row) { return (row_len(row) + PA_UNIT - 1) / PA_UNIT; };
   // an idle row still has its zeros to write: one unit
   auto row_units = [&](int row) {
     int first;
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       continue;
     }
     int first;
-    const int n = row_tokens(row, first), len = max(a.lens[row], 0), tiles = row_tiles(n);
+    const int n = row_tokens(row, first), len = row_len(row), tiles = row_tiles(n);
     // (32-bit divisions: a row's units are counted in 32 bits)
     const uint32_t in = static_cast<uint32_t>(u - base), upp_u = max((len + PA_UNIT - 1) / PA_UNIT, 1), local_pair = in / upp_u;
     const int upp = upp_u, ua = in - local_pair * upp_u;
@@ -292,6 +303,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
     }
+    const uint32_t plane = static_cast<uint32_t>(n_kv) * HD << cp.page_shift, page_bytes = 2 * plane;
+    const int8_t* heads = cp.codes + (static_cast<size_t>(g) * HD << cp.page_shift);  // head g of page 0
     float vref = 0.f;  // the largest value scale so far: O is in units of vref / kPOff
 
     for (int kb = kbeg; kb < kend; kb += PA_GROUPS * 16) {
@@ -330,12 +343,12 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       auto ask = [&](int gi, int stage) {
         uint8_t* dst = ring + stage * STAGE;
         uint64_t* bar = &s_full[warp][stage];
-        const size_t plane = static_cast<size_t>(n_kv) * HD << cp.page_shift;
         if (GP == 1 || cp.page_shift > 4) {
           const int pg = s_page[gi];
           mbar_arrive_expect_tx(bar, pg < 0 ? 0 : STAGE);
           if (pg >= 0) {
-            const int8_t* at = kv_head_ptr(cp, pg, 0, g) + ((kb + gi * 16) & page_mask) * HD;
+            const int8_t* at = heads + static_cast<uint64_t>(static_cast<uint32_t>(pg)) * page_bytes +
+                               ((kb + gi * 16) & page_mask) * HD;
             bulk_load(dst, at, HALF, bar);
             bulk_load(dst + HALF, at + plane, HALF, bar);
           }
@@ -347,7 +360,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 #pragma unroll
           for (int p = 0; p < GP; ++p)
             if (s_page[gi + p] >= 0) {
-              const int8_t* at = kv_head_ptr(cp, s_page[gi + p], 0, g);
+              const int8_t* at = heads + static_cast<uint64_t>(static_cast<uint32_t>(s_page[gi + p])) * page_bytes;
               bulk_load(dst + p * 16 * HD, at, 16 * HD, bar);
               bulk_load(dst + HALF + p * 16 * HD, at + plane, 16 * HD, bar);
             }
@@ -477,44 +490,73 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
             }
           centre();
         }
-        uint32_t pb[GP][NT][2], pl[SPLIT ? GP : 1][NT][2];
+        float least = INFINITY;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int p = 0; p < GP; ++p) {
-            float y[4];
+            float(&y)[4] = x[p][t];
+            float z[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[e] = ex2_approx(x[p][t][e]);
-              l[t][e & 1] += y[e];
-              y[e] *= vr[p];
+            for (int e = 0; e < 4; ++e) z[e] = ex2_approx(y[e]);
+            add2_acc(l[t][0], l[t][1], z[0], z[1]);
+            add2_acc(l[t][0], l[t][1], z[2], z[3]);
+            if (masked) {  // 0 even where the scale is NaN
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = y[e] == -INFINITY ? 0.f : z[e] * vr[p];
+            } else {
+              fma2_sc(z[0], z[1], vr[p], 0.f, y[0], y[1]);
+              fma2_sc(z[2], z[3], vr[p], 0.f, y[2], y[3]);
             }
-            if (masked)  // 0 even where the scale is NaN
+            least = fminf(fminf(least, fminf(y[0], y[1])), fminf(y[2], y[3]));
+          }
+        const bool narrow = !SPLIT || __all_sync(0xffffffffu, least >= kF16Normal);
+        if (narrow) {
+          uint32_t pb[GP][NT][2];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (x[p][t][e] == -INFINITY) y[e] = 0.f;
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if constexpr (SPLIT) {
+            for (int p = 0; p < GP; ++p)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) pb[p][t][e] = movmatrix_trans(pack_f16x2(x[p][t][2 * e], x[p][t][2 * e + 1]));
+#pragma unroll
+          for (int p = 0; p < GP; ++p)
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+              const uint4 x4 = *reinterpret_cast<const uint4*>(block + HALF + p * 16 * HD + lane_v + j * 128);
+              const uint32_t w[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t a0, a1, a2, a3;
+                i8x4_to_f16x4(w[2 * h], a0, a2);
+                i8x4_to_f16x4(w[2 * h + 1], a1, a3);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma_16816(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
+              }
+            }
+        } else if constexpr (SPLIT) {
+          uint32_t pb[GP][NT][2], pl[GP][NT][2];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int p = 0; p < GP; ++p)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float(&y)[4] = x[p][t];
                 const uint32_t hi = pack_bf16x2(y[2 * e], y[2 * e + 1]);
                 const float2 f = unpack_bf16x2(hi);
                 pb[p][t][e] = movmatrix_trans(hi);
                 pl[p][t][e] = movmatrix_trans(pack_bf16x2(y[2 * e] - f.x, y[2 * e + 1] - f.y));
-              } else {
-                pb[p][t][e] = movmatrix_trans(pack_f16x2(y[2 * e], y[2 * e + 1]));
               }
-            }
-          }
 #pragma unroll
-        for (int p = 0; p < GP; ++p)
+          for (int p = 0; p < GP; ++p)
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            const uint4 x4 = *reinterpret_cast<const uint4*>(block + HALF + p * 16 * HD + lane_v + j * 128);
-            const uint32_t w[4] = {x4.x, x4.y, x4.z, x4.w};
+            for (int j = 0; j < HD / 32; ++j) {
+              const uint4 x4 = *reinterpret_cast<const uint4*>(block + HALF + p * 16 * HD + lane_v + j * 128);
+              const uint32_t w[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t a0, a1, a2, a3;
-              if constexpr (SPLIT) {
+              for (int h = 0; h < 2; ++h) {
+                uint32_t a0, a1, a2, a3;
                 i8x4_to_bf16x4(w[2 * h], a0, a2);
                 i8x4_to_bf16x4(w[2 * h + 1], a1, a3);
 #pragma unroll
@@ -522,14 +564,9 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
                   mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
                   mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pl[p][t][0], pl[p][t][1]);
                 }
-              } else {
-                i8x4_to_f16x4(w[2 * h], a0, a2);
-                i8x4_to_f16x4(w[2 * h + 1], a1, a3);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) mma_16816(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
               }
             }
-          }
+        }
         // every lane has used the stage's bytes: it is asked for again
         __syncwarp();
         if (lane == 0 && left > STAGES) ask(gi + STAGES * PA_WARPS * GP, st);
@@ -646,7 +683,8 @@ __global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_
   const int q8 = TC ? in % 8 : in / (J::DIMS / 4), d4 = (TC ? in / 8 : in % (J::DIMS / 4)) * 4;
   const int dim = blockIdx.z * J::DIMS + d4;
   auto join = [&](int cta, const int4& d) {
-    const int first = a.cu ? a.cu[d.x] : d.x, n = a.cu ? a.cu[d.x + 1] - first : 1;
+    int first;
+    const int n = paged_row_tokens(a, d.x, first);
     const int pieces = d.w - cta + 1, i = blockIdx.y * 8 + q8, qr = d.y * ROWS + i;
     float m = kLow, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

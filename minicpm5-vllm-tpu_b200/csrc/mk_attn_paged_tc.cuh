@@ -15,7 +15,10 @@
 //               K-major operands; a 32-bit word of the value plane is four neighbouring keys of one channel already
 //
 // Queries are scaled by a power of two to f16 without loss (its inverse joins the score's factor), codes are exact, and
-// p = exp(s - m) * vscale goes in as f16 (11 bits), as for the wide tiles of mk_attn_paged.cuh.
+// p = exp(s - m) * vscale goes in as f16 (11 bits), as for the wide tiles of mk_attn_paged.cuh, here held times kTcPOff:
+// a rescaling waits for the product before it and passes O through registers, so m may lag more (16 rows of
+// up to 64 tokens over up to 8192 keys: 65.3 us so, 66.3 with 1024 and 5); a key that weighs less than 2^-31 of the
+// maximum is lost.
 #pragma once
 
 #include "mk_attn_paged.cuh"
@@ -35,6 +38,7 @@ __host__ __device__ constexpr uint32_t pt_raw_bytes(int hd) { return 2 * PT_KEYS
 __host__ __device__ constexpr size_t pt_smem_bytes(int hd) {
   return 1024 + 4 * PT_QCHUNK + PT_KV * pt_kv_bytes(hd) + PT_RAW * pt_raw_bytes(hd) + 1024;
 }
+constexpr float kTcPOff = 128.f, kTcLag = 8.f;
 // In place of a key scale of 0 (a page of zeros): the scores are 0 all the same, and those masked as -inf stay that.
 constexpr float kTinyScale = 1e-30f;
 // Instruction descriptor for kind::f16 with f16 operands, both K-major.
@@ -101,12 +105,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   pdl_wait();
 
   // Work in equal shares of units, as in attn_paged_kernel, here with 256 rows a pair.
-  auto row_tokens = [&](int row, int& first) {
-    first = a.cu ? a.cu[row] : row;
-    return a.cu ? a.cu[row + 1] - first : 1;
-  };
+  auto row_tokens = [&](int row, int& first) { return paged_row_tokens(a, row, first); };
+  auto row_len = [&](int row) { return kv_row_len(a.lens, row, a.width, cp.page_shift, a.err); };
   auto row_tiles = [&](int n) { return (n * G + PT_ROWS - 1) / PT_ROWS; };
-  auto pair_units = [&](int row) { return max((max(a.lens[row], 0) + PT_KEYS - 1) / PT_KEYS, 1); };
+  auto pair_units = [&](int row) { return max((row_len(row) + PT_KEYS - 1) / PT_KEYS, 1); };
   auto row_units = [&](int row) {
     int first;
     const int n = row_tokens(row, first);
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     if (u >= u1) return false;
     p.row = row;
     p.n = row_tokens(row, p.first);
-    p.len = max(a.lens[row], 0);
+    p.len = row_len(row);
     p.R = p.n * G;
     // (32-bit divisions: a row's units are counted in 32 bits)
     const uint32_t in = static_cast<uint32_t>(u - base), upp = max((p.len + PT_KEYS - 1) / PT_KEYS, 1);
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
             vs = *kv_scale_ptr(cp, page, 1, p.g);
           }
           if (ks == 0.f) ks = kTinyScale;
-          vs = ref > 0.f ? vs / ref * kPOff : vs;
+          vs = ref > 0.f ? vs / ref * kTcPOff : vs;
           none8 = static_cast<int>(__ballot_sync(0xffffffffu, wanted && page < 0));
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[st], ((j / PT_RAW) & 1) ^ 1u, abort_flag));
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
           float m_tile = -INFINITY;
 #pragma unroll
           for (int q = 0; q < 4; ++q) m_tile = fmaxf(m_tile, fmaxf(mx[q][0], mx[q][1]) * ks[q]);
-          const bool need = m_tile > m + kLag;
+          const bool need = m_tile > m + kTcLag;
           bool pv_waited = i == 0;
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? ex2_approx(m - m_tile) : 1.f;
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
       if (p.tiles64 > 0) ++piece;
       // the row's result, or its piece of one (all of a piece's rows are written: the join reads them)
       const size_t slot = (static_cast<size_t>(cta) * 2 + (p.begins ? 1 : 0)) * PT_ROWS + t * 128 + trow;
-      const float f = p.whole ? (l == 0.f ? 0.f : ref / kPOff / l) : ref / kPOff;
+      const float f = p.whole ? (l == 0.f ? 0.f : ref / kTcPOff / l) : ref / kTcPOff;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];

@@ -36,6 +36,9 @@ mk_status kv_pages(KvPages* out, void* codes, float* scales, int num_pages, int 
   return MK_OK;
 }
 
+// Tables hold less than 2^31 - 256 tokens a row, so that positions stay 32-bit numbers.
+bool table_fits(int width, int page) { return width <= (INT_MAX - 256) / page; }
+
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 size_t page_bytes(int n_kv, int page, int hd) { return static_cast<size_t>(2) * n_kv * page * hd; }
@@ -118,7 +121,7 @@ mk_status mk_kv_append(const void* k, const void* v, int64_t ld_k, int64_t head_
   if (!k || !v || !block_table || !lens) return MK_ERR_BAD_ARG;
   if (!aligned16(k) || !aligned16(v) || ld_k % 8 || ld_v % 8 || head_ld_k % 8 || head_ld_v % 8) return MK_ERR_BAD_ALIGN;
   const int touched = (std::max(1, cu_new ? max_new : 1) + page_size - 2) / page_size + 1;
-  if (static_cast<int64_t>(rows) * touched > INT_MAX || n_kv > 65535) return MK_ERR_TOO_LARGE;
+  if (static_cast<int64_t>(rows) * touched > INT_MAX || n_kv > 65535 || !table_fits(width, page_size)) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   using Kernel = decltype(&mk::kv_append_kernel<96, 4>);
@@ -143,7 +146,7 @@ mk_status mk_kv_read(const void* codes, const float* scales, int32_t num_pages, 
   if (!k || !v || !block_table || !start || !count) return MK_ERR_BAD_ARG;
   if (!aligned16(k) || !aligned16(v)) return MK_ERR_BAD_ALIGN;
   const int64_t items = (static_cast<int64_t>(max_count) / 4 + 2) * (head_dim / 8);
-  if (items > INT_MAX || rows > 65535 || n_kv > 32767) return MK_ERR_TOO_LARGE;
+  if (items > INT_MAX || rows > 65535 || n_kv > 32767 || !table_fits(width, page_size)) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   const int blocks = static_cast<int>((items + mk::KVR_THREADS - 1) / mk::KVR_THREADS);
@@ -183,6 +186,7 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.ld_q = ld_q;
   a.hs_q = head_ld_q;
+  a.T = T;
   a.n_q = n_q;
   a.group = n_q / n_kv;
   a.rows = rows;
@@ -241,7 +245,7 @@ mk_status mk_kv_fork(void* codes, float* scales, int32_t layers, int32_t num_pag
   if (new_rows && (new_table == block_table || new_lens == lens)) return MK_ERR_BAD_ARG;
   if (workspace_bytes < mk_kv_move_workspace(new_rows, num_pages)) return MK_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MK_ERR_BAD_ALIGN;
-  if (new_rows > mk::PG_ROWS_MAX || layers > 65534) return MK_ERR_TOO_LARGE;
+  if (new_rows > mk::PG_ROWS_MAX || layers > 65534 || !table_fits(width, page_size)) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -275,7 +279,7 @@ mk_status mk_kv_reserve(int32_t* block_table, const int32_t* lens, int32_t rows,
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return MK_ERR_BAD_SHAPE;
   if (rows == 0) return MK_OK;
   if (!refs || !block_table || !lens) return MK_ERR_BAD_ARG;
-  if (rows > mk::PG_ROWS_MAX) return MK_ERR_TOO_LARGE;
+  if (rows > mk::PG_ROWS_MAX || !table_fits(width, page_size)) return MK_ERR_TOO_LARGE;
   HostDevice d;
   MK_TRY(mk::host_device(&d));
   const int shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;

@@ -32,9 +32,19 @@ __device__ __forceinline__ float* kv_scale_ptr(const KvPages& c, int page, int p
   return c.scales + (static_cast<size_t>(page) * 2 + plane) * c.n_kv + head;
 }
 
+// A row's length, cut to what its table holds (a longer one sets the error word: its pages are missing).  Tables hold
+// less than 2^31 - 256 tokens (checked on the host), so that sums of a length and a page do not overflow.
+__device__ __forceinline__ int kv_row_len(const int32_t* lens, int row, int width, int page_shift, int* err) {
+  const int len = max(lens[row], 0), most = width << page_shift;
+  if (len <= most) return len;
+  if (err) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+  return most;
+}
+
 // Page of slot `slot` of row `row`, -1 (and the error word set) where the table has no such page.
 __device__ __forceinline__ int kv_page_of(const int32_t* table, int width, int num_pages, int row, int slot, int* err) {
-  const int page = slot < width ? table[static_cast<size_t>(row) * width + slot] : -1;
+  const bool in = static_cast<unsigned>(slot) < static_cast<unsigned>(width);
+  const int page = in ? table[static_cast<size_t>(row) * width + slot] : -1;
   if (page >= 0 && page < num_pages) return page;
   if (err) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
   return -1;
@@ -101,11 +111,15 @@ __global__ void __launch_bounds__(kva_threads(HD, SHIFT))
   pdl_trigger();
   const int row = blockIdx.x / touched, plane = blockIdx.y, head = blockIdx.z;
   const int tok0 = cu ? cu[row] : row, n = cu ? cu[row + 1] - tok0 : 1;
-  const int len = lens[row];
-  if (n <= 0 || len < 0 || tok0 < 0 || tok0 + n > T) return;
+  if (n <= 0 || lens[row] < 0) return;
+  if (tok0 < 0 || n > T - tok0) {  // tokens that are not there
+    atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+    return;
+  }
+  const int len = kv_row_len(lens, row, width, SHIFT, err);
   const int slot = (len >> SHIFT) + blockIdx.x % touched;
   const int pos0 = slot << SHIFT;
-  if (pos0 >= len + n) return;
+  if (slot > width || pos0 - len >= n) return;  // (the first slot past the table is an error below)
   const int page = kv_page_of(table, width, c.num_pages, row, slot, err);
   if (page < 0) return;
   const long long ld = plane ? ld_v : ld_k;
@@ -128,7 +142,7 @@ __global__ void __launch_bounds__(kva_threads(HD, SHIFT))
     for (int t = 0; t < 4; ++t) {
       const int pos = pos0 + 4 * g + t;
       x[i][t] = make_uint4(0, 0, 0, 0);
-      if (mine && pos >= len && pos < len + n) x[i][t] = __ldg(reinterpret_cast<const uint4*>(at + t * ld));
+      if (mine && pos >= len && pos - len < n) x[i][t] = __ldg(reinterpret_cast<const uint4*>(at + t * ld));
       const uint32_t a = __vmaxu2(x[i][t].x & 0x7fff7fffu, x[i][t].y & 0x7fff7fffu);
       const uint32_t b = __vmaxu2(x[i][t].z & 0x7fff7fffu, x[i][t].w & 0x7fff7fffu);
       top = __vmaxu2(top, __vmaxu2(a, b));
@@ -158,7 +172,7 @@ __global__ void __launch_bounds__(kva_threads(HD, SHIFT))
     if (!mine) continue;
     const int pos = pos0 + 4 * g;
     // tokens of this group: [0, o) were there, [o, m) are new, [m, 4) are past the end
-    const int o = min(4, max(0, len - pos)), m = min(4, max(0, len + n - pos));
+    const int o = min(4, max(0, len - pos)), m = min(4, max(0, n - (pos - len)));
     if (m == o && !(again && o > 0)) continue;
     if (fast && o == 0 && m == 4) {  // four new tokens: nothing of the page's bytes is read
       uint32_t t[4][8];
@@ -261,9 +275,10 @@ __global__ void __launch_bounds__(KVR_THREADS)
   pdl_wait();
   pdl_trigger();
   const int row = blockIdx.y, plane = blockIdx.z >= c.n_kv, head = blockIdx.z - (plane ? c.n_kv : 0);
-  const int s0 = start[row], n = s0 < 0 ? 0 : min(count[row], max_count);
+  const int s0 = kv_row_len(start, row, width, c.page_shift, err);
+  const int n = start[row] < 0 ? 0 : min(count[row], max_count);
   const int it = blockIdx.x * KVR_THREADS + threadIdx.x, g = it / chunks, ch = it % chunks;
-  const int lead = max(s0, 0) & 3;           // tokens of the first group before the range
+  const int lead = s0 & 3;                   // tokens of the first group before the range
   const int i0 = 4 * g - lead;               // output row of the group's first token
   if (i0 >= max_count) return;
   uint32_t u[4][4] = {};
@@ -349,9 +364,8 @@ __global__ void __launch_bounds__(FORK_THREADS)
     if (threadIdx.x == 0) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
     p = -1;
   }
-  int len = p < 0 ? 0 : max(0, lens[p]);
-  const int n = min(width, (len + (1 << page_shift) - 1) >> page_shift);
-  if (threadIdx.x == 0 && len > (width << page_shift)) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+  const int len = p < 0 ? 0 : kv_row_len(lens, p, width, page_shift, err);
+  const int n = (len + (1 << page_shift) - 1) >> page_shift;
   bool twin = false;  // an earlier row continues the same parent
   if (p >= 0)
     for (int j = threadIdx.x; j < i; j += FORK_THREADS) twin |= parents[j] == p;
@@ -371,6 +385,15 @@ __global__ void __launch_bounds__(FORK_THREADS)
   }
 }
 
+// One past the last slot that a row needs for its next n_new tokens, cut to the table (more sets the error word).
+__device__ __forceinline__ int kv_reserve_end(const int32_t* lens, const int32_t* n_new, int row, int width, int page_shift,
+                                              int* err) {
+  const long long end = static_cast<long long>(max(lens[row], 0)) + (n_new ? max(n_new[row], 0) : 1);
+  const long long slots = (end + (1 << page_shift) - 1) >> page_shift;
+  if (slots > width && err) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
+  return static_cast<int>(min(slots, static_cast<long long>(width)));
+}
+
 // Hands free pages (refs == 0, lowest first) to the rows that ask for them, in row order; upto[i] is the number of
 // requests of rows 0 .. i, in shared memory.  One pass of the CTA over refs, 4 bytes a page, which stops once every
 // request is served.
@@ -381,7 +404,6 @@ __device__ __forceinline__ void deal_pages(const int* upto, int asked, int32_t* 
                                            int width, const int32_t* n_new, const int32_t* src, int2* pairs,
                                            int32_t* n_pairs, int32_t* refs, int num_pages, int page_shift, int* sums,
                                            int* err) {
-  const int page_tokens = 1 << page_shift;
   int given = 0;
   for (int base = 0; base < num_pages && given < asked; base += PG_THREADS) {
     const int page = base + threadIdx.x;
@@ -394,16 +416,14 @@ __device__ __forceinline__ void deal_pages(const int* upto, int asked, int32_t* 
         const int mid = (lo + hi) >> 1;
         if (upto[mid] > k) hi = mid; else lo = mid + 1;
       }
-      const int len = max(0, lens[lo]);
       int32_t* mine = table + static_cast<size_t>(lo) * width;
       if (src) {
-        mine[min(width, (len + page_tokens - 1) >> page_shift) - 1] = page;
+        mine[((lens[lo] + (1 << page_shift) - 1) >> page_shift) - 1] = page;  // (cut to the table before)
         pairs[k] = make_int2(src[lo], page);
       } else {
         // the row's r-th missing slot: a row's slots with pages come before those without
-        const int r = k - (lo ? upto[lo - 1] : 0), add = n_new ? max(0, n_new[lo]) : 1;
-        const int end = min(width, (len + add + page_tokens - 1) >> page_shift), mine_n = upto[lo] - (lo ? upto[lo - 1] : 0);
-        mine[end - mine_n + r] = page;
+        const int r = k - (lo ? upto[lo - 1] : 0), mine_n = upto[lo] - (lo ? upto[lo - 1] : 0);
+        mine[kv_reserve_end(lens, n_new, lo, width, page_shift, nullptr) - mine_n + r] = page;
       }
       refs[page] = 1;
     }
@@ -432,10 +452,9 @@ __global__ void __launch_bounds__(PG_THREADS)
       if (src) {
         want = src[i] >= 0;
       } else {
-        const int len = max(0, lens[i]), add = n_new ? max(0, n_new[i]) : 1;
-        const int first = len >> page_shift, end = (len + add + (1 << page_shift) - 1) >> page_shift;
-        if (add > 0 && end > width) atomicCAS(err, 0, DEV_ERR_NO_PAGE);
-        for (int j = first; j < min(end, width); ++j) want += table[static_cast<size_t>(i) * width + j] < 0;
+        const int first = kv_row_len(lens, i, width, page_shift, err) >> page_shift;
+        const int end = kv_reserve_end(lens, n_new, i, width, page_shift, err);
+        for (int j = first; j < end; ++j) want += table[static_cast<size_t>(i) * width + j] < 0;
       }
     }
     int total;
@@ -479,8 +498,7 @@ __global__ void __launch_bounds__(PG_THREADS)
         atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
         p = -1;
       }
-      const int len = p < 0 ? 0 : max(0, lens[p]), n = min(width, (len + (1 << page_shift) - 1) >> page_shift);
-      if (len > (width << page_shift)) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+      const int len = p < 0 ? 0 : kv_row_len(lens, p, width, page_shift, err), n = (len + (1 << page_shift) - 1) >> page_shift;
       new_lens[i] = len;
       src[i] = -1;
       if (p >= 0 && n > 0 && eldest[p] < i && (len & ((1 << page_shift) - 1))) {
@@ -499,7 +517,7 @@ __global__ void __launch_bounds__(PG_THREADS)
     const int i = e / width, j = e - i * width, p = parents[i];
     const int n = (new_lens[i] + (1 << page_shift) - 1) >> page_shift;
     const bool ok = p >= 0 && p < rows_in && j < n;
-    const bool copy = ok && j == min(n, width) - 1 && eldest[p] < i && (new_lens[i] & ((1 << page_shift) - 1));
+    const bool copy = ok && j == n - 1 && eldest[p] < i && (new_lens[i] & ((1 << page_shift) - 1));
     int page = -1;
     if (ok && !copy) page = kv_page_of(table, width, num_pages, p, j, err);
     if (page >= 0) atomicAdd(refs + page, 1);

@@ -266,6 +266,48 @@ def test_attention_missing_page_is_reported(dev):
     assert _err() == (0, 0)
 
 
+@pytest.mark.parametrize("top", [1, 40])
+def test_lengths_and_tokens_out_of_range_are_reported(dev, top):
+    """Lengths past the table (up to the largest int) and token ranges past T read and write nothing outside; the
+    other rows are right."""
+    from minicpm5_mk import ops
+    lens, page, hd = [60, 60, 60], 16, 96
+    codes, scales = ref.pool(13, 2, page, hd, 4)
+    table = ref.tables(lens, page, 13, 4)
+    T = 3 * top
+    q = torch.randn((T, 16, hd), generator=torch.Generator().manual_seed(1)).to(BF)
+    cu = _i32([0, top, 2 * top, 3 * top])
+    want = ref.attend(q, codes, scales, table, lens, cu, 0.1)
+    one = dict(cu_q=cu.to(dev), max_q=top) if top > 1 else {}
+    keep = list(range(top)) + list(range(2 * top, T))
+    for bad in (65, 2 ** 31 - 1):
+        o, lse = ops.attention_paged(*_gpu(dev, q, codes, scales, table, _i32([60, bad, 60])), **one, softmax_scale=0.1)
+        assert _err() == (10, 0x500)
+        _close(o[keep], lse[keep], *[w[keep] for w in want])
+    for bad in ([0, top, 2 * top, 2 ** 31 - 1], [0, top, 2 * top, T + 1], [0, top, -5, T], [0, -2 ** 31, 2 * top, T]):
+        o, lse = ops.attention_paged(*_gpu(dev, q, codes, scales, table, _i32(lens)), cu_q=_i32(bad).to(dev), max_q=top,
+                                     softmax_scale=0.1)
+        assert _err()[0] in (0, 10)
+        if bad[1] == top:
+            _close(o[:top], lse[:top], *[w[:top] for w in want])
+    cd, sd = _gpu(dev, codes, scales)
+    x = torch.ones((2, 2, hd), dtype=BF, device=dev)
+    for ln, c in (([64, 2 ** 31 - 1, 0], [0, 1, 2, 2]), ([0, 0, 0], [0, 3, 3, 3]), ([0, 0, 0], [0, -1, 0, 2 ** 31 - 1])):
+        ops.kv_append(x, x, cd, sd, *_gpu(dev, table, _i32(ln), _i32(c)), max_new=5)
+        assert _err() == (10, 0x500)
+    # (the last of them wrote row 1's token -1 .. 0 nowhere, and the pool is as it was)
+    assert cd.cpu().equal(codes) and sd.cpu().equal(scales)
+    k, v = ops.kv_read(cd, sd, *_gpu(dev, table, _i32([2 ** 31 - 1, 64, 60]), _i32([4, 4, 2 ** 31 - 1])), 8)
+    assert _err() == (10, 0x500)
+    assert not bool(k[:2].any()) and not bool(k[2, 4:].any())
+    pool6 = cd[None].contiguous(), sd[None].contiguous()
+    refs = torch.ones(13, dtype=torch.int32, device=dev)
+    t, n, f = ops.kv_fork(*pool6, *_gpu(dev, table, _i32([60, 2 ** 31 - 1, 60])), refs, _i32([1, 1, 0, 2 ** 31 - 1]).to(dev))
+    assert _err() == (10, 0x500) and n.cpu().tolist() == [64, 64, 60, 0]
+    ops.kv_reserve(t, _i32([2 ** 31 - 1, 64, 60, 0]).to(dev), f, _i32([2 ** 31 - 1, 1, 0, 0]).to(dev), page)
+    assert _err()[0] == 10
+
+
 # ---------------------------------------------------------------------------------------- append, read
 def _check_pool(codes, scales, got_codes, got_scales, ids):
     ids = [int(i) for i in ids]
