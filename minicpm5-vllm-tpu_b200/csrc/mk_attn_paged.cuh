@@ -108,16 +108,42 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A row's queries: [first, first + n); rows that name tokens outside [0, T) have none, and set the error word.
-__device__ __forceinline__ int paged_row_tokens(const PagedAttnArgs& a, int row, int& first) {
-  first = row;
-  if (!a.cu) return 1;
-  first = a.cu[row];
-  const int n = max(a.cu[row + 1] - first, 0);
-  if (n == 0 || (first >= 0 && n <= a.T - first)) return n;
-  atomicCAS(a.err, 0, DEV_ERR_BAD_PAGE);
-  return 0;
+// A row's queries are tokens [first, first + n), its cached tokens [0, len).  Rows that name tokens outside [0, T) have no
+// queries, and a length past the table is cut to it; both set the error word.
+struct PagedRow {
+  int first, n, len;
+};
+__device__ __forceinline__ PagedRow paged_row(const PagedAttnArgs& a, int page_shift, int row) {
+  // (three loads at once)
+  const int len = a.lens[row], first = a.cu ? a.cu[row] : row, end = a.cu ? a.cu[row + 1] : row + 1;
+  PagedRow p = {first, max(end - first, 0), min(max(len, 0), a.width << page_shift)};
+  if (len > p.len) atomicCAS(a.err, 0, DEV_ERR_BAD_PAGE);
+  if (p.n > 0 && (first < 0 || p.n > a.T - first)) {
+    atomicCAS(a.err, 0, DEV_ERR_BAD_PAGE);
+    p.n = 0;
+  }
+  return p;
 }
+
+// N units of work in equal contiguous shares for C CTAs, the first N % C of them one unit longer.
+struct PagedShares {
+  long long q;
+  uint32_t rest, C;
+  bool small;  // N in 32 bits: short divisions
+  __device__ __forceinline__ PagedShares(long long N, uint32_t grid) {
+    C = static_cast<uint32_t>(min(static_cast<long long>(grid), N));
+    small = N >> 32 == 0;
+    q = C == 0 ? 0 : small ? static_cast<uint32_t>(N) / C : N / C;
+    rest = static_cast<uint32_t>(N - q * C);
+  }
+  __device__ __forceinline__ long long begin(uint32_t cta) const { return cta * q + min(cta, rest); }
+  __device__ __forceinline__ int owner(long long u) const {
+    const long long longer = rest * (q + 1);
+    const bool in = u < longer;
+    const long long x = in ? u : u - longer, d = in ? q + 1 : q;
+    return static_cast<int>((in ? 0 : rest) + (small ? static_cast<uint32_t>(x) / static_cast<uint32_t>(d) : x / d));
+  }
+};
 
 // Work.  A pair is (row, tile of 8 NT query rows, key/value head), a query row being (token, head of the
 // group); a pair's keys are cut into units of PA_UNIT.  All units of all pairs, in order, are dealt out in equal
@@ -157,21 +183,17 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int G = a.group, n_kv = cp.n_kv, page_mask = (1 << cp.page_shift) - 1;
 
-  auto row_tokens = [&](int row, int& first) { return paged_row_tokens(a, row, first); };
-  auto row_len = [&](int row) { return kv_row_len(a.lens, row, a.width, cp.page_shift, a.err); };
+  auto row_of = [&](int row) { return paged_row(a, cp.page_shift, row); };
   auto row_tiles = [&](int n) { return (n * G + ROWS - 1) / ROWS; };
-  auto pair_units = [&](int row) { return (row_len(row) + PA_UNIT - 1) / PA_UNIT; };
   // an idle row still has its zeros to write: one unit
-  auto row_units = [&](int row) {
-    int first;
-    const int n = row_tokens(row, first);
-    return n <= 0 ? 0u : static_cast<uint32_t>(max(pair_units(row), 1)) * row_tiles(n) * n_kv;
+  auto units = [&](const PagedRow& p) {
+    return p.n == 0 ? 0u : static_cast<uint32_t>(max((p.len + PA_UNIT - 1) / PA_UNIT, 1)) * row_tiles(p.n) * n_kv;
   };
 
   // this CTA's share [u0, u1) of the N units, and the row where it begins
   const int per = (a.rows + PA_THREADS - 1) / PA_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
   long long mine = 0;
-  for (int i = i0; i < i1; ++i) mine += row_units(i);
+  for (int i = i0; i < i1; ++i) mine += units(row_of(i));
   long long inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -186,14 +208,15 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
     if (w < warp) inc += s_scan[w];
     N += s_scan[w];
   }
-  const long long C = min(static_cast<long long>(gridDim.x), N), cta = blockIdx.x;
+  const PagedShares shares(N, gridDim.x);
+  const uint32_t cta = blockIdx.x;
   if (tid == 0) a.desc[cta] = make_int4(-1, 0, 0, 0);
-  if (cta >= C) return;
-  const long long u0 = cta * N / C, u1 = (cta + 1) * N / C;
+  if (cta >= shares.C) return;
+  const long long u0 = shares.begin(cta), u1 = shares.begin(cta + 1);
   if (inc - mine <= u0 && u0 < inc) {
     long long base = inc - mine;
     int i = i0;
-    for (uint32_t n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
+    for (uint32_t n = units(row_of(i)); base + n <= u0; n = units(row_of(++i))) base += n;
     s_row = i;
     s_base = base;
   }
@@ -205,14 +228,14 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   uint32_t phase = 0;
 
   for (long long u = u0; u < u1;) {
-    const uint32_t ru = row_units(row);
+    const PagedRow pr = row_of(row);
+    const uint32_t ru = units(pr);
     if (u >= base + ru) {
       base += ru;
       ++row;
       continue;
     }
-    int first;
-    const int n = row_tokens(row, first), len = row_len(row), tiles = row_tiles(n);
+    const int first = pr.first, n = pr.n, len = pr.len, tiles = row_tiles(n);
     // (32-bit divisions: a row's units are counted in 32 bits)
     const uint32_t in = static_cast<uint32_t>(u - base), upp_u = max((len + PA_UNIT - 1) / PA_UNIT, 1), local_pair = in / upp_u;
     const int upp = upp_u, ua = in - local_pair * upp_u;
@@ -648,7 +671,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
     }
     if (!whole && ua == 0 && tid == 0) {
       const long long last = base + (local_pair + 1) * upp_u - 1;  // the pair's last unit
-      a.desc[cta] = make_int4(row, rt, g, static_cast<int>(((last + 1) * C - 1) / N));
+      a.desc[cta] = make_int4(first, rt, g, shares.owner(last) | min(ROWS, R - r0) << 16);
     }
     fence_proxy_async_smem();  // the results before the next copies into the same bytes
     __syncthreads();           // s_o and s_q are free again
@@ -659,20 +682,96 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
   if (tid == 0 && s_abort) atomicCAS(a.err, 0, DEV_ERR_TIMEOUT_ATTN_PAGED);
 }
 
-// Joins the pieces of the pairs that several CTAs worked on: eight rows of a pair and DIMS of their channels at a
-// time.  A thread owns four channels of a row; PARTS groups of threads take every PARTS-th piece in turn, and their
-// results are joined in order.
-//   LONG  (few pairs, each in many pieces): the CTAs first number the unfinished pairs, and CTA (x, y, z) takes every
-//         gridDim.x-th from the x-th, rows 8y .. and channels 32z .. (8 groups, 32 channels: all SMs have work)
-//   else  CTA (c, y) takes rows 8y .. of the pair that began in CTA c, if one did and was not finished there
-// A piece's O is [row][channel], or (TC: from mk_attn_paged_tc.cuh) [four channels][row][4].
-template <int HD, bool LONG>
-struct PagedJoin {
-  static constexpr int PARTS = LONG ? 8 : 2, DIMS = LONG ? 32 : HD, LANES = 8 * DIMS / 4, THREADS = PARTS * LANES;
+// Joins the pieces of the pairs that several CTAs worked on.  A piece's O is [row][channel], or (TC: from
+// mk_attn_paged_tc.cuh) [four channels][row][4]; a thread takes four channels of a row.
+struct PagedSum {
+  float m = kLow, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float2 ml, float4 x) {
+    const float top = fmaxf(m, ml.x), f = ex2_approx(m - top), e = ex2_approx(ml.x - top);
+    m = top;
+    l = l * f + ml.y * e;
+    o.x = o.x * f + x.x * e;
+    o.y = o.y * f + x.y * e;
+    o.z = o.z * f + x.z * e;
+    o.w = o.w * f + x.w * e;
+  }
+  // row `at` (token times heads), channels dim ..
+  __device__ __forceinline__ void finish(const PagedAttnArgs& a, long long at, int hd, int dim) const {
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(a.out + at * hd + dim) =
+        make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
+    if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
+  }
 };
-template <int HD, bool LONG, bool TC>
-__global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_kernel(PagedAttnArgs a, int ctas) {
-  using J = PagedJoin<HD, LONG>;
+// Adds pieces p0, p0 + step, .. of the pair that began in CTA cta to ITEMS sums, 16 channels apart, of row i; the loads
+// of several pieces are on the way at a time (also of the last few: one that is not there counts as empty).
+template <int HD, bool TC, int ITEMS>
+__device__ __forceinline__ void add_pieces(const PagedAttnArgs& a, int cta, int pieces, int p0, int step, int rows, int i,
+                                           int dim, PagedSum (&sum)[ITEMS]) {
+  constexpr int AHEAD = ITEMS == 1 ? 4 : 2;
+  for (int p = p0; p < pieces; p += AHEAD * step) {
+    float2 ml[AHEAD];
+    float4 x[AHEAD][ITEMS];
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      const int q = min(p + e * step, pieces - 1);
+      const size_t slot = static_cast<size_t>(cta + q) * 2 + (q == 0 ? 1 : 0);
+      ml[e] = a.part_ml[slot * rows + i];
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int at = dim + 16 * k;
+        x[e][k] = *reinterpret_cast<const float4*>(TC ? a.part_o + ((slot * (HD / 4) + at / 4) * rows + i) * 4
+                                                      : a.part_o + (slot * rows + i) * HD + at);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e)
+      if (p + e * step >= pieces) {
+        ml[e] = make_float2(kLow, 0.f);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) x[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e)
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) sum[k].add(ml[e], x[e][k]);
+  }
+}
+
+// CTA (c, y) joins rows RJ y .. of the pair that began in CTA c, if one did and was not finished there: 8 rows, or 32
+// (TC: all CTAs in one wave; a warp reads 8 rows x 16 channels).
+template <int HD, bool TC>
+struct PagedJoin {
+  static constexpr int RJ = TC ? 32 : 8, THREADS = TC ? 256 : 8 * HD / 4, ITEMS = TC ? HD / 32 : 1;
+};
+template <int HD, bool TC>
+__global__ void __launch_bounds__(PagedJoin<HD, TC>::THREADS) attn_paged_join_kernel(PagedAttnArgs a, int ROWS) {
+  using J = PagedJoin<HD, TC>;
+  pdl_wait();
+  pdl_trigger();
+  const int cta = blockIdx.x, G = a.group, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int4 d = a.desc[cta];
+  if (d.x < 0) return;
+  const int i = blockIdx.y * J::RJ + (TC ? (warp & 3) * 8 + (lane & 7) : tid / (HD / 4)), qr = d.y * ROWS + i;
+  const int dim0 = TC ? (warp >> 2) * (HD / 2) + (lane >> 3) * 4 : tid % (HD / 4) * 4;
+  if (i >= d.w >> 16) return;
+  PagedSum sum[J::ITEMS];
+  add_pieces<HD, TC>(a, cta, (d.w & 0xffff) - cta + 1, 0, 1, ROWS, i, dim0, sum);
+  const long long at = static_cast<long long>(d.x + qr / G) * a.n_q + d.z * G + qr % G;
+#pragma unroll
+  for (int k = 0; k < J::ITEMS; ++k) sum[k].finish(a, at, HD, dim0 + 16 * k);
+}
+
+// Few pairs, each in many pieces: the CTAs first number the unfinished pairs, and CTA (x, y, z) takes every gridDim.x-th
+// from the x-th, rows 8y .. and channels 32z ..; PARTS groups of threads take every PARTS-th piece in turn, and their
+// results are joined in order (so that all SMs have work).
+struct PagedLongJoin {
+  static constexpr int PARTS = 8, DIMS = 32, LANES = 8 * DIMS / 4, THREADS = PARTS * LANES;
+};
+template <int HD, bool TC>
+__global__ void __launch_bounds__(PagedLongJoin::THREADS) attn_paged_long_join_kernel(PagedAttnArgs a, int ctas) {
+  using J = PagedLongJoin;
   __shared__ __align__(16) float s_o[J::PARTS][8][J::DIMS];
   __shared__ float2 s_ml[J::PARTS][8];
   __shared__ int s_sum[J::THREADS / 32], s_mine[J::THREADS];
@@ -683,64 +782,38 @@ __global__ void __launch_bounds__(PagedJoin<HD, LONG>::THREADS) attn_paged_join_
   const int q8 = TC ? in % 8 : in / (J::DIMS / 4), d4 = (TC ? in / 8 : in % (J::DIMS / 4)) * 4;
   const int dim = blockIdx.z * J::DIMS + d4;
   auto join = [&](int cta, const int4& d) {
-    int first;
-    const int n = paged_row_tokens(a, d.x, first);
-    const int pieces = d.w - cta + 1, i = blockIdx.y * 8 + q8, qr = d.y * ROWS + i;
-    float m = kLow, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float2 ml, float4 x) {
-      const float top = fmaxf(m, ml.x), f = ex2_approx(m - top), e = ex2_approx(ml.x - top);
-      m = top;
-      l = l * f + ml.y * e;
-      o.x = o.x * f + x.x * e;
-      o.y = o.y * f + x.y * e;
-      o.z = o.z * f + x.z * e;
-      o.w = o.w * f + x.w * e;
-    };
-#pragma unroll 4
-    for (int p = grp; p < pieces; p += J::PARTS) {
-      const size_t slot = static_cast<size_t>(cta + p) * 2 + (p == 0 ? 1 : 0), at = slot * ROWS + i;
-      const float* o4 = TC ? a.part_o + ((slot * (HD / 4) + dim / 4) * ROWS + i) * 4 : a.part_o + at * HD + dim;
-      add(a.part_ml[at], *reinterpret_cast<const float4*>(o4));
-    }
-    *reinterpret_cast<float4*>(&s_o[grp][q8][d4]) = o;
-    if (d4 == 0) s_ml[grp][q8] = make_float2(m, l);
+    const int i = blockIdx.y * 8 + q8, qr = d.y * ROWS + i;
+    PagedSum sums[1], &sum = sums[0];
+    if (i < d.w >> 16) add_pieces<HD, TC>(a, cta, (d.w & 0xffff) - cta + 1, grp, J::PARTS, ROWS, i, dim, sums);
+    *reinterpret_cast<float4*>(&s_o[grp][q8][d4]) = sum.o;
+    if (d4 == 0) s_ml[grp][q8] = make_float2(sum.m, sum.l);
     __syncthreads();
-    if (grp == 0 && qr < n * G) {
+    if (grp == 0 && i < d.w >> 16) {
 #pragma unroll
-      for (int p = 1; p < J::PARTS; ++p) add(s_ml[p][q8], *reinterpret_cast<const float4*>(&s_o[p][q8][d4]));
-      const long long at = static_cast<long long>(first + qr / G) * a.n_q + d.z * G + qr % G;
-      const float f = l == 0.f ? 0.f : 1.f / l;
-      *reinterpret_cast<uint2*>(a.out + at * HD + dim) =
-          make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
-      if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
+      for (int p = 1; p < J::PARTS; ++p) sum.add(s_ml[p][q8], *reinterpret_cast<const float4*>(&s_o[p][q8][d4]));
+      sum.finish(a, static_cast<long long>(d.x + qr / G) * a.n_q + d.z * G + qr % G, HD, dim);
     }
     __syncthreads();
   };
-  if constexpr (!LONG) {
-    const int4 d = a.desc[blockIdx.x];
-    if (d.x >= 0) join(blockIdx.x, d);
-  } else {
-    const int gx = gridDim.x, x = blockIdx.x;
-    int before = 0;  // unfinished pairs of earlier rounds
-    for (int c0 = 0; c0 < ctas; c0 += J::THREADS) {
-      const bool open = c0 + tid < ctas && a.desc[c0 + tid].x >= 0;
-      const uint32_t votes = __ballot_sync(0xffffffffu, open);
-      if (lane == 0) s_sum[warp] = __popc(votes);
-      __syncthreads();
-      int number = before + __popc(votes & ((1u << lane) - 1)), total = 0;
-      for (int w = 0; w < J::THREADS / 32; ++w) {
-        if (w < warp) number += s_sum[w];
-        total += s_sum[w];
-      }
-      const int had = (before + gx - 1 - x) / gx;  // of this CTA's pairs
-      if (open && number % gx == x) s_mine[number / gx - had] = c0 + tid;
-      before += total;
-      const int mine = (before + gx - 1 - x) / gx - had;
-      __syncthreads();
-      for (int j = 0; j < mine; ++j) join(s_mine[j], a.desc[s_mine[j]]);
-      __syncthreads();
+  const int gx = gridDim.x, x = blockIdx.x;
+  int before = 0;  // unfinished pairs of earlier rounds
+  for (int c0 = 0; c0 < ctas; c0 += J::THREADS) {
+    const bool open = c0 + tid < ctas && a.desc[c0 + tid].x >= 0;
+    const uint32_t votes = __ballot_sync(0xffffffffu, open);
+    if (lane == 0) s_sum[warp] = __popc(votes);
+    __syncthreads();
+    int number = before + __popc(votes & ((1u << lane) - 1)), total = 0;
+    for (int w = 0; w < J::THREADS / 32; ++w) {
+      if (w < warp) number += s_sum[w];
+      total += s_sum[w];
     }
+    const int had = (before + gx - 1 - x) / gx;  // of this CTA's pairs
+    if (open && number % gx == x) s_mine[number / gx - had] = c0 + tid;
+    before += total;
+    const int mine = (before + gx - 1 - x) / gx - had;
+    __syncthreads();
+    for (int j = 0; j < mine; ++j) join(s_mine[j], a.desc[s_mine[j]]);
+    __syncthreads();
   }
 }
 

@@ -7,7 +7,8 @@
 // else; S and O lie in TMEM, and the exponentials (16 a clock and SM: 1024 cycles for 256 x 64) are what bounds the
 // loop once it runs.
 //
-//   warp 0      asks for the tile's codes (bulk copies, 3 stages) and looks up its pages and scales
+//   warp 0      asks for the tile's codes (bulk copies, 3 stages)
+//   warp 3      looks up its scales
 //   warps 1, 2  MMA issuers of row tiles 0 and 1 (128 rows each), as in mk_attn_tc.cuh:
 //                 S_t(j+1) = Q_t K(j+1)^T (f16, M 128, N 64), then O_t += P_t(j) V(j) (P from TMEM, N hd)
 //   warps 4-11  softmax of tiles 0 and 1, one thread per row, and the rows' queries and results
@@ -62,8 +63,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   uint64_t* kv_empty = kv_full + PT_KV;
   uint64_t* s_full = kv_empty + PT_KV;  // [tile][buffer]
   uint64_t* p_ready = s_full + 4;       // [tile][buffer]
-  uint64_t* pv_done = p_ready + 4;      // [tile]
-  uint64_t* q_ready = pv_done + 2;      // [tile]
+  uint64_t* pv_done = p_ready + 4;      // [tile][buffer]
+  uint64_t* q_ready = pv_done + 4;      // [tile]
   uint64_t* drain = q_ready + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   const int G = a.group, n_kv = cp.n_kv;
   if (tid == 0) {
     for (int i = 0; i < PT_RAW; ++i) {
-      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_full[i], 2);
       mbar_init(&raw_empty[i], 4);
     }
     for (int i = 0; i < PT_KV; ++i) {
@@ -85,11 +86,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);
+      mbar_init(&pv_done[i], 1);
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&pv_done[t], 1);
-      mbar_init(&q_ready[t], 4);
-    }
+    for (int t = 0; t < 2; ++t) mbar_init(&q_ready[t], 4);
     mbar_init(drain, 2);
     *abort_flag = 0;
     fence_mbar_init();
@@ -105,18 +104,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   pdl_wait();
 
   // Work in equal shares of units, as in attn_paged_kernel, here with 256 rows a pair.
-  auto row_tokens = [&](int row, int& first) { return paged_row_tokens(a, row, first); };
-  auto row_len = [&](int row) { return kv_row_len(a.lens, row, a.width, cp.page_shift, a.err); };
+  auto row_of = [&](int row) { return paged_row(a, cp.page_shift, row); };
   auto row_tiles = [&](int n) { return (n * G + PT_ROWS - 1) / PT_ROWS; };
-  auto pair_units = [&](int row) { return max((row_len(row) + PT_KEYS - 1) / PT_KEYS, 1); };
-  auto row_units = [&](int row) {
-    int first;
-    const int n = row_tokens(row, first);
-    return n <= 0 ? 0u : static_cast<uint32_t>(pair_units(row)) * row_tiles(n) * n_kv;
+  auto units = [&](const PagedRow& p) {
+    return p.n == 0 ? 0u : static_cast<uint32_t>(max((p.len + PT_KEYS - 1) / PT_KEYS, 1)) * row_tiles(p.n) * n_kv;
   };
   const int per = (a.rows + PT_THREADS - 1) / PT_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
   long long mine = 0;
-  for (int i = i0; i < i1; ++i) mine += row_units(i);
+  for (int i = i0; i < i1; ++i) mine += units(row_of(i));
   long long inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -130,14 +125,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     if (w < warp) inc += s_scan[w];
     N += s_scan[w];
   }
-  const long long C = min(static_cast<long long>(gridDim.x), N), cta = blockIdx.x;
-  const bool idle = cta >= C;
-  const long long u0 = idle ? 0 : cta * N / C, u1 = idle ? 0 : (cta + 1) * N / C;
+  const PagedShares shares(N, gridDim.x);
+  const uint32_t cta = blockIdx.x;
+  const bool idle = cta >= shares.C;
+  const long long u0 = idle ? 0 : shares.begin(cta), u1 = idle ? 0 : shares.begin(cta + 1);
   if (tid == 0) a.desc[cta] = make_int4(-1, 0, 0, 0);
   if (!idle && inc - mine <= u0 && u0 < inc) {
     long long base = inc - mine;
     int i = i0;
-    for (uint32_t n = row_units(i); base + n <= u0; n = row_units(++i)) base += n;
+    for (uint32_t n = units(row_of(i)); base + n <= u0; n = units(row_of(++i))) base += n;
     s_row = i;
     s_base = base;
   }
@@ -152,15 +148,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   long long u = u0, base = idle ? 0 : s_base;
   int row = idle ? 0 : s_row;
   auto next = [&](Piece& p) {
-    uint32_t ru = 0;
-    while (u < u1 && u >= base + (ru = row_units(row))) {
-      base += ru;
-      ++row;
-    }
     if (u >= u1) return false;
+    PagedRow pr = row_of(row);
+    for (uint32_t ru = units(pr); u >= base + ru; ru = units(pr)) {
+      base += ru;
+      pr = row_of(++row);
+    }
     p.row = row;
-    p.n = row_tokens(row, p.first);
-    p.len = row_len(row);
+    p.first = pr.first;
+    p.n = pr.n;
+    p.len = pr.len;
     p.R = p.n * G;
     // (32-bit divisions: a row's units are counted in 32 bits)
     const uint32_t in = static_cast<uint32_t>(u - base), upp = max((p.len + PT_KEYS - 1) / PT_KEYS, 1);
@@ -185,47 +182,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
   if (warp == 0) {
-    // ---------------------------------------------------------------- codes, pages and scales
-    int j = 0, piece = 0;
+    // ---------------------------------------------------------------- codes
+    int j = 0;
+    const int run = min(1 << cp.page_shift, PT_KEYS);  // keys that lie together
     while (ok && next(p)) {
-      if (p.tiles64 == 0) continue;
-      float ref = 0.f;
-      for (int s = (p.kbeg >> cp.page_shift) + lane; s <= (p.kend - 1) >> cp.page_shift; s += 32) {
-        const int page = s < a.width ? a.table[static_cast<size_t>(p.row) * a.width + s] : -1;
-        if (page >= 0 && page < cp.num_pages) ref = fmaxf(ref, *kv_scale_ptr(cp, page, 1, p.g));
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-      if (lane == 0) s_ref[piece & 15] = ref;
-      ++piece;
-      const int run = min(1 << cp.page_shift, PT_KEYS);  // keys that lie together
-      int page = -1, none8 = 0;
-      float ks = 0.f, vs = 0.f;
+      int page = -1;
       for (int i = 0; ok && i < p.tiles64; ++i, ++j) {
         const int st = j % PT_RAW, i8 = i & 7;
         if (i8 == 0) {  // lane l looks up group l of the next eight tiles
           const int key = p.kbeg + i * PT_KEYS + 16 * lane;
           page = -1;
-          ks = vs = 0.f;
-          const bool wanted = key < p.kend;
-          if (wanted) page = kv_page_of(a.table, a.width, cp.num_pages, p.row, key >> cp.page_shift, a.err);
-          if (page >= 0) {
-            ks = *kv_scale_ptr(cp, page, 0, p.g);
-            vs = *kv_scale_ptr(cp, page, 1, p.g);
-          }
-          if (ks == 0.f) ks = kTinyScale;
-          vs = ref > 0.f ? vs / ref * kTcPOff : vs;
-          none8 = static_cast<int>(__ballot_sync(0xffffffffu, wanted && page < 0));
+          if (key < p.kend) page = kv_page_of(a.table, a.width, cp.num_pages, p.row, key >> cp.page_shift, nullptr);
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[st], ((j / PT_RAW) & 1) ^ 1u, abort_flag));
         if (!ok) break;
-        const bool here = lane >> 2 == i8;
         const int in = lane & 3;  // group of the tile
-        if (here) s_sc[(j & 7) * 4 + in] = make_float2(ks, vs);
-        if (lane == 0) s_none[j & 7] = none8 >> (4 * i8) & 15;
-        const bool asks = here && page >= 0 && (16 * in) % run == 0;
+        const bool asks = lane >> 2 == i8 && page >= 0 && (16 * in) % run == 0;
         const uint32_t bytes = __reduce_add_sync(0xffffffffu, asks ? 2u * run * HD : 0u);
-        __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], bytes);
         __syncwarp();
         if (asks) {
@@ -240,6 +213,57 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     }
     // every copy that was asked for lands before the CTA may leave
     for (int i = max(0, j - PT_RAW); i < j; ++i) mbar_wait_drain(&raw_full[i % PT_RAW], (i / PT_RAW) & 1);
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- scales
+    int j = 0, piece = 0;
+    while (ok && next(p)) {
+      if (p.tiles64 == 0) continue;
+      auto page_at = [&](int slot, int* err) {
+        return kv_page_of(a.table, a.width, cp.num_pages, p.row, slot, err);
+      };
+      // what the piece's value scales are relative to: the largest of them
+      float ref = 0.f;
+      for (int s0 = p.kbeg >> cp.page_shift; s0 <= (p.kend - 1) >> cp.page_shift; s0 += 128) {
+        int page[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int s = s0 + 32 * e + lane;
+          page[e] = s <= (p.kend - 1) >> cp.page_shift ? page_at(s, nullptr) : -1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (page[e] >= 0) ref = fmaxf(ref, *kv_scale_ptr(cp, page[e], 1, p.g));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+      if (lane == 0) s_ref[piece & 15] = ref;
+      ++piece;
+      int none8 = 0;
+      float ks = 0.f, vs = 0.f;
+      for (int i = 0; ok && i < p.tiles64; ++i, ++j) {
+        const int st = j % PT_RAW, i8 = i & 7;
+        if (i8 == 0) {  // lane l looks up group l of the next eight tiles
+          const int key = p.kbeg + i * PT_KEYS + 16 * lane;
+          const bool wanted = key < p.kend;
+          const int page = wanted ? page_at(key >> cp.page_shift, a.err) : -1;
+          ks = vs = 0.f;
+          if (page >= 0) {
+            ks = *kv_scale_ptr(cp, page, 0, p.g);
+            vs = *kv_scale_ptr(cp, page, 1, p.g);
+          }
+          if (ks == 0.f) ks = kTinyScale;
+          vs = ref > 0.f ? vs / ref * kTcPOff : vs;
+          none8 = static_cast<int>(__ballot_sync(0xffffffffu, wanted && page < 0));
+        }
+        // (that the stage is free says that the softmax is done with tile j - 8)
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[st], ((j / PT_RAW) & 1) ^ 1u, abort_flag));
+        if (!ok) break;
+        if (lane >> 2 == i8) s_sc[(j & 7) * 4 + (lane & 3)] = make_float2(ks, vs);
+        if (lane == 0) s_none[j & 7] = none8 >> (4 * i8) & 15;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_full[st]);
+      }
+    }
   } else if (warp == 1 || warp == 2) {
     // ---------------------------------------------------------------- MMA issuers
     const int t = warp - 1;
@@ -294,7 +318,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
             mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + (jt & 1) * 64 + ks * 8, db, idesc_pv,
                        (i > 0 || ks > 0) ? 1u : 0u);
           }
-          mma_commit(&pv_done[t]);
+          mma_commit(&pv_done[t * 2 + (jt & 1)]);
           mma_commit(&kv_empty[st]);
         }
         __syncwarp();
@@ -358,44 +382,66 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + lane_off + t * 128, tO = tmem + lane_off + 256 + t * 128;
     int j = 0, jt = 0, piece = 0;
+    // O_t += P_t(x) V(x) is done.  (Not waited for in every phase: S_t(x + 2), which was issued after it and has been
+    // waited for since, says so too, and a buffer's next product starts only after that.)
+    auto pv_wait = [&](int x) {
+      return __all_sync(0xffffffffu, mbar_wait(&pv_done[t * 2 + (x & 1)], (x >> 1) & 1, abort_flag));
+    };
     while (ok && next(p)) {
       const int qr = p.r0 + t * 128 + trow;
       const bool has = qr < p.R;
       const bool tile_on = p.r0 + t * 128 < p.R;
       const int limit = has ? p.len - p.n + qr / G + 1 : 0;
       const long long at = has ? static_cast<long long>(p.first + qr / G) * a.n_q + p.g * G + qr % G : 0;
-      float m = kLow, l = 0.f, ref = 0.f;
+      float m = kLow, l = 0.f, ref = 0.f, sf = 0.f;
       if (p.tiles64 > 0 && tile_on) {
-        // the row's query, as f16 with its largest channel near 1, into the swizzled operand
-        const __nv_bfloat16* qp = a.q;
-        if (has) qp += static_cast<long long>(p.first + qr / G) * a.ld_q + static_cast<long long>(p.g * G + qr % G) * a.hs_q;
-        float top = 0.f;
-        uint4 qv[HD / 8];
+        // the queries, as f16 with a row's largest channel near 1, into the swizzled operand: four lanes a row
+        const long long qp = has ? static_cast<long long>(p.first + qr / G) * a.ld_q +
+                                       static_cast<long long>(p.g * G + qr % G) * a.hs_q
+                                 : LLONG_MIN;
+        uint4 qv[4][HD / 32];
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          qv[c] = has ? __ldg(reinterpret_cast<const uint4*>(qp + c * 8)) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {qv[c].x, qv[c].y, qv[c].z, qv[c].w};
+        for (int it = 0; it < 4; ++it) {
+          const long long from = __shfl_sync(0xffffffffu, qp, it * 8 + (lane >> 2));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(w[e]);
-            top = max3f(top, fabsf(f.x), fabsf(f.y));
+          for (int k = 0; k < HD / 32; ++k) {
+            qv[it][k] = make_uint4(0, 0, 0, 0);
+            if (from != LLONG_MIN) qv[it][k] = __ldg(reinterpret_cast<const uint4*>(a.q + from + ((lane & 3) + 4 * k) * 8));
           }
         }
-        const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-        // (a negative scale turns the queries, so that the scores' factor is not negative)
-        const float down = copysignf(__uint_as_float((254u - ex) << 23), a.scale);
-        const float sf = __uint_as_float(ex << 23) * fabsf(a.scale);
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          const uint32_t w[4] = {qv[c].x, qv[c].y, qv[c].z, qv[c].w};
-          uint32_t h[4];
+        for (int it = 0; it < 4; ++it) {
+          float top = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(w[e]);
-            h[e] = pack_f16x2(f.x * down, f.y * down);
+          for (int k = 0; k < HD / 32; ++k) {
+            const uint32_t w[4] = {qv[it][k].x, qv[it][k].y, qv[it][k].z, qv[it][k].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack_bf16x2(w[e]);
+              top = max3f(top, fabsf(f.x), fabsf(f.y));
+            }
           }
-          *reinterpret_cast<uint4*>(sQ + (t * 2 + (c >> 3)) * PT_QCHUNK + trow * 128 + (((c & 7) ^ (trow & 7)) << 4)) =
-              make_uint4(h[0], h[1], h[2], h[3]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+          // (a negative scale turns the queries, so that the scores' factor is not negative)
+          const float down = copysignf(__uint_as_float((254u - ex) << 23), a.scale);
+          const float up = __shfl_sync(0xffffffffu, __uint_as_float(ex << 23) * fabsf(a.scale), (lane & 7) * 4);
+          if (lane >> 3 == it) sf = up;
+          const int r = quarter * 32 + it * 8 + (lane >> 2);
+#pragma unroll
+          for (int k = 0; k < HD / 32; ++k) {
+            const int c = (lane & 3) + 4 * k;
+            const uint32_t w[4] = {qv[it][k].x, qv[it][k].y, qv[it][k].z, qv[it][k].w};
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack_bf16x2(w[e]);
+              h[e] = pack_f16x2(f.x * down, f.y * down);
+            }
+            *reinterpret_cast<uint4*>(sQ + (t * 2 + (c >> 3)) * PT_QCHUNK + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -434,15 +480,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
 #pragma unroll
           for (int q = 0; q < 4; ++q) m_tile = fmaxf(m_tile, fmaxf(mx[q][0], mx[q][1]) * ks[q]);
           const bool need = m_tile > m + kTcLag;
-          bool pv_waited = i == 0;
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? ex2_approx(m - m_tile) : 1.f;
             if (i > 0) {
               // O_t += P_t(j-1) V(j-1) must have landed before O_t is rescaled
-              ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (jt - 1) & 1, abort_flag));
+              ok = pv_wait(jt - 1);
               if (!ok) break;
               tc_fence_after();
-              pv_waited = true;
 #pragma unroll
               for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
@@ -476,10 +520,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
             }
           }
           l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-          if (!pv_waited) {  // a parity barrier is waited for once per phase
-            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (jt - 1) & 1, abort_flag));
-            if (!ok) break;
-          }
           tmem_st_32x32b_x32(tS + b * 64, pk);  // P_t(j) over the scores just read
           tmem_st_wait();
           tc_fence_before();
@@ -487,7 +527,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
           if (lane == 0) mbar_arrive(&p_ready[t * 2 + b]);
         }
         if (ok) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (jt - 1) & 1, abort_flag));
+          ok = pv_wait(jt - 1);
           tc_fence_after();
         }
         if (!ok) break;
@@ -537,7 +577,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
           a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
       }
       if (!p.whole && p.begins && t == 0 && trow == 0)
-        a.desc[cta] = make_int4(p.row, p.rt, p.g, static_cast<int>(((p.last + 1) * C - 1) / N));
+        a.desc[cta] = make_int4(p.first, p.rt, p.g, shares.owner(p.last) | min(PT_ROWS, p.R - p.r0) << 16);
       __syncwarp();
       tc_fence_before();  // O_t is read before the next piece's first product (ordered by its q_ready and p_ready)
     }

@@ -217,10 +217,11 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
     constexpr int HD = decltype(hd)::value;
     constexpr bool TC = decltype(of_tc)::value;
     if (p.long_join > 0)
-      return launch_k(mk::attn_paged_join_kernel<HD, true, TC>, dim3(p.long_join, p.nt, HD / 32),
-                      dim3(mk::PagedJoin<HD, true>::THREADS), 0, st, true, a, p.ctas);
-    return launch_k(mk::attn_paged_join_kernel<HD, false, TC>, dim3(p.ctas, p.nt), dim3(mk::PagedJoin<HD, false>::THREADS),
-                    0, st, true, a, p.ctas);
+      return launch_k(mk::attn_paged_long_join_kernel<HD, TC>, dim3(p.long_join, p.nt, HD / 32),
+                      dim3(mk::PagedLongJoin::THREADS), 0, st, true, a, p.ctas);
+    using Join = mk::PagedJoin<HD, TC>;
+    return launch_k(mk::attn_paged_join_kernel<HD, TC>, dim3(p.ctas, 8 * p.nt / Join::RJ), dim3(Join::THREADS), 0, st, true,
+                    a, 8 * p.nt);
   };
   const auto by_size = [&](auto hd) { return tc ? join(hd, std::true_type()) : join(hd, std::false_type()); };
   return head_dim == 96 ? by_size(std::integral_constant<int, 96>()) : by_size(std::integral_constant<int, 128>());
