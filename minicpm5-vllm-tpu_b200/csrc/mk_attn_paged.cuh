@@ -44,7 +44,7 @@ constexpr int PA_THREADS = PA_WARPS * 32;
 // other's latencies; wider tiles have work enough, and no registers left.
 __host__ __device__ constexpr int pa_groups(int nt) { return nt == 1 ? 2 : 1; }
 __host__ __device__ constexpr int pa_unit(int nt) { return 16 * pa_groups(nt) * PA_WARPS; }  // keys of one unit of work
-constexpr int PA_GROUPS = 64;           // groups whose pages and scales are staged at a time
+constexpr int PA_GROUPS = PA_THREADS;   // groups whose pages and scales are staged at a time
 // m may lag the true maximum by up to 2^kLag: it moves only then, which spares a warp reduction and a rescaling
 // of O per block.
 //
@@ -247,7 +247,16 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
     const int lim_min = r0 + ROWS <= R ? limit(r0) : 0, lim_max = limit(min(r0 + ROWS, R) - 1);
     const int kbeg = ua * PA_UNIT, kend = min(ub * PA_UNIT, lim_max);
 
-    // Asked for first, all at once: the queries, then the pages of the first keys and the scales of those pages.
+    // Asked for first, all at once: the pages of the first keys and the queries.  Once the pages are there, their scales
+    // and the first keys themselves.
+    int page = -1;
+    float page_vs = 0.f, page_ks = 0.f;
+    auto groups_at = [&](int kb) { return min(PA_GROUPS, (kend - kb + 15) >> 4); };
+    auto load_page = [&](int kb) {  // thread i: the page of group i
+      page = -1;
+      if (tid < groups_at(kb)) page = kv_page_of(a.table, a.width, cp.num_pages, row, (kb + tid * 16) >> cp.page_shift, a.err);
+    };
+    if (kbeg < kend) load_page(kbeg);
     uint32_t qw[NT][KS][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -264,19 +273,48 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
         qw[t][s + 1][1] = v.w;
       }
     }
-    int page = -1;
-    float page_vs = 0.f, page_ks = 0.f;
-    auto load_pages = [&](int kb, int ng) {  // thread i: the page of group i
-      page = -1;
-      page_vs = page_ks = 0.f;
-      if (tid < ng) page = kv_page_of(a.table, a.width, cp.num_pages, row, (kb + tid * 16) >> cp.page_shift, a.err);
-      if (page >= 0) {
-        page_vs = *kv_scale_ptr(cp, page, 1, g);
-        page_ks = *kv_scale_ptr(cp, page, 0, g);
+    const uint32_t plane = static_cast<uint32_t>(n_kv) * HD << cp.page_shift, page_bytes = 2 * plane;
+    const int8_t* heads = cp.codes + (static_cast<size_t>(g) * HD << cp.page_shift);  // head g of page 0
+    // Asks for the block at group gi (in one page from 32 tokens on).  A missing page is not read: what the stage
+    // holds instead weighs nothing.
+    auto ask = [&](int kb, int gi, int stage) {
+      uint8_t* dst = ring + stage * STAGE;
+      uint64_t* bar = &s_full[warp][stage];
+      if (GP == 1 || cp.page_shift > 4) {
+        const int pg = s_page[gi];
+        mbar_arrive_expect_tx(bar, pg < 0 ? 0 : STAGE);
+        if (pg >= 0) {
+          const int8_t* at = heads + static_cast<uint64_t>(static_cast<uint32_t>(pg)) * page_bytes +
+                             ((kb + gi * 16) & page_mask) * HD;
+          bulk_load(dst, at, HALF, bar);
+          bulk_load(dst + HALF, at + plane, HALF, bar);
+        }
+      } else {
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int p = 0; p < GP; ++p) bytes += s_page[gi + p] < 0 ? 0 : STAGE / GP;
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int p = 0; p < GP; ++p)
+          if (s_page[gi + p] >= 0) {
+            const int8_t* at = heads + static_cast<uint64_t>(static_cast<uint32_t>(s_page[gi + p])) * page_bytes;
+            bulk_load(dst + p * 16 * HD, at, 16 * HD, bar);
+            bulk_load(dst + HALF + p * 16 * HD, at + plane, 16 * HD, bar);
+          }
       }
     };
-    auto groups_at = [&](int kb) { return min(PA_GROUPS, (kend - kb + 15) >> 4); };
-    if (kbeg < kend) load_pages(kbeg, groups_at(kbeg));
+    // The pages go to shared memory, their scales and each warp's first blocks are asked for.
+    int blocks = 0;  // of this warp
+    auto start = [&](int kb) {
+      s_page[tid] = page;  // (past the last group: none)
+      page_vs = page >= 0 ? *kv_scale_ptr(cp, page, 1, g) : 0.f;
+      page_ks = page >= 0 ? *kv_scale_ptr(cp, page, 0, g) : 0.f;
+      __syncthreads();
+      blocks = (groups_at(kb) - warp * GP + PA_WARPS * GP - 1) / (PA_WARPS * GP);  // (none: <= 0)
+      if (lane == 0)
+        for (int i = 0; i < min(blocks, STAGES); ++i) ask(kb, (warp + i * PA_WARPS) * GP, (st + i) % STAGES);
+    };
+    if (kbeg < kend) start(kbeg);
 
     // queries as f16, each row scaled by a power of two to about 1 (its exponent joins the score's factor)
     uint32_t qf[NT == 1 ? KS : 1][2];
@@ -326,15 +364,14 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
     }
-    const uint32_t plane = static_cast<uint32_t>(n_kv) * HD << cp.page_shift, page_bytes = 2 * plane;
-    const int8_t* heads = cp.codes + (static_cast<size_t>(g) * HD << cp.page_shift);  // head g of page 0
     float vref = 0.f;  // the largest value scale so far: O is in units of vref / kPOff
 
     for (int kb = kbeg; kb < kend; kb += PA_GROUPS * 16) {
       const int ng = groups_at(kb);
       if (kb != kbeg) {
-        load_pages(kb, ng);
+        load_page(kb);
         __syncthreads();  // the last groups' pages and scales are no longer read
+        start(kb);
       }
       float top = page_vs;  // (a NaN scale does not take part, and makes its own group NaN)
 #pragma unroll
@@ -344,11 +381,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_red[w]);
       const float nref = fmaxf(vref, top);
-      if (tid < PA_GROUPS) {  // (past ng: no page)
-        s_page[tid] = page;
-        s_ks[tid] = page_ks;
-        s_vs[tid] = nref > 0.f ? page_vs / nref * kPOff : page_vs;
-      }
+      s_ks[tid] = page_ks;
+      s_vs[tid] = nref > 0.f ? page_vs / nref * kPOff : page_vs;
       if (nref != vref && vref > 0.f) {
         const float f = vref / nref;
 #pragma unroll
@@ -361,37 +395,6 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       vref = nref;
       __syncthreads();
 
-      // Asks for the block at group gi (in one page from 32 tokens on).  A missing page is not read: what the stage
-      // holds instead weighs nothing.
-      auto ask = [&](int gi, int stage) {
-        uint8_t* dst = ring + stage * STAGE;
-        uint64_t* bar = &s_full[warp][stage];
-        if (GP == 1 || cp.page_shift > 4) {
-          const int pg = s_page[gi];
-          mbar_arrive_expect_tx(bar, pg < 0 ? 0 : STAGE);
-          if (pg >= 0) {
-            const int8_t* at = heads + static_cast<uint64_t>(static_cast<uint32_t>(pg)) * page_bytes +
-                               ((kb + gi * 16) & page_mask) * HD;
-            bulk_load(dst, at, HALF, bar);
-            bulk_load(dst + HALF, at + plane, HALF, bar);
-          }
-        } else {
-          uint32_t bytes = 0;
-#pragma unroll
-          for (int p = 0; p < GP; ++p) bytes += s_page[gi + p] < 0 ? 0 : STAGE / GP;
-          mbar_arrive_expect_tx(bar, bytes);
-#pragma unroll
-          for (int p = 0; p < GP; ++p)
-            if (s_page[gi + p] >= 0) {
-              const int8_t* at = heads + static_cast<uint64_t>(static_cast<uint32_t>(s_page[gi + p])) * page_bytes;
-              bulk_load(dst + p * 16 * HD, at, 16 * HD, bar);
-              bulk_load(dst + HALF + p * 16 * HD, at + plane, 16 * HD, bar);
-            }
-        }
-      };
-      const int blocks = (ng - warp * GP + PA_WARPS * GP - 1) / (PA_WARPS * GP);  // of this warp (none: <= 0)
-      if (lane == 0)
-        for (int i = 0; i < min(blocks, STAGES); ++i) ask((warp + i * PA_WARPS) * GP, (st + i) % STAGES);
       const int lane_k = (4 * (r >> 1) + (r & 1)) * HD + c * 16, lane_k8 = (4 * (r >> 1) + (r & 1)) * HD + 64 + c * 8;
       const int lane_v = (c * HD + 4 * r) * 4;
       int left = blocks;
@@ -592,7 +595,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
         }
         // every lane has used the stage's bytes: it is asked for again
         __syncwarp();
-        if (lane == 0 && left > STAGES) ask(gi + STAGES * PA_WARPS * GP, st);
+        if (lane == 0 && left > STAGES) ask(kb, gi + STAGES * PA_WARPS * GP, st);
         --left;
         if (++st == STAGES) {
           st = 0;
