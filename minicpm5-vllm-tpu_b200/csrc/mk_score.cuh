@@ -89,14 +89,16 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 // where there are rows enough), each with a slice of it.
 //
 // Alternatives.  An entry can only be among the k largest if it reaches tau, any value that k entries reach.  A
-// warp's lanes keep the maxima of two halves of what they have seen, and the k-th largest of the 64 is such a value;
-// it is taken after the first 1024 logits of the warp, again when four times as many have been seen, and so on,
-// and the largest that any warp of the CTA has published serves them all.  (A tau of the whole CTA is closer to the
-// k-th largest, but costs each warp more rounds: 105 us instead of 78 at 2047 x 73448, k = 5.)  16-byte vectors
-// that hold a logit that reaches it go into a list in shared memory; at the end their logits are cut to what
-// reaches the last tau and put in order by counting.  After the first step no warp waits for another before the end.
-// Rows that defeat it (long runs of equal or rising logits that fill the list; fewer than k logits above -inf) fall
-// back to one search of the slice for each alternative missing.
+// warp's lanes keep the maxima of two halves of what they have seen: 64 entries.  If each of W warps has ceil(k / W)
+// maxima that reach a value, the least of those values over the warps is such a tau.  It is taken after the first 1024
+// logits of a warp, again when twice as many have been seen, and so on; a warp publishes its part when it gets there
+// (parts only rise: an old one is valid).  16-byte vectors that hold a logit that reaches tau go into a list in shared
+// memory; at the end their logits are cut to what reaches the last tau and put in order by counting.  After the first
+// step no warp waits for another before the end.  The list holds what random logits need at k = 64 (470 vectors of
+// 130560 logits; 70 at k = 5, 150 at k = 20).
+// Rows that defeat it (rising logits; a warp whose share is lower than the others') are read once more, with the best
+// tau that is then known, of the shares or of one warp alone; where that does not do either (long runs of equal
+// logits; fewer than k above -inf), each alternative that is missing is searched for.
 //
 // What bounds it: the bytes of the logits.  Per bf16 logit the arithmetic is about six instructions and one
 // exponential, two thirds of what an SM can issue at the rate at which HBM delivers them.
@@ -105,8 +107,7 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 constexpr int TL_FEW = 128, TL_MANY = 512;
 constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
-constexpr int TL_LIST = 512;      // vectors listed
-constexpr int TL_SHORT = 32;      // a list that is expanded with the tau at hand
+constexpr int TL_LIST = 640;      // vectors listed
 constexpr int TL_CAP = 1024;      // logits put in order
 constexpr int TL_CLUSTER_MAX = 8;
 static_assert(TL_TOPK_MAX <= 64 && TL_CLUSTER_MAX * TL_TOPK_MAX <= TL_CAP, "alternatives");
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
   __shared__ int s_id[TL_LIST];
   __shared__ unsigned long long s_kept[TL_CAP], s_top[TL_TOPK_MAX];
   __shared__ unsigned long long s_pick[TL_THREADS / 32];
-  __shared__ __align__(16) volatile float s_tau[TL_THREADS / 32];
+  __shared__ __align__(16) volatile float s_tau[TL_THREADS / 32], s_own[TL_THREADS / 32];
   __shared__ int s_n, s_kept_n, s_have;
   __shared__ RowStats s_st[TL_THREADS / 32];
   __shared__ int s_above[TL_THREADS / 32];
@@ -186,10 +187,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
       s_id[at] = id;
     }
   };
-  // the warp's tau: one maximum is struck out per round, the lowest lane's among equals
-  auto threshold = [&]() {
+  // the n-th largest of the warp's maxima: one is struck out per round, the lowest lane's among equals
+  constexpr int WARPS = TL_THREADS / 32;
+  const int share = (k + WARPS - 1) / WARPS;
+  auto nth_largest = [&](int n) {
     uint32_t hi = order_key(fmaxf(top, top1)), lo = order_key(fminf(top, top1)), last = 0;
-    for (int r = 0; r < k; ++r) {
+    for (int r = 0; r < n; ++r) {
       last = __reduce_max_sync(0xffffffffu, hi);
       const uint32_t with = __ballot_sync(0xffffffffu, hi == last);
       if (lane == __ffs(with) - 1) {
@@ -197,7 +200,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
         lo = 0;
       }
     }
-    tau = last == 0 ? -INFINITY : __uint_as_float(last & 0x80000000u ? last & 0x7fffffffu : ~last);
+    return last == 0 ? -INFINITY : __uint_as_float(last & 0x80000000u ? last & 0x7fffffffu : ~last);
+  };
+  auto take_tau = [&]() {  // of what the warps have published
+    float least = s_tau[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) least = fminf(least, s_tau[i]);
+    tau = least;
   };
 
   // a loose logit of the head or tail: at most one per thread
@@ -308,13 +317,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
     st.w = fmaf((w0 + w1) * kLn2, back, st.w);
     if (k > 0) {
       if (step == retake) {
-        threshold();
-        if (lane == 0) s_tau[wp] = tau;
-        if (step == 0) __syncthreads();  // the list begins with the best tau of all warps
-        retake = step * 4 + 3;
+        const float part = nth_largest(share);
+        if (lane == 0) s_tau[wp] = part;
+        if (step == 0) __syncthreads();  // every warp has a part
+        retake = step * 2 + 1;
       }
-#pragma unroll
-      for (int i = 0; i < TL_THREADS / 32; ++i) tau = fmaxf(tau, s_tau[i]);
+      take_tau();
       if (step == 0 && loose_x >= tau && loose_x > -INFINITY) {  // as the first logit of a vector
         uint32_t first = __float_as_uint(loose_x);
         if (BF) first = first >> 16 | 0xff800000u;
@@ -354,21 +362,31 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
   const int want = min(k, hi - lo);
   if (k > 0) {
     const int n = s_n;
-    if (n <= TL_LIST) {
-      if (steps > 1 && n > TL_SHORT) {  // tau of all that each warp has seen
-        threshold();
-        if (lane == 0) s_tau[wp] = tau;
-        __syncthreads();
+    auto keep = [&](float f, int id) {
+      if (f >= tau && f > -INFINITY) {
+        const int at = atomicAdd(&s_kept_n, 1);
+        if (at < TL_CAP) s_kept[at] = order_entry(order_key(f), id);
+      }
+    };
+    if (steps > 1) {  // tau of all that each warp has seen
+      const float part = nth_largest(share);
+      if (lane == 0) s_tau[wp] = part;
+      __syncthreads();
+      take_tau();
+    }
+    if (n <= TL_LIST)
+      for (int i = tid; i < n * EPV; i += TL_THREADS)
+        keep(logit_at(reinterpret_cast<const E*>(s_vec), i), s_id[i / EPV] + i % EPV);
+    __syncthreads();
+    if (n > TL_LIST || s_kept_n > TL_CAP) {
+      const float own = nth_largest(k);
+      if (lane == 0) s_own[wp] = own;
+      __syncthreads();
+      if (tid == 0) s_kept_n = 0;
 #pragma unroll
-        for (int i = 0; i < TL_THREADS / 32; ++i) tau = fmaxf(tau, s_tau[i]);
-      }
-      for (int i = tid; i < n * EPV; i += TL_THREADS) {
-        const float f = logit_at(reinterpret_cast<const E*>(s_vec), i);
-        if (f >= tau && f > -INFINITY) {
-          const int at = atomicAdd(&s_kept_n, 1);
-          if (at < TL_CAP) s_kept[at] = order_entry(order_key(f), s_id[i / EPV] + i % EPV);
-        }
-      }
+      for (int i = 0; i < WARPS; ++i) tau = fmaxf(tau, s_own[i]);
+      __syncthreads();
+      for (int i = lo + tid; i < hi; i += TL_THREADS) keep(logit_at(row, i), i);
     }
     __syncthreads();
     const int kept = s_kept_n <= TL_CAP ? s_kept_n : 0;
