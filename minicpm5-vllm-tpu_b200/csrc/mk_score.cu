@@ -104,15 +104,19 @@ mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, 
   a.rank = ranks;
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
-  // A row is shared by as many CTAs (up to eight) as still have two steps' 8192 logits each, while the GPU has room:
-  // 512 threads run two to an SM.
+  // A row is shared by as many CTAs of 512 threads (up to eight) as still have half a step's 8192 logits each, while
+  // there are SMs for them (us at 130560 f32, k = 5, with 1, 2, 4, 8 CTAs a row: 8 rows 21, 15, 12, 10.5; 74 rows 22,
+  // 18, 24, 31; 148 rows 24, 23, 37, 51).  From there on a row has one CTA: of 512 threads while the rows are up to three
+  // an SM (296 rows 33, with 128 threads 60; 400 rows 50 and 65; bf16 27 and 44, 40 and 47), then of 128, eight to an SM
+  // (1184 rows 117 with 512 threads, 113 with 128; bf16 95 and 75).
   int cluster = 1;
-  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= static_cast<int64_t>(d.sm_count) * 2 &&
-         V / (cluster * 2) >= 8192)
+  while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= d.sm_count && V / (cluster * 2) >= 8192)
     cluster *= 2;
-  if (cluster > 1) {
+  const bool many = cluster > 1 || (T <= static_cast<int64_t>(d.sm_count) * 3 && V >= mk::TL_MANY * mk::TL_VALUES);
+  if (many) {
     void (*k)(mk::LogitsArgs, int) = logits_bits == 32 ? mk::token_logprobs_kernel<float, mk::TL_MANY>
                                                        : mk::token_logprobs_kernel<__nv_bfloat16, mk::TL_MANY>;
+    if (cluster == 1) return launch_k(k, dim3(static_cast<unsigned>(T)), dim3(mk::TL_MANY), 0, st, true, a, 1);
     return launch_k_cluster(cluster, k, dim3(static_cast<unsigned>(T) * cluster), dim3(mk::TL_MANY), 0, st, true, a, cluster);
   }
   void (*k)(mk::LogitsArgs, int) = logits_bits == 32 ? mk::token_logprobs_kernel<float, mk::TL_FEW>

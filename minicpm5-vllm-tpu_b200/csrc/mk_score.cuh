@@ -107,7 +107,7 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 constexpr int TL_FEW = 128, TL_MANY = 512;
 constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
-constexpr int TL_LIST = 640;      // vectors listed
+constexpr int TL_LIST = 736;      // vectors listed (as many as leave eight CTAs of an SM with 32 KB of L1 or more)
 constexpr int TL_CAP = 1024;      // logits put in order
 constexpr int TL_CLUSTER_MAX = 8;
 static_assert(TL_TOPK_MAX <= 64 && TL_CLUSTER_MAX * TL_TOPK_MAX <= TL_CAP, "alternatives");
