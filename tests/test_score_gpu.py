@@ -62,6 +62,23 @@ def test_token_logprobs_orders(dev, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("T,k", [(2, 64), (160, 20), (460, 64)])
+def test_token_logprobs_uneven_parts(dev, T, k, dtype):
+    """Rows whose best logits lie where few threads read, rise to the end, or are all the same: with a CTA cluster, 512
+    threads and 128 threads a row."""
+    from minicpm5_mk import ops
+    V = 20011
+    i = torch.arange(V)
+    noise = torch.randn(V, generator=torch.Generator().manual_seed(k))
+    per = 16 // dtype.itemsize  # logits of a thread's load
+    x = torch.stack([noise + torch.where((i // per) // 32 % 4 == 1, 0.0, -40.0), noise + i / 500, i / 100.0,
+                     torch.where(i > V - 1500, noise + 20, noise), torch.full((V,), 2.5)]).to(dtype)
+    x = x[torch.arange(T) % 5]
+    t = (torch.arange(T, dtype=torch.int32) * 977) % V
+    _check(ops.token_logprobs(x.to(dev), t.to(dev), k), ref.scores(x, t, k), x.double(), k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
 @pytest.mark.parametrize("V", [9, 5000])
 def test_token_logprobs_masked_and_not_finite(dev, V, dtype):
     """Rows of -inf alone, one finite logit, the type's lowest value, a NaN, a +inf, a masked target, and targets
