@@ -80,8 +80,8 @@ PagedPlan paged_plan(int group, int n_kv, int hd, int rows, int max_q, int max_l
   return p;
 }
 
-// Once per device: the rings are larger than a kernel's default shared memory.
-mk_status paged_ready() {
+// Once per device: some kernels take more shared memory than the default.
+mk_status cache_ready() {
   static std::mutex mu;
   static bool ready[64];
   int dev = 0;
@@ -102,6 +102,8 @@ mk_status paged_ready() {
                                static_cast<int>(mk::pt_smem_bytes(96))));
   MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(mk::pt_smem_bytes(128))));
+  MK_CUDA(cudaFuncSetAttribute(mk::kv_fork_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               mk::FORK_INTS * static_cast<int>(sizeof(int))));
   ready[dev] = true;
   return MK_OK;
 }
@@ -210,7 +212,7 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
                                                                              : mk::attn_paged_kernel<96, 4>)
                      : (p.nt == 1 ? mk::attn_paged_kernel<128, 1> : p.nt == 2 ? mk::attn_paged_kernel<128, 2>
                                                                               : mk::attn_paged_kernel<128, 4>);
-  MK_TRY(paged_ready());
+  MK_TRY(cache_ready());
   MK_TRY(launch_k(k, dim3(p.ctas), dim3(tc ? mk::PT_THREADS : mk::PA_THREADS),
                   tc ? mk::pt_smem_bytes(head_dim) : mk::pa_ring_bytes(head_dim, p.nt), st, true, c, a));
   const auto join = [&](auto hd, auto of_tc) {
@@ -258,10 +260,12 @@ mk_status mk_kv_fork(void* codes, float* scales, int32_t layers, int32_t num_pag
     MK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(num_pages) * sizeof(int32_t), st));
     return MK_OK;
   }
-  if (static_cast<int64_t>(new_rows) * width <= mk::FORK_SMALL && num_pages <= mk::FORK_SMALL && new_rows + rows <= 12000) {
-    MK_TRY(launch_k(mk::kv_fork_small_kernel, dim3(1), dim3(mk::PG_THREADS),
-                    (static_cast<size_t>(new_rows) + rows) * sizeof(int), st, true, block_table, lens, rows, width, parents,
-                    new_rows, num_pages, c.page_shift, new_table, new_lens, refs, src, pairs, count, d.err));
+  const int64_t ints = mk::fork_ints(new_rows, rows, num_pages);
+  if (static_cast<int64_t>(new_rows) * width <= mk::FORK_ENTRIES && ints <= mk::FORK_INTS) {
+    MK_TRY(cache_ready());
+    MK_TRY(launch_k(mk::kv_fork_small_kernel, dim3(1), dim3(mk::PG_THREADS), static_cast<size_t>(ints) * sizeof(int), st, true,
+                    block_table, lens, rows, width, parents, new_rows, num_pages, c.page_shift, new_table, new_lens, refs,
+                    pairs, count, d.err));
   } else {
     MK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(num_pages) * sizeof(int32_t), st));
     MK_TRY(launch_k(mk::kv_fork_rows_kernel, dim3(new_rows), dim3(mk::FORK_THREADS), 0, st, false, block_table, lens, rows,

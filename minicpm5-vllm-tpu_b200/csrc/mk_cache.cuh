@@ -65,13 +65,13 @@ __device__ __forceinline__ void quant8(const uint4& x, float inv, float s, uint3
   const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float2 p = unpack_bf16x2(u[e]);
-    const float f[2] = {p.x, p.y};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float q = f[i] * inv;
-      t[2 * e + i] = __float_as_uint(fmaf(fmaf(-q, s, f[i]), inv, q) + 12582912.f);
-    }
+    const float2 f = unpack_bf16x2(u[e]);
+    float q0, q1, d0, d1;  // (two at a time: packed f32 arithmetic rounds as the single does)
+    mul2_sc(f.x, f.y, inv, q0, q1);
+    fma2_v(q0, q1, -s, f.x, f.y, d0, d1);
+    fma2_v(d0, d1, inv, q0, q1, d0, d1);
+    t[2 * e] = __float_as_uint(d0 + 12582912.f);
+    t[2 * e + 1] = __float_as_uint(d1 + 12582912.f);
   }
 }
 // the low bytes of four words as one word
@@ -407,7 +407,7 @@ __device__ __forceinline__ void deal_pages(const int* upto, int asked, int32_t* 
   int given = 0;
   for (int base = 0; base < num_pages && given < asked; base += PG_THREADS) {
     const int page = base + threadIdx.x;
-    const int is_free = page < num_pages && __ldcg(refs + page) == 0;
+    const int is_free = page < num_pages && refs[page] == 0;
     int total;
     const int k = given + block_scan(is_free, sums, total) - 1;
     if (is_free && k < asked) {
@@ -467,66 +467,65 @@ __global__ void __launch_bounds__(PG_THREADS)
 }
 
 // kv_fork_rows_kernel and kv_assign_kernel in one CTA, for tables and pools that one SM walks through faster than
-// two more launches take: 256 rows of 9 slots over 1500 pages fork in 5 us instead of 12.
-constexpr int FORK_SMALL = 32768;  // table entries, and pages
+// two more launches take; the counts and all that a row needs twice lie in shared memory, so that only three loads follow
+// on one another.  256 rows of 7 slots over 1500 pages fork in 8.4 us; a step of
+// a beam search over 24 layers takes 33.3 us with it, 37.1 with the two kernels and a memset.
+constexpr int FORK_ENTRIES = 32768;  // of the new table
+constexpr int FORK_INTS = 50000;     // of shared memory
+constexpr int64_t fork_ints(int64_t rows, int64_t rows_in, int64_t num_pages) { return num_pages + rows_in + 4 * rows; }
 __global__ void __launch_bounds__(PG_THREADS)
     kv_fork_small_kernel(const int32_t* __restrict__ table, const int32_t* __restrict__ lens, int rows_in, int width,
                          const int32_t* __restrict__ parents, int rows, int num_pages, int page_shift,
-                         int32_t* __restrict__ new_table, int32_t* __restrict__ new_lens, int32_t* refs,
-                         int32_t* __restrict__ src, int2* __restrict__ pairs, int32_t* __restrict__ n_pairs, int* err) {
-  extern __shared__ int smem[];  // [rows] upto, [rows_in] the first child of each parent
+                         int32_t* new_table, int32_t* __restrict__ new_lens, int32_t* __restrict__ refs,
+                         int2* __restrict__ pairs, int32_t* __restrict__ n_pairs, int* err) {
+  // per page: rows that list it; per parent: its first child; per row: parent, length, page to copy, requests up to it
+  extern __shared__ int smem[];
   __shared__ int sums[32];
-  int *upto = smem, *eldest = smem + rows;
+  int *s_refs = smem, *eldest = s_refs + num_pages, *par = eldest + rows_in, *len = par + rows, *src = len + rows,
+      *upto = src + rows;
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x;
-  for (int p = tid; p < num_pages; p += PG_THREADS) refs[p] = 0;
+  for (int p = tid; p < num_pages; p += PG_THREADS) s_refs[p] = 0;
   for (int p = tid; p < rows_in; p += PG_THREADS) eldest[p] = rows;
   __syncthreads();
   for (int i = tid; i < rows; i += PG_THREADS) {
-    const int p = parents[i];
-    if (p >= 0 && p < rows_in) atomicMin(eldest + p, i);
+    int p = parents[i];
+    if (p >= rows_in) {
+      atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+      p = -1;
+    }
+    if (p >= 0) atomicMin(eldest + p, i);
+    par[i] = p;
+    len[i] = p < 0 ? 0 : kv_row_len(lens, p, width, page_shift, err);
+    src[i] = -1;
+    new_lens[i] = len[i];
+  }
+  __syncthreads();
+  for (int e = tid; e < rows * width; e += PG_THREADS) {
+    const int i = e / width, j = e - i * width, p = par[i], n = (len[i] + (1 << page_shift) - 1) >> page_shift;
+    const int page = p >= 0 && j < n ? kv_page_of(table, width, num_pages, p, j, err) : -1;
+    const bool copy = page >= 0 && j == n - 1 && eldest[p] < i && (len[i] & ((1 << page_shift) - 1));
+    if (copy)
+      src[i] = page;
+    else if (page >= 0)
+      atomicAdd(s_refs + page, 1);
+    new_table[e] = copy ? -1 : page;
   }
   __syncthreads();
   int asked = 0;
   for (int base = 0; base < rows; base += PG_THREADS) {
     const int i = base + tid;
-    int want = 0;
-    if (i < rows) {
-      int p = parents[i];
-      if (p >= rows_in) {
-        atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
-        p = -1;
-      }
-      const int len = p < 0 ? 0 : kv_row_len(lens, p, width, page_shift, err), n = (len + (1 << page_shift) - 1) >> page_shift;
-      new_lens[i] = len;
-      src[i] = -1;
-      if (p >= 0 && n > 0 && eldest[p] < i && (len & ((1 << page_shift) - 1))) {
-        const int page = kv_page_of(table, width, num_pages, p, n - 1, err);
-        src[i] = page;
-        want = page >= 0;
-      }
-    }
     int total;
-    const int inc = block_scan(want, sums, total);
+    const int inc = block_scan(i < rows && src[i] >= 0, sums, total);
     if (i < rows) upto[i] = asked + inc;
     asked += total;
   }
   __syncthreads();
-  for (int e = tid; e < rows * width; e += PG_THREADS) {
-    const int i = e / width, j = e - i * width, p = parents[i];
-    const int n = (new_lens[i] + (1 << page_shift) - 1) >> page_shift;
-    const bool ok = p >= 0 && p < rows_in && j < n;
-    const bool copy = ok && j == n - 1 && eldest[p] < i && (new_lens[i] & ((1 << page_shift) - 1));
-    int page = -1;
-    if (ok && !copy) page = kv_page_of(table, width, num_pages, p, j, err);
-    if (page >= 0) atomicAdd(refs + page, 1);
-    new_table[e] = page;
-  }
-  __threadfence();
-  __syncthreads();
-  deal_pages(upto, asked, new_table, new_lens, rows, width, nullptr, src, pairs, n_pairs, refs, num_pages, page_shift, sums,
+  deal_pages(upto, asked, new_table, len, rows, width, nullptr, src, pairs, n_pairs, s_refs, num_pages, page_shift, sums,
              err);
+  __syncthreads();
+  for (int p = tid; p < num_pages; p += PG_THREADS) refs[p] = s_refs[p];
 }
 
 // Compaction: with `used` live pages, those at `used` and above move into the holes below, lowest to lowest.

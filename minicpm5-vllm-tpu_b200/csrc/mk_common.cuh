@@ -440,6 +440,21 @@ __device__ __forceinline__ void fma2_sc(float a0, float a1, float s, float c, fl
       : "=f"(d0), "=f"(d1)
       : "f"(a0), "f"(a1), "f"(s), "f"(c));
 }
+// (a0, a1) * s + (c0, c1), and (a0, a1) * s, likewise.
+__device__ __forceinline__ void fma2_v(float a0, float a1, float s, float c0, float c1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 x, y, z, r;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %6};\n\t"
+      "fma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(s), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2_sc(float a0, float a1, float s, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 x, y, r;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+      "mul.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(s));
+}
 // (d0, d1) += (a0, a1) in one packed f32x2 add.
 __device__ __forceinline__ void add2_acc(float& d0, float& d1, float a0, float a1) {
   asm("{\n\t.reg .b64 x, y;\n\t"
