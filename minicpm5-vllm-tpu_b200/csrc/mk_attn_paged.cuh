@@ -40,32 +40,31 @@ struct PagedAttnArgs {
 
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
-// 16-key groups that a warp works on at a time: with 8 query rows two neighbouring ones, whose instructions fill each
-// other's latencies; wider tiles have work enough, and no registers left.
-__host__ __device__ constexpr int pa_groups(int nt) { return nt == 1 ? 2 : 1; }
-__host__ __device__ constexpr int pa_unit(int nt) { return 16 * pa_groups(nt) * PA_WARPS; }  // keys of one unit of work
+constexpr int PA_ROWS = 8;  // query rows of a tile
+// 16-key groups that a warp works on at a time: two neighbouring ones, whose instructions fill each other's latencies.
+constexpr int PA_GP = 2;
+constexpr int PA_UNIT = 16 * PA_GP * PA_WARPS;  // keys of one unit of work
 constexpr int PA_GROUPS = PA_THREADS;   // groups whose pages and scales are staged at a time
 // m may lag the true maximum by up to 2^kLag: it moves only then, which spares a warp reduction and a rescaling
 // of O per block.
 //
 // The probabilities p = exp(s - m) * vscale are rounded for their product with the codes: to one f16 (11 bits), held
-// times kPOff, so that the largest operand is 2^15.  With up to 16 query rows a block whose smallest p is below f16's
-// normal range (2^-24 of the maximum; or masked) is multiplied in another way, with p as two bf16 parts (p rounded, and
-// what that left over): 17 bits and the range of f32, so that keys far below the maximum still count where the others
-// have a zero.  That conversion and its second product cost a block a quarter more instructions.  With 32 rows the
-// products are the limit, and a key that weighs less than 2^-34 of the maximum is lost.
+// times kPOff, so that the largest operand is 2^15.  A block whose smallest p is below f16's normal range (2^-24 of the
+// maximum; or masked) is multiplied in another way, with p as two bf16 parts (p rounded, and what that left over): 17
+// bits and the range of f32, so that keys far below the maximum still count where the others have a zero.  That
+// conversion and its second product cost a block a quarter more instructions.
 constexpr float kPOff = 1024.f;
 constexpr float kLag = 5.f;
 constexpr float kF16Normal = 0x1p-14f;
 // m before the first key: low enough that any score raises it, and finite, so that m - m is 0
 constexpr float kLow = -1e30f;
 
-__host__ __device__ constexpr int pa_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int PA_CTAS_PER_SM = 3;
 // Ring of a warp: a stage holds a block's keys and values, and a CTA's rings fill its part of an SM's shared memory
 // (up to 72 KB of 227).
-__host__ __device__ constexpr int pa_stage_bytes(int hd, int nt) { return 2 * 16 * pa_groups(nt) * hd; }
-__host__ __device__ constexpr int pa_stages(int hd, int nt) { return nt == 1 ? (hd == 96 ? 3 : 2) : 4; }
-__host__ __device__ constexpr int pa_ring_bytes(int hd, int nt) { return PA_WARPS * pa_stages(hd, nt) * pa_stage_bytes(hd, nt); }
+__host__ __device__ constexpr int pa_stage_bytes(int hd) { return 2 * 16 * PA_GP * hd; }
+__host__ __device__ constexpr int pa_stages(int hd) { return hd == 96 ? 3 : 2; }
+__host__ __device__ constexpr int pa_ring_bytes(int hd) { return PA_WARPS * pa_stages(hd) * pa_stage_bytes(hd); }
 
 // Bulk copy global -> shared (both 16-byte aligned, bytes a multiple of 16), counted on `bar`.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -145,7 +144,7 @@ struct PagedShares {
   }
 };
 
-// Work.  A pair is (row, tile of 8 NT query rows, key/value head), a query row being (token, head of the
+// Work.  A pair is (row, tile of 8 query rows, key/value head), a query row being (token, head of the
 // group); a pair's keys are cut into units of PA_UNIT.  All units of all pairs, in order, are dealt out in equal
 // contiguous shares, one per CTA, from the lengths on the device: ragged batches, one long row and many short
 // ones all fill the GPU alike.  A pair that lies inside one share is finished there; a share holds at most one
@@ -158,23 +157,20 @@ struct PagedShares {
 //           or 64 + 8c .., hd 96), and the queries' B fragments the same channels.
 //   V^T P^T after a transpose of P (movmatrix) lane c's k-slots are keys 4c .. 4c + 3, one word of the value
 //           plane; a 16-byte load holds them for channels 32j + 4r .. + 3, two of each 16-row tile.
-template <int HD, int NT>
-__global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
-  constexpr int GP = pa_groups(NT), PA_UNIT = pa_unit(NT);
-  constexpr int KS = HD / 16, MT = HD / 16, ROWS = 8 * NT, LDO = HD + 4;
-  constexpr bool SPLIT = NT <= 2;  // p as two bf16 parts where f16 would lose some
-  constexpr int STAGES = pa_stages(HD, NT), STAGE = pa_stage_bytes(HD, NT), HALF = STAGE / 2;
+template <int HD>
+__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
+  constexpr int GP = PA_GP, KS = HD / 16, MT = HD / 16, ROWS = PA_ROWS, LDO = HD + 4;
+  constexpr int STAGES = pa_stages(HD), STAGE = pa_stage_bytes(HD), HALF = STAGE / 2;
   __shared__ long long s_scan[PA_WARPS], s_base;
   __shared__ int s_row;
   __shared__ int s_page[PA_GROUPS];
   __shared__ float s_ks[PA_GROUPS], s_vs[PA_GROUPS], s_red[PA_WARPS];
-  __shared__ uint2 s_q[NT > 1 ? NT * KS * 32 : 1];
   __shared__ float s_m[PA_WARPS][ROWS], s_l[PA_WARPS][ROWS];
   __shared__ uint64_t s_full[PA_WARPS][STAGES];
   __shared__ int s_abort;
   // the rings; after a pair's last block the same bytes hold the warps' results
   extern __shared__ __align__(128) uint8_t s_ring[];
-  static_assert(sizeof(float) * PA_WARPS * 8 * LDO <= pa_ring_bytes(HD, NT), "results fit");
+  static_assert(sizeof(float) * PA_WARPS * 8 * LDO <= pa_ring_bytes(HD), "results fit");
   float (*s_o)[8][LDO] = reinterpret_cast<float (*)[8][LDO]>(s_ring);
   if (threadIdx.x < PA_WARPS * STAGES) mbar_init(&s_full[0][0] + threadIdx.x, 1);
   if (threadIdx.x == 0) s_abort = 0;
@@ -257,21 +253,18 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       if (tid < groups_at(kb)) page = kv_page_of(a.table, a.width, cp.num_pages, row, (kb + tid * 16) >> cp.page_shift, a.err);
     };
     if (kbeg < kend) load_page(kbeg);
-    uint32_t qw[NT][KS][2];
+    uint32_t qw[KS][2];
+    const int qr = r0 + r;
+    const __nv_bfloat16* qp = a.q;
+    if (qr < R) qp += static_cast<long long>(first + qr / G) * a.ld_q + static_cast<long long>(g * G + qr % G) * a.hs_q;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int qr = r0 + t * 8 + r;
-      const __nv_bfloat16* qp = a.q;
-      if (qr < R) qp += static_cast<long long>(first + qr / G) * a.ld_q + static_cast<long long>(g * G + qr % G) * a.hs_q;
-#pragma unroll
-      for (int s = 0; s < KS; s += 2) {  // 8 channels: two words' worth
-        const int ch = s < 4 ? 16 * c + 4 * s : HD == 128 ? 64 + 16 * c + 4 * (s - 4) : 64 + 8 * c;
-        const uint4 v = qr < R ? __ldg(reinterpret_cast<const uint4*>(qp + ch)) : make_uint4(0, 0, 0, 0);
-        qw[t][s][0] = v.x;
-        qw[t][s][1] = v.y;
-        qw[t][s + 1][0] = v.z;
-        qw[t][s + 1][1] = v.w;
-      }
+    for (int s = 0; s < KS; s += 2) {  // 8 channels: two words' worth
+      const int ch = s < 4 ? 16 * c + 4 * s : HD == 128 ? 64 + 16 * c + 4 * (s - 4) : 64 + 8 * c;
+      const uint4 v = qr < R ? __ldg(reinterpret_cast<const uint4*>(qp + ch)) : make_uint4(0, 0, 0, 0);
+      qw[s][0] = v.x;
+      qw[s][1] = v.y;
+      qw[s + 1][0] = v.z;
+      qw[s + 1][1] = v.w;
     }
     const uint32_t plane = static_cast<uint32_t>(n_kv) * HD << cp.page_shift, page_bytes = 2 * plane;
     const int8_t* heads = cp.codes + (static_cast<size_t>(g) * HD << cp.page_shift);  // head g of page 0
@@ -280,7 +273,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
     auto ask = [&](int kb, int gi, int stage) {
       uint8_t* dst = ring + stage * STAGE;
       uint64_t* bar = &s_full[warp][stage];
-      if (GP == 1 || cp.page_shift > 4) {
+      if (cp.page_shift > 4) {
         const int pg = s_page[gi];
         mbar_arrive_expect_tx(bar, pg < 0 ? 0 : STAGE);
         if (pg >= 0) {
@@ -317,53 +310,37 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
     if (kbeg < kend) start(kbeg);
 
     // queries as f16, each row scaled by a power of two to about 1 (its exponent joins the score's factor)
-    uint32_t qf[NT == 1 ? KS : 1][2];
-    float rf[NT][2];   // score factor of this lane's two columns of each 8-row tile
-    int lim[NT][2];
+    uint32_t qf[KS][2];
+    float rf[2];   // score factor of this lane's two columns
+    int lim[2];
+    float big = 0.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float top = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack_bf16x2(qw[t][s][e]);
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-      const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        uint32_t h[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack_bf16x2(qw[t][s][e]);
-          h[e] = pack_f16x2(f.x * down, f.y * down);
-        }
-        if constexpr (NT == 1) {
-          qf[s][0] = h[0];
-          qf[s][1] = h[1];
-        } else if (warp == t % PA_WARPS) {
-          s_q[(t * KS + s) * 32 + lane] = make_uint2(h[0], h[1]);
-        }
-      }
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        rf[t][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4) * a.scale;
-        lim[t][e] = limit(r0 + t * 8 + 2 * c + e);
+        const float2 f = unpack_bf16x2(qw[s][e]);
+        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
       }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const uint32_t ex = min(max(__float_as_uint(big) >> 23, 1u), 253u);
+    const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = unpack_bf16x2(qw[s][e]);
+        qf[s][e] = pack_f16x2(f.x * down, f.y * down);
+      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      rf[e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4) * a.scale;
+      lim[e] = limit(r0 + 2 * c + e);
     }
 
-    float m[NT][2], l[NT][2], o[MT][NT][4];
+    float m[2] = {kLow, kLow}, l[2] = {0.f, 0.f}, o[MT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      m[t][0] = m[t][1] = kLow;
-      l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
-    }
+    for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float vref = 0.f;  // the largest value scale so far: O is in units of vref / kPOff
 
     for (int kb = kbeg; kb < kend; kb += PA_GROUPS * 16) {
@@ -388,9 +365,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][t][e] *= f;
+          for (int e = 0; e < 4; ++e) o[i][e] *= f;
       }
       vref = nref;
       __syncthreads();
@@ -406,7 +381,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
           break;
         }
         const uint8_t* block = ring + st * STAGE;
-        float s[GP][NT][4];
+        float s[GP][4];
 #pragma unroll
         for (int p = 0; p < GP; ++p) {
           uint32_t kw[2][KS];  // two keys' words
@@ -430,33 +405,22 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
             }
           }
           // even and odd steps in sums of their own: two chains of products half as long
-          float s1[NT][4];
+          float s1[4];
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[p][t][e] = s1[t][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[p][e] = s1[e] = 0.f;
 #pragma unroll
           for (int w = 0; w < KS; ++w) {
             uint32_t a0, a1, a2, a3;
             i8x4_to_f16x4(kw[0][w], a0, a2);
             i8x4_to_f16x4(kw[1][w], a1, a3);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              if constexpr (NT == 1) {
-                mma_16816(w & 1 ? s1[t] : s[p][t], a0, a1, a2, a3, qf[w][0], qf[w][1]);
-              } else {
-                const uint2 b = s_q[(t * KS + w) * 32 + lane];
-                mma_16816(s[p][t], a0, a1, a2, a3, b.x, b.y);
-              }
-            }
+            mma_16816(w & 1 ? s1 : s[p], a0, a1, a2, a3, qf[w][0], qf[w][1]);
           }
-          if constexpr (NT == 1)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[p][0][e] += s1[0][e];
+          for (int e = 0; e < 4; ++e) s[p][e] += s1[e];
         }
         // keys past a row's limit or of a missing page weigh nothing
         bool none[GP];
-        float vr[GP], sf[GP][NT][2];
+        float vr[GP], sf[GP][2];
         bool masked = kb + (gi + GP) * 16 > lim_min;
 #pragma unroll
         for (int p = 0; p < GP; ++p) {
@@ -464,87 +428,75 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
           masked |= none[p];
           const float ks = s_ks[gi + p];
           vr[p] = s_vs[gi + p];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            sf[p][t][0] = rf[t][0] * ks;
-            sf[p][t][1] = rf[t][1] * ks;
-          }
+          sf[p][0] = rf[0] * ks;
+          sf[p][1] = rf[1] * ks;
         }
         // x = s - m, in units of log 2
-        float x[GP][NT][4];
+        float x[GP][4];
         float top = 0.f;
         auto centre = [&]() {
           top = -INFINITY;
 #pragma unroll
-          for (int p = 0; p < GP; ++p)
+          for (int p = 0; p < GP; ++p) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
+            for (int e = 0; e < 4; ++e) x[p][e] = fmaf(s[p][e], sf[p][e & 1], -m[e & 1]);
+            if (masked) {
+              const int key = kb + (gi + p) * 16 + 4 * (r >> 1) + (r & 1);  // and key + 2
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[p][t][e] = fmaf(s[p][t][e], sf[p][t][e & 1], -m[t][e & 1]);
-              if (masked) {
-                const int key = kb + (gi + p) * 16 + 4 * (r >> 1) + (r & 1);  // and key + 2
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (none[p] || key + (e & 2) >= lim[t][e & 1]) x[p][t][e] = -INFINITY;
-              }
-              top = max3f(max3f(top, x[p][t][0], x[p][t][1]), x[p][t][2], x[p][t][3]);
+              for (int e = 0; e < 4; ++e)
+                if (none[p] || key + (e & 2) >= lim[e & 1]) x[p][e] = -INFINITY;
             }
+            top = max3f(max3f(top, x[p][0], x[p][1]), x[p][2], x[p][3]);
+          }
         };
         centre();
         if (__any_sync(0xffffffffu, top > kLag)) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int e = 0; e < 2; ++e) {
+            float top_s = m[e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top_s = m[t][e];
+            for (int p = 0; p < GP; ++p)
 #pragma unroll
-              for (int p = 0; p < GP; ++p)
+              for (int i = e; i < 4; i += 2)
+                if (x[p][i] > 0.f) top_s = fmaxf(top_s, s[p][i] * sf[p][e]);
+            top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 4));
+            top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 8));
+            top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 16));
+            const float f = ex2_approx(m[e] - top_s);
+            m[e] = top_s;
+            l[e] *= f;
 #pragma unroll
-                for (int i = e; i < 4; i += 2)
-                  if (x[p][t][i] > 0.f) top_s = fmaxf(top_s, s[p][t][i] * sf[p][t][e]);
-              top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 4));
-              top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 8));
-              top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, 16));
-              const float f = ex2_approx(m[t][e] - top_s);
-              m[t][e] = top_s;
-              l[t][e] *= f;
-#pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                o[i][t][e] *= f;
-                o[i][t][e + 2] *= f;
-              }
+            for (int i = 0; i < MT; ++i) {
+              o[i][e] *= f;
+              o[i][e + 2] *= f;
             }
+          }
           centre();
         }
         float least = INFINITY;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int p = 0; p < GP; ++p) {
+          float(&y)[4] = x[p];
+          float z[4];
 #pragma unroll
-          for (int p = 0; p < GP; ++p) {
-            float(&y)[4] = x[p][t];
-            float z[4];
+          for (int e = 0; e < 4; ++e) z[e] = ex2_approx(y[e]);
+          add2_acc(l[0], l[1], z[0], z[1]);
+          add2_acc(l[0], l[1], z[2], z[3]);
+          if (masked) {  // 0 even where the scale is NaN
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = ex2_approx(y[e]);
-            add2_acc(l[t][0], l[t][1], z[0], z[1]);
-            add2_acc(l[t][0], l[t][1], z[2], z[3]);
-            if (masked) {  // 0 even where the scale is NaN
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = y[e] == -INFINITY ? 0.f : z[e] * vr[p];
-            } else {
-              fma2_sc(z[0], z[1], vr[p], 0.f, y[0], y[1]);
-              fma2_sc(z[2], z[3], vr[p], 0.f, y[2], y[3]);
-            }
-            least = fminf(fminf(least, fminf(y[0], y[1])), fminf(y[2], y[3]));
+            for (int e = 0; e < 4; ++e) y[e] = y[e] == -INFINITY ? 0.f : z[e] * vr[p];
+          } else {
+            fma2_sc(z[0], z[1], vr[p], 0.f, y[0], y[1]);
+            fma2_sc(z[2], z[3], vr[p], 0.f, y[2], y[3]);
           }
-        const bool narrow = !SPLIT || __all_sync(0xffffffffu, least >= kF16Normal);
-        if (narrow) {
-          uint32_t pb[GP][NT][2];
+          least = fminf(fminf(least, fminf(y[0], y[1])), fminf(y[2], y[3]));
+        }
+        if (__all_sync(0xffffffffu, least >= kF16Normal)) {
+          uint32_t pb[GP][2];
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int p = 0; p < GP; ++p)
 #pragma unroll
-            for (int p = 0; p < GP; ++p)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) pb[p][t][e] = movmatrix_trans(pack_f16x2(x[p][t][2 * e], x[p][t][2 * e + 1]));
+            for (int e = 0; e < 2; ++e) pb[p][e] = movmatrix_trans(pack_f16x2(x[p][2 * e], x[p][2 * e + 1]));
 #pragma unroll
           for (int p = 0; p < GP; ++p)
 #pragma unroll
@@ -556,24 +508,21 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
                 uint32_t a0, a1, a2, a3;
                 i8x4_to_f16x4(w[2 * h], a0, a2);
                 i8x4_to_f16x4(w[2 * h + 1], a1, a3);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) mma_16816(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
+                mma_16816(o[2 * j + h], a0, a1, a2, a3, pb[p][0], pb[p][1]);
               }
             }
-        } else if constexpr (SPLIT) {
-          uint32_t pb[GP][NT][2], pl[GP][NT][2];
+        } else {
+          uint32_t pb[GP][2], pl[GP][2];
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int p = 0; p < GP; ++p)
 #pragma unroll
-            for (int p = 0; p < GP; ++p)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float(&y)[4] = x[p][t];
-                const uint32_t hi = pack_bf16x2(y[2 * e], y[2 * e + 1]);
-                const float2 f = unpack_bf16x2(hi);
-                pb[p][t][e] = movmatrix_trans(hi);
-                pl[p][t][e] = movmatrix_trans(pack_bf16x2(y[2 * e] - f.x, y[2 * e + 1] - f.y));
-              }
+            for (int e = 0; e < 2; ++e) {
+              const float(&y)[4] = x[p];
+              const uint32_t hi = pack_bf16x2(y[2 * e], y[2 * e + 1]);
+              const float2 f = unpack_bf16x2(hi);
+              pb[p][e] = movmatrix_trans(hi);
+              pl[p][e] = movmatrix_trans(pack_bf16x2(y[2 * e] - f.x, y[2 * e + 1] - f.y));
+            }
 #pragma unroll
           for (int p = 0; p < GP; ++p)
 #pragma unroll
@@ -585,11 +534,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
                 uint32_t a0, a1, a2, a3;
                 i8x4_to_bf16x4(w[2 * h], a0, a2);
                 i8x4_to_bf16x4(w[2 * h + 1], a1, a3);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                  mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pb[p][t][0], pb[p][t][1]);
-                  mma_16816_bf16(o[2 * j + h][t], a0, a1, a2, a3, pl[p][t][0], pl[p][t][1]);
-                }
+                mma_16816_bf16(o[2 * j + h], a0, a1, a2, a3, pb[p][0], pb[p][1]);
+                mma_16816_bf16(o[2 * j + h], a0, a1, a2, a3, pl[p][0], pl[p][1]);
               }
             }
         }
@@ -606,70 +552,65 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
 
     // the warps' pieces, joined in order
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], d);
-        if (r == 0) {
-          s_m[warp][t * 8 + 2 * c + e] = m[t][e];
-          s_l[warp][t * 8 + 2 * c + e] = l[t][e];
-        }
+      for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+      if (r == 0) {
+        s_m[warp][2 * c + e] = m[e];
+        s_l[warp][2 * c + e] = l[e];
       }
+    }
     __syncthreads();  // every warp is done with its ring
     const bool whole = ua == 0 && ub == upp;
     const int slot = static_cast<int>(cta) * 2 + (ua == 0 ? 1 : 0);
     const float unit = vref / kPOff;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      __syncthreads();
+    for (int e = 0; e < 2; ++e) {
+      const int q8 = 2 * c + e;
+      float top = kLow;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int q8 = 2 * c + e;
-        float top = kLow;
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][q8]);
+      const float f = ex2_approx(m[e] - top);
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][t * 8 + q8]);
-        const float f = ex2_approx(m[t][e] - top);
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j)
-          *reinterpret_cast<float4*>(&s_o[warp][q8][32 * j + 4 * r]) =
-              make_float4(o[2 * j][t][e] * f, o[2 * j][t][e + 2] * f, o[2 * j + 1][t][e] * f, o[2 * j + 1][t][e + 2] * f);
-      }
-      __syncthreads();
-      const int q8 = tid >> 4, qr = r0 + t * 8 + q8;
+      for (int j = 0; j < HD / 32; ++j)
+        *reinterpret_cast<float4*>(&s_o[warp][q8][32 * j + 4 * r]) =
+            make_float4(o[2 * j][e] * f, o[2 * j][e + 2] * f, o[2 * j + 1][e] * f, o[2 * j + 1][e + 2] * f);
+    }
+    __syncthreads();
+    const int q8 = tid >> 4;
+    if (r0 + q8 < R) {
       float top = kLow, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][t * 8 + q8]);
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w][q8]);
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) sum += s_l[w][t * 8 + q8] * ex2_approx(s_m[w][t * 8 + q8] - top);
-      if (qr < R) {
-        const long long at = static_cast<long long>(first + qr / G) * a.n_q + g * G + qr % G;
+      for (int w = 0; w < PA_WARPS; ++w) sum += s_l[w][q8] * ex2_approx(s_m[w][q8] - top);
+      const int to = r0 + q8;
+      const long long at = static_cast<long long>(first + to / G) * a.n_q + g * G + to % G;
 #pragma unroll
-        for (int d = (tid & 15) * 4; d < HD; d += 64) {
-          float4 x = *reinterpret_cast<const float4*>(&s_o[0][q8][d]);
+      for (int d = (tid & 15) * 4; d < HD; d += 64) {
+        float4 x = *reinterpret_cast<const float4*>(&s_o[0][q8][d]);
 #pragma unroll
-          for (int w = 1; w < PA_WARPS; ++w) {
-            const float4 y = *reinterpret_cast<const float4*>(&s_o[w][q8][d]);
-            x.x += y.x;
-            x.y += y.y;
-            x.z += y.z;
-            x.w += y.w;
-          }
-          if (whole) {
-            const float f = sum == 0.f ? 0.f : unit / sum;
-            *reinterpret_cast<uint2*>(a.out + at * HD + d) =
-                make_uint2(pack_bf16x2(x.x * f, x.y * f), pack_bf16x2(x.z * f, x.w * f));
-          } else {
-            *reinterpret_cast<float4*>(a.part_o + (static_cast<size_t>(slot) * ROWS + t * 8 + q8) * HD + d) =
-                make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
-          }
+        for (int w = 1; w < PA_WARPS; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(&s_o[w][q8][d]);
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
         }
-        if ((tid & 15) == 0) {
-          if (!whole)
-            a.part_ml[static_cast<size_t>(slot) * ROWS + t * 8 + q8] = make_float2(top, sum);
-          else if (a.lse)
-            a.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.693147180559945f;
+        if (whole) {
+          const float f = sum == 0.f ? 0.f : unit / sum;
+          *reinterpret_cast<uint2*>(a.out + at * HD + d) =
+              make_uint2(pack_bf16x2(x.x * f, x.y * f), pack_bf16x2(x.z * f, x.w * f));
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + (static_cast<size_t>(slot) * ROWS + q8) * HD + d) =
+              make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
         }
+      }
+      if ((tid & 15) == 0) {
+        if (!whole)
+          a.part_ml[static_cast<size_t>(slot) * ROWS + q8] = make_float2(top, sum);
+        else if (a.lse)
+          a.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.693147180559945f;
       }
     }
     if (!whole && ua == 0 && tid == 0) {
@@ -677,7 +618,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas_per_sm(NT)) attn_paged_ker
       a.desc[cta] = make_int4(first, rt, g, shares.owner(last) | min(ROWS, R - r0) << 16);
     }
     fence_proxy_async_smem();  // the results before the next copies into the same bytes
-    __syncthreads();           // s_o and s_q are free again
+    __syncthreads();           // s_o is free again
     u += ub - ua;
     if (s_abort) break;
   }

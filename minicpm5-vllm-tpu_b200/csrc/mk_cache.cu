@@ -51,31 +51,36 @@ mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int 
                   page_bytes(n_kv, page, hd), 2 * n_kv, pairs, n_pairs, layers, table, entries, to, new_table, err);
 }
 
-// Launch shape and workspace of the paged attention.  Query rows (tokens times heads of a group) per tile: 8, 16
-// or 32, the smallest that holds a row's queries (a wider tile reads and converts the cache less often but
-// leaves room for two CTAs per SM instead of three), or 256 with tcgen05 above kPagedWide.  One wave of CTAs on 148 SMs, fewer when the bounds say that
-// there are fewer units of work.
-constexpr int kPagedTc = mk::PT_ROWS / 8;  // the tcgen05 kernel's rows, in eights
-constexpr int kPagedWide = 128;
+// Launch shape and workspace of the paged attention.  Up to kPagedWide query rows (tokens times heads of a group) per
+// key/value head go through attn_paged_kernel in tiles of 8, which read and convert the cache once a tile; more through
+// attn_paged_tc_kernel, 256 at a time.  us with 32, 48, 64 and 128 rows (hd 96, 2 key/value heads): 16 rows of 4096
+// tokens 26, 32, 39, 68 in tiles of 8 and 37, 37, 37, 36 with tcgen05; one row of 32768 20, 23, 26, 40 and 28, 28, 29,
+// 29; 64 rows of 256 16, 17, 23, 36 and 23, 23, 23, 24.  One wave of CTAs, fewer when the bounds say that there are
+// fewer units of work.
+constexpr int kPagedWide = 56;
 struct PagedPlan {
-  int nt, ctas, long_join;  // long_join: CTAs that join few pairs of many pieces, 0: one per CTA of the products
+  bool tc;
+  int rows, ctas;  // rows of a tile
+  int long_join;   // CTAs that join few pairs of many pieces, 0: one per CTA of the products
   size_t o_bytes, ml_bytes, bytes;
 };
 PagedPlan paged_plan(int group, int n_kv, int hd, int rows, int max_q, int max_len) {
   PagedPlan p;
   const int64_t q_rows = static_cast<int64_t>(std::max(max_q, 1)) * group;
-  p.nt = q_rows <= 8 ? 1 : q_rows <= 16 ? 2 : q_rows <= kPagedWide ? 4 : kPagedTc;
-  const int64_t tiles = (q_rows + 8 * p.nt - 1) / (8 * p.nt);
-  const int unit = p.nt == kPagedTc ? mk::PT_KEYS : mk::pa_unit(p.nt);
+  p.tc = q_rows > kPagedWide;
+  p.rows = p.tc ? mk::PT_ROWS : mk::PA_ROWS;
+  const int64_t tiles = (q_rows + p.rows - 1) / p.rows;
+  const int unit = p.tc ? mk::PT_KEYS : mk::PA_UNIT;
   const int64_t per_pair = std::max(1, max_len / unit + (max_len % unit != 0));
-  const int64_t most = p.nt == kPagedTc ? mk::PT_CTAS : 148 * mk::pa_ctas_per_sm(p.nt);
+  const int64_t most = mk::PT_CTAS * (p.tc ? 1 : mk::PA_CTAS_PER_SM);
   // (each factor is below 2^31: cut before the product can overflow)
   const int64_t pairs = std::min<int64_t>(most, static_cast<int64_t>(rows) * n_kv) * std::min<int64_t>(most, tiles);
   p.ctas = static_cast<int>(std::max<int64_t>(1, std::min(most, std::min(most, pairs) * per_pair)));
-  // 8 pairs of 55 pieces join in 7.5 us this way and in 17 the other, 128 pairs of 4 in 7.6 and 5.8
+  // 8 pairs in 55 pieces each take 54 us with the long join and 60 with the other, 2 pairs in 222 pieces 16 and 38; 128
+  // pairs of 3 or 4 pieces 38 and 34 (hd 128)
   p.long_join = pairs * 8 <= p.ctas ? static_cast<int>(pairs) : 0;
-  p.o_bytes = static_cast<size_t>(2) * p.ctas * 8 * p.nt * hd * sizeof(float);
-  p.ml_bytes = static_cast<size_t>(2) * p.ctas * 8 * p.nt * sizeof(float2);
+  p.o_bytes = static_cast<size_t>(2) * p.ctas * p.rows * hd * sizeof(float);
+  p.ml_bytes = static_cast<size_t>(2) * p.ctas * p.rows * sizeof(float2);
   p.bytes = p.o_bytes + p.ml_bytes + static_cast<size_t>(p.ctas) * sizeof(int4);
   return p;
 }
@@ -89,15 +94,10 @@ mk_status cache_ready() {
   if (dev < 0 || dev >= 64) return MK_ERR_BAD_ARG;
   std::lock_guard<std::mutex> lk(mu);
   if (ready[dev]) return MK_OK;
-  const auto allow = [](void (*k)(KvPages, mk::PagedAttnArgs), int hd, int nt) {
-    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, mk::pa_ring_bytes(hd, nt));
-  };
-  MK_CUDA(allow(mk::attn_paged_kernel<96, 1>, 96, 1));
-  MK_CUDA(allow(mk::attn_paged_kernel<96, 2>, 96, 2));
-  MK_CUDA(allow(mk::attn_paged_kernel<96, 4>, 96, 4));
-  MK_CUDA(allow(mk::attn_paged_kernel<128, 1>, 128, 1));
-  MK_CUDA(allow(mk::attn_paged_kernel<128, 2>, 128, 2));
-  MK_CUDA(allow(mk::attn_paged_kernel<128, 4>, 128, 4));
+  MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_kernel<96>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               mk::pa_ring_bytes(96)));
+  MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               mk::pa_ring_bytes(128)));
   MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<96>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(mk::pt_smem_bytes(96))));
   MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -205,27 +205,23 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
   a.desc = reinterpret_cast<int4*>(ws + p.o_bytes + p.ml_bytes);
   a.err = d.err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool tc = p.nt == kPagedTc;
   void (*k)(KvPages, mk::PagedAttnArgs) =
-      tc               ? (head_dim == 96 ? mk::attn_paged_tc_kernel<96> : mk::attn_paged_tc_kernel<128>)
-      : head_dim == 96 ? (p.nt == 1 ? mk::attn_paged_kernel<96, 1> : p.nt == 2 ? mk::attn_paged_kernel<96, 2>
-                                                                             : mk::attn_paged_kernel<96, 4>)
-                     : (p.nt == 1 ? mk::attn_paged_kernel<128, 1> : p.nt == 2 ? mk::attn_paged_kernel<128, 2>
-                                                                              : mk::attn_paged_kernel<128, 4>);
+      p.tc ? (head_dim == 96 ? mk::attn_paged_tc_kernel<96> : mk::attn_paged_tc_kernel<128>)
+           : (head_dim == 96 ? mk::attn_paged_kernel<96> : mk::attn_paged_kernel<128>);
   MK_TRY(cache_ready());
-  MK_TRY(launch_k(k, dim3(p.ctas), dim3(tc ? mk::PT_THREADS : mk::PA_THREADS),
-                  tc ? mk::pt_smem_bytes(head_dim) : mk::pa_ring_bytes(head_dim, p.nt), st, true, c, a));
+  MK_TRY(launch_k(k, dim3(p.ctas), dim3(p.tc ? mk::PT_THREADS : mk::PA_THREADS),
+                  p.tc ? mk::pt_smem_bytes(head_dim) : mk::pa_ring_bytes(head_dim), st, true, c, a));
   const auto join = [&](auto hd, auto of_tc) {
     constexpr int HD = decltype(hd)::value;
     constexpr bool TC = decltype(of_tc)::value;
     if (p.long_join > 0)
-      return launch_k(mk::attn_paged_long_join_kernel<HD, TC>, dim3(p.long_join, p.nt, HD / 32),
+      return launch_k(mk::attn_paged_long_join_kernel<HD, TC>, dim3(p.long_join, p.rows / 8, HD / 32),
                       dim3(mk::PagedLongJoin::THREADS), 0, st, true, a, p.ctas);
     using Join = mk::PagedJoin<HD, TC>;
-    return launch_k(mk::attn_paged_join_kernel<HD, TC>, dim3(p.ctas, 8 * p.nt / Join::RJ), dim3(Join::THREADS), 0, st, true,
-                    a, 8 * p.nt);
+    return launch_k(mk::attn_paged_join_kernel<HD, TC>, dim3(p.ctas, p.rows / Join::RJ), dim3(Join::THREADS), 0, st, true,
+                    a, p.rows);
   };
-  const auto by_size = [&](auto hd) { return tc ? join(hd, std::true_type()) : join(hd, std::false_type()); };
+  const auto by_size = [&](auto hd) { return p.tc ? join(hd, std::true_type()) : join(hd, std::false_type()); };
   return head_dim == 96 ? by_size(std::integral_constant<int, 96>()) : by_size(std::integral_constant<int, 128>());
 }
 
