@@ -20,6 +20,11 @@
 // a rescaling waits for the product before it and passes O through registers, so m may lag more (16 rows of
 // up to 64 tokens over up to 8192 keys: 65.3 us so, 66.3 with 1024 and 5); a key that weighs less than 2^-31 of the
 // maximum is lost.
+//
+// Measured: those 16 rows (470 tokens over 69268 cached, hd 96) 53.1 us with the join, where the exponentials of its
+// 3374 tiles would take 12.  A CTA's 23 tiles take 2000 cycles each: 1590 from the scores to the weights (1100 where only
+// one of the two row tiles has rows), the rest is barriers and TMEM.  Before the first tile come 13000 cycles (the walk
+// over the lengths, queries, pages, the first codes), after the last 4000, and the join is 8 us.
 #pragma once
 
 #include "mk_attn_paged.cuh"

@@ -100,10 +100,14 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 // tau that is then known, of the shares or of one warp alone; where that does not do either (long runs of equal
 // logits; fewer than k above -inf), each alternative that is missing is searched for.
 //
-// What bounds it: the bytes of the logits.  Per bf16 logit the arithmetic is about six instructions and one
-// exponential, two thirds of what an SM can issue at the rate at which HBM delivers them.
+// What bounds it: the bytes of the logits where they are f32 (2047 x 130560, k = 5: 188 us, 5.7 TB/s; k = 0: 165, the
+// rate of a plain copy), the issue slots and the wait for the loads where they are bf16 (2047 x 73448, k = 5: 77 us, 3.9
+// TB/s; k = 0: 61): per bf16 logit the arithmetic is about six instructions and one exponential, two thirds of what an SM
+// can issue at the rate at which HBM delivers them.  Three rows of 130560 f32 take 10.8 us: a launch, two waits for
+// memory and the cluster's join.
 // Threads per CTA.  128 where there are rows enough (the work at a row's end is the same for every warp, and with
-// 256 threads it was a third of all); 512 where a cluster shares a row, so that a slice of 16384 logits is one step.
+// 256 threads it was a third of all); 512 where a cluster shares a row, so that a slice of 16384 logits is one step, and
+// where there are few rows an SM.
 constexpr int TL_FEW = 128, TL_MANY = 512;
 constexpr int TL_VALUES = 32;     // logits per thread and step
 constexpr int TL_TOPK_MAX = 64;
@@ -478,6 +482,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
 // What bounds it: 2 H operations per logit against five instructions and one exponential in the epilogue; with
 // H = 1536 the tensor cores take 12288 cycles for a 128 x 256 tile and the exponentials 2048, hidden behind the
 // next tile's products (two accumulators fill the 512 TMEM columns).  With few tokens W's bytes are the bound.
+// Measured: 8192 tokens x 73448 ids, H 1536, 1079 us (1713 TFLOP/s, alone) and 1.28 ms in a row of calls under the power
+// limit, with 19 us for the join of the parts; 37 tokens x 130560 ids 63 us, 6.4 TB/s of W, and 5 us for the join.
 //
 // Layout.  PAIR (more than 128 tokens): two CTAs work on 256 tokens x 256 ids with 2-SM MMAs, each holding its 128
 // tokens and half of the ids, which halves the operand bytes that each SM takes in per product.  Otherwise one
