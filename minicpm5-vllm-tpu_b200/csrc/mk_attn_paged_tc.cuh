@@ -21,7 +21,7 @@
 // up to 64 tokens over up to 8192 keys: 65.3 us so, 66.3 with 1024 and 5); a key that weighs less than 2^-31 of the
 // maximum is lost.
 //
-// Measured: those 16 rows (470 tokens over 69268 cached, hd 96) 53.1 us with the join, where the exponentials of its
+// Measured: those 16 rows (470 tokens over 69268 cached, hd 96) 51.9 us with the join, where the exponentials of its
 // 3374 tiles would take 12.  A CTA's 23 tiles take 2000 cycles each: 1590 from the scores to the weights (1100 where only
 // one of the two row tiles has rows), the rest is barriers and TMEM.  Before the first tile come 13000 cycles (the walk
 // over the lengths, queries, pages, the first codes), after the last 4000, and the join is 8 us.
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
   Piece p;
   bool ok = true;
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   }
   if (warp == 0) {
     // ---------------------------------------------------------------- codes
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     mbar_wait_drain(drain, 0);
   } else if (warp >= 12) {
     // ---------------------------------------------------------------- int8 -> f16
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int ct = tid - 12 * 32;
     int j = 0;
     while (ok && next(p)) {
@@ -381,8 +381,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attn_paged_tc_kernel(KvPages cp
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax, queries, results
-    // 512 threads x 128 registers at launch: these 256 take 168 each, the others 88
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    // 512 threads x 128 registers at launch: these 256 take 184 each, the others 72 (with 168 and 88 the chunk above takes
+    // 53.3 us instead of 51.9, with 152 and 104 54.8)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int t = (warp - 4) >> 2, quarter = warp & 3, trow = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + lane_off + t * 128, tO = tmem + lane_off + 256 + t * 128;
