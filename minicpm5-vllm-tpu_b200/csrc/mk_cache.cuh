@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(PG_THREADS)
 
 // kv_fork_rows_kernel and kv_assign_kernel in one CTA, for tables and pools that one SM walks through faster than
 // two more launches take; the counts and all that a row needs twice lie in shared memory, so that only three loads follow
-// on one another.  256 rows of 7 slots over 1500 pages fork in 8.4 us; a step of
-// a beam search over 24 layers takes 33.3 us with it, 37.1 with the two kernels and a memset.
+// on one another.  256 rows of 8 slots over 1500 pages fork in 8 us; a step of
+// a beam search over 24 layers takes 33.2 us with it, 37.1 with the two kernels and a memset.
 constexpr int FORK_ENTRIES = 32768;  // of the new table
 constexpr int FORK_INTS = 50000;     // of shared memory
 constexpr int64_t fork_ints(int64_t rows, int64_t rows_in, int64_t num_pages) { return num_pages + rows_in + 4 * rows; }
@@ -509,15 +509,30 @@ __global__ void __launch_bounds__(PG_THREADS)
     new_lens[i] = len[i];
   }
   __syncthreads();
-  for (int e = tid; e < rows * width; e += PG_THREADS) {
-    const int i = e / width, j = e - i * width, p = par[i], n = (len[i] + (1 << page_shift) - 1) >> page_shift;
-    const int page = p >= 0 && j < n ? kv_page_of(table, width, num_pages, p, j, err) : -1;
-    const bool copy = page >= 0 && j == n - 1 && eldest[p] < i && (len[i] & ((1 << page_shift) - 1));
-    if (copy)
-      src[i] = page;
-    else if (page >= 0)
-      atomicAdd(s_refs + page, 1);
-    new_table[e] = copy ? -1 : page;
+  constexpr int AHEAD = 4;  // entries of a thread whose loads are on the way together
+  for (int e0 = tid; e0 < rows * width; e0 += AHEAD * PG_THREADS) {
+    int page[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int e = e0 + k * PG_THREADS, i = min(e / width, rows - 1), j = e - i * width, p = par[i];
+      const bool listed = e < rows * width && p >= 0 && j < (len[i] + (1 << page_shift) - 1) >> page_shift;
+      page[k] = listed ? max(table[static_cast<size_t>(p) * width + j], -1) : INT_MIN;  // (-1: missing)
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int e = e0 + k * PG_THREADS, i = min(e / width, rows - 1), j = e - i * width, p = par[i];
+      if (e >= rows * width) break;
+      if (page[k] != INT_MIN && static_cast<unsigned>(page[k]) >= static_cast<unsigned>(num_pages)) {
+        atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
+        page[k] = INT_MIN;
+      }
+      const bool copy = page[k] >= 0 && eldest[p] < i && j == (len[i] - 1) >> page_shift && (len[i] & ((1 << page_shift) - 1));
+      if (copy)
+        src[i] = page[k];
+      else if (page[k] >= 0)
+        atomicAdd(s_refs + page[k], 1);
+      new_table[e] = copy || page[k] < 0 ? -1 : page[k];
+    }
   }
   __syncthreads();
   int asked = 0;
