@@ -18,7 +18,7 @@
 // Measured, with the join: 64 rows of up to 8192 tokens (291198 together, hd 128, 2 key/value heads; 150 MB) 36.6 us, 4.1
 // TB/s; 4 rows of up to 131001 (302602) 37.4 us.  Between the first copy and the last HBM delivers what a plain copy
 // reaches; what is over is the launch, the walk over the lengths and the page lookup before the first copy (3 us), the
-// results (1 us) and the join (5 to 6 us).  A single row of 999 tokens takes 5 us here and 3 in the join.
+// results (1 us) and the join (5 to 6 us).  A single row of 999 tokens takes 6.5 us, by one launch of a few CTAs.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -65,6 +65,8 @@ constexpr float kF16Normal = 0x1p-14f;
 constexpr float kLow = -1e30f;
 
 constexpr int PA_CTAS_PER_SM = 3;
+constexpr int PA_CLUSTER = 8;  // CTAs of a (row, key/value head), where rows are few: one for each query row
+static_assert(PA_CLUSTER == PA_ROWS, "a row each");
 // Ring of a warp: a stage holds a block's keys and values, and a CTA's rings fill its part of an SM's shared memory
 // (up to 72 KB of 227).
 __host__ __device__ constexpr int pa_stage_bytes(int hd) { return 2 * 16 * PA_GP * hd; }
@@ -149,6 +151,44 @@ struct PagedShares {
   }
 };
 
+// Four channels of a row's result, put together from pieces in order.
+struct PagedSum {
+  float m = kLow, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float2 ml, float4 x) {
+    const float top = fmaxf(m, ml.x), f = ex2_approx(m - top), e = ex2_approx(ml.x - top);
+    m = top;
+    l = l * f + ml.y * e;
+    o.x = o.x * f + x.x * e;
+    o.y = o.y * f + x.y * e;
+    o.z = o.z * f + x.z * e;
+    o.w = o.w * f + x.w * e;
+  }
+  // row `at` (token times heads), channels dim ..
+  __device__ __forceinline__ void finish(const PagedAttnArgs& a, long long at, int hd, int dim) const {
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(a.out + at * hd + dim) =
+        make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
+    if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
+  }
+};
+__device__ __forceinline__ float2 ld_cluster_f2(const void* p, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(mapa_cluster(smem_u32(p), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(const void* p, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(mapa_cluster(smem_u32(p), rank))
+               : "memory");
+  return v;
+}
+
 // Work.  A pair is (row, tile of 8 query rows, key/value head), a query row being (token, head of the
 // group); a pair's keys are cut into units of PA_UNIT.  All units of all pairs, in order, are dealt out in equal
 // contiguous shares, one per CTA, from the lengths on the device: ragged batches, one long row and many short
@@ -162,12 +202,17 @@ struct PagedShares {
 //           or 64 + 8c .., hd 96), and the queries' B fragments the same channels.
 //   V^T P^T after a transpose of P (movmatrix) lane c's k-slots are keys 4c .. 4c + 3, one word of the value
 //           plane; a 16-byte load holds them for channels 32j + 4r .. + 3, two of each 16-row tile.
-template <int HD>
+//
+// ONE: single tokens of few rows (one per row, up to 8 heads a group).  A cluster of PA_CLUSTER CTAs takes a (row,
+// key/value head), its keys in equal shares, and CTA i puts query row i together from the others' shared memory: no
+// walk over the lengths, nothing in memory, no second launch.
+template <int HD, bool ONE>
 __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(KvPages cp, PagedAttnArgs a) {
   constexpr int GP = PA_GP, KS = HD / 16, MT = HD / 16, ROWS = PA_ROWS, LDO = HD + 4;
   constexpr int STAGES = pa_stages(HD), STAGE = pa_stage_bytes(HD), HALF = STAGE / 2;
   __shared__ long long s_scan[PA_WARPS], s_base;
   __shared__ int s_row;
+  __shared__ float2 s_ml[ROWS];  // ONE: this CTA's m and l
   __shared__ int s_page[PA_GROUPS];
   __shared__ float s_ks[PA_GROUPS], s_vs[PA_GROUPS], s_red[PA_WARPS];
   __shared__ float s_m[PA_WARPS][ROWS], s_l[PA_WARPS][ROWS];
@@ -192,55 +237,67 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(
   };
 
   // this CTA's share [u0, u1) of the N units, and the row where it begins
-  const int per = (a.rows + PA_THREADS - 1) / PA_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
-  long long mine = 0;
-  for (int i = i0; i < i1; ++i) mine += units(row_of(i));
-  long long inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += t;
-  }
-  if (lane == 31) s_scan[warp] = inc;
-  __syncthreads();
-  long long N = 0;
-#pragma unroll
-  for (int w = 0; w < PA_WARPS; ++w) {
-    if (w < warp) inc += s_scan[w];
-    N += s_scan[w];
-  }
-  const PagedShares shares(N, gridDim.x);
   const uint32_t cta = blockIdx.x;
-  if (tid == 0) a.desc[cta] = make_int4(-1, 0, 0, 0);
-  if (cta >= shares.C) return;
-  const long long u0 = shares.begin(cta), u1 = shares.begin(cta + 1);
-  if (inc - mine <= u0 && u0 < inc) {
-    long long base = inc - mine;
-    int i = i0;
-    for (uint32_t n = units(row_of(i)); base + n <= u0; n = units(row_of(++i))) base += n;
-    s_row = i;
-    s_base = base;
+  PagedShares shares(0, 0);
+  long long u0 = 0, u1 = 1, base = 0;
+  int row;
+  if constexpr (ONE) {
+    row = cta / PA_CLUSTER / n_kv;
+  } else {
+    const int per = (a.rows + PA_THREADS - 1) / PA_THREADS, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) mine += units(row_of(i));
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    long long N = 0;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) {
+      if (w < warp) inc += s_scan[w];
+      N += s_scan[w];
+    }
+    shares = PagedShares(N, gridDim.x);
+    if (tid == 0) a.desc[cta] = make_int4(-1, 0, 0, 0);
+    if (cta >= shares.C) return;
+    u0 = shares.begin(cta);
+    u1 = shares.begin(cta + 1);
+    if (inc - mine <= u0 && u0 < inc) {
+      long long at = inc - mine;
+      int i = i0;
+      for (uint32_t n = units(row_of(i)); at + n <= u0; n = units(row_of(++i))) at += n;
+      s_row = i;
+      s_base = at;
+    }
+    __syncthreads();
+    row = s_row;
+    base = s_base;
   }
-  __syncthreads();
-  int row = s_row;
-  long long base = s_base;
   uint8_t* ring = s_ring + warp * STAGES * STAGE;
   int st = 0;           // stage of the next block to be read
   uint32_t phase = 0;
 
   for (long long u = u0; u < u1;) {
     const PagedRow pr = row_of(row);
-    const uint32_t ru = units(pr);
-    if (u >= base + ru) {
-      base += ru;
-      ++row;
-      continue;
+    if constexpr (!ONE) {
+      const uint32_t ru = units(pr);
+      if (u >= base + ru) {
+        base += ru;
+        ++row;
+        continue;
+      }
     }
     const int first = pr.first, n = pr.n, len = pr.len, tiles = row_tiles(n);
     // (32-bit divisions: a row's units are counted in 32 bits)
-    const uint32_t in = static_cast<uint32_t>(u - base), upp_u = max((len + PA_UNIT - 1) / PA_UNIT, 1), local_pair = in / upp_u;
-    const int upp = upp_u, ua = in - local_pair * upp_u;
-    const int ub = static_cast<int>(min(static_cast<long long>(upp), ua + (u1 - u)));
+    const uint32_t in = static_cast<uint32_t>(u - base), upp_u = max((len + PA_UNIT - 1) / PA_UNIT, 1);
+    const uint32_t local_pair = ONE ? cta / PA_CLUSTER % n_kv : in / upp_u, share = ONE ? cluster_ctarank() : 0;
+    const int upp = upp_u, ua = ONE ? static_cast<long long>(upp) * share / PA_CLUSTER : in - local_pair * upp_u;
+    const int ub = static_cast<int>(ONE ? static_cast<long long>(upp) * (share + 1) / PA_CLUSTER
+                                        : min(static_cast<long long>(upp), ua + (u1 - u)));
     const int g = tiles == 1 ? local_pair : local_pair / tiles, rt = local_pair - g * tiles;
     const int r0 = rt * ROWS, R = n * G;
     // a query row's token sees the keys below its limit
@@ -566,7 +623,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(
       }
     }
     __syncthreads();  // every warp is done with its ring
-    const bool whole = ua == 0 && ub == upp;
+    const bool whole = !ONE && ua == 0 && ub == upp;
     const int slot = static_cast<int>(cta) * 2 + (ua == 0 ? 1 : 0);
     const float unit = vref / kPOff;
 #pragma unroll
@@ -602,7 +659,9 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(
           x.z += y.z;
           x.w += y.w;
         }
-        if (whole) {
+        if constexpr (ONE) {
+          *reinterpret_cast<float4*>(&s_o[0][q8][d]) = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
+        } else if (whole) {
           const float f = sum == 0.f ? 0.f : unit / sum;
           *reinterpret_cast<uint2*>(a.out + at * HD + d) =
               make_uint2(pack_bf16x2(x.x * f, x.y * f), pack_bf16x2(x.z * f, x.w * f));
@@ -612,11 +671,33 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(
         }
       }
       if ((tid & 15) == 0) {
-        if (!whole)
+        if (ONE)
+          s_ml[q8] = make_float2(top, sum);
+        else if (!whole)
           a.part_ml[static_cast<size_t>(slot) * ROWS + q8] = make_float2(top, sum);
         else if (a.lse)
           a.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.693147180559945f;
       }
+    }
+    if constexpr (ONE) {
+      __syncthreads();
+      cluster_sync();
+      if (static_cast<int>(share) < R && tid < HD / 4) {
+        float2 ml[PA_CLUSTER];
+        float4 x[PA_CLUSTER];
+#pragma unroll
+        for (int i = 0; i < PA_CLUSTER; ++i) {
+          ml[i] = ld_cluster_f2(&s_ml[share], i);
+          x[i] = ld_cluster_f4(&s_o[0][share][tid * 4], i);
+        }
+        PagedSum all;
+#pragma unroll
+        for (int i = 0; i < PA_CLUSTER; ++i) all.add(ml[i], x[i]);
+        all.finish(a, static_cast<long long>(first) * a.n_q + g * G + share, HD, tid * 4);
+      }
+      __syncthreads();
+      cluster_sync();  // no CTA leaves while its results may be read
+      break;
     }
     if (!whole && ua == 0 && tid == 0) {
       const long long last = base + (local_pair + 1) * upp_u - 1;  // the pair's last unit
@@ -633,26 +714,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) attn_paged_kernel(
 
 // Joins the pieces of the pairs that several CTAs worked on.  A piece's O is [row][channel], or (TC: from
 // mk_attn_paged_tc.cuh) [four channels][row][4]; a thread takes four channels of a row.
-struct PagedSum {
-  float m = kLow, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  __device__ __forceinline__ void add(float2 ml, float4 x) {
-    const float top = fmaxf(m, ml.x), f = ex2_approx(m - top), e = ex2_approx(ml.x - top);
-    m = top;
-    l = l * f + ml.y * e;
-    o.x = o.x * f + x.x * e;
-    o.y = o.y * f + x.y * e;
-    o.z = o.z * f + x.z * e;
-    o.w = o.w * f + x.w * e;
-  }
-  // row `at` (token times heads), channels dim ..
-  __device__ __forceinline__ void finish(const PagedAttnArgs& a, long long at, int hd, int dim) const {
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(a.out + at * hd + dim) =
-        make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
-    if (dim == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945f;
-  }
-};
+//
 // Adds pieces p0, p0 + step, .. of the pair that began in CTA cta to ITEMS sums, 16 channels apart, of row i; the loads
 // of several pieces are on the way at a time (also of the last few: one that is not there counts as empty).
 template <int HD, bool TC, int ITEMS>

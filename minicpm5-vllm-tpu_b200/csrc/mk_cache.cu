@@ -58,6 +58,13 @@ mk_status copy_pages(void* codes, float* scales, int layers, int num_pages, int 
 // 29; 64 rows of 256 16, 17, 23, 36 and 23, 23, 23, 24.  One wave of CTAs, fewer when the bounds say that there are
 // fewer units of work.
 constexpr int kPagedWide = 56;
+// Single tokens of few rows: one launch, a cluster of 8 CTAs per (row, key/value head), while the clusters are at most two
+// CTAs an SM (three do not all fit at once) and a cluster's share of the keys is short.  us with it and with equal shares
+// and a join (hd 96, 2 key/value heads; hd 128 alike): 1 row of 1000 tokens 6.4 and 9.2, of 4096 8.7 and 9.0, of 8192 12.2
+// and 10.1; 16 rows of 1000 7.0 and 10.7, of 8192 15.2 and 19.9; 27 rows of 1000 13.0 and 11.7.
+bool paged_one(int64_t pairs, int group, int max_len) {
+  return group <= mk::PA_ROWS && pairs * mk::PA_CLUSTER <= 2 * mk::PT_CTAS && max_len <= (pairs < 16 ? 4096 : 8192);
+}
 struct PagedPlan {
   bool tc;
   int rows, ctas;  // rows of a tile
@@ -94,10 +101,13 @@ mk_status cache_ready() {
   if (dev < 0 || dev >= 64) return MK_ERR_BAD_ARG;
   std::lock_guard<std::mutex> lk(mu);
   if (ready[dev]) return MK_OK;
-  MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_kernel<96>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               mk::pa_ring_bytes(96)));
-  MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               mk::pa_ring_bytes(128)));
+  const auto allow = [](void (*k)(KvPages, mk::PagedAttnArgs), int hd) {
+    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, mk::pa_ring_bytes(hd));
+  };
+  MK_CUDA(allow(mk::attn_paged_kernel<96, false>, 96));
+  MK_CUDA(allow(mk::attn_paged_kernel<96, true>, 96));
+  MK_CUDA(allow(mk::attn_paged_kernel<128, false>, 128));
+  MK_CUDA(allow(mk::attn_paged_kernel<128, true>, 128));
   MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<96>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(mk::pt_smem_bytes(96))));
   MK_CUDA(cudaFuncSetAttribute(mk::attn_paged_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -207,8 +217,14 @@ mk_status mk_attention_paged(const void* q, int64_t ld_q, int64_t head_ld_q, int
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   void (*k)(KvPages, mk::PagedAttnArgs) =
       p.tc ? (head_dim == 96 ? mk::attn_paged_tc_kernel<96> : mk::attn_paged_tc_kernel<128>)
-           : (head_dim == 96 ? mk::attn_paged_kernel<96> : mk::attn_paged_kernel<128>);
+           : (head_dim == 96 ? mk::attn_paged_kernel<96, false> : mk::attn_paged_kernel<128, false>);
   MK_TRY(cache_ready());
+  const int64_t pairs = static_cast<int64_t>(rows) * n_kv;
+  if (!cu_q && paged_one(pairs, a.group, max_len))
+    return mk::launch_k_cluster(mk::PA_CLUSTER,
+                                head_dim == 96 ? mk::attn_paged_kernel<96, true> : mk::attn_paged_kernel<128, true>,
+                                dim3(static_cast<unsigned>(pairs * mk::PA_CLUSTER)), dim3(mk::PA_THREADS),
+                                mk::pa_ring_bytes(head_dim), st, true, c, a);
   MK_TRY(launch_k(k, dim3(p.ctas), dim3(p.tc ? mk::PT_THREADS : mk::PA_THREADS),
                   p.tc ? mk::pt_smem_bytes(head_dim) : mk::pa_ring_bytes(head_dim), st, true, c, a));
   const auto join = [&](auto hd, auto of_tc) {

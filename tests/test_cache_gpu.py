@@ -266,6 +266,31 @@ def test_attention_missing_page_is_reported(dev):
     assert _err() == (0, 0)
 
 
+@pytest.mark.parametrize("hd,page,n_q,n_kv", [(96, 64, 16, 2), (128, 16, 16, 2), (96, 128, 2, 2), (128, 32, 10, 2)])
+@pytest.mark.parametrize("top", [4096, 8192])
+def test_attention_single_tokens_of_few_rows(dev, hd, page, n_q, n_kv, top):
+    """Lengths around where the shares of eight CTAs begin and end, and up to where the launch changes its form."""
+    lens = [0, 1, 127, 128, 129, 1023, 1024, 1025, 1151, 2047, top - 129, top][: 7 if top == 4096 else 12]
+    _attend(dev, lens, [1] * len(lens), n_q, n_kv, hd, page, 5 + hd + n_q, max_len=top)
+
+
+@pytest.mark.parametrize("case", [test_attention_large_scores, test_attention_contiguous_queries_and_tight_bound,
+                                  test_attention_value_scales_far_apart, test_attention_nan_scale_shows,
+                                  test_attention_zero_and_tiny_queries, test_attention_offsets_past_32_bits,
+                                  test_attention_on_another_stream, test_attention_missing_page_is_reported])
+def test_attention_single_tokens_as_chunks(dev, monkeypatch, case):
+    """Single tokens given as chunks of one take another way through the library: the cases above hold there too."""
+    from minicpm5_mk import ops
+    plain = ops.attention_paged
+
+    def chunks(q, *args, cu_q=None, **kw):
+        each = torch.arange(q.shape[0] + 1, dtype=torch.int32, device=q.device)
+        return plain(q, *args, cu_q=each if cu_q is None else cu_q, **kw)
+
+    monkeypatch.setattr(ops, "attention_paged", chunks)
+    case(dev)
+
+
 @pytest.mark.parametrize("top", [1, 40])
 def test_lengths_and_tokens_out_of_range_are_reported(dev, top):
     """Lengths past the table (up to the largest int) and token ranges past T read and write nothing outside; the
