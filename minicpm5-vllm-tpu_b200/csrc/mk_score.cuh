@@ -33,9 +33,11 @@ __device__ __forceinline__ RowStats stats_join(const RowStats& a, const RowStats
 __device__ __forceinline__ void stats_add(RowStats& s, float x) {
   s = stats_join(s, {x, x == -INFINITY ? 0.f : x - x == 0.f ? 1.f : __int_as_float(0x7fffffff), 0.f});
 }
+// Over groups of N lanes.
+template <int N = 32>
 __device__ __forceinline__ RowStats stats_warp(RowStats s) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
+  for (int o = N / 2; o; o >>= 1) {
     RowStats t;
     t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
     t.z = __shfl_xor_sync(0xffffffffu, s.z, o);
@@ -167,16 +169,27 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
   const int part = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const long long b = blockIdx.x / cluster;
   const E* row = static_cast<const E*>(a.logits) + b * a.ld;
-  const int t = a.targets[b];
-  const bool given = t >= 0 && t < V;
-  const float mine = given ? logit_at(row, t) : INFINITY;
-
   // the row: `head` logits up to a 16-byte boundary, nvec vectors, a tail; this CTA's vectors and loose logits
   const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(E)));
   const int nvec = (V - head) / EPV, tail0 = head + nvec * EPV;
   const int per = (nvec + cluster - 1) / cluster, vec0 = min(nvec, part * per), vec1 = min(nvec, vec0 + per);
   const int lo = part == 0 ? 0 : head + vec0 * EPV, hi = part == cluster - 1 ? V : head + vec1 * EPV;
   const uint4* vecs = reinterpret_cast<const uint4*>(row + head);
+  const int steps = max(1, (vec1 - vec0 + TL_THREADS * VECS - 1) / (TL_THREADS * VECS));
+  uint4 x[VECS];
+  auto load = [&](int step) {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = vec0 + (step * VECS + v) * TL_THREADS + tid;
+      x[v] = make_uint4(kNone, kNone, kNone, kNone);
+      if (at < vec1) x[v] = ldg_once(vecs + at);
+    }
+  };
+  load(0);
+
+  const int t = a.targets[b];
+  const bool given = t >= 0 && t < V;
+  const float mine = given ? logit_at(row, t) : INFINITY;
 
   RowStats st = stats_empty();
   float top = -INFINITY, top1 = -INFINITY, tau = -INFINITY;  // maxima of the even and odd vectors
@@ -225,17 +238,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
     above += loose_x > mine;
   }
 
-  const int steps = max(1, (vec1 - vec0 + TL_THREADS * VECS - 1) / (TL_THREADS * VECS));
-  uint4 x[VECS];
-  auto load = [&](int step) {
-#pragma unroll
-    for (int v = 0; v < VECS; ++v) {
-      const int at = vec0 + (step * VECS + v) * TL_THREADS + tid;
-      x[v] = make_uint4(kNone, kNone, kNone, kNone);
-      if (at < vec1) x[v] = ldg_once(vecs + at);
-    }
-  };
-  load(0);
   int retake = 0;  // the step after which tau is taken next
   for (int step = 0; step < steps; ++step) {
     const int v0 = vec0 + step * TL_THREADS * VECS + tid;
@@ -425,13 +427,21 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
   // the row's
   if (cluster > 1) cluster_sync(); else __syncthreads();
   if (part == 0) {
-    st = {s_res[0], s_res[1], s_res[2]};
-    above = __float_as_int(s_res[3]);
-    for (int c = 1; c < cluster; ++c) {
-      const unsigned long long mz = ld_cluster_u64(&s_res[0], c), wa = ld_cluster_u64(&s_res[2], c);
-      st = stats_join(st, {__uint_as_float(static_cast<uint32_t>(mz)), __uint_as_float(static_cast<uint32_t>(mz >> 32)),
-                           __uint_as_float(static_cast<uint32_t>(wa))});
-      above += static_cast<int>(wa >> 32);
+    const int all = cluster * k;
+    if (cluster > 1) {  // each eight lanes of each warp: lane c has CTA c's statistics
+      const int c = lane % TL_CLUSTER_MAX;
+      const bool has = c < cluster;
+      const unsigned long long mz = ld_cluster_u64(&s_res[0], has ? c : 0), wa = ld_cluster_u64(&s_res[2], has ? c : 0);
+      for (int i = tid; i < all; i += TL_THREADS) s_kept[i] = ld_cluster_u64(&s_top[i % k], i / k);
+      st = stats_empty();
+      if (has)
+        st = {__uint_as_float(static_cast<uint32_t>(mz)), __uint_as_float(static_cast<uint32_t>(mz >> 32)),
+              __uint_as_float(static_cast<uint32_t>(wa))};
+      st = stats_warp<TL_CLUSTER_MAX>(st);
+      above = __reduce_add_sync(0xffffffffu, lane < cluster ? static_cast<int>(wa >> 32) : 0);
+    } else {
+      st = {s_res[0], s_res[1], s_res[2]};
+      above = __float_as_int(s_res[3]);
     }
     if (given && mine != mine) {  // a NaN ranks below every number
       int numbers = 0;
@@ -452,11 +462,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
       a.ent[b] = st.z == 0.f ? 0.f : lz - st.w / st.z;
       a.rank[b] = given ? above + 1 : 0;
     }
-    const int all = cluster * k;
-    if (cluster > 1) {
-      for (int i = tid; i < all; i += TL_THREADS) s_kept[i] = ld_cluster_u64(&s_top[i % k], i / k);
-      __syncthreads();
-    }
+    if (cluster > 1) __syncthreads();
     for (int i = tid; i < all; i += TL_THREADS) {
       const unsigned long long e = cluster > 1 ? s_kept[i] : s_top[i];
       int r = i;
