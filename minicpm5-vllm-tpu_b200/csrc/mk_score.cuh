@@ -466,9 +466,15 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
     for (int i = tid; i < all; i += TL_THREADS) {
       const unsigned long long e = cluster > 1 ? s_kept[i] : s_top[i];
       int r = i;
-      if (cluster > 1) {
+      if (cluster > 1) {  // how many of each CTA's alternatives, in order, come before it
+        int before[TL_CLUSTER_MAX] = {};
+        for (int step = 1 << (31 - __clz(k)); step; step >>= 1)
+#pragma unroll
+          for (int c = 0; c < TL_CLUSTER_MAX; ++c)
+            if (c < cluster && before[c] + step <= k && s_kept[c * k + before[c] + step - 1] > e) before[c] += step;
         r = 0;
-        for (int j = 0; j < all; ++j) r += s_kept[j] > e;
+#pragma unroll
+        for (int c = 0; c < TL_CLUSTER_MAX; ++c) r += before[c];
       }
       if (r < k && e) {
         a.top_ids[b * k + r] = order_id(e);
