@@ -105,10 +105,10 @@ mk_status mk_token_logprobs(const void* logits, int32_t logits_bits, int32_t T, 
   a.top_ids = top_ids;
   a.top_lp = top_logprobs;
   // A row is shared by as many CTAs of 512 threads (up to eight) as still have half a step's 8192 logits each, while
-  // there are SMs for them (us at 130560 f32, k = 5, with 1, 2, 4, 8 CTAs a row: 8 rows 21, 15, 12, 10.5; 74 rows 22,
-  // 18, 24, 31; 148 rows 24, 23, 37, 51).  From there on a row has one CTA: of 512 threads while the rows are up to three
-  // an SM (296 rows 33, with 128 threads 60; 400 rows 50 and 65; bf16 27 and 44, 40 and 47), then of 128, eight to an SM
-  // (1184 rows 117 with 512 threads, 113 with 128; bf16 95 and 75).
+  // there are SMs for them (us at 130560 f32, k = 5, with 1, 2, 4, 8 CTAs a row: 8 rows 21, 15, 11, 10; 74 rows 22, 18,
+  // 23, 29; 148 rows 24, 22, 35, 48).  From there on a row has one CTA: of 512 threads while the rows are up to three an
+  // SM (296 rows 32, with 128 threads 56; 400 rows 49 and 60; bf16 26 and 44, 40 and 47), then of 128, eight to an SM
+  // (1184 rows 125 with 512 threads, 101 with 128; bf16 94 and 74).
   int cluster = 1;
   while (cluster < mk::TL_CLUSTER_MAX && static_cast<int64_t>(T) * cluster * 2 <= d.sm_count && V / (cluster * 2) >= 8192)
     cluster *= 2;

@@ -105,7 +105,7 @@ __device__ __forceinline__ int order_id(unsigned long long e) { return static_ca
 // What bounds it: the bytes of the logits where they are f32 (2047 x 130560, k = 5: 188 us, 5.7 TB/s; k = 0: 165, the
 // rate of a plain copy), the issue slots and the wait for the loads where they are bf16 (2047 x 73448, k = 5: 77 us, 3.9
 // TB/s; k = 0: 61): per bf16 logit the arithmetic is about six instructions and one exponential, two thirds of what an SM
-// can issue at the rate at which HBM delivers them.  Three rows of 130560 f32 take 10.8 us: a launch, two waits for
+// can issue at the rate at which HBM delivers them.  Three rows of 130560 f32 take 9.9 us: a launch, two waits for
 // memory and the cluster's join.
 // Threads per CTA.  128 where there are rows enough (the work at a row's end is the same for every warp, and with
 // 256 threads it was a third of all); 512 where a cluster shares a row, so that a slice of 16384 logits is one step, and
