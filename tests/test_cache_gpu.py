@@ -436,6 +436,57 @@ def test_read_ranges(dev):
     assert _err() == (0, 0)
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+def test_decoding_step_in_a_graph(dev, rows):
+    """Pages reserved, keys appended, attention and scores of one step captured once: each replay gives what the calls
+    give outside."""
+    from minicpm5_mk import ops
+    page, hd, n_kv, steps = 16, 96, 2, 20
+    lens = [(7 * r) % 50 for r in range(rows)]
+    width, pages = 5, 5 * rows + 1
+    codes, scales = ref.pool(pages, n_kv, page, hd, 3)
+    start = ref.tables(lens, page, pages, 3)
+    table = torch.full((rows, width), -1, dtype=torch.int32)
+    table[:, :start.shape[1]] = start
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[table[table >= 0].long()] = 1
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((steps + 3, rows, 12, hd), generator=g).to(BF).to(dev)
+    logits = torch.randn((steps + 3, rows, 5000), generator=g).to(dev)
+    ids = torch.randint(0, 5000, (rows,), generator=g, dtype=torch.int32).to(dev)
+
+    def state():
+        return [t.clone() for t in _gpu(dev, codes, scales, table, _i32(lens), refs)]
+
+    def step(st, xs, lg):
+        cd, sd, t, n, f = st
+        ops.kv_reserve(t, n, f, None, page)
+        ops.kv_append(xs[:, 8:10], xs[:, 10:12], cd, sd, t, n)
+        n += 1
+        return (*ops.attention_paged(xs[:, :8], cd, sd, t, n, softmax_scale=0.1), *ops.token_logprobs(lg, ids, 3))
+
+    there, here = state(), state()
+    xs, lg = x[0].clone(), logits[0].clone()
+    side = torch.cuda.Stream(dev)
+    with torch.cuda.stream(side):
+        step(state(), xs, lg)  # outside a capture first
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(there, xs, lg)
+    for t, w in zip(there, state()):
+        t.copy_(w)
+    for i in range(steps):
+        xs.copy_(x[i])
+        lg.copy_(logits[i])
+        graph.replay()
+        for a, b in zip(got, step(here, x[i], logits[i])):
+            assert a.equal(b)
+    for a, b in zip(there, here):
+        assert a.equal(b)
+    assert _err() == (0, 0)
+
+
 def test_append_without_a_page_is_reported(dev):
     from minicpm5_mk import ops
     codes, scales = ref.pool(4, 2, 16, 96, 1)
