@@ -175,7 +175,11 @@ mk_status mk_score_tokens(const void* h, int32_t T, int32_t H, int64_t ld, const
   else
     MK_TRY(launch_k(mk::score_tokens_kernel<false>, dim3(units), dim3(mk::SC_THREADS),
                     mk::SC_SMEM_BYTES, st, true, mh, mw, a));
-  return launch_k(mk::score_join_kernel, dim3((T + mk::SJ_TOKENS - 1) / mk::SJ_TOKENS), dim3(mk::SJ_THREADS), 0, st, true, a, logprobs, entropy);
+  // (many tokens fill the GPU with fewer slices each: 8192 tokens' 287 parts join in 11 us
+  // with 256 threads a CTA, in 13.5 with 512, 19 with 1024, 16 with 128)
+  const int join = T > d.sm_count * 16 ? 256 : mk::SJ_THREADS;
+  return launch_k(mk::score_join_kernel, dim3((T + mk::SJ_TOKENS - 1) / mk::SJ_TOKENS), dim3(join), 0, st, true, a, logprobs,
+                  entropy);
 }
 
 }  // extern "C"

@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
 // H = 1536 the tensor cores take 12288 cycles for a 128 x 256 tile and the exponentials 2048, hidden behind the
 // next tile's products (two accumulators fill the 512 TMEM columns).  With few tokens W's bytes are the bound.
 // Measured: 8192 tokens x 73448 ids, H 1536, 1079 us (1713 TFLOP/s, alone) and 1.28 ms in a row of calls under the power
-// limit, with 19 us for the join of the parts; 37 tokens x 130560 ids 63 us, 6.4 TB/s of W, and 5 us for the join.
+// limit, with 11 us for the join of the parts; 37 tokens x 130560 ids 63 us, 6.4 TB/s of W, and 5 us for the join.
 //
 // Layout.  PAIR (more than 128 tokens): two CTAs work on 256 tokens x 256 ids with 2-SM MMAs, each holding its 128
 // tokens and half of the ids, which halves the operand bytes that each SM takes in per product.  Otherwise one
@@ -792,10 +792,10 @@ __device__ __forceinline__ RowStats stats_join2(const RowStats& a, const RowStat
   r.w = (a.w + a.z * fmaxf(da, kFar)) * ea + (b.w + b.z * fmaxf(db, kFar)) * eb;
   return r;
 }
-// Joins a token's parts: 8 tokens x 128 slices of the parts per CTA; a slice in order, then the slices in a
+// Joins a token's parts: 8 tokens x (threads / 8) slices of the parts per CTA; a slice in order, then the slices in a
 // fixed order.
 constexpr int SJ_TOKENS = 8;
-constexpr int SJ_THREADS = 1024;
+constexpr int SJ_THREADS = 1024;  // at most
 __global__ void __launch_bounds__(SJ_THREADS)
     score_join_kernel(const ScoreArgs args, float* __restrict__ lp, float* __restrict__ ent) {
   __shared__ RowStats s_p[SJ_THREADS / 32][SJ_TOKENS];
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(SJ_THREADS)
   RowStats s = stats_empty();
   if (t < args.T) {
 #pragma unroll 4
-    for (int vt = threadIdx.x / SJ_TOKENS; vt < args.parts; vt += SJ_THREADS / SJ_TOKENS) {
+    for (int vt = threadIdx.x / SJ_TOKENS; vt < args.parts; vt += blockDim.x / SJ_TOKENS) {
       const float* p = args.part + static_cast<long long>(vt) * 3 * args.ld_part + t;
       s = stats_join2(s, {p[0], p[args.ld_part], p[2 * args.ld_part]});
     }
@@ -821,8 +821,8 @@ __global__ void __launch_bounds__(SJ_THREADS)
   __syncthreads();
   if (warp) return;
   s = s_p[lane / SJ_TOKENS][k];
-#pragma unroll
-  for (int i = 4; i < SJ_THREADS / 32; i += 4) s = stats_join2(s, s_p[i + lane / SJ_TOKENS][k]);
+#pragma unroll 4
+  for (int i = 4; i < static_cast<int>(blockDim.x) / 32; i += 4) s = stats_join2(s, s_p[i + lane / SJ_TOKENS][k]);
   s = stats_join2(s, across(8));
   s = stats_join2(s, across(16));
   if (lane >= SJ_TOKENS || t >= args.T) return;
