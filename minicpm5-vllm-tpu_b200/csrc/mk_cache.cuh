@@ -126,6 +126,8 @@ __global__ void __launch_bounds__(kva_threads(HD, SHIFT))
   const int slot = (len >> SHIFT) + blockIdx.x % touched;
   const int pos0 = slot << SHIFT;
   if (slot > width || pos0 - len >= n) return;  // (the first slot past the table is an error below)
+  // more tokens than the launch was told of: those in the pages that follow are not written
+  if (blockIdx.x % touched == touched - 1 && pos0 + (1 << SHIFT) - len < n) atomicCAS(err, 0, DEV_ERR_BAD_PAGE);
   const int page = kv_page_of(table, width, c.num_pages, row, slot, err);
   if (page < 0) return;
   const long long ld = plane ? ld_v : ld_k;

@@ -436,6 +436,27 @@ def test_read_ranges(dev):
     assert _err() == (0, 0)
 
 
+def test_append_of_more_tokens_than_announced_is_reported(dev):
+    """max_new bounds a row's new tokens: pages past those that so many can touch are left alone, and the error word
+    says so.  40 tokens from position 3 touch three pages of 16, 18 may as well, 2 touch two at most."""
+    from minicpm5_mk import ops
+    codes, scales = ref.pool(5, 2, 16, 96, 1)
+    table = ref.tables([64], 16, 5, 1)
+    x = torch.randn((40, 2, 96), generator=torch.Generator().manual_seed(3)).to(BF).to(dev)
+    cd, sd = codes.to(dev), scales.to(dev)
+    ops.kv_append(x, x, cd, sd, *_gpu(dev, table, _i32([3]), _i32([0, 40])), max_new=2)
+    assert _err() == (10, 0x500)
+    for p in (*table[0, 2:].tolist(), *sorted(set(range(5)) - set(table[0].tolist()))):
+        assert cd[p].cpu().equal(codes[p]) and sd[p].cpu().equal(scales[p])
+    for bound in (18, 40):
+        cd, sd = codes.to(dev), scales.to(dev)
+        ops.kv_append(x, x, cd, sd, *_gpu(dev, table, _i32([3]), _i32([0, 40])), max_new=bound)
+        c, s = codes.clone(), scales.clone()
+        ref.append(x.cpu(), x.cpu(), c, s, table, [3], [0, 40])
+        _check_pool(c, s, cd, sd, range(5))
+    assert _err() == (0, 0)
+
+
 @pytest.mark.parametrize("rows", [2, 40])
 def test_decoding_step_in_a_graph(dev, rows):
     """Pages reserved, keys appended, attention and scores of one step captured once: each replay gives what the calls
